@@ -204,8 +204,9 @@ def _experts(s):
 def _quantise(s):
     x = s["x"].float()
     most = x.abs().amax(1, keepdim=True)
-    q = torch.clamp(torch.round(x * (127.0 / most)), -127, 127)
-    return {"q": q.to(torch.int8), "scale": (most / 127.0)[:, 0]}
+    top = torch.full_like(most, 127.0)  # a tensor: torch divides by a number as a product with its reciprocal
+    q = torch.clamp(torch.round(x * (top / most)), -127, 127)
+    return {"q": q.to(torch.int8), "scale": (most / top)[:, 0]}
 
 
 def _product(s):
