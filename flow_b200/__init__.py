@@ -21,12 +21,14 @@ import ctypes
 from typing import Sequence
 
 from . import _native
-from .records import (ExprOp, GpuProfile, KSplit, MoveSite, TileRead, TileSite, conv2d_site, fir_site,
-                      matmul_site, program, transpose_site)
+from .records import (DTYPES, ExpertSite, ExprOp, GpuProfile, I8Site, KSplit, MoveSite, NormSite, QuantSite, TileRead,
+                      TileSite, conv2d_site, expert_site, fir_site, matmul_i8_site, matmul_site, norm_site, program,
+                      quant_site, transpose_site)
 
 __all__ = [
     "Context", "MapalTrap", "MapalInfraError", "Unsupported", "TileSite", "TileRead", "KSplit",
     "MoveSite", "GpuProfile", "matmul_site", "fir_site", "conv2d_site", "transpose_site",
+    "NormSite", "ExpertSite", "QuantSite", "I8Site", "norm_site", "expert_site", "quant_site", "matmul_i8_site",
     "STRICT", "TF32X3", "U11", "U01", "OP_ADD", "OP_SUB", "OP_MUL", "OP_DIV", "OP_MOD",
     "shard_range", "render_f32", "render_f64", "lib",
 ]
@@ -91,6 +93,42 @@ def _ptr(t) -> int:
 
 def _arr(ptrs: Sequence) -> ctypes.Array:
     return (ctypes.c_void_p * len(ptrs))(*[_ptr(p) for p in ptrs])
+
+
+_torch_types: dict[int, object] = {}  # MAPAL_DTYPE_* (and 4: int32) -> torch dtype, filled on first use
+
+
+def _span(rows: int, cols: int, ld: int) -> int:
+    """Elements from the first to the last of rows x cols at row stride ld."""
+    return (rows - 1) * ld + cols if rows and cols else 0
+
+
+def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0) -> int:
+    """Address of a device buffer of a row-wise operator: None (0), an int address taken as given, or a torch
+    tensor, which must be of the record's type, on the context's device, with `need` elements from its first."""
+    if t is None:
+        return 0
+    if isinstance(t, int):
+        return t
+    if not _torch_types:
+        import torch
+        _torch_types.update({DTYPES[str(d).replace("torch.", "")]: d
+                             for d in (torch.float32, torch.float16, torch.bfloat16, torch.int8)})
+        _torch_types[4] = torch.int32
+    if t.dtype is not _torch_types.get(code):
+        raise ValueError(f"{what} is {t.dtype}, the record says {_torch_types.get(code)}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, the context drives cuda:{device}")
+    if not (t.is_contiguous() and t.numel() >= need):
+        if t.numel() and t.dim():
+            if t.stride(-1) != 1 and t.size(-1) > 1:
+                raise ValueError(f"{what}: the elements of a row must be contiguous")
+            if ld and t.dim() > 1 and t.size(-2) > 1 and t.stride(-2) != ld:
+                raise ValueError(f"{what} has row stride {t.stride(-2)}, the record says {ld}")
+        have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+        if have < need:
+            raise ValueError(f"{what} holds {have} elements, the record needs {need}")
+    return t.data_ptr()
 
 
 def _u64s(vals: Sequence[int]) -> ctypes.Array:
@@ -292,6 +330,96 @@ class Context:
 
     def tile_site(self, site: TileSite, a, b, out, mode: int = STRICT) -> None:
         _check(lib().mapal_gpu_tile_site_f32(self._h, ctypes.byref(site), _ptr(a), _ptr(b), _ptr(out), mode))
+
+    # ---- rows of a model's layer (local device 0) --------------------------------------
+    def layer_norm(self, site: NormSite, x, w, b, y, mean=None, rstd=None) -> None:
+        """y = (x - mean(x)) / sqrt(var(x) + eps) * w + b for each row; mean and rstd for the gradient."""
+        dev, rows, d, t, ldx, ldy = self.devices[0], site.rows, site.d, site.dtype, site.ldx, site.ldy
+        _check(lib().mapal_gpu_layer_norm(
+            self._h, ctypes.byref(site), _buf(x, t, _span(rows, d, ldx), dev, "x", ldx),
+            _buf(w, site.wtype, d, dev, "w"), _buf(b, site.wtype, d, dev, "b"),
+            _buf(y, t, _span(rows, d, ldy), dev, "y", ldy), _buf(mean, 0, rows, dev, "mean"),
+            _buf(rstd, 0, rows, dev, "rstd")))
+
+    def layer_norm_grad_workspace(self, site: NormSite) -> int:
+        """Bytes of scratch that layer_norm_grad takes."""
+        n = ctypes.c_uint64()
+        _check(lib().mapal_gpu_layer_norm_grad_workspace(self._h, ctypes.byref(site), ctypes.byref(n)))
+        return n.value
+
+    def layer_norm_grad(self, site: NormSite, x, w, mean, rstd, dy, dx, dw, db, work) -> None:
+        """dx, dw and db (f32; either may be None) of layer_norm. `work`: a CUDA buffer of at least
+        layer_norm_grad_workspace(site) bytes, its own for calls that may overlap."""
+        dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
+        if work is not None and work.get_device() != dev:
+            raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
+        _check(lib().mapal_gpu_layer_norm_grad(
+            self._h, ctypes.byref(site), _buf(x, t, _span(rows, d, site.ldx), dev, "x", site.ldx),
+            _buf(w, site.wtype, d, dev, "w"), _buf(mean, 0, rows, dev, "mean"), _buf(rstd, 0, rows, dev, "rstd"),
+            _buf(dy, t, _span(rows, d, site.lddy), dev, "dy", site.lddy),
+            _buf(dx, t, _span(rows, d, site.lddx), dev, "dx", site.lddx), _buf(dw, 0, d, dev, "dw"),
+            _buf(db, 0, d, dev, "db"), 0 if work is None else work.data_ptr(),
+            0 if work is None else work.numel() * work.element_size()))
+
+    def expert_sort(self, site: ExpertSite, ids, offsets, order, pos) -> None:
+        """Slots sorted by expert, stably: offsets (experts + 1), order (place -> slot; may be None) and pos
+        (slot -> place, -1 where ids is -1), all int32."""
+        dev, n = self.devices[0], site.tokens * site.k
+        _check(lib().mapal_gpu_expert_sort(
+            self._h, ctypes.byref(site), _buf(ids, 4, n, dev, "ids"),
+            _buf(offsets, 4, site.experts + 1, dev, "offsets"), _buf(order, 4, n, dev, "order"),
+            _buf(pos, 4, n, dev, "pos")))
+
+    def expert_dispatch(self, site: ExpertSite, x, pos, xs, scale=None, scale_out=None) -> None:
+        """xs[pos[t, j]] = x[t], and scale_out likewise from scale (the scales of 8-bit rows)."""
+        dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
+        _check(lib().mapal_gpu_expert_dispatch(
+            self._h, ctypes.byref(site), _buf(x, t, _span(tokens, d, site.ldt), dev, "x", site.ldt),
+            _buf(scale, 0, tokens, dev, "scale"), _buf(pos, 4, tokens * site.k, dev, "pos"),
+            _buf(xs, t, _span(site.rows, d, site.ldr), dev, "xs", site.ldr),
+            _buf(scale_out, 0, site.rows, dev, "scale_out")))
+
+    def expert_combine(self, site: ExpertSite, h, w, pos, y) -> None:
+        """y[t] = sum over j of w[t, j] * h[pos[t, j]] (w None: 1)."""
+        dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
+        _check(lib().mapal_gpu_expert_combine(
+            self._h, ctypes.byref(site), _buf(h, t, _span(site.rows, d, site.ldr), dev, "h", site.ldr),
+            _buf(w, 0, tokens * site.k, dev, "w"), _buf(pos, 4, tokens * site.k, dev, "pos"),
+            _buf(y, t, _span(tokens, d, site.ldt), dev, "y", site.ldt)))
+
+    def expert_dispatch_grad(self, site: ExpertSite, dxs, pos, dx) -> None:
+        """dx[t] = sum over j of dxs[pos[t, j]]."""
+        dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
+        _check(lib().mapal_gpu_expert_dispatch_grad(
+            self._h, ctypes.byref(site), _buf(dxs, t, _span(site.rows, d, site.ldr), dev, "dxs", site.ldr),
+            _buf(pos, 4, tokens * site.k, dev, "pos"), _buf(dx, t, _span(tokens, d, site.ldt), dev, "dx", site.ldt)))
+
+    def expert_combine_grad(self, site: ExpertSite, h, w, pos, dy, dh, dw) -> None:
+        """dh[pos[t, j]] = w[t, j] * dy[t] and dw[t, j] = <dy[t], h[pos[t, j]]> (dw may be None)."""
+        dev, t, d, tokens, n = self.devices[0], site.dtype, site.d, site.tokens, site.tokens * site.k
+        sorted_span = _span(site.rows, d, site.ldr)
+        _check(lib().mapal_gpu_expert_combine_grad(
+            self._h, ctypes.byref(site), _buf(h, t, sorted_span, dev, "h", site.ldr), _buf(w, 0, n, dev, "w"),
+            _buf(pos, 4, n, dev, "pos"), _buf(dy, t, _span(tokens, d, site.ldt), dev, "dy", site.ldt),
+            _buf(dh, t, sorted_span, dev, "dh", site.ldr), _buf(dw, 0, n, dev, "dw")))
+
+    def quantize_rows_i8(self, site: QuantSite, x, q, scale) -> None:
+        """scale = max|x|/127 and q = x/scale rounded to int8, for each row."""
+        dev, rows, d = self.devices[0], site.rows, site.d
+        _check(lib().mapal_gpu_quantize_rows_i8(
+            self._h, ctypes.byref(site), _buf(x, site.dtype, _span(rows, d, site.ldx), dev, "x", site.ldx),
+            _buf(q, 3, _span(rows, d, site.ldq), dev, "q", site.ldq), _buf(scale, 0, rows, dev, "scale")))
+
+    def matmul_i8(self, site: I8Site, A, scale_a, B, scale_b, C, offsets=None) -> None:
+        """C[i] = (A[i] . B[g]^T) * scale_a[i] * scale_b[g] with exact integer sums; rows offsets[g] to
+        offsets[g + 1] belong to g (offsets None: one matrix for all rows)."""
+        dev, m, n, k, groups, ldb = self.devices[0], site.m, site.n, site.k, site.groups, site.ldb
+        _check(lib().mapal_gpu_matmul_i8(
+            self._h, ctypes.byref(site), _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),
+            _buf(scale_a, 0, m, dev, "scale_a"),
+            _buf(B, 3, _span(groups, _span(n, k, ldb), site.ldg), dev, "B", ldb),
+            _buf(scale_b, 0, groups * n, dev, "scale_b"), _buf(offsets, 4, groups + 1, dev, "offsets"),
+            _buf(C, site.dtype, _span(m, n, site.ldc), dev, "C", site.ldc)))
 
     # ---- sharded sites (one buffer per local device) --------------------------------
     def saxpy_sharded(self, a: float, xs, y0s, outs) -> None:

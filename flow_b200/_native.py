@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-from .records import ExprOp, GpuProfile, MoveSite, TileSite
+from .records import ExpertSite, ExprOp, GpuProfile, I8Site, MoveSite, NormSite, QuantSite, TileSite
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmapal_gpu.so")
 
@@ -67,6 +67,17 @@ SIGNATURES: dict[str, tuple] = {
     "mapal_gpu_broadcast_f32": (_int, [_vp, _pp, _u64, _int]),
     "mapal_gpu_gather_sharded": (_int, [_vp, _pp, _u64, _pp, _pp, _pu64]),
     "mapal_gpu_matmul_f32_sharded": (_int, [_vp, _c.POINTER(TileSite), _pp, _pp, _pp, _pu64, _int, _int]),
+    "mapal_gpu_layer_norm": (_int, [_vp, _c.POINTER(NormSite), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mapal_gpu_layer_norm_grad_workspace": (_int, [_vp, _c.POINTER(NormSite), _pu64]),
+    "mapal_gpu_layer_norm_grad": (_int, [_vp, _c.POINTER(NormSite), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                         _u64]),
+    "mapal_gpu_expert_sort": (_int, [_vp, _c.POINTER(ExpertSite), _vp, _vp, _vp, _vp]),
+    "mapal_gpu_expert_dispatch": (_int, [_vp, _c.POINTER(ExpertSite), _vp, _vp, _vp, _vp, _vp]),
+    "mapal_gpu_expert_combine": (_int, [_vp, _c.POINTER(ExpertSite), _vp, _vp, _vp, _vp]),
+    "mapal_gpu_expert_dispatch_grad": (_int, [_vp, _c.POINTER(ExpertSite), _vp, _vp, _vp]),
+    "mapal_gpu_expert_combine_grad": (_int, [_vp, _c.POINTER(ExpertSite), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mapal_gpu_quantize_rows_i8": (_int, [_vp, _c.POINTER(QuantSite), _vp, _vp, _vp]),
+    "mapal_gpu_matmul_i8": (_int, [_vp, _c.POINTER(I8Site), _vp, _vp, _vp, _vp, _vp, _vp]),
     "mapal_gpu_probe_mma_peak": (_int, [_vp, _int, _c.c_uint32, _c.POINTER(_c.c_double)]),
     "mapal_gpu_probe_launch_floor": (_int, [_vp, _int, _vp, _u64, _vp]),
     # mapal-rt re-exports (include/mapal_rt.h)

@@ -150,3 +150,71 @@ def transpose_site(R: int, C: int) -> MoveSite:
     s = MoveSite()
     s.width, s.rows, s.cq, s.cr, s.len = R, C, 1, C, R * C
     return s
+
+
+# ---- records of the row-wise operators -----------------------------------------------------------
+
+DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3}  # MAPAL_DTYPE_*
+
+
+def dtype_code(dtype) -> int:
+    """MAPAL_DTYPE_* of a torch or numpy dtype, a name, or the code itself."""
+    if isinstance(dtype, int):
+        return dtype
+    name = str(dtype).replace("torch.", "")
+    if name not in DTYPES:
+        raise ValueError(f"no element type {dtype!r}: one of {sorted(DTYPES)}")
+    return DTYPES[name]
+
+
+class NormSite(ctypes.Structure):
+    """Rows to normalise (MapalNormSite)."""
+    _fields_ = [("rows", ctypes.c_uint64), ("d", ctypes.c_uint64), ("ldx", ctypes.c_uint64), ("ldy", ctypes.c_uint64),
+                ("lddy", ctypes.c_uint64), ("lddx", ctypes.c_uint64), ("eps", ctypes.c_float),
+                ("dtype", ctypes.c_int32), ("wtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class ExpertSite(ctypes.Structure):
+    """Tokens that go to k of several experts each (MapalExpertSite)."""
+    _fields_ = [("tokens", ctypes.c_uint64), ("d", ctypes.c_uint64), ("rows", ctypes.c_uint64),
+                ("ldt", ctypes.c_uint64), ("ldr", ctypes.c_uint64), ("k", ctypes.c_uint32),
+                ("experts", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class QuantSite(ctypes.Structure):
+    """Rows to 8 bits (MapalQuantSite)."""
+    _fields_ = [("rows", ctypes.c_uint64), ("d", ctypes.c_uint64), ("ldx", ctypes.c_uint64), ("ldq", ctypes.c_uint64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class I8Site(ctypes.Structure):
+    """An 8-bit product, of one matrix or one per group of rows (MapalI8Site)."""
+    _fields_ = [("m", ctypes.c_uint64), ("n", ctypes.c_uint64), ("k", ctypes.c_uint64), ("lda", ctypes.c_uint64),
+                ("ldb", ctypes.c_uint64), ("ldg", ctypes.c_uint64), ("ldc", ctypes.c_uint64),
+                ("groups", ctypes.c_uint32), ("dtype", ctypes.c_int32)]
+
+
+def norm_site(rows: int, d: int, dtype, wdtype=None, eps: float = 1e-5, ldx: int = 0, ldy: int = 0, lddy: int = 0,
+              lddx: int = 0) -> NormSite:
+    """rows x d elements of `dtype`, w and b of `wdtype` (default: the same); strides 0: contiguous rows."""
+    code = dtype_code(dtype)
+    return NormSite(rows, d, ldx or d, ldy or d, lddy or d, lddx or d, eps, code,
+                    code if wdtype is None else dtype_code(wdtype), 0)
+
+
+def expert_site(tokens: int, k: int, experts: int, d: int, dtype, rows: int | None = None, ldt: int = 0,
+                ldr: int = 0) -> ExpertSite:
+    """tokens rows of d elements, k experts each; `rows`: rows of the sorted arrays (default tokens*k)."""
+    return ExpertSite(tokens, d, tokens * k if rows is None else rows, ldt or d, ldr or d, k, experts,
+                      dtype_code(dtype), 0)
+
+
+def quant_site(rows: int, d: int, dtype, ldx: int = 0, ldq: int = 0) -> QuantSite:
+    return QuantSite(rows, d, ldx or d, ldq or d, dtype_code(dtype), 0)
+
+
+def matmul_i8_site(m: int, n: int, k: int, dtype, groups: int = 1, lda: int = 0, ldb: int = 0, ldg: int = 0,
+                   ldc: int = 0) -> I8Site:
+    """C (m x n, of `dtype`) from A (m x k) and `groups` matrices B (n x k); strides 0: contiguous."""
+    ldb = ldb or k
+    return I8Site(m, n, k, lda or k, ldb, ldg or n * ldb, ldc or n, groups, dtype_code(dtype))

@@ -465,6 +465,157 @@ int mapal_gpu_matmul_f32_sharded(MapalGpuCtx* ctx, const MapalTileSite* site,
                                  const float* const* A, float* const* B, float* const* C,
                                  const uint64_t* m, int root, int mode);
 
+/* ---- rows of a model's layer ----------------------------------------------------
+ * No counterpart in the reference, whose arrays are f32 and i32: the row-wise
+ * operators around a feed-forward layer of experts, for training and serving.
+ * They keep this ABI's manner: a record of sizes and strides, caller-owned
+ * device buffers, stream order on local device 0's stream, traps by the flag.
+ * Nothing is allocated and no scratch of the context is used, so two contexts
+ * may run at once and a call may be captured into a CUDA graph (sync mode off,
+ * the capturing stream set with mapal_gpu_set_stream); a trap raised by a
+ * replay surfaces at the next mapal_gpu_synchronize. The calling thread's
+ * current device is left as it was. Strides are in elements; a row's elements
+ * are contiguous. Any alignment of a type is accepted, 16-byte aligned rows
+ * are the fast ones. Arithmetic is f32 (exact 32-bit integers for the 8-bit
+ * product); values are rounded to a 16-bit type once, on writing. Outputs do
+ * not depend on timing: no floating-point atomics. */
+#define MAPAL_DTYPE_F32 0
+#define MAPAL_DTYPE_F16 1
+#define MAPAL_DTYPE_BF16 2
+#define MAPAL_DTYPE_I8 3 /* where stated */
+
+/* Rows of `d` elements to normalise. wtype: the type of w and b. */
+typedef struct MapalNormSite {
+  uint64_t rows;
+  uint64_t d;
+  uint64_t ldx;  /* row strides of x, y, dy and dx */
+  uint64_t ldy;
+  uint64_t lddy;
+  uint64_t lddx;
+  float eps;
+  int32_t dtype; /* x, y, dy, dx */
+  int32_t wtype; /* w, b: dtype or MAPAL_DTYPE_F32 */
+  int32_t reserved;
+} MapalNormSite;
+
+/* Layer norm: mu = mean(x), r = 1/sqrt(mean((x - mu)^2) + eps),
+ * y = (x - mu)*r*w + b for each row. w and b (d values; NULL: 1 and 0);
+ * mean and rstd (one float a row, what the gradient needs; either may be
+ * NULL). The variance is taken around the mean, not as a difference of
+ * squares. y may be x itself (same pointer and stride). */
+int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site, const void* x, const void* w, const void* b,
+                         void* y, float* mean, float* rstd);
+
+/* Bytes of scratch that mapal_gpu_layer_norm_grad takes for this site on this
+ * context's device, for dw and db together. */
+int mapal_gpu_layer_norm_grad_workspace(MapalGpuCtx* ctx, const MapalNormSite* site, uint64_t* bytes);
+
+/* The gradient of layer norm from the forward call's x, w, mean and rstd:
+ * with h = (x - mean)*rstd and g = dy*w,
+ *   dx = rstd*(g - mean(g) - h*mean(g*h)),  dw = sum over rows of dy*h,
+ *   db = sum over rows of dy.
+ * dw and db are d floats whatever the types, written (not added to); either
+ * may be NULL. They are summed in f32 in an order fixed by the record and the
+ * device, so they are the same on every run. `work` is scratch of at least
+ * the stated bytes, 16-byte aligned, used until the call's work has finished:
+ * calls that may overlap need one each (NULL when both dw and db are).
+ * dx may be dy itself. rows = 0 writes zeros to dw and db. */
+int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* site, const void* x, const void* w,
+                              const float* mean, const float* rstd, const void* dy, void* dx, float* dw, float* db,
+                              void* work, uint64_t work_bytes);
+
+/* Tokens that go to k of `experts` each. Token arrays (x, y, dy, dx) have
+ * `tokens` rows at stride ldt, sorted arrays (xs, h, dh, dxs) `rows` rows at
+ * stride ldr. tokens*k < 2^31, experts <= 1024. */
+typedef struct MapalExpertSite {
+  uint64_t tokens;
+  uint64_t d;
+  uint64_t rows;
+  uint64_t ldt;
+  uint64_t ldr;
+  uint32_t k;
+  uint32_t experts;
+  int32_t dtype; /* MAPAL_DTYPE_I8 in mapal_gpu_expert_dispatch alone */
+  int32_t reserved;
+} MapalExpertSite;
+
+/* Sort the slots t*k + j by the expert ids[t*k + j], stably:
+ *   offsets[e] = number of slots of experts before e (experts + 1 values),
+ *   order[p] = the slot at sorted place p (may be NULL),
+ *   pos[slot] = its place, -1 for a slot without an expert.
+ * An id of -1 names no expert (padding). Any other id outside [0, experts)
+ * traps index_oob; its slot is treated as without an expert. order is written
+ * up to offsets[experts]; what lies behind is left as it was. */
+int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* site, const int32_t* ids, int32_t* offsets,
+                          int32_t* order, int32_t* pos);
+
+/* xs[pos[t*k + j]] = x[t], and where scale is given (one float a token, the
+ * scales of 8-bit rows) scale_out[pos[t*k + j]] = scale[t]. A negative pos is
+ * skipped, one at or above site->rows traps index_oob and is skipped; rows
+ * that no pos names are left as they were. Two slots with the same place give
+ * that row either token's values. */
+int mapal_gpu_expert_dispatch(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* x, const float* scale,
+                              const int32_t* pos, void* xs, float* scale_out);
+
+/* y[t] = sum over j ascending of w[t*k + j]*h[pos[t*k + j]] in f32 (w NULL:
+ * 1). A slot without a place adds nothing, whatever its weight; a token
+ * without any gets zeros. */
+int mapal_gpu_expert_combine(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* h, const float* w,
+                             const int32_t* pos, void* y);
+
+/* The gradient of dispatch: dx[t] = sum over j ascending of dxs[pos[t*k + j]]. */
+int mapal_gpu_expert_dispatch_grad(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* dxs,
+                                   const int32_t* pos, void* dx);
+
+/* The gradient of combine: dh[pos[t*k + j]] = w[t*k + j]*dy[t] and
+ * dw[t*k + j] = <dy[t], h[pos[t*k + j]]> (0 for a slot without a place).
+ * w NULL: 1; dw may be NULL. Rows of dh that no pos names are left as they
+ * were. dh may be h itself. */
+int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* h, const float* w,
+                                  const int32_t* pos, const void* dy, void* dh, float* dw);
+
+/* Rows of `d` elements to 8 bits. */
+typedef struct MapalQuantSite {
+  uint64_t rows;
+  uint64_t d;
+  uint64_t ldx;
+  uint64_t ldq;
+  int32_t dtype; /* x */
+  int32_t reserved;
+} MapalQuantSite;
+
+/* Symmetric 8-bit rows: with a = max|x| of the row, scale = a/127 and
+ * q = x*(127/a) rounded to nearest even and kept within [-127, 127], every
+ * step in f32, so q*scale stands for x. A row of zeros, and one so small that
+ * 127/a overflows (a below 3.74e-37), has scale 0 and q = 0; a row that holds
+ * a NaN or an infinity has scale NaN and q = 0. */
+int mapal_gpu_quantize_rows_i8(MapalGpuCtx* ctx, const MapalQuantSite* site, const void* x, int8_t* q, float* scale);
+
+/* An 8-bit product: A is m x k, B holds `groups` matrices of n x k (a weight's
+ * rows are its output channels, contiguous along k, as A's), C is m x n. */
+typedef struct MapalI8Site {
+  uint64_t m;
+  uint64_t n;
+  uint64_t k;
+  uint64_t lda;
+  uint64_t ldb;
+  uint64_t ldg;  /* from one of B's matrices to the next */
+  uint64_t ldc;
+  uint32_t groups;
+  int32_t dtype; /* C */
+} MapalI8Site;
+
+/* C[i, j] = (sum over k of A[i, k]*B[g][j, k]) * scale_a[i] * scale_b[g*n + j],
+ * the sum exact in 32-bit integers (k < 131072), converted to f32 and
+ * multiplied by scale_a, then by scale_b, each rounded to f32 (NULL scales:
+ * 1). offsets NULL: groups is 1 and every row belongs to it. Otherwise rows
+ * offsets[g] to offsets[g + 1] (groups + 1 values on the device, as
+ * mapal_gpu_expert_sort writes them) belong to g; rows of C in no group are
+ * left as they were. Offsets that descend or leave [0, m] trap index_oob and
+ * are taken as if clamped. k = 0 gives zeros times the scales. */
+int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, const int8_t* A, const float* scale_a,
+                        const int8_t* B, const float* scale_b, const int32_t* offsets, void* C);
+
 /* ---- measurement --------------------------------------------------------------
  * No counterpart in the reference: the roofline of MAPAL_MATMUL_TF32X3.
  * Issues the 3xTF32 GEMM's own tensor-core instruction (tcgen05.mma M128 N256,
