@@ -6,7 +6,12 @@
 // is exact in 32 bits for k < 2^17 (127^2 and even 128^2 times k stays below
 // 2^31), so any split or order of it gives the same bits; the float steps are
 // one conversion and two multiplications, each rounded to f32.
+#include <cooperative_groups.h>
+
 #include "rows.cuh"
+#include "tcgen05.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -81,6 +86,402 @@ __global__ void __launch_bounds__(kThreads) mm_i8_tile_kernel(const MapalI8Site 
   }
 }
 
+// ---- tensor cores ------------------------------------------------------------------
+//
+// The product is taken as D = B*A^T: B's rows (channels) are the M dimension
+// of tcgen05.mma and A's rows (tokens) the N dimension, so that a tile may be
+// as narrow in tokens as there are tokens (16 at least) while the weights,
+// which a small batch spends its time reading, always fill the 128 lanes, and
+// so that neighbouring lanes hold neighbouring elements of a row of C.
+//
+// One CTA owns a tile of 128 channels and up to NT tokens of one group:
+//   warp 0     walks the tiles; one lane issues the TMA loads of each 128-byte
+//              block of k (128-byte swizzle) into a ring of STAGES stages. k's
+//              tail and channels beyond n read as zeros;
+//   warp 1     allocates TMEM (two accumulators, so the next tile's products
+//              run beside this tile's output) and issues kind::i8, K32, with N
+//              the tile's tokens rounded up to 16;
+//   warps 2-5  read the accumulator, scale and store C.
+// Tiles are numbered channel tiles first, then token tiles, then groups, and a
+// persistent grid takes every gridDim-th; each warp finds a tile's group by a
+// scan over the offsets, 32 groups at a time.
+//
+// With few tiles (a few tokens on one matrix) k is split over a cluster of
+// `split` CTAs: each leaves its integer partial sums in the shared memory of
+// the CTA that writes those tokens, which adds them up. Integer sums are exact
+// in any order, so the split does not change a bit.
+
+constexpr int kLanes = 128;           // channels of a CTA's tile
+constexpr int kBlockK = 128;          // bytes of k in a stage
+constexpr int kWTile = kLanes * kBlockK;
+constexpr int kTcThreads = 192;
+
+template <int NT, int STAGES>
+struct TcSmem {
+  static constexpr int kStage = kWTile + NT * kBlockK;
+  uint8_t stage[STAGES][kStage];  // weights, then tokens; 1024-byte aligned for the swizzle
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t parts, drained;
+  uint32_t tmem_base;
+  int abort;
+};
+
+// Shared-memory matrix descriptor, K-major, 128-byte swizzle: rows of 128
+// bytes, 8-row groups 1024 bytes apart, version 1 (sm_100), layout type 2.
+__device__ __forceinline__ uint64_t desc128(const void* p) {
+  return (uint64_t)((sa(p) & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// D 32-bit integers, A and B signed 8-bit, both K-major.
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+struct Tile {
+  uint32_t group, token0, tokens, channel0;
+};
+
+// A warp's walk over the tiles in ascending order; every lane gets the answer.
+struct TileWalk {
+  const int32_t* offsets;
+  uint32_t groups, m, nt, channels, channel_tiles;
+  unsigned* trap;
+  uint32_t base = 0, before = 0;       // the chunk's first group, token tiles before it
+  uint32_t lo = 0, hi = 0, incl = 0;   // this lane's group: rows, token tiles up to and with it
+  uint32_t chunk = 0;                  // token tiles of the chunk
+
+  __device__ void load() {
+    const uint32_t lane = threadIdx.x & 31, g = base + lane;
+    lo = hi = 0;
+    if (g < groups) {
+      if (offsets)
+        group_rows(offsets, g, m, trap, lo, hi);
+      else
+        hi = m;
+    }
+    incl = (hi - lo + nt - 1) / nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    chunk = __shfl_sync(0xffffffffu, incl, 31);
+  }
+
+  __device__ bool at(uint64_t tile, Tile& t) {
+    const uint64_t token_tile = tile / channel_tiles;
+    while (token_tile >= (uint64_t)before + chunk) {
+      base += 32;
+      if (base >= groups) return false;
+      before += chunk;
+      load();
+    }
+    const uint32_t want = (uint32_t)(token_tile - before);
+    const int src = __ffs(__ballot_sync(0xffffffffu, incl > want)) - 1;
+    const uint32_t glo = __shfl_sync(0xffffffffu, lo, src), ghi = __shfl_sync(0xffffffffu, hi, src);
+    const uint32_t first = __shfl_sync(0xffffffffu, incl, src) - (ghi - glo + nt - 1) / nt;
+    t.group = base + src;
+    t.token0 = glo + (want - first) * nt;
+    t.tokens = min(nt, ghi - t.token0);
+    t.channel0 = (uint32_t)(tile % channel_tiles) * channels;
+    return true;
+  }
+};
+
+struct TcArgs {
+  const int32_t* offsets;
+  const float* sa;
+  const float* sb;
+  void* C;
+  unsigned* trap;
+  uint64_t ldc;
+  uint32_t m, n, k_blocks, groups, split;
+};
+
+// Writes one column (token) of a warp's 32 channels.
+template <typename T>
+__device__ __forceinline__ void put(const TcArgs& P, T* c, uint32_t token, uint32_t channel, int acc, float sb) {
+  if (channel < P.n) c[(uint64_t)token * P.ldc + channel] = scaled<T>(acc, P.sa ? __ldg(P.sa + token) : 1.0f, sb);
+}
+
+template <typename T, int NT, int STAGES>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    mm_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                    const __grid_constant__ TcArgs P) {
+  using Smem = TcSmem<NT, STAGES>;
+  constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  int* partial = reinterpret_cast<int*>(&sm + 1);  // split > 1: NT x 128 partial sums
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t split = P.split, rank = split > 1 ? blockIdx.x % split : 0;
+  const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
+  const uint32_t kb_lo = (uint32_t)((uint64_t)P.k_blocks * rank / split);
+  const uint32_t kbs = (uint32_t)((uint64_t)P.k_blocks * (rank + 1) / split) - kb_lo;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 4);
+    }
+    mbar_init(&sm.parts, split * 128);
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
+                 "r"(kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if (split > 1)
+    cg::this_cluster().sync();  // the others' barriers are there before any arrival
+  else
+    __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* abort = &sm.abort;
+
+  TileWalk walk{P.offsets, P.groups, P.m, NT, kLanes, (P.n + kLanes - 1) / kLanes, P.trap};
+  walk.load();
+  Tile t;
+  uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
+  if (warp == 0) {
+    // ---- loads ----
+    for (uint64_t tile = first; walk.at(tile, t); tile += step) {
+      if (lane == 0)
+        for (uint32_t kb = 0; kb < kbs; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!mbar_wait(&sm.empty[s], ((it / STAGES) & 1) ^ 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          mbar_expect_tx(&sm.full[s], Smem::kStage);
+          const int k0 = (int)(kb_lo + kb) * kBlockK;
+          tma_load_3d(sm.stage[s], &map_w, k0, (int)t.channel0, (int)t.group, &sm.full[s]);
+          tma_load_2d(sm.stage[s] + kWTile, &map_x, k0, (int)t.token0, &sm.full[s]);
+        }
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else if (warp == 1) {
+    // ---- products ----
+    uint32_t n = 0;
+    for (uint64_t tile = first; walk.at(tile, t); tile += step, ++n) {
+      const uint32_t b = n & 1;
+      if (lane == 0) {
+        const uint32_t idesc = idesc_i8(kLanes, (int)((t.tokens + 15) / 16 * 16));
+        if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (uint32_t kb = 0; kb < kbs && !*abort; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + kWTile);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            mma_i8(tmem + b * NT, dw + kk * 2, dx + kk * 2, idesc, kb > 0 || kk > 0);
+          mma_commit(&sm.empty[s]);
+        }
+        mma_commit(&sm.acc_full[b]);
+      }
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else {
+    // ---- scales and output ----
+    T* C = static_cast<T*>(P.C);
+    const int quarter = warp & 3;  // TMEM lanes 32*quarter to +31
+    uint32_t n = 0;
+    for (uint64_t tile = first; walk.at(tile, t); tile += step, ++n) {
+      const uint32_t b = n & 1;
+      const uint32_t channel = t.channel0 + quarter * 32 + lane;
+      const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
+      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+        *abort = 1;
+        break;
+      }
+      if (*abort) break;  // the last commit of an aborted tile
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
+      constexpr int kTokens = NT < 16 ? NT : 16;
+      for (uint32_t j0 = 0; j0 < t.tokens; j0 += kTokens) {
+        int r[16];
+        tmem_ld16(col + j0, r);
+        if (split > 1) {
+          const uint32_t share = NT / split;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint32_t at = ((rank * share + (j0 + j) % share) * kLanes + quarter * 32 + lane) * 4;
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sa(partial) + at), "r"((j0 + j) / share));
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(r[j]) : "memory");
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j0 + j < t.tokens) put<T>(P, C, t.token0 + j0 + j, channel, r[j], sb);
+        }
+      }
+      if (split > 1) {
+        for (uint32_t q = 0; q < split; ++q) {
+          uint32_t to;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sa(&sm.parts)), "r"(q));
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(to) : "memory");
+        }
+        if (!mbar_wait_cluster(&sm.parts, 0, abort)) {
+          *abort = 1;
+          break;
+        }
+        const uint32_t share = NT / split;
+        for (uint32_t j = 0; j < share && rank * share + j < t.tokens; ++j) {
+          int acc = 0;
+          for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + j) * kLanes + quarter * 32 + lane];
+          put<T>(P, C, t.token0 + rank * share + j, channel, acc, sb);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if (split > 1)
+    cg::this_cluster().sync();  // nobody leaves while another may still write here
+  else
+    __syncthreads();
+  if (*abort) {
+    // a wait gave up: what is still in flight ends before shared memory and TMEM are given back
+    if (warp == 0 && lane == 0) {
+      atomicOr(P.trap, kDeviceTimeout);
+      for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+        mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1, nullptr);
+    }
+    if (warp == 1 && lane == 0) {
+      mma_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, nullptr);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+  }
+}
+
+// rows x k bytes (x matrices) in boxes of 128 bytes x box_rows.
+int make_map(CUtensorMap* map, const int8_t* base, uint64_t k, uint64_t rows, uint64_t ld, uint64_t mats, uint64_t ldm,
+             int dims, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const uint64_t k16 = (k + 15) & ~15ull;
+  // a stride that no access uses (one row, one matrix) may be anything: any valid one stands in
+  cuuint64_t dim[3] = {k, rows, mats};
+  cuuint64_t stride[2] = {rows > 1 ? ld : k16, mats > 1 ? ldm : (rows > 1 ? ld : k16) * rows};
+  if (mats <= 1) stride[1] = (stride[1] + 15) & ~15ull;
+  cuuint32_t box[3] = {kBlockK, box_rows, 1}, one[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, (void*)base, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return 0;
+}
+
+// Whether TMA can read both operands where they lie.
+bool tma_reads(const MapalI8Site& s, const int8_t* A, const int8_t* B) {
+  const uint64_t lim = 1ull << 39;
+  const bool a = aligned16(A) && (s.m == 1 || (s.lda % 16 == 0 && s.lda < lim));
+  const bool b = aligned16(B) && (s.n == 1 || (s.ldb % 16 == 0 && s.ldb < lim)) &&
+                 (s.groups == 1 || (s.ldg % 16 == 0 && s.ldg < lim));
+  return s.k > 0 && a && b && s.n * (s.n == 1 ? s.k : s.ldb) < lim;
+}
+
+template <typename T, int NT, int STAGES>
+int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, TcArgs P, uint64_t tiles) {
+  CUtensorMap mw, mx;
+  MAPAL_TRY(make_map(&mw, B, s.k, s.n, s.ldb, s.groups, s.ldg, 3, kLanes));
+  MAPAL_TRY(make_map(&mx, A, s.k, s.m, s.lda, 1, 0, 2, NT));
+  const size_t most = sizeof(TcSmem<NT, STAGES>) + 1024 + (NT <= 64 ? NT * kLanes * 4 : 0);
+  const size_t smem = sizeof(TcSmem<NT, STAGES>) + 1024 + (P.split > 1 ? NT * kLanes * 4 : 0);
+  static std::atomic<uint64_t> done{0};
+  auto kernel = mm_i8_tc_kernel<T, NT, STAGES>;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "matmul_i8 shared memory"));
+  const uint64_t cap = P.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * P.split));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = D.stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = P.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = P.split > 1 ? 1 : 0;
+  MAPAL_CUDA(cudaLaunchKernelEx(&cfg, kernel, mw, mx, P));
+  count_launch();
+  return 0;
+}
+
+template <typename T>
+int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float* sa, const int8_t* B, const float* sb,
+           const int32_t* offsets, void* C) {
+  TcArgs P{};
+  P.offsets = offsets;
+  P.sa = sa;
+  P.sb = sb;
+  P.C = C;
+  P.trap = D.trap;
+  P.ldc = s.ldc;
+  P.m = (uint32_t)s.m;
+  P.n = (uint32_t)s.n;
+  P.groups = s.groups;
+  P.k_blocks = (uint32_t)((s.k + kBlockK - 1) / kBlockK);
+  P.split = 1;
+  const uint64_t nt = s.m <= 16ull * s.groups ? 16 : s.m <= 32ull * s.groups ? 32 : s.m <= 64ull * s.groups ? 64 : s.m <= 128ull * s.groups ? 128 : 256;
+  // an upper bound of the tiles: every group with rows has at most one part-filled token tile
+  const uint64_t token_tiles = s.m / nt + (s.groups < s.m ? s.groups : s.m);
+  const uint64_t tiles = (offsets ? token_tiles : (s.m + nt - 1) / nt) * ((s.n + kLanes - 1) / kLanes);
+  if (nt <= 64)
+    while (P.split < 8 && tiles * P.split * 2 <= (uint64_t)D.prof.sm_count && P.split * 4 <= P.k_blocks) P.split *= 2;
+  switch (nt) {
+    case 16: return launch_tc<T, 16, 8>(D, s, A, B, P, tiles);
+    case 32: return launch_tc<T, 32, 8>(D, s, A, B, P, tiles);
+    case 64: return launch_tc<T, 64, 7>(D, s, A, B, P, tiles);
+    case 128: return launch_tc<T, 128, 6>(D, s, A, B, P, tiles);
+    default: return launch_tc<T, 256, 4>(D, s, A, B, P, tiles);
+  }
+}
+
 int check_site(const MapalI8Site* s) {
   if (!s) return set_error(MAPAL_ERR_INVALID, "site is null");
   const int es = dtype_bytes(s->dtype);
@@ -122,14 +523,14 @@ extern "C" int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, co
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
     MAPAL_TRY(enter(ctx));
     DeviceSlot& D = ctx->dev[0];
-    int rc;
-    if (s.dtype == MAPAL_DTYPE_F32)
-      rc = launch_tiles<float>(D, s, A, scale_a, B, scale_b, offsets, C);
-    else if (s.dtype == MAPAL_DTYPE_F16)
-      rc = launch_tiles<__half>(D, s, A, scale_a, B, scale_b, offsets, C);
-    else
-      rc = launch_tiles<__nv_bfloat16>(D, s, A, scale_a, B, scale_b, offsets, C);
-    MAPAL_TRY(rc);
-    return finish(ctx, 0, offsets != nullptr);
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      return tma_reads(s, A, B) ? run_tc<T>(D, s, A, scale_a, B, scale_b, offsets, C)
+                                : launch_tiles<T>(D, s, A, scale_a, B, scale_b, offsets, C);
+    };
+    MAPAL_TRY(s.dtype == MAPAL_DTYPE_F32   ? go(float{})
+              : s.dtype == MAPAL_DTYPE_F16 ? go(__half{})
+                                           : go(__nv_bfloat16{}));
+    return finish(ctx, 0, true);
   });
 }

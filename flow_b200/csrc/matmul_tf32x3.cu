@@ -35,9 +35,8 @@
 // kDeviceTimeout (reported as MAPAL_ERR_TIMEOUT), all roles leave their
 // loops, in-flight copies and MMAs are waited for (bounded again) and TMEM
 // is freed before the CTA exits.
-#include <cuda.h>
-
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -52,8 +51,6 @@ constexpr uint32_t kTmemCols = 2 * kAccCols;
 constexpr int kATile = BM * BK * 4;  // bytes of one A tile (hi or lo)
 constexpr int kBTile = BN * BK * 4;  // bytes of one B tile (hi or lo)
 constexpr int kStageBytes = 2 * kATile + 2 * kBTile;
-constexpr uint32_t kDeviceTimeout = 0x100u;
-constexpr uint64_t kWaitLimitNs = 2000000000ull;  // a wait gives up after 2 s
 
 struct Smem {
   // stage buffers first, each 1024-byte aligned (the swizzle pattern repeats
@@ -65,55 +62,6 @@ struct Smem {
   uint32_t tmem_base;
   int abort;
 };
-
-__device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(b)), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sa(b)), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(sa(b)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait on a phase: false when kWaitLimitNs ran out, or (abort given)
-// when another role has aborted.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
-  const uint64_t t0 = now_ns();
-  for (uint32_t i = 0;; ++i) {
-    if (mbar_try(b, parity)) return true;
-    if ((i & 255) == 255) {
-      if (abort && *abort) return false;
-      if (now_ns() - t0 > kWaitLimitNs) return false;
-    }
-  }
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          sa(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(sa(bar))
-      : "memory");
-}
 
 // Shared-memory matrix descriptor, K-major, 64-byte swizzle: rows of 64 bytes
 // (16 tf32), 8-row groups 512 bytes apart (SBO), LBO 16 bytes (unused for
@@ -139,11 +87,6 @@ __device__ __forceinline__ void mma_tf32(uint32_t tmem, uint64_t a, uint64_t b, 
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
       "l"(a), "l"(b), "r"(kIdesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sa(bar))
-               : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
@@ -368,10 +311,6 @@ struct SmemF {
 constexpr int kConvThreads = 128;
 static_assert(kATile / 16 % kConvThreads == 0, "the converter's float4 share must be whole");
 constexpr uint32_t kLoadStageBytes = kATile + 2 * kBTile;  // TMA bytes per stage
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sa(b)) : "memory");
-}
 
 // lo part of x for the truncated hi: x - trunc(x) is exact in f32 and is
 // rounded to TF32 (nearest, ties away) with integer operations. A NaN or
@@ -754,24 +693,6 @@ __global__ void __launch_bounds__(kTT* kTRows) split_transpose_kernel(const floa
 }
 
 // ---- host: tensor maps ----------------------------------------------------------------------
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's cuTensorMapEncodeTiled, looked up once (a function-local
-// static is initialised exactly once, also when threads race to it).
-EncodeTiledFn encode_fn() {
-  static const EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      return (EncodeTiledFn)p;
-    return (EncodeTiledFn) nullptr;
-  }();
-  return fn;
-}
 
 // rows x K f32 matrix with row stride kp (elements), box = box_rows x BK.
 int make_map(CUtensorMap* map, const float* base, uint64_t rows, uint64_t K, uint64_t kp, uint32_t box_rows) {
