@@ -183,13 +183,13 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__
         const int32_t p = place_of(pos, t * k + j, rows, trap);
         if (p < 0) continue;
         const float g = w ? __ldg(w + t * k + j) : 1.0f;
-        const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i);
+        float f[V];
+        reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i)->get(f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = __fmaf_rn(g, to_f32(v.v[e]), acc[e]);
+        for (int e = 0; e < V; ++e) acc[e] = __fmaf_rn(g, f[e], acc[e]);
       }
       Pack<T, V> o;
-#pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = from_f32<T>(acc[e]);
+      o.set(acc);
       *reinterpret_cast<Pack<T, V>*>(y + t * ldt + i) = o;
     }
   }
@@ -212,15 +212,16 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* h, cons
       const float g = w ? __ldg(w + s) : 1.0f;
       const T* dyr = dy + s / k * ldt;
       for (uint64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
-        const Pack<T, V> a = *reinterpret_cast<const Pack<T, V>*>(dyr + i);
-        const Pack<T, V> b = *reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i);
+        float a[V], b[V];
+        reinterpret_cast<const Pack<T, V>*>(dyr + i)->get(a);
+        reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i)->get(b);
         Pack<T, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = to_f32(a.v[e]);
-          dot = __fmaf_rn(v, to_f32(b.v[e]), dot);
-          o.v[e] = from_f32<T>(g * v);
+          dot = __fmaf_rn(a[e], b[e], dot);
+          a[e] *= g;
         }
+        o.set(a);
         *reinterpret_cast<Pack<T, V>*>(dh + (uint64_t)p * ldr + i) = o;
       }
     }

@@ -4,40 +4,547 @@
 // Forward: mu = mean(x), r = 1/sqrt(mean((x - mu)^2) + eps), y = (x - mu)*r*w + b.
 // Backward, with h = (x - mu)*r and g = dy*w:
 //   dx = r*(g - mean(g) - h*mean(g*h)), dw = sum_rows dy*h, db = sum_rows dy.
+#include "f32x2.cuh"
 #include "rows.cuh"
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of the kernels for long rows
+constexpr int kMostFlow = 8192;  // elements of the longest row of the kernels for many rows
 
-template <typename TW>
-__device__ __forceinline__ float weight_at(const void* w, uint64_t i, float none) {
-  return w ? to_f32(static_cast<const TW*>(w)[i]) : none;
+// V weights of type TW as floats; `none` where there are no weights.
+template <typename TW, int V>
+__device__ __forceinline__ void weights(const void* w, int64_t i, float none, float (&out)[V]) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = none;
+  } else {
+    constexpr int U = V * sizeof(TW) > 16 ? 16 / sizeof(TW) : V;  // elements of an access
+#pragma unroll
+    for (int u = 0; u < V; u += U) {
+      float f[U];
+      reinterpret_cast<const Pack<TW, U>*>(static_cast<const TW*>(w) + i + u)->get(f);
+#pragma unroll
+      for (int e = 0; e < U; ++e) out[u + e] = f[e];
+    }
+  }
 }
 
 __device__ __forceinline__ float inv_std(float var, float eps) { return __fdiv_rn(1.0f, __fsqrt_rn(var + eps)); }
 
-// One block a row, three passes over it.
-template <typename T, typename TW>
+// G threads (whole warps) of a block that share a row. A group of one warp
+// needs no barrier; others meet at a named barrier of their own.
+struct Group {
+  int size, tid, id;
+  __device__ explicit Group(int g) : size(g), tid(threadIdx.x % g), id(threadIdx.x / g) {}
+  __device__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(size) : "memory"); }
+  // N sums over the group at once, in every thread. Lanes halve the values
+  // they carry while they add, so 4 sums take 6 shuffles instead of 20. `red`
+  // is the group's own, and not that of the sums before (two sets taken in
+  // turn are enough).
+  template <int N>
+  __device__ void sums(float (&a)[N], float (*red)[16]) const {
+    static_assert(N == 1 || N == 2 || N == 4, "");
+    constexpr unsigned kAll = 0xffffffffu;
+    constexpr int L = 32 / N;  // lanes that end with the same value
+    const int lane = tid & 31;
+    float v;
+    if constexpr (N == 1) {
+      v = a[0];
+    } else if constexpr (N == 2) {
+      const bool up = lane & 16;
+      v = (up ? a[1] : a[0]) + __shfl_xor_sync(kAll, up ? a[0] : a[1], 16);
+    } else {
+      const bool up = lane & 16, up2 = lane & 8;
+      const float p = (up ? a[2] : a[0]) + __shfl_xor_sync(kAll, up ? a[0] : a[2], 16);
+      const float q = (up ? a[3] : a[1]) + __shfl_xor_sync(kAll, up ? a[1] : a[3], 16);
+      v = (up2 ? q : p) + __shfl_xor_sync(kAll, up2 ? p : q, 8);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if (size > 32) {
+      const int at = lane % L, warps = size / 32;
+      if (at == 0) red[lane / L][tid >> 5] = v;
+      sync();
+      v = at < warps ? red[lane / L][at] : 0.0f;
+      if (L < 16 && at + L < warps) v += red[lane / L][at + L];
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) a[k] = __shfl_sync(kAll, v, k * L);
+  }
+  __device__ float sum(float a, float* red) const {
+    a = warp_sum(a);
+    if (size == 32) return a;
+    const int lane = tid & 31, warp = tid >> 5;
+    if (lane == 0) red[warp] = a;
+    sync();
+    return warp_sum(lane < size / 32 ? red[lane] : 0.0f);
+  }
+};
+constexpr int kMostGroups = 16;
+
+// ---- few rows ------------------------------------------------------------------------
+//
+// Forward: a row lives, packed as it was read, in the registers of a group of
+// warps, EACH elements a thread, so it is read once and both sums run over
+// registers. 8 elements a thread spread a row's loads and sums as wide as they
+// go; rows of more than 8192 elements take 16 or 32 a thread.
+
+template <typename T, typename TW, int V, int EACH>
+__global__ void __launch_bounds__(1024)
+    norm_held_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const void* __restrict__ b, T* y,
+                     float* __restrict__ mean, float* __restrict__ rstd, int group) {
+  using P = Pack<T, V>;
+  constexpr int NV = EACH / V;
+  __shared__ float red[32][2][32];  // at most 32 groups
+  const Group G(group);
+  const uint64_t stride = (uint64_t)gridDim.x * (blockDim.x / group);
+  const int d = (int)S.d;
+  const float n = (float)d;
+  for (uint64_t r = (uint64_t)blockIdx.x * (blockDim.x / group) + G.id; r < S.rows; r += stride) {
+    const T* xr = x + r * S.ldx;
+    P v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * group + G.tid) * V;
+      if (i < d)
+        v[j] = ld_once(reinterpret_cast<const P*>(xr + i));
+      else
+        v[j].clear();
+    }
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[V];
+      v[j].get(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[e];
+    }
+    const float mu = __fdiv_rn(G.sum(s, red[G.id][0]), n);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if ((j * group + G.tid) * V < d) {
+        if constexpr (EACH > 8) v[j].forget();
+        float f[V];
+        v[j].get(f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float c = f[e] - mu;
+          q = __fmaf_rn(c, c, q);
+        }
+      }
+    const float rs = inv_std(__fdiv_rn(G.sum(q, red[G.id][1]), n), S.eps);
+    T* yr = y + r * S.ldy;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * group + G.tid) * V;
+      if (i < d) {
+        if constexpr (EACH > 8) v[j].forget();
+        float f[V], fw[V], fb[V];
+        v[j].get(f);
+        weights<TW, V>(w, i, 1.0f, fw);
+        weights<TW, V>(b, i, 0.0f, fb);
+        P o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = __fmaf_rn((f[e] - mu) * rs, fw[e], fb[e]);
+        o.set(f);
+        st_once(reinterpret_cast<P*>(yr + i), o);
+      }
+      if constexpr (EACH > 8) asm volatile("" ::: "memory");  // keeps the weights' loads from piling up in registers
+    }
+    if (G.tid == 0) {
+      if (mean) mean[r] = mu;
+      if (rstd) rstd[r] = rs;
+    }
+  }
+}
+
+// ---- many rows of up to 8192 elements ------------------------------------------------
+//
+// A group of threads takes ROWS rows at a time, EACH columns a thread, and
+// keeps its columns' weights (and, in the gradient, their sums over rows) in
+// registers from row to row. Rows arrive through a ring in shared memory: every
+// thread copies its own elements with cp.async and reads them back itself, so
+// there is nothing to wait for but its own copies, and rows stay in flight
+// without holding registers. What is left is instructions, so the arithmetic is
+// on packed pairs and the sums of ROWS rows share their shuffles and barrier.
+// 16-bit rows at odd addresses, which cp.async cannot copy, are loaded into
+// registers one turn ahead.
+
+constexpr int kFlow = 512;  // threads of a block; one block an SM
+
+// V: elements of an access; ARRAYS: 1 (x) or 2 (x and dy).
+template <typename T, int V, int EACH, int ROWS, int ARRAYS>
+struct Ring {
+  using P = Pack<T, V>;
+  static constexpr int NV = EACH / V;
+  static constexpr bool kAsync = sizeof(P) >= 4;
+  static constexpr int kSlots = ARRAYS * ROWS * NV;  // of a thread in a stage
+  static constexpr int kStages = !kAsync ? 1 : sizeof(T) == 4 ? 3 : 4;
+  static constexpr size_t kBytes = kAsync ? (size_t)kStages * kSlots * sizeof(P) * kFlow : 0;
+  P* base;
+  P ahead[kAsync ? 1 : kSlots];
+  int stage = 0;
+  __device__ explicit Ring(void* p) : base(static_cast<P*>(p)) {}
+
+  __device__ __forceinline__ P* slot(int st, int s) { return base + (size_t)(st * kSlots + s) * kFlow + threadIdx.x; }
+  __device__ __forceinline__ void copy(int st, int s, const T* from) {
+    if constexpr (kAsync) {
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot(st, s));
+      if constexpr (sizeof(P) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+    } else {
+      ahead[s] = ld_once(reinterpret_cast<const P*>(from));
+    }
+  }
+  __device__ __forceinline__ void commit() {
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // This turn's rows are there.
+  __device__ __forceinline__ void wait() {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+  }
+  __device__ __forceinline__ P take(int s) { return kAsync ? *slot(stage, s) : ahead[kAsync ? 0 : s]; }
+  __device__ __forceinline__ void next() { stage = stage + 1 == kStages ? 0 : stage + 1; }
+};
+
+__device__ __forceinline__ float f2_sum(f2 v) { return f2_lo(v) + f2_hi(v); }
+
+template <typename T, typename TW, int V, int EACH, int ROWS>
+__global__ void __launch_bounds__(kFlow, 1)
+    norm_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const void* __restrict__ b, T* y,
+                     float* __restrict__ mean, float* __restrict__ rstd, int group) {
+  using R = Ring<T, V, EACH, ROWS, 1>;
+  using P = Pack<T, V>;
+  constexpr int NV = EACH / V;
+  __shared__ float red[kMostGroups][2][4][16];
+  extern __shared__ __align__(16) uint8_t dyn[];
+  R ring(dyn);
+  const Group G(group);
+  const int groups = blockDim.x / group, d = (int)S.d;
+  const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
+  uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
+  const float n = (float)d;
+  auto start = [&](int st, uint64_t row) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (row + k < S.rows) {
+        const T* from = x + (row + k) * S.ldx + G.tid * V;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if ((j * group + G.tid) * V < d) ring.copy(st, k * NV + j, from + j * group * V);
+      }
+    ring.commit();
+  };
+#pragma unroll
+  for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
+  f2 fw[EACH / 2], fb[EACH / 2];
+  {
+    float a[EACH], c[EACH];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * group + G.tid) * V;
+      float pa[V] = {}, pc[V] = {};
+      if (i < d) {
+        weights<TW, V>(w, i, 1.0f, pa);
+        weights<TW, V>(b, i, 0.0f, pc);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        a[j * V + e] = pa[e];
+        c[j * V + e] = pc[e];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < EACH / 2; ++u) {
+      fw[u] = f2_pack(a[2 * u], a[2 * u + 1]);
+      fb[u] = f2_pack(c[2 * u], c[2 * u + 1]);
+    }
+  }
+  for (; r < S.rows; r += step) {
+    ring.wait();
+    f2 v[ROWS][EACH / 2];
+    float s[ROWS], q[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      float f[EACH];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        P p;
+        if ((j * group + G.tid) * V < d && r + k < S.rows)
+          p = ring.take(k * NV + j);
+        else
+          p.clear();
+        float g[V];
+        p.get(g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[j * V + e] = g[e];
+      }
+      f2 t = f2_splat(0.0f);
+#pragma unroll
+      for (int u = 0; u < EACH / 2; ++u) {
+        v[k][u] = f2_pack(f[2 * u], f[2 * u + 1]);
+        t = f2_add(t, v[k][u]);
+      }
+      s[k] = f2_sum(t);
+    }
+    G.sums(s, red[G.id][0]);
+    start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
+    ring.next();
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      s[k] = __fdiv_rn(s[k], n);
+      const f2 m = f2_splat(-s[k]);
+#pragma unroll
+      for (int u = 0; u < EACH / 2; ++u) v[k][u] = f2_add(v[k][u], m);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if ((j * group + G.tid) * V >= d) {  // no elements here
+          if constexpr (V > 1) {
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) v[k][j * (V / 2) + e] = f2_splat(0.0f);
+          } else {
+            v[k][j / 2] = j % 2 ? f2_pack(f2_lo(v[k][j / 2]), 0.0f) : f2_pack(0.0f, f2_hi(v[k][j / 2]));
+          }
+        }
+      f2 t = f2_splat(0.0f);
+#pragma unroll
+      for (int u = 0; u < EACH / 2; ++u) t = f2_fma(v[k][u], v[k][u], t);
+      q[k] = f2_sum(t);
+    }
+    G.sums(q, red[G.id][1]);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const float rs = inv_std(__fdiv_rn(q[k], n), S.eps);
+      if (r + k >= S.rows) break;
+      const f2 m = f2_splat(rs);
+      float f[EACH];
+#pragma unroll
+      for (int u = 0; u < EACH / 2; ++u) {
+        const f2 o = f2_fma(f2_mul(v[k][u], m), fw[u], fb[u]);
+        f[2 * u] = f2_lo(o);
+        f[2 * u + 1] = f2_hi(o);
+      }
+      T* to = y + (r + k) * S.ldy + G.tid * V;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float g[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[e] = f[j * V + e];
+        P p;
+        p.set(g);
+        if ((j * group + G.tid) * V < d) st_once(reinterpret_cast<P*>(to + j * group * V), p);
+      }
+      if (G.tid == 0) {
+        if (mean) mean[r + k] = s[k];
+        if (rstd) rstd[r + k] = rs;
+      }
+    }
+  }
+}
+
+// The gradient: dx, and where work is given this block's sums of dy*h and dy
+// as rows 2*block and 2*block + 1 of it (the groups add theirs in order).
+template <typename T, typename TW, int V, int EACH, int ROWS>
+__global__ void __launch_bounds__(kFlow, 1)
+    norm_grad_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const float* __restrict__ mean,
+                          const float* __restrict__ rstd, const T* dy, T* dx, float* __restrict__ work, int group) {
+  using R = Ring<T, V, EACH, ROWS, 2>;
+  using P = Pack<T, V>;
+  constexpr int NV = EACH / V, H = EACH / 2;
+  __shared__ float red[kMostGroups][2][2 * ROWS][16];
+  extern __shared__ __align__(16) uint8_t dyn[];
+  R ring(dyn);
+  float* sums = reinterpret_cast<float*>(dyn + R::kBytes);  // several groups: 2*d floats
+  const Group G(group);
+  const int groups = blockDim.x / group, d = (int)S.d;
+  const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
+  uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
+  const float inv_n = __fdiv_rn(1.0f, (float)d);
+  auto start = [&](int st, uint64_t row) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (row + k < S.rows) {
+        const T* from = x + (row + k) * S.ldx + G.tid * V;
+        const T* from2 = dy + (row + k) * S.lddy + G.tid * V;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if ((j * group + G.tid) * V < d) {
+            ring.copy(st, k * NV + j, from + j * group * V);
+            ring.copy(st, (ROWS + k) * NV + j, from2 + j * group * V);
+          }
+      }
+    ring.commit();
+  };
+#pragma unroll
+  for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
+  float nmu[ROWS], nrs[ROWS];
+  auto stats = [&](uint64_t row) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const bool in = row + k < S.rows;
+      nmu[k] = in ? __ldg(mean + row + k) : 0.0f;
+      nrs[k] = in ? __ldg(rstd + row + k) : 0.0f;
+    }
+  };
+  stats(r);
+  f2 fw[H], aw[H], ab[H];
+  {
+    float a[EACH];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * group + G.tid) * V;
+      float pa[V] = {};
+      if (i < d) weights<TW, V>(w, i, 1.0f, pa);
+#pragma unroll
+      for (int e = 0; e < V; ++e) a[j * V + e] = pa[e];
+    }
+#pragma unroll
+    for (int u = 0; u < H; ++u) {
+      fw[u] = f2_pack(a[2 * u], a[2 * u + 1]);
+      aw[u] = ab[u] = f2_splat(0.0f);
+    }
+  }
+  int par = 0;
+  for (; r < S.rows; r += step, par ^= 1) {
+    ring.wait();
+    f2 h[ROWS][H], g[ROWS][H];
+    float c[2 * ROWS], rs[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      float fx[EACH], fy[EACH];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        P px, py;
+        if ((j * group + G.tid) * V < d && r + k < S.rows) {
+          px = ring.take(k * NV + j);
+          py = ring.take((ROWS + k) * NV + j);
+        } else {
+          px.clear();
+          py.clear();
+        }
+        float a[V], e2[V];
+        px.get(a);
+        py.get(e2);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          fx[j * V + e] = a[e];
+          fy[j * V + e] = e2[e];
+        }
+      }
+      rs[k] = nrs[k];
+      const f2 m = f2_splat(-nmu[k]), sc = f2_splat(nrs[k]);
+      f2 c1 = f2_splat(0.0f), c2 = c1;
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        const f2 t = f2_pack(fy[2 * u], fy[2 * u + 1]);
+        h[k][u] = f2_mul(f2_add(f2_pack(fx[2 * u], fx[2 * u + 1]), m), sc);
+        g[k][u] = f2_mul(t, fw[u]);
+        aw[u] = f2_fma(t, h[k][u], aw[u]);
+        ab[u] = f2_add(ab[u], t);
+        c1 = f2_add(c1, g[k][u]);
+        c2 = f2_fma(g[k][u], h[k][u], c2);
+      }
+      c[2 * k] = f2_sum(c1);
+      c[2 * k + 1] = f2_sum(c2);
+    }
+    stats(r + step);
+    G.sums(c, red[G.id][par]);
+    start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
+    ring.next();
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      if (r + k >= S.rows) break;
+      const f2 c1 = f2_splat(-c[2 * k] * inv_n), c2 = f2_splat(-c[2 * k + 1] * inv_n), sc = f2_splat(rs[k]);
+      float f[EACH];
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        const f2 o = f2_mul(f2_fma(h[k][u], c2, f2_add(g[k][u], c1)), sc);
+        f[2 * u] = f2_lo(o);
+        f[2 * u + 1] = f2_hi(o);
+      }
+      T* to = dx + (r + k) * S.lddx + G.tid * V;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = f[j * V + e];
+        P p;
+        p.set(o);
+        if ((j * group + G.tid) * V < d) st_once(reinterpret_cast<P*>(to + j * group * V), p);
+      }
+    }
+  }
+  if (!work) return;
+  float* out = work + 2ull * blockIdx.x * S.d;
+  for (int k = 0; k < groups; ++k) {
+    if (G.id == k) {
+      const bool first = k == 0, last = k == groups - 1;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * group + G.tid) * V;
+        if (i >= d) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int u = j * V + e;
+          const float a = u % 2 ? f2_hi(aw[u / 2]) : f2_lo(aw[u / 2]), c = u % 2 ? f2_hi(ab[u / 2]) : f2_lo(ab[u / 2]);
+          (last ? out : sums)[i + e] = first ? a : sums[i + e] + a;
+          (last ? out : sums)[d + i + e] = first ? c : sums[d + i + e] + c;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- longer rows -------------------------------------------------------------------
+//
+// One block a row, which is read again for each pass (from L1 or L2: rows of a
+// few hundred KB); sums over rows by column, with partial sums in `work`.
+
+template <typename T, typename TW, int V>
 __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const MapalNormSite S, const T* x, const void* w,
                                                              const void* b, T* y, float* mean, float* rstd) {
   __shared__ float red[2][32];
+  const int64_t d = (int64_t)S.d;
   const float n = (float)S.d;
   for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x) {
     const T* xr = x + r * S.ldx;
     T* yr = y + r * S.ldy;
     float s = 0.0f;
-    for (uint64_t i = threadIdx.x; i < S.d; i += kThreads) s += to_f32(xr[i]);
+    for (int64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
+      float f[V];
+      reinterpret_cast<const Pack<T, V>*>(xr + i)->get(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[e];
+    }
     const float mu = __fdiv_rn(block_sum(s, red[0]), n);
     float q = 0.0f;
-    for (uint64_t i = threadIdx.x; i < S.d; i += kThreads) {
-      const float c = to_f32(xr[i]) - mu;
-      q = __fmaf_rn(c, c, q);
+    for (int64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
+      float f[V];
+      reinterpret_cast<const Pack<T, V>*>(xr + i)->get(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float c = f[e] - mu;
+        q = __fmaf_rn(c, c, q);
+      }
     }
     const float rs = inv_std(__fdiv_rn(block_sum(q, red[1]), n), S.eps);
-    for (uint64_t i = threadIdx.x; i < S.d; i += kThreads)
-      yr[i] = from_f32<T>(
-          __fmaf_rn((to_f32(xr[i]) - mu) * rs, weight_at<TW>(w, i, 1.0f), weight_at<TW>(b, i, 0.0f)));
+    for (int64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
+      float f[V], fw[V], fb[V];
+      reinterpret_cast<const Pack<T, V>*>(xr + i)->get(f);
+      weights<TW, V>(w, i, 1.0f, fw);
+      weights<TW, V>(b, i, 0.0f, fb);
+      Pack<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = __fmaf_rn((f[e] - mu) * rs, fw[e], fb[e]);
+      o.set(f);
+      st_once(reinterpret_cast<Pack<T, V>*>(yr + i), o);
+    }
     if (threadIdx.x == 0) {
       if (mean) mean[r] = mu;
       if (rstd) rstd[r] = rs;
@@ -45,80 +552,112 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const MapalNormSite
   }
 }
 
-// One block a row: the row's two means, then dx.
-template <typename T, typename TW>
+template <typename T, typename TW, int V>
 __global__ void __launch_bounds__(kThreads) norm_grad_rows_kernel(const MapalNormSite S, const T* x, const void* w,
                                                                   const float* mean, const float* rstd, const T* dy,
                                                                   T* dx) {
   __shared__ float red[2][2][32];
+  const int64_t d = (int64_t)S.d;
   const float n = (float)S.d;
   int par = 0;
   for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x, par ^= 1) {
     const T* xr = x + r * S.ldx;
     const T* dyr = dy + r * S.lddy;
-    T* dxr = dx + r * S.lddx;
     const float mu = mean[r], rs = rstd[r];
     float c1 = 0.0f, c2 = 0.0f;
-    for (uint64_t i = threadIdx.x; i < S.d; i += kThreads) {
-      const float g = to_f32(dyr[i]) * weight_at<TW>(w, i, 1.0f);
-      c1 += g;
-      c2 = __fmaf_rn(g, (to_f32(xr[i]) - mu) * rs, c2);
+    for (int64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
+      float fx[V], fy[V], fw[V];
+      reinterpret_cast<const Pack<T, V>*>(xr + i)->get(fx);
+      reinterpret_cast<const Pack<T, V>*>(dyr + i)->get(fy);
+      weights<TW, V>(w, i, 1.0f, fw);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float g = fy[e] * fw[e];
+        c1 += g;
+        c2 = __fmaf_rn(g, (fx[e] - mu) * rs, c2);
+      }
     }
     c1 = __fdiv_rn(block_sum(c1, red[par][0]), n);
     c2 = __fdiv_rn(block_sum(c2, red[par][1]), n);
-    for (uint64_t i = threadIdx.x; i < S.d; i += kThreads) {
-      const float g = to_f32(dyr[i]) * weight_at<TW>(w, i, 1.0f);
-      const float h = (to_f32(xr[i]) - mu) * rs;
-      dxr[i] = from_f32<T>((g - c1 - h * c2) * rs);
+    for (int64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
+      float fx[V], fy[V], fw[V];
+      reinterpret_cast<const Pack<T, V>*>(xr + i)->get(fx);
+      reinterpret_cast<const Pack<T, V>*>(dyr + i)->get(fy);
+      weights<TW, V>(w, i, 1.0f, fw);
+      Pack<T, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) fx[e] = __fmaf_rn(-((fx[e] - mu) * rs), c2, fy[e] * fw[e] - c1) * rs;
+      o.set(fx);
+      st_once(reinterpret_cast<Pack<T, V>*>(dx + r * S.lddx + i), o);
     }
   }
 }
 
-// dw and db over rows p, p + parts, ...: part p writes its sums of 32 columns.
-template <typename T>
+// dw and db over rows p*8 + sub, then every parts*8-th: part p's sums of 32*V columns.
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const MapalNormSite S, const T* x, const float* mean,
                                                                   const float* rstd, const T* dy, float* work,
                                                                   uint32_t parts) {
-  __shared__ float sw[8][32], sb[8][32];
+  __shared__ float sw[8][32 * V], sb[8][32 * V];
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
-  float aw = 0.0f, ab = 0.0f;
+  const uint64_t c = ((uint64_t)blockIdx.x * 32 + lane) * V;
+  float aw[V] = {}, ab[V] = {};
   if (c < S.d)
     for (uint64_t r = blockIdx.y * 8ull + sub; r < S.rows; r += parts * 8ull) {
-      const float g = to_f32(dy[r * S.lddy + c]);
-      aw = __fmaf_rn(g, (to_f32(x[r * S.ldx + c]) - mean[r]) * rstd[r], aw);
-      ab += g;
+      const Pack<T, V> p = ld_once(reinterpret_cast<const Pack<T, V>*>(x + r * S.ldx + c));
+      const Pack<T, V> t = ld_once(reinterpret_cast<const Pack<T, V>*>(dy + r * S.lddy + c));
+      const float mu = __ldg(mean + r), rs = __ldg(rstd + r);
+      float fx[V], fy[V];
+      p.get(fx);
+      t.get(fy);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float g = fy[e];
+        aw[e] = __fmaf_rn(g, (fx[e] - mu) * rs, aw[e]);
+        ab[e] += g;
+      }
     }
-  sw[sub][lane] = aw;
-  sb[sub][lane] = ab;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    sw[sub][e * 32 + lane] = aw[e];
+    sb[sub][e * 32 + lane] = ab[e];
+  }
   __syncthreads();
   if (sub == 0 && c < S.d) {
-    for (int k = 1; k < 8; ++k) {
-      aw += sw[k][lane];
-      ab += sb[k][lane];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      for (int k = 1; k < 8; ++k) {
+        aw[e] += sw[k][e * 32 + lane];
+        ab[e] += sb[k][e * 32 + lane];
+      }
+      work[(2ull * blockIdx.y) * S.d + c + e] = aw[e];
+      work[(2ull * blockIdx.y + 1) * S.d + c + e] = ab[e];
     }
-    work[(2ull * blockIdx.y) * S.d + c] = aw;
-    work[(2ull * blockIdx.y + 1) * S.d + c] = ab;
   }
 }
 
-// dw and db from the parts' sums, in part order.
-__global__ void __launch_bounds__(kThreads) norm_grad_join_kernel(const float* work, uint64_t d, uint32_t parts,
-                                                                  float* dw, float* db) {
-  __shared__ float red[8][32];
+// dw and db from the parts' sums: 32 runs of parts in order, then the runs.
+__global__ void __launch_bounds__(1024) norm_grad_join_kernel(const float* __restrict__ work, uint64_t d,
+                                                                  uint32_t parts, float* dw, float* db) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;  // 0..d: dw, d..2d: db
   float a = 0.0f;
-  if (c < 2 * d)
-    for (uint32_t p = sub; p < parts; p += 8) a += work[2ull * p * d + c];
-  red[sub][lane] = a;
+  if (c < 2 * d) {
+#pragma unroll 10
+    for (uint32_t p = sub; p < parts; p += 32) a += __ldcs(work + 2ull * p * d + c);
+  }
+  red[lane][sub] = a;
   __syncthreads();
-  if (sub == 0 && c < 2 * d) {
-    for (int k = 1; k < 8; ++k) a += red[k][lane];
-    float* out = c < d ? dw : db;
-    if (out) out[c < d ? c : c - d] = a;
+  a = warp_sum(red[sub][lane]);  // warp `sub` joins column `sub`
+  const uint64_t o = (uint64_t)blockIdx.x * 32 + sub;
+  if (lane == 0 && o < 2 * d) {
+    float* out = o < d ? dw : db;
+    if (out) out[o < d ? o : o - d] = a;
   }
 }
+
+// ---- host --------------------------------------------------------------------------
 
 int check_norm(const MapalNormSite* s) {
   if (!s) return set_error(MAPAL_ERR_INVALID, "site is null");
@@ -131,48 +670,148 @@ int check_norm(const MapalNormSite* s) {
   return 0;
 }
 
+// How the kernels for many rows are launched: threads of a group, of a block,
+// blocks. `rows` at a time; rows of more than 4096 elements twice the columns
+// a thread.
+struct Plan {
+  int group, threads;
+  unsigned blocks;
+};
+
+Plan flow_plan(const MapalNormSite& s, int sms, int rows) {
+  Plan p;
+  const uint64_t each = s.d > 4096 ? 16 : 8, turn = s.d > 4096 ? rows / 2 : rows;
+  p.group = (int)((s.d + 32 * each - 1) / (32 * each)) * 32;
+  p.threads = kFlow / p.group * p.group;
+  const uint64_t groups = p.threads / p.group, want = (s.rows + groups * turn - 1) / (groups * turn);
+  p.blocks = (unsigned)(want < (uint64_t)sms ? want : sms);
+  return p;
+}
+
 uint32_t grad_parts(const MapalNormSite& s, int sms) {
+  if (s.d <= kMostFlow && s.rows) return flow_plan(s, sms, 2).blocks;
   const uint64_t want = (s.rows + 7) / 8, cap = 2ull * sms;
   return (uint32_t)(want < 1 ? 1 : want < cap ? want : cap);
 }
 
 uint64_t grad_bytes(const MapalNormSite& s, int sms) { return grad_parts(s, sms) * 2ull * s.d * sizeof(float); }
 
-template <typename T, typename TW>
-void launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
+unsigned row_blocks(const MapalNormSite& s, int sms) { return (unsigned)(s.rows < 8ull * sms ? s.rows : 8ull * sms); }
+
+template <typename T, typename TW, int V, int EACH>
+void launch_held(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                  float* mean, float* rstd) {
-  const unsigned grid = (unsigned)(s.rows < 8ull * D.prof.sm_count ? s.rows : 8ull * D.prof.sm_count);
-  norm_rows_kernel<T, TW><<<grid, kThreads, 0, D.stream>>>(s, (const T*)x, w, b, (T*)y, mean, rstd);
-  count_launch();
+  const int group = (int)((s.d + 32 * EACH - 1) / (32 * EACH)) * 32;
+  // one row a block while that leaves no SM with two
+  const int threads = group >= 256 || s.rows <= (uint64_t)D.prof.sm_count ? group : 256 / group * group;
+  const uint64_t want = (s.rows + threads / group - 1) / (threads / group),
+                 cap = (uint64_t)D.prof.sm_count * (1024 / threads);
+  norm_held_kernel<T, TW, V, EACH><<<(unsigned)(want < cap ? want : cap), threads, 0, D.stream>>>(
+      s, (const T*)x, w, b, (T*)y, mean, rstd, group);
 }
 
-template <typename T, typename TW>
+template <typename T, typename TW, int V, int EACH, int ROWS>
+int launch_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
+                float* mean, float* rstd) {
+  constexpr size_t smem = Ring<T, V, EACH, ROWS, 1>::kBytes;
+  static std::atomic<uint64_t> done{0};
+  auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS>;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "layer_norm shared memory"));
+  const Plan p = flow_plan(s, D.prof.sm_count, 4);
+  kernel<<<p.blocks, p.threads, smem, D.stream>>>(s, (const T*)x, w, b, (T*)y, mean, rstd, p.group);
+  return 0;
+}
+
+template <typename T, typename TW, int V>
+int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
+                float* mean, float* rstd) {
+  constexpr int kMid = V == 1 ? 16 : 32;
+  // many: every thread of the device gets at least two turns of 32 elements
+  const bool many = s.rows * s.d >= 64ull * kFlow * D.prof.sm_count;
+  if (s.d <= 4096 && many)
+    MAPAL_TRY((launch_flow<T, TW, V, 8, 4>(D, s, x, w, b, y, mean, rstd)));
+  else if (s.d <= kMostFlow && many)
+    MAPAL_TRY((launch_flow<T, TW, V, 16, 2>(D, s, x, w, b, y, mean, rstd)));
+  else if (s.d <= 1024 * 8)
+    launch_held<T, TW, V, 8>(D, s, x, w, b, y, mean, rstd);
+  else if (s.d <= 1024 * kMid)
+    launch_held<T, TW, V, kMid>(D, s, x, w, b, y, mean, rstd);
+  else
+    norm_rows_kernel<T, TW, V><<<row_blocks(s, D.prof.sm_count), kThreads, 0, D.stream>>>(s, (const T*)x, w, b, (T*)y,
+                                                                                         mean, rstd);
+  count_launch();
+  return 0;
+}
+
+template <typename T, typename TW, int V, int EACH, int ROWS>
+int launch_grad_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
+                     const float* rstd, const void* dy, void* dx, float* work) {
+  constexpr size_t ring = Ring<T, V, EACH, ROWS, 2>::kBytes;
+  static std::atomic<uint64_t> done{0};
+  auto kernel = norm_grad_flow_kernel<T, TW, V, EACH, ROWS>;
+  const Plan p = flow_plan(s, D.prof.sm_count, 2);
+  const size_t sums = work && p.threads > p.group ? 2 * s.d * sizeof(float) : 0;  // at most 16 KB: d <= 2048
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, ring + 16384, "layer_norm_grad shared memory"));
+  kernel<<<p.blocks, p.threads, ring + sums, D.stream>>>(s, (const T*)x, w, mean, rstd, (const T*)dy, (T*)dx, work,
+                                                         p.group);
+  count_launch();
+  return 0;
+}
+
+template <typename T, typename TW, int V>
 int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
                      const float* rstd, const void* dy, void* dx, float* dw, float* db, float* work) {
-  const uint32_t parts = grad_parts(s, D.prof.sm_count);
-  const unsigned blocks = (unsigned)((s.d + 31) / 32);
-  if (dw || db) {
-    norm_grad_cols_kernel<T><<<dim3(blocks, parts), kThreads, 0, D.stream>>>(s, (const T*)x, mean, rstd,
-                                                                             (const T*)dy, work, parts);
-    count_launch();
-    norm_grad_join_kernel<<<(unsigned)((2 * s.d + 31) / 32), kThreads, 0, D.stream>>>(work, s.d, parts, dw, db);
+  const int sms = D.prof.sm_count;
+  const uint32_t parts = grad_parts(s, sms);
+  if (!dw && !db) work = nullptr;
+  const bool flow = s.d <= kMostFlow && s.rows;
+  if (flow && s.d <= 4096) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2>(D, s, x, w, mean, rstd, dy, dx, work)));
+  } else if (flow) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1>(D, s, x, w, mean, rstd, dy, dx, work)));
+  } else if (work) {
+    // before dx is written, which may be dy
+    norm_grad_cols_kernel<T, V><<<dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0, D.stream>>>(
+        s, (const T*)x, mean, rstd, (const T*)dy, work, parts);
     count_launch();
   }
-  if (s.rows) {
-    const unsigned grid = (unsigned)(s.rows < 8ull * D.prof.sm_count ? s.rows : 8ull * D.prof.sm_count);
-    norm_grad_rows_kernel<T, TW><<<grid, kThreads, 0, D.stream>>>(s, (const T*)x, w, mean, rstd, (const T*)dy, (T*)dx);
+  if (work) {
+    norm_grad_join_kernel<<<(unsigned)((2 * s.d + 31) / 32), 1024, 0, D.stream>>>(work, s.d, parts, dw, db);
+    count_launch();
+  }
+  if (!flow && s.rows) {
+    norm_grad_rows_kernel<T, TW, V><<<row_blocks(s, sms), kThreads, 0, D.stream>>>(s, (const T*)x, w, mean, rstd,
+                                                                                  (const T*)dy, (T*)dx);
     count_launch();
   }
   return 0;
 }
 
-// f(T, TW) for the site's types.
+// f(T, TW, V) for the site's types and the widest access (16, 4 or an element's
+// bytes) that a row is a multiple of and all arrays' rows begin at.
 template <typename F>
-auto by_type(const MapalNormSite& s, F&& f) {
+int by_type(const MapalNormSite& s, int width, const void* w, const void* b, F&& f) {
+  using std::integral_constant;
+  const int ww = align_of(w, 0, 1) < align_of(b, 0, 1) ? align_of(w, 0, 1) : align_of(b, 0, 1);
+  const int ws = dtype_bytes(s.wtype);
+  if (s.dtype == MAPAL_DTYPE_F32) {
+    if (width >= 16 && ww >= 16) return f(float{}, float{}, integral_constant<int, 4>{});
+    return f(float{}, float{}, integral_constant<int, 1>{});
+  }
+  auto half = [&](auto t, auto tw) {
+    if (width >= 16 && ww >= 16) return f(t, tw, integral_constant<int, 8>{});
+    if (width >= 4 && ww >= 2 * ws) return f(t, tw, integral_constant<int, 2>{});
+    return f(t, tw, integral_constant<int, 1>{});
+  };
   const bool wide = s.wtype == MAPAL_DTYPE_F32;
-  if (s.dtype == MAPAL_DTYPE_F32) return f(float{}, float{});
-  if (s.dtype == MAPAL_DTYPE_F16) return wide ? f(__half{}, float{}) : f(__half{}, __half{});
-  return wide ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
+  if (s.dtype == MAPAL_DTYPE_F16) return wide ? half(__half{}, float{}) : half(__half{}, __half{});
+  return wide ? half(__nv_bfloat16{}, float{}) : half(__nv_bfloat16{}, __nv_bfloat16{});
+}
+
+int narrowest(std::initializer_list<int> widths) {
+  int w = 16;
+  for (const int o : widths) w = o < w ? o : w;
+  return w;
 }
 
 bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
@@ -192,10 +831,11 @@ extern "C" int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site,
         !aligned_to(mean, 4) || !aligned_to(rstd, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
     MAPAL_TRY(enter(ctx));
-    by_type(*site, [&](auto t, auto tw) {
-      launch_norm<decltype(t), decltype(tw)>(ctx->dev[0], *site, x, w, b, y, mean, rstd);
-      return 0;
-    });
+    const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(y, site->ldy * es, site->rows),
+                                 align_of(nullptr, site->d * es, 2)});
+    MAPAL_TRY(by_type(*site, width, w, b, [&](auto t, auto tw, auto v) {
+      return launch_norm<decltype(t), decltype(tw), v.value>(ctx->dev[0], *site, x, w, b, y, mean, rstd);
+    }));
     return finish(ctx, 0, false);
   });
 }
@@ -230,9 +870,11 @@ extern "C" int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* 
     MAPAL_TRY(enter(ctx));
     if ((dw || db) && work_bytes < grad_bytes(*site, ctx->dev[0].prof.sm_count))
       return set_error(MAPAL_ERR_INVALID, "work is shorter than mapal_gpu_layer_norm_grad_workspace says");
-    MAPAL_TRY(by_type(*site, [&](auto t, auto tw) {
-      return launch_norm_grad<decltype(t), decltype(tw)>(ctx->dev[0], *site, x, w, mean, rstd, dy, dx, dw, db,
-                                                         (float*)work);
+    const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(dy, site->lddy * es, site->rows),
+                                 align_of(dx, site->lddx * es, site->rows), align_of(nullptr, site->d * es, 2)});
+    MAPAL_TRY(by_type(*site, width, w, w, [&](auto t, auto tw, auto v) {
+      return launch_norm_grad<decltype(t), decltype(tw), v.value>(ctx->dev[0], *site, x, w, mean, rstd, dy, dx, dw, db,
+                                                                  (float*)work);
     }));
     return finish(ctx, 0, false);
   });

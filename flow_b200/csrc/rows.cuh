@@ -6,7 +6,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <string.h>
+
 #include <exception>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -32,11 +35,110 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// V elements moved as one access.
+// V elements moved as one access, held as 32-bit words (or one 16-bit value).
+// Converted a word at a time: two bf16 are a shift and a mask, and pairs are
+// rounded by one instruction.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
-  T v[V];
+  static constexpr int W = sizeof(T) * V / 4;  // 0: a single 16-bit element
+  using Word = std::conditional_t<W == 0, uint16_t, uint32_t>;
+  Word w[W == 0 ? 1 : W];
+
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      if constexpr (W == 0) {
+        f[0] = __uint_as_float((uint32_t)w[0] << 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          f[2 * i] = __uint_as_float(w[i] << 16);
+          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    } else {
+      if constexpr (W == 0) {
+        f[0] = __half2float(__ushort_as_half(w[0]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          __half2 h;
+          memcpy(&h, &w[i], 4);
+          const float2 g = __half22float2(h);
+          f[2 * i] = g.x;
+          f[2 * i + 1] = g.y;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(f[i]);
+    } else if constexpr (W == 0) {
+      const T v = from_f32<T>(f[0]);
+      memcpy(&w[0], &v, 2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          memcpy(&w[i], &v, 4);
+        } else {
+          const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+          memcpy(&w[i], &v, 4);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (W == 0 ? 1 : W); ++i) w[i] = 0;
+  }
+
+  // Hides where the bits come from, so that a later use converts them again
+  // instead of keeping the floats of an earlier one in registers.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < (W == 0 ? 1 : W); ++i) {
+      if constexpr (W == 0)
+        asm volatile("" : "+h"(w[i]));
+      else
+        asm volatile("" : "+r"(w[i]));
+    }
+  }
 };
+
+// A pack read or written once (no reuse expected in this kernel).
+template <typename P>
+__device__ __forceinline__ P ld_once(const P* p) {
+  P r;
+  if constexpr (sizeof(P) == 16) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+    r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+  } else if constexpr (sizeof(P) == 4) {
+    r.w[0] = __ldcs(reinterpret_cast<const unsigned*>(p));
+  } else {
+    static_assert(sizeof(P) == 2, "packs of 2, 4 or 16 bytes");
+    r.w[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
+  }
+  return r;
+}
+template <typename P>
+__device__ __forceinline__ void st_once(P* p, const P& r) {
+  if constexpr (sizeof(P) == 16) {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]));
+  } else if constexpr (sizeof(P) == 4) {
+    __stcs(reinterpret_cast<unsigned*>(p), r.w[0]);
+  } else {
+    static_assert(sizeof(P) == 2, "packs of 2, 4 or 16 bytes");
+    __stcs(reinterpret_cast<unsigned short*>(p), r.w[0]);
+  }
+}
 
 inline int dtype_bytes(int dtype) {
   return dtype == MAPAL_DTYPE_F32 ? 4 : dtype == MAPAL_DTYPE_F16 || dtype == MAPAL_DTYPE_BF16 ? 2 : dtype == MAPAL_DTYPE_I8 ? 1 : 0;
