@@ -32,8 +32,10 @@ __device__ __forceinline__ void weights(const void* w, int64_t i, float none, fl
 
 __device__ __forceinline__ float inv_std(float var, float eps) { return __fdiv_rn(1.0f, __fsqrt_rn(var + eps)); }
 
-// G threads (whole warps) of a block that share a row. A group of one warp
-// needs no barrier; others meet at a named barrier of their own.
+// Threads of a block that share a row: 8 or 16 lanes of a warp (SUB), a warp,
+// which need no barrier, or several warps, which meet at a named barrier of
+// their own.
+template <bool SUB>
 struct Group {
   int size, tid, id;
   __device__ explicit Group(int g) : size(g), tid(threadIdx.x % g), id(threadIdx.x / g) {}
@@ -45,6 +47,13 @@ struct Group {
   template <int N>
   __device__ void sums(float (&a)[N], float (*red)[16]) const {
     static_assert(N == 1 || N == 2 || N == 4, "");
+    if constexpr (SUB) {  // other groups of the warp may have no row left
+      const unsigned lanes = ((1u << size) - 1) << (threadIdx.x & 31 & ~(size - 1));
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        for (int o = size / 2; o > 0; o >>= 1) a[k] += __shfl_xor_sync(lanes, a[k], o);
+      return;
+    }
     constexpr unsigned kAll = 0xffffffffu;
     constexpr int L = 32 / N;  // lanes that end with the same value
     const int lane = tid & 31;
@@ -83,7 +92,7 @@ struct Group {
     return warp_sum(lane < size / 32 ? red[lane] : 0.0f);
   }
 };
-constexpr int kMostGroups = 16;
+constexpr int kMostGroups = 8;  // of more than a warp in a block
 
 // ---- few rows ------------------------------------------------------------------------
 //
@@ -99,7 +108,7 @@ __global__ void __launch_bounds__(1024)
   using P = Pack<T, V>;
   constexpr int NV = EACH / V;
   __shared__ float red[32][2][32];  // at most 32 groups
-  const Group G(group);
+  const Group<false> G(group);
   const uint64_t stride = (uint64_t)gridDim.x * (blockDim.x / group);
   const int d = (int)S.d;
   const float n = (float)d;
@@ -214,17 +223,18 @@ struct Ring {
 
 __device__ __forceinline__ float f2_sum(f2 v) { return f2_lo(v) + f2_hi(v); }
 
-template <typename T, typename TW, int V, int EACH, int ROWS>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
 __global__ void __launch_bounds__(kFlow, 1)
     norm_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const void* __restrict__ b, T* y,
                      float* __restrict__ mean, float* __restrict__ rstd, int group) {
   using R = Ring<T, V, EACH, ROWS, 1>;
   using P = Pack<T, V>;
   constexpr int NV = EACH / V;
-  __shared__ float red[kMostGroups][2][4][16];
+  __shared__ float sets[kMostGroups][2][4][16];
   extern __shared__ __align__(16) uint8_t dyn[];
   R ring(dyn);
-  const Group G(group);
+  const Group<SUB> G(group);
+  auto* red = sets[SUB || group == 32 ? 0 : G.id];
   const int groups = blockDim.x / group, d = (int)S.d;
   const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
   uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(kFlow, 1)
       }
       s[k] = f2_sum(t);
     }
-    G.sums(s, red[G.id][0]);
+    G.sums(s, red[0]);
     start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
     ring.next();
 #pragma unroll
@@ -316,7 +326,7 @@ __global__ void __launch_bounds__(kFlow, 1)
       for (int u = 0; u < EACH / 2; ++u) t = f2_fma(v[k][u], v[k][u], t);
       q[k] = f2_sum(t);
     }
-    G.sums(q, red[G.id][1]);
+    G.sums(q, red[1]);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       const float rs = inv_std(__fdiv_rn(q[k], n), S.eps);
@@ -349,18 +359,19 @@ __global__ void __launch_bounds__(kFlow, 1)
 
 // The gradient: dx, and where work is given this block's sums of dy*h and dy
 // as rows 2*block and 2*block + 1 of it (the groups add theirs in order).
-template <typename T, typename TW, int V, int EACH, int ROWS>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
 __global__ void __launch_bounds__(kFlow, 1)
     norm_grad_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const float* __restrict__ mean,
                           const float* __restrict__ rstd, const T* dy, T* dx, float* __restrict__ work, int group) {
   using R = Ring<T, V, EACH, ROWS, 2>;
   using P = Pack<T, V>;
   constexpr int NV = EACH / V, H = EACH / 2;
-  __shared__ float red[kMostGroups][2][2 * ROWS][16];
+  __shared__ float sets[kMostGroups][2][2 * ROWS][16];
   extern __shared__ __align__(16) uint8_t dyn[];
   R ring(dyn);
-  float* sums = reinterpret_cast<float*>(dyn + R::kBytes);  // several groups: 2*d floats
-  const Group G(group);
+  float* sums = reinterpret_cast<float*>(dyn);  // 2*d floats, when the ring is done
+  const Group<SUB> G(group);
+  auto* red = sets[SUB || group == 32 ? 0 : G.id];
   const int groups = blockDim.x / group, d = (int)S.d;
   const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
   uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
@@ -453,7 +464,7 @@ __global__ void __launch_bounds__(kFlow, 1)
       c[2 * k + 1] = f2_sum(c2);
     }
     stats(r + step);
-    G.sums(c, red[G.id][par]);
+    G.sums(c, red[par]);
     start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
     ring.next();
 #pragma unroll
@@ -480,10 +491,23 @@ __global__ void __launch_bounds__(kFlow, 1)
     }
   }
   if (!work) return;
+  // groups of one warp first, then warps or larger groups in order
+  if constexpr (SUB) {
+    __syncwarp();
+    for (int o = group; o < 32; o <<= 1)
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        aw[u] = f2_add(aw[u], __shfl_xor_sync(0xffffffffu, aw[u], o));
+        ab[u] = f2_add(ab[u], __shfl_xor_sync(0xffffffffu, ab[u], o));
+      }
+  }
+  const int turns = SUB ? blockDim.x / 32 : groups;
+  const int turn = !SUB ? G.id : (int)(threadIdx.x % 32) < group ? (int)(threadIdx.x / 32) : -1;
   float* out = work + 2ull * blockIdx.x * S.d;
-  for (int k = 0; k < groups; ++k) {
-    if (G.id == k) {
-      const bool first = k == 0, last = k == groups - 1;
+  __syncthreads();  // every group has taken its last rows out of the ring
+  for (int k = 0; k < turns; ++k) {
+    if (turn == k) {
+      const bool first = k == 0, last = k == turns - 1;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int i = (j * group + G.tid) * V;
@@ -671,26 +695,24 @@ int check_norm(const MapalNormSite* s) {
 }
 
 // How the kernels for many rows are launched: threads of a group, of a block,
-// blocks. `rows` at a time; rows of more than 4096 elements twice the columns
-// a thread.
+// blocks.
 struct Plan {
   int group, threads;
   unsigned blocks;
 };
 
-Plan flow_plan(const MapalNormSite& s, int sms, int rows) {
+Plan flow_plan(const MapalNormSite& s, int sms, uint64_t each, uint64_t turn) {
   Plan p;
-  const uint64_t each = s.d > 4096 ? 16 : 8, turn = s.d > 4096 ? rows / 2 : rows;
-  p.group = (int)((s.d + 32 * each - 1) / (32 * each)) * 32;
+  p.group = s.d <= 64 ? 8 : s.d <= 128 ? 16 : (int)((s.d + 32 * each - 1) / (32 * each)) * 32;
   p.threads = kFlow / p.group * p.group;
   const uint64_t groups = p.threads / p.group, want = (s.rows + groups * turn - 1) / (groups * turn);
   p.blocks = (unsigned)(want < (uint64_t)sms ? want : sms);
   return p;
 }
 
+// Partial sums that the gradient's scratch has room for: a block each.
 uint32_t grad_parts(const MapalNormSite& s, int sms) {
-  if (s.d <= kMostFlow && s.rows) return flow_plan(s, sms, 2).blocks;
-  const uint64_t want = (s.rows + 7) / 8, cap = 2ull * sms;
+  const uint64_t want = s.d <= kMostFlow ? s.rows : (s.rows + 7) / 8, cap = s.d <= kMostFlow ? sms : 2ull * sms;
   return (uint32_t)(want < 1 ? 1 : want < cap ? want : cap);
 }
 
@@ -710,14 +732,14 @@ void launch_held(const DeviceSlot& D, const MapalNormSite& s, const void* x, con
       s, (const T*)x, w, b, (T*)y, mean, rstd, group);
 }
 
-template <typename T, typename TW, int V, int EACH, int ROWS>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
 int launch_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                 float* mean, float* rstd) {
   constexpr size_t smem = Ring<T, V, EACH, ROWS, 1>::kBytes;
   static std::atomic<uint64_t> done{0};
-  auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS>;
+  auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS, SUB>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "layer_norm shared memory"));
-  const Plan p = flow_plan(s, D.prof.sm_count, 4);
+  const Plan p = flow_plan(s, D.prof.sm_count, EACH, ROWS);
   kernel<<<p.blocks, p.threads, smem, D.stream>>>(s, (const T*)x, w, b, (T*)y, mean, rstd, p.group);
   return 0;
 }
@@ -726,12 +748,22 @@ template <typename T, typename TW, int V>
 int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                 float* mean, float* rstd) {
   constexpr int kMid = V == 1 ? 16 : 32;
-  // many: every thread of the device gets at least two turns of 32 elements
-  const bool many = s.rows * s.d >= 64ull * kFlow * D.prof.sm_count;
-  if (s.d <= 4096 && many)
-    MAPAL_TRY((launch_flow<T, TW, V, 8, 4>(D, s, x, w, b, y, mean, rstd)));
+  constexpr int kLong = V == 1 ? 16 : 32;
+  // Many rows: a thread of the device gets at least two turns of 32 elements
+  // (eight where it loads them one by one and a turn is slower to start).
+  const bool many = s.rows * s.d >= (V == 1 ? 256ull : 64ull) * kFlow * D.prof.sm_count;
+  // 16-byte accesses of 16-bit types do better with 16 columns a thread (and
+  // half the warps at each barrier) from 512 columns on: 16384 x 4096 bf16 52
+  // against 60 us, 60000 x 1024 45 against 54; f32 and narrow accesses do not.
+  constexpr uint64_t kNarrow = sizeof(T) * V == 16 && sizeof(T) == 2 ? 512 : 4096;
+  if (s.d <= 128 && many)
+    MAPAL_TRY((launch_flow<T, TW, V, 8, 4, true>(D, s, x, w, b, y, mean, rstd)));
+  else if (s.d <= kNarrow && many)
+    MAPAL_TRY((launch_flow<T, TW, V, 8, 4, false>(D, s, x, w, b, y, mean, rstd)));
   else if (s.d <= kMostFlow && many)
-    MAPAL_TRY((launch_flow<T, TW, V, 16, 2>(D, s, x, w, b, y, mean, rstd)));
+    MAPAL_TRY((launch_flow<T, TW, V, 16, 2, false>(D, s, x, w, b, y, mean, rstd)));
+  else if (V > 1 && s.d <= 2 * kMostFlow && many)
+    MAPAL_TRY((launch_flow<T, TW, V, kLong, 32 / kLong, false>(D, s, x, w, b, y, mean, rstd)));
   else if (s.d <= 1024 * 8)
     launch_held<T, TW, V, 8>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= 1024 * kMid)
@@ -743,16 +775,18 @@ int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
   return 0;
 }
 
-template <typename T, typename TW, int V, int EACH, int ROWS>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
 int launch_grad_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
-                     const float* rstd, const void* dy, void* dx, float* work) {
+                     const float* rstd, const void* dy, void* dx, float* work, uint32_t& parts) {
   constexpr size_t ring = Ring<T, V, EACH, ROWS, 2>::kBytes;
   static std::atomic<uint64_t> done{0};
-  auto kernel = norm_grad_flow_kernel<T, TW, V, EACH, ROWS>;
-  const Plan p = flow_plan(s, D.prof.sm_count, 2);
-  const size_t sums = work && p.threads > p.group ? 2 * s.d * sizeof(float) : 0;  // at most 16 KB: d <= 2048
-  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, ring + 16384, "layer_norm_grad shared memory"));
-  kernel<<<p.blocks, p.threads, ring + sums, D.stream>>>(s, (const T*)x, w, mean, rstd, (const T*)dy, (T*)dx, work,
+  auto kernel = norm_grad_flow_kernel<T, TW, V, EACH, ROWS, SUB>;
+  const Plan p = flow_plan(s, D.prof.sm_count, EACH, ROWS);
+  parts = p.blocks;
+  const size_t sums = p.threads > p.group ? 2 * s.d * sizeof(float) : 0;  // at most 32 KB: d <= 4096
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, ring > 32768 ? ring : 32768,
+                             "layer_norm_grad shared memory"));
+  kernel<<<p.blocks, p.threads, ring > sums ? ring : sums, D.stream>>>(s, (const T*)x, w, mean, rstd, (const T*)dy, (T*)dx, work,
                                                          p.group);
   count_launch();
   return 0;
@@ -762,13 +796,18 @@ template <typename T, typename TW, int V>
 int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
                      const float* rstd, const void* dy, void* dx, float* dw, float* db, float* work) {
   const int sms = D.prof.sm_count;
-  const uint32_t parts = grad_parts(s, sms);
+  uint32_t parts = grad_parts(s, sms);
   if (!dw && !db) work = nullptr;
   const bool flow = s.d <= kMostFlow && s.rows;
-  if (flow && s.d <= 4096) {
-    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2>(D, s, x, w, mean, rstd, dy, dx, work)));
+  // as in the forward pass, but more registers hang on a column: 16384 x 4096
+  // bf16 75 against 77 us, 60000 x 1024 73 against 69
+  constexpr uint64_t kNarrow = sizeof(T) * V == 16 && sizeof(T) == 2 ? 2048 : 4096;
+  if (flow && s.d <= 128) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, true>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
+  } else if (flow && s.d <= kNarrow) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, false>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (flow) {
-    MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1>(D, s, x, w, mean, rstd, dy, dx, work)));
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1, false>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (work) {
     // before dx is written, which may be dy
     norm_grad_cols_kernel<T, V><<<dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0, D.stream>>>(
