@@ -19,8 +19,10 @@ constexpr unsigned kTrapOob = 2;  // the trap flag's index_oob
 // ---- sort --------------------------------------------------------------------------
 
 constexpr int kMaxExperts = 1024;
-constexpr int kSortWarps = 32;
+constexpr int kSortWarps = 32;  // at most, in a block
 constexpr int kSortThreads = kSortWarps * 32;
+constexpr uint32_t kSortBlocks = 8;  // at most, in the cluster
+constexpr int kThreads = 256;
 constexpr int kSortUnroll = 8;  // ids in flight for each lane
 
 // One cluster sorts all slots, each warp a contiguous run of them in order.
@@ -31,33 +33,37 @@ constexpr int kSortUnroll = 8;  // ids in flight for each lane
 // Second walk: a slot's place is its expert's counter plus the lanes before it
 // with the same expert. Slots keep their order within an expert, no atomics,
 // no memory but the arrays.
-__global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t E,
-                                                                   uint32_t chunk, int32_t* __restrict__ offsets,
-                                                                   int32_t* __restrict__ order,
-                                                                   int32_t* __restrict__ pos, unsigned* trap) {
+__global__ void __launch_bounds__(kSortThreads)
+    expert_sort_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t E, uint32_t chunk,
+                       int32_t* __restrict__ offsets, int32_t* __restrict__ order, int32_t* __restrict__ pos,
+                       unsigned* trap) {
   extern __shared__ uint32_t sm[];
-  uint32_t* cnt = sm;                      // [warp][E]
-  uint32_t* total = sm + kSortWarps * E;   // [E]: this block's slots
-  uint32_t* start = total + E;             // [E]: where this block's slots of an expert begin
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  uint32_t* cnt = sm;                 // [warp][E]
+  uint32_t* total = sm + warps * E;   // [E]: this block's slots
+  uint32_t* start = total + E;        // [E]: where this block's slots of an expert begin
   __shared__ uint32_t wsum[32];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t lt = (1u << lane) - 1;
-  const uint64_t lo64 = (uint64_t)(rank * kSortWarps + warp) * chunk;
+  const uint64_t lo64 = (uint64_t)(rank * warps + warp) * chunk;
   const uint32_t lo = (uint32_t)(lo64 < n ? lo64 : n), hi = (uint32_t)(lo64 + chunk < n ? lo64 + chunk : n);
   uint32_t* mine = cnt + warp * E;
 
-  for (uint32_t e = lane; e < E; e += 32) mine[e] = 0;
-  __syncwarp();
-  bool bad = false;
-  for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortUnroll) {
-    int32_t id[kSortUnroll];
+  auto load = [&](int32_t (&id)[kSortUnroll], uint32_t i0) {
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) {
       const uint32_t i = i0 + u * 32 + lane;
       id[u] = i < hi ? __ldg(ids + i) : -1;
     }
+  };
+  int32_t id[kSortUnroll];
+  load(id, lo);
+  for (uint32_t e = lane; e < E; e += 32) mine[e] = 0;
+  __syncwarp();
+  bool bad = false;
+  for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortUnroll) {
+    if (i0 != lo) load(id, i0);
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) {
       if (i0 + u * 32 >= hi) break;
@@ -70,50 +76,60 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const int32_t
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicMax(trap, kTrapOob);
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < E; e += kSortThreads) {
+  for (uint32_t e = threadIdx.x; e < E; e += blockDim.x) {
     uint32_t run = 0;
-#pragma unroll 8
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = cnt[w * E + e];
-      cnt[w * E + e] = run;
-      run += c;
+    for (uint32_t w0 = 0; w0 < warps; w0 += 8) {
+      uint32_t c[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) c[w] = w0 + w < warps ? cnt[(w0 + w) * E + e] : 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (w0 + w < warps) cnt[(w0 + w) * E + e] = run;
+        run += c[w];
+      }
     }
     total[e] = run;
   }
-  cluster.sync();
-  // E <= kSortThreads: one expert a thread
-  uint32_t before = 0, all = 0;
-  if (threadIdx.x < E)
-    for (uint32_t r = 0; r < blocks; ++r) {
-      const uint32_t c = *cluster.map_shared_rank(total + threadIdx.x, r);
-      before += r < rank ? c : 0;
-      all += c;
-    }
-  uint32_t incl = all;
+  if (blocks > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  // blocks of blockDim.x experts in turn, one a thread
+  uint32_t done = 0;
+  for (uint32_t e0 = 0; e0 < E; e0 += blockDim.x) {
+    const uint32_t e = e0 + threadIdx.x;
+    uint32_t before = 0, all = 0;
+    if (e < E) {
+      uint32_t c[kSortBlocks];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) wsum[warp] = incl;
-  __syncthreads();
-  uint32_t base = 0;
-  for (uint32_t w = 0; w < warp; ++w) base += wsum[w];
-  if (threadIdx.x < E) {
-    start[threadIdx.x] = base + incl - all + before;
-    if (rank == 0) {
-      offsets[threadIdx.x] = (int32_t)(base + incl - all);
-      if (threadIdx.x == E - 1) offsets[E] = (int32_t)(base + incl);
+      for (uint32_t r = 0; r < kSortBlocks; ++r)
+        c[r] = r >= blocks ? 0 : blocks > 1 ? *cluster.map_shared_rank(total + e, r) : total[e];
+#pragma unroll
+      for (uint32_t r = 0; r < kSortBlocks; ++r) {
+        before += r < rank ? c[r] : 0;
+        all += c[r];
+      }
     }
+    uint32_t incl = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    const uint32_t part = lane < warps ? wsum[lane] : 0;
+    const uint32_t base = done + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
+    done += __reduce_add_sync(0xffffffffu, part);
+    if (e < E) {
+      start[e] = base + incl - all + before;
+      if (rank == 0) offsets[e] = (int32_t)(base + incl - all);
+    }
+    __syncthreads();
   }
-  cluster.sync();  // `start` is written, and no block leaves while another reads its counts
+  if (rank == 0 && threadIdx.x == 0) offsets[E] = (int32_t)done;
   for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortUnroll) {
-    int32_t id[kSortUnroll];
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) {
-      const uint32_t i = i0 + u * 32 + lane;
-      id[u] = i < hi ? __ldg(ids + i) : -1;
-    }
+    if (chunk > 32 * kSortUnroll) load(id, i0);  // a shorter run is still held
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) {
       if (i0 + u * 32 >= hi) break;
@@ -131,13 +147,20 @@ __global__ void __launch_bounds__(kSortThreads) expert_sort_kernel(const int32_t
       if (i < hi) pos[i] = p;
     }
   }
+  if (blocks > 1) cluster.sync();  // no block leaves while another reads its counts
 }
 
 // ---- rows --------------------------------------------------------------------------
+//
+// Bound by HBM: dispatch reads a token's row once and writes k, combine reads k
+// and writes one. A block takes a piece of a token's row (a few accesses a
+// thread), so that even a few tokens spread over the device, and each thread
+// has all of its loads in flight at once.
 
-constexpr int kThreads = 256;
+constexpr int kRowThreads = 128;
+constexpr int kAtOnce = 4;  // slots of a token whose rows are in flight together
 
-// Token t's place for slot j, -1 for none; out of range raises the trap.
+// Slot's place, -1 for none; out of range raises the trap.
 __device__ __forceinline__ int32_t place_of(const int32_t* pos, uint64_t slot, uint64_t rows, unsigned* trap) {
   const int32_t p = __ldg(pos + slot);
   if (p >= 0 && (uint64_t)p >= rows) {
@@ -147,87 +170,163 @@ __device__ __forceinline__ int32_t place_of(const int32_t* pos, uint64_t slot, u
   return p;
 }
 
-// xs[pos[t, j]] = x[t] in units U of a row; one block a token.
-template <typename U>
-__global__ void __launch_bounds__(kThreads) dispatch_kernel(const U* __restrict__ x, const float* __restrict__ scale,
-                                                            const int32_t* __restrict__ pos, U* __restrict__ xs,
-                                                            float* __restrict__ scale_out, uint64_t tokens, uint32_t k,
-                                                            uint64_t units, uint64_t ldt, uint64_t ldr, uint64_t rows,
-                                                            unsigned* trap) {
-  for (uint64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
-    for (uint64_t i = threadIdx.x; i < units; i += kThreads) {
-      const U v = x[t * ldt + i];
-      for (uint32_t j = 0; j < k; ++j) {
-        const int32_t p = place_of(pos, t * k + j, rows, trap);
-        if (p >= 0) xs[(uint64_t)p * ldr + i] = v;
-      }
-    }
-    if (scale)
-      for (uint32_t j = threadIdx.x; j < k; j += kThreads) {
-        const int32_t p = place_of(pos, t * k + j, rows, trap);
-        if (p >= 0) scale_out[p] = scale[t];
-      }
-  }
-}
+// A row in pieces of `piece` accesses; item = token * pieces + piece.
+struct Pieces {
+  uint64_t items;
+  uint32_t pieces;
+};
 
-// y[t] = sum_j w[t, j]*h[pos[t, j]]; one block a token.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__ h, const float* __restrict__ w,
-                                                           const int32_t* __restrict__ pos, T* __restrict__ y,
-                                                           uint64_t tokens, uint32_t k, uint64_t d, uint64_t ldt,
-                                                           uint64_t ldr, uint64_t rows, unsigned* trap) {
-  for (uint64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
-    for (uint64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
-      float acc[V] = {};
-      for (uint32_t j = 0; j < k; ++j) {
-        const int32_t p = place_of(pos, t * k + j, rows, trap);
-        if (p < 0) continue;
-        const float g = w ? __ldg(w + t * k + j) : 1.0f;
-        float f[V];
-        reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i)->get(f);
+// xs[pos[t, j]] = x[t] in units U of a row, NV units a thread.
+template <typename U, int NV>
+__global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const U* __restrict__ x, const float* __restrict__ scale,
+                                                               const int32_t* __restrict__ pos, U* __restrict__ xs,
+                                                               float* __restrict__ scale_out, Pieces Q, uint32_t k,
+                                                               uint64_t units, uint64_t ldt, uint64_t ldr,
+                                                               uint64_t rows, unsigned* trap) {
+  for (uint64_t item = blockIdx.x; item < Q.items; item += gridDim.x) {
+    const uint64_t t = item / Q.pieces;
+    const uint32_t piece = (uint32_t)(item % Q.pieces);
+    const uint64_t i0 = (uint64_t)piece * (kRowThreads * NV) + threadIdx.x;
+    U v[NV];
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = __fmaf_rn(g, f[e], acc[e]);
-      }
-      Pack<T, V> o;
-      o.set(acc);
-      *reinterpret_cast<Pack<T, V>*>(y + t * ldt + i) = o;
+    for (int u = 0; u < NV; ++u)
+      if (i0 + u * kRowThreads < units) v[u] = x[t * ldt + i0 + u * kRowThreads];
+    for (uint32_t j = 0; j < k; ++j) {
+      const int32_t p = place_of(pos, t * k + j, rows, trap);
+      if (p < 0) continue;
+      U* to = xs + (uint64_t)p * ldr + i0;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        if (i0 + u * kRowThreads < units) to[u * kRowThreads] = v[u];
+      if (scale && piece == 0 && threadIdx.x == 0) scale_out[p] = scale[t];
     }
   }
 }
 
-// dh[p] = w*dy[t] and dw = <dy[t], h[p]>; one block a slot. An element of h is
-// read by the thread that writes it in dh.
-template <typename T, int V>
+// y[t] = sum_j w[t, j]*h[pos[t, j]], NV packs a thread.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kRowThreads) combine_kernel(const T* __restrict__ h, const float* __restrict__ w,
+                                                              const int32_t* __restrict__ pos, T* __restrict__ y,
+                                                              Pieces Q, uint32_t k, uint64_t d, uint64_t ldt,
+                                                              uint64_t ldr, uint64_t rows, unsigned* trap) {
+  using P = Pack<T, V>;
+  for (uint64_t item = blockIdx.x; item < Q.items; item += gridDim.x) {
+    const uint64_t t = item / Q.pieces;
+    const uint64_t i0 = ((item % Q.pieces) * (kRowThreads * NV) + threadIdx.x) * V;
+    float acc[NV][V] = {};
+    for (uint32_t j0 = 0; j0 < k; j0 += kAtOnce) {
+      P v[kAtOnce][NV];
+      float g[kAtOnce];
+      bool on[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const uint64_t slot = t * k + j0 + u;
+        const int32_t p = j0 + u < k ? place_of(pos, slot, rows, trap) : -1;
+        on[u] = p >= 0;
+        g[u] = on[u] && w ? __ldg(w + slot) : 1.0f;
+        const T* from = h + (uint64_t)(on[u] ? p : 0) * ldr + i0;
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+          if (on[u] && i0 + c * (kRowThreads * V) < d) v[u][c] = ld_once(reinterpret_cast<const P*>(from + c * (kRowThreads * V)));
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (on[u]) {
+#pragma unroll
+          for (int c = 0; c < NV; ++c) {
+            float f[V];
+            v[u][c].get(f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[c][e] = __fmaf_rn(g[u], f[e], acc[c][e]);
+          }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      P o;
+      o.set(acc[c]);
+      if (i0 + c * (kRowThreads * V) < d) st_once(reinterpret_cast<P*>(y + t * ldt + i0 + c * (kRowThreads * V)), o);
+    }
+  }
+}
+
+// dh[p] = w*dy[t] and dw = <dy[t], h[p]> for SLOTS slots of a token at once,
+// over which dy is read once; a block owns whole rows, so dw needs no atomics.
+// An element of h is read by the thread that writes it in dh.
+template <typename T, int V, int SLOTS>
 __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* h, const float* __restrict__ w,
                                                                 const int32_t* __restrict__ pos,
                                                                 const T* __restrict__ dy, T* dh, float* __restrict__ dw,
-                                                                uint64_t slots, uint32_t k, uint64_t d, uint64_t ldt,
+                                                                uint64_t items, uint32_t k, uint64_t d, uint64_t ldt,
                                                                 uint64_t ldr, uint64_t rows, unsigned* trap) {
-  __shared__ float red[2][32];
+  using P = Pack<T, V>;
+  __shared__ float red[2][SLOTS][kThreads / 32];
+  const uint32_t turns = (k + SLOTS - 1) / SLOTS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int par = 0;
-  for (uint64_t s = blockIdx.x; s < slots; s += gridDim.x, par ^= 1) {
-    const int32_t p = place_of(pos, s, rows, trap);
-    float dot = 0.0f;
-    if (p >= 0) {
-      const float g = w ? __ldg(w + s) : 1.0f;
-      const T* dyr = dy + s / k * ldt;
-      for (uint64_t i = threadIdx.x * V; i < d; i += kThreads * V) {
-        float a[V], b[V];
-        reinterpret_cast<const Pack<T, V>*>(dyr + i)->get(a);
-        reinterpret_cast<const Pack<T, V>*>(h + (uint64_t)p * ldr + i)->get(b);
-        Pack<T, V> o;
+  for (uint64_t item = blockIdx.x; item < items; item += gridDim.x, par ^= 1) {
+    const uint64_t t = item / turns;
+    const uint32_t j0 = (uint32_t)(item % turns) * SLOTS;
+    float dot[SLOTS], g[SLOTS];
+    uint64_t at[SLOTS];
+    bool on[SLOTS];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          dot = __fmaf_rn(a[e], b[e], dot);
-          a[e] *= g;
+    for (int u = 0; u < SLOTS; ++u) {
+      const uint64_t slot = t * k + j0 + u;
+      const int32_t p = j0 + u < k ? place_of(pos, slot, rows, trap) : -1;
+      on[u] = p >= 0;
+      g[u] = on[u] && w ? __ldg(w + slot) : 1.0f;
+      at[u] = (uint64_t)(on[u] ? p : 0) * ldr;
+      dot[u] = 0.0f;
+    }
+    const T* dyr = dy + t * ldt;
+    // all loads of a turn before its stores: dh may be h, so the compiler keeps their order
+    constexpr int NV = sizeof(P) == 16 ? 1 : 4;
+    const uint64_t step = blockDim.x * V;
+    for (uint64_t i0 = threadIdx.x * V; i0 < d; i0 += step * NV) {
+      P a[NV], b[SLOTS][NV];
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+        if (i0 + c * step < d) a[c] = *reinterpret_cast<const P*>(dyr + i0 + c * step);
+#pragma unroll
+      for (int u = 0; u < SLOTS; ++u)
+        if (on[u]) {
+#pragma unroll
+          for (int c = 0; c < NV; ++c)
+            if (i0 + c * step < d) b[u][c] = ld_once(reinterpret_cast<const P*>(h + at[u] + i0 + c * step));
         }
-        o.set(a);
-        *reinterpret_cast<Pack<T, V>*>(dh + (uint64_t)p * ldr + i) = o;
-      }
+#pragma unroll
+      for (int u = 0; u < SLOTS; ++u)
+        if (on[u]) {
+#pragma unroll
+          for (int c = 0; c < NV; ++c)
+            if (i0 + c * step < d) {
+              float fa[V], fb[V];
+              a[c].get(fa);
+              b[u][c].get(fb);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                dot[u] = __fmaf_rn(fa[e], fb[e], dot[u]);
+                fb[e] = fa[e] * g[u];
+              }
+              P o;
+              o.set(fb);
+              st_once(reinterpret_cast<P*>(dh + at[u] + i0 + c * step), o);
+            }
+        }
     }
     if (dw) {
-      dot = block_sum(dot, red[par]);
-      if (threadIdx.x == 0) dw[s] = dot;
+#pragma unroll
+      for (int u = 0; u < SLOTS; ++u) {
+        dot[u] = warp_sum(dot[u]);
+        if (lane == 0) red[par][u][warp] = dot[u];
+      }
+      __syncthreads();
+      if (threadIdx.x < SLOTS && j0 + threadIdx.x < k) {
+        float s = 0.0f;
+        for (int q = 0; q < warps; ++q) s += red[par][threadIdx.x][q];
+        dw[t * k + j0 + threadIdx.x] = s;
+      }
     }
   }
 }
@@ -251,15 +350,26 @@ int check_site(const MapalExpertSite* s, bool rows_arrays, bool bytes_too) {
 
 bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
-unsigned token_grid(uint64_t n, int sms) { return (unsigned)(n < 32ull * sms ? n : 32ull * sms); }
+constexpr uint64_t kMostBlocks = 1u << 20;  // what lies beyond is walked
+
+// `accesses` of a row, NV a thread.
+Pieces pieces_of(uint64_t tokens, uint64_t accesses, int nv) {
+  Pieces q;
+  const uint64_t one = (uint64_t)kRowThreads * nv;
+  q.pieces = (uint32_t)((accesses + one - 1) / one);
+  if (q.pieces == 0) q.pieces = 1;
+  q.items = tokens * q.pieces;
+  return q;
+}
 
 template <typename U>
 void launch_dispatch(const DeviceSlot& D, const MapalExpertSite& s, const void* x, const float* scale, const int32_t* pos,
                      void* xs, float* scale_out) {
   const uint64_t es = dtype_bytes(s.dtype), u = sizeof(U);
-  dispatch_kernel<U><<<token_grid(s.tokens, D.prof.sm_count), kThreads, 0, D.stream>>>(
-      (const U*)x, scale, pos, (U*)xs, scale_out, s.tokens, s.k, s.d * es / u, s.ldt * es / u, s.ldr * es / u, s.rows,
-      D.trap);
+  constexpr int NV = sizeof(U) == 16 ? 2 : 4;
+  const Pieces q = pieces_of(s.tokens, s.d * es / u, NV);
+  dispatch_kernel<U, NV><<<(unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0, D.stream>>>(
+      (const U*)x, scale, pos, (U*)xs, scale_out, q, s.k, s.d * es / u, s.ldt * es / u, s.ldr * es / u, s.rows, D.trap);
   count_launch();
 }
 
@@ -303,16 +413,20 @@ extern "C" int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* si
     MAPAL_TRY(enter(ctx));
     DeviceSlot& D = ctx->dev[0];
     const uint32_t E = site->experts;
-    const size_t smem = (size_t)(kSortWarps + 2) * E * sizeof(uint32_t);
     static std::atomic<uint64_t> done{0};
     MAPAL_TRY(ensure_smem_attr(done, (const void*)expert_sort_kernel, D.device,
                                (size_t)(kSortWarps + 2) * kMaxExperts * sizeof(uint32_t), "expert_sort shared memory"));
-    const unsigned blocks = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
-    const uint64_t warps = (uint64_t)blocks * kSortWarps;
-    const uint32_t chunk = (uint32_t)(((n + warps - 1) / warps + 31) / 32 * 32);
+    // About 64 slots a warp (a few warps sort a generated batch), then up to
+    // 8 blocks of 32 warps.
+    const uint64_t want = (n + 63) / 64;
+    const unsigned blocks = want <= 2 * kSortWarps ? 1 : want <= 4 * kSortWarps ? 2 : want <= 8 * kSortWarps ? 4 : 8;
+    const uint32_t warps = (uint32_t)(want < 4 ? 4 : want < kSortWarps ? want : kSortWarps);
+    const uint64_t all = (uint64_t)blocks * warps;
+    const uint32_t chunk = (uint32_t)(((n + all - 1) / all + 31) / 32 * 32);
+    const size_t smem = (size_t)(warps + 2) * E * sizeof(uint32_t);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kSortThreads);
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = D.stream;
     cudaLaunchAttribute at[1];
@@ -320,7 +434,7 @@ extern "C" int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* si
     at[0].val.clusterDim.x = blocks;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = blocks > 1 ? 1 : 0;
     MAPAL_CUDA(cudaLaunchKernelEx(&cfg, expert_sort_kernel, ids, (uint32_t)n, E, chunk, offsets, order, pos, D.trap));
     count_launch();
     return finish(ctx, 0, true);
@@ -364,8 +478,10 @@ static int combine_rows(MapalGpuCtx* ctx, const MapalExpertSite* site, const voi
   const MapalExpertSite& s = *site;
   by_type(s, row_width(s, y, y, h, h), [&](auto t, auto v) {
     using T = decltype(t);
-    combine_kernel<T, v.value><<<token_grid(s.tokens, D.prof.sm_count), kThreads, 0, D.stream>>>(
-        (const T*)h, w, pos, (T*)y, s.tokens, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
+    constexpr int V = v.value, NV = V * sizeof(T) == 16 ? 1 : 4;
+    const Pieces q = pieces_of(s.tokens, s.d / V, NV);
+    combine_kernel<T, V, NV><<<(unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0, D.stream>>>(
+        (const T*)h, w, pos, (T*)y, q, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
     count_launch();
   });
   return finish(ctx, 0, true);
@@ -397,9 +513,15 @@ extern "C" int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpert
     const MapalExpertSite& s = *site;
     by_type(s, row_width(s, dy, dy, h, dh), [&](auto t, auto v) {
       using T = decltype(t);
-      const uint64_t slots = s.tokens * s.k;
-      combine_grad_kernel<T, v.value><<<token_grid(slots, D.prof.sm_count), kThreads, 0, D.stream>>>(
-          (const T*)h, w, pos, (const T*)dy, (T*)dh, dw, slots, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
+      constexpr int V = v.value;
+      const uint64_t wide = (s.d / V + 31) / 32 * 32;
+      const unsigned threads = wide < 32 ? 32 : wide < kThreads ? (unsigned)wide : kThreads;
+      // tokens that do not fill the device go slot by slot
+      const bool few = s.tokens < 8ull * D.prof.sm_count;
+      const uint64_t items = s.tokens * (few ? s.k : (s.k + kAtOnce - 1) / kAtOnce);
+      auto kernel = few ? combine_grad_kernel<T, V, 1> : combine_grad_kernel<T, V, kAtOnce>;
+      kernel<<<(unsigned)(items < kMostBlocks ? items : kMostBlocks), threads, 0, D.stream>>>(
+          (const T*)h, w, pos, (const T*)dy, (T*)dh, dw, items, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
       count_launch();
     });
     return finish(ctx, 0, true);
