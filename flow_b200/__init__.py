@@ -95,7 +95,8 @@ def _arr(ptrs: Sequence) -> ctypes.Array:
     return (ctypes.c_void_p * len(ptrs))(*[_ptr(p) for p in ptrs])
 
 
-_torch_types: dict[int, object] = {}  # MAPAL_DTYPE_* (and 4: int32) -> torch dtype, filled on first use
+_tensor = None  # torch.Tensor, and torch dtypes by MAPAL_DTYPE_* (4: int32), from the first tensor on
+_dtypes: list = [None] * 5
 
 
 def _span(rows: int, cols: int, ld: int) -> int:
@@ -103,20 +104,25 @@ def _span(rows: int, cols: int, ld: int) -> int:
     return (rows - 1) * ld + cols if rows and cols else 0
 
 
-def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0) -> int:
-    """Address of a device buffer of a row-wise operator: None (0), an int address taken as given, or a torch
-    tensor, which must be of the record's type, on the context's device, with `need` elements from its first."""
-    if t is None:
-        return 0
+def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0):
+    """Address of a device buffer of a row-wise operator: None, an int address taken as given, or a torch tensor,
+    which must be of the record's type, on the context's device, with `need` elements from its first."""
+    if (t.__class__ is _tensor and t.dtype is _dtypes[code] and t.get_device() == device and t.numel() >= need
+            and t.is_contiguous()):
+        return t.data_ptr()
+    return t if t is None else _buf_checked(t, code, need, device, what, ld)
+
+
+def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int) -> int:
+    global _tensor
     if isinstance(t, int):
         return t
-    if not _torch_types:
+    if _tensor is None:
         import torch
-        _torch_types.update({DTYPES[str(d).replace("torch.", "")]: d
-                             for d in (torch.float32, torch.float16, torch.bfloat16, torch.int8)})
-        _torch_types[4] = torch.int32
-    if t.dtype is not _torch_types.get(code):
-        raise ValueError(f"{what} is {t.dtype}, the record says {_torch_types.get(code)}")
+        _dtypes[:] = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.int32
+        _tensor = torch.Tensor
+    if not 0 <= code < len(_dtypes) or t.dtype is not _dtypes[code]:
+        raise ValueError(f"{what} is {t.dtype}, the record says {_dtypes[code] if 0 <= code < len(_dtypes) else code}")
     if t.get_device() != device:
         raise ValueError(f"{what} is on {t.device}, the context drives cuda:{device}")
     if not (t.is_contiguous() and t.numel() >= need):
@@ -335,8 +341,8 @@ class Context:
     def layer_norm(self, site: NormSite, x, w, b, y, mean=None, rstd=None) -> None:
         """y = (x - mean(x)) / sqrt(var(x) + eps) * w + b for each row; mean and rstd for the gradient."""
         dev, rows, d, t, ldx, ldy = self.devices[0], site.rows, site.d, site.dtype, site.ldx, site.ldy
-        _check(lib().mapal_gpu_layer_norm(
-            self._h, ctypes.byref(site), _buf(x, t, _span(rows, d, ldx), dev, "x", ldx),
+        _check(_native.load().mapal_gpu_layer_norm(
+            self._h, site, _buf(x, t, _span(rows, d, ldx), dev, "x", ldx),
             _buf(w, site.wtype, d, dev, "w"), _buf(b, site.wtype, d, dev, "b"),
             _buf(y, t, _span(rows, d, ldy), dev, "y", ldy), _buf(mean, 0, rows, dev, "mean"),
             _buf(rstd, 0, rows, dev, "rstd")))
@@ -344,7 +350,7 @@ class Context:
     def layer_norm_grad_workspace(self, site: NormSite) -> int:
         """Bytes of scratch that layer_norm_grad takes."""
         n = ctypes.c_uint64()
-        _check(lib().mapal_gpu_layer_norm_grad_workspace(self._h, ctypes.byref(site), ctypes.byref(n)))
+        _check(_native.load().mapal_gpu_layer_norm_grad_workspace(self._h, site, ctypes.byref(n)))
         return n.value
 
     def layer_norm_grad(self, site: NormSite, x, w, mean, rstd, dy, dx, dw, db, work) -> None:
@@ -353,8 +359,8 @@ class Context:
         dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
         if work is not None and work.get_device() != dev:
             raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
-        _check(lib().mapal_gpu_layer_norm_grad(
-            self._h, ctypes.byref(site), _buf(x, t, _span(rows, d, site.ldx), dev, "x", site.ldx),
+        _check(_native.load().mapal_gpu_layer_norm_grad(
+            self._h, site, _buf(x, t, _span(rows, d, site.ldx), dev, "x", site.ldx),
             _buf(w, site.wtype, d, dev, "w"), _buf(mean, 0, rows, dev, "mean"), _buf(rstd, 0, rows, dev, "rstd"),
             _buf(dy, t, _span(rows, d, site.lddy), dev, "dy", site.lddy),
             _buf(dx, t, _span(rows, d, site.lddx), dev, "dx", site.lddx), _buf(dw, 0, d, dev, "dw"),
@@ -365,16 +371,16 @@ class Context:
         """Slots sorted by expert, stably: offsets (experts + 1), order (place -> slot; may be None) and pos
         (slot -> place, -1 where ids is -1), all int32."""
         dev, n = self.devices[0], site.tokens * site.k
-        _check(lib().mapal_gpu_expert_sort(
-            self._h, ctypes.byref(site), _buf(ids, 4, n, dev, "ids"),
+        _check(_native.load().mapal_gpu_expert_sort(
+            self._h, site, _buf(ids, 4, n, dev, "ids"),
             _buf(offsets, 4, site.experts + 1, dev, "offsets"), _buf(order, 4, n, dev, "order"),
             _buf(pos, 4, n, dev, "pos")))
 
     def expert_dispatch(self, site: ExpertSite, x, pos, xs, scale=None, scale_out=None) -> None:
         """xs[pos[t, j]] = x[t], and scale_out likewise from scale (the scales of 8-bit rows)."""
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
-        _check(lib().mapal_gpu_expert_dispatch(
-            self._h, ctypes.byref(site), _buf(x, t, _span(tokens, d, site.ldt), dev, "x", site.ldt),
+        _check(_native.load().mapal_gpu_expert_dispatch(
+            self._h, site, _buf(x, t, _span(tokens, d, site.ldt), dev, "x", site.ldt),
             _buf(scale, 0, tokens, dev, "scale"), _buf(pos, 4, tokens * site.k, dev, "pos"),
             _buf(xs, t, _span(site.rows, d, site.ldr), dev, "xs", site.ldr),
             _buf(scale_out, 0, site.rows, dev, "scale_out")))
@@ -382,40 +388,40 @@ class Context:
     def expert_combine(self, site: ExpertSite, h, w, pos, y) -> None:
         """y[t] = sum over j of w[t, j] * h[pos[t, j]] (w None: 1)."""
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
-        _check(lib().mapal_gpu_expert_combine(
-            self._h, ctypes.byref(site), _buf(h, t, _span(site.rows, d, site.ldr), dev, "h", site.ldr),
+        _check(_native.load().mapal_gpu_expert_combine(
+            self._h, site, _buf(h, t, _span(site.rows, d, site.ldr), dev, "h", site.ldr),
             _buf(w, 0, tokens * site.k, dev, "w"), _buf(pos, 4, tokens * site.k, dev, "pos"),
             _buf(y, t, _span(tokens, d, site.ldt), dev, "y", site.ldt)))
 
     def expert_dispatch_grad(self, site: ExpertSite, dxs, pos, dx) -> None:
         """dx[t] = sum over j of dxs[pos[t, j]]."""
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
-        _check(lib().mapal_gpu_expert_dispatch_grad(
-            self._h, ctypes.byref(site), _buf(dxs, t, _span(site.rows, d, site.ldr), dev, "dxs", site.ldr),
+        _check(_native.load().mapal_gpu_expert_dispatch_grad(
+            self._h, site, _buf(dxs, t, _span(site.rows, d, site.ldr), dev, "dxs", site.ldr),
             _buf(pos, 4, tokens * site.k, dev, "pos"), _buf(dx, t, _span(tokens, d, site.ldt), dev, "dx", site.ldt)))
 
     def expert_combine_grad(self, site: ExpertSite, h, w, pos, dy, dh, dw) -> None:
         """dh[pos[t, j]] = w[t, j] * dy[t] and dw[t, j] = <dy[t], h[pos[t, j]]> (dw may be None)."""
         dev, t, d, tokens, n = self.devices[0], site.dtype, site.d, site.tokens, site.tokens * site.k
         sorted_span = _span(site.rows, d, site.ldr)
-        _check(lib().mapal_gpu_expert_combine_grad(
-            self._h, ctypes.byref(site), _buf(h, t, sorted_span, dev, "h", site.ldr), _buf(w, 0, n, dev, "w"),
+        _check(_native.load().mapal_gpu_expert_combine_grad(
+            self._h, site, _buf(h, t, sorted_span, dev, "h", site.ldr), _buf(w, 0, n, dev, "w"),
             _buf(pos, 4, n, dev, "pos"), _buf(dy, t, _span(tokens, d, site.ldt), dev, "dy", site.ldt),
             _buf(dh, t, sorted_span, dev, "dh", site.ldr), _buf(dw, 0, n, dev, "dw")))
 
     def quantize_rows_i8(self, site: QuantSite, x, q, scale) -> None:
         """scale = max|x|/127 and q = x/scale rounded to int8, for each row."""
         dev, rows, d = self.devices[0], site.rows, site.d
-        _check(lib().mapal_gpu_quantize_rows_i8(
-            self._h, ctypes.byref(site), _buf(x, site.dtype, _span(rows, d, site.ldx), dev, "x", site.ldx),
+        _check(_native.load().mapal_gpu_quantize_rows_i8(
+            self._h, site, _buf(x, site.dtype, _span(rows, d, site.ldx), dev, "x", site.ldx),
             _buf(q, 3, _span(rows, d, site.ldq), dev, "q", site.ldq), _buf(scale, 0, rows, dev, "scale")))
 
     def matmul_i8(self, site: I8Site, A, scale_a, B, scale_b, C, offsets=None) -> None:
         """C[i] = (A[i] . B[g]^T) * scale_a[i] * scale_b[g] with exact integer sums; rows offsets[g] to
         offsets[g + 1] belong to g (offsets None: one matrix for all rows)."""
         dev, m, n, k, groups, ldb = self.devices[0], site.m, site.n, site.k, site.groups, site.ldb
-        _check(lib().mapal_gpu_matmul_i8(
-            self._h, ctypes.byref(site), _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),
+        _check(_native.load().mapal_gpu_matmul_i8(
+            self._h, site, _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),
             _buf(scale_a, 0, m, dev, "scale_a"),
             _buf(B, 3, _span(groups, _span(n, k, ldb), site.ldg), dev, "B", ldb),
             _buf(scale_b, 0, groups * n, dev, "scale_b"), _buf(offsets, 4, groups + 1, dev, "offsets"),

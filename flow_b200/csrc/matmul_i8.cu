@@ -91,41 +91,23 @@ __global__ void __launch_bounds__(kThreads) mm_i8_tile_kernel(const MapalI8Site 
 // The product is taken as D = B*A^T: B's rows (channels) are the M dimension
 // of tcgen05.mma and A's rows (tokens) the N dimension, so that a tile may be
 // as narrow in tokens as there are tokens (16 at least) while the weights,
-// which a small batch spends its time reading, always fill the 128 lanes, and
-// so that neighbouring lanes hold neighbouring elements of a row of C.
+// which a small batch spends its time reading, always fill the lanes, and so
+// that neighbouring lanes hold neighbouring elements of a row of C.
 //
-// One CTA owns a tile of 128 channels and up to NT tokens of one group:
+// Both kernels have the same roles:
 //   warp 0     walks the tiles; one lane issues the TMA loads of each 128-byte
 //              block of k (128-byte swizzle) into a ring of STAGES stages. k's
 //              tail and channels beyond n read as zeros;
 //   warp 1     allocates TMEM (two accumulators, so the next tile's products
 //              run beside this tile's output) and issues kind::i8, K32, with N
-//              the tile's tokens rounded up to 16;
+//              the tile's tokens rounded up;
 //   warps 2-5  read the accumulator, scale and store C.
 // Tiles are numbered channel tiles first, then token tiles, then groups, and a
 // persistent grid takes every gridDim-th; each warp finds a tile's group by a
 // scan over the offsets, 32 groups at a time.
-//
-// With few tiles (a few tokens on one matrix) k is split over a cluster of
-// `split` CTAs: each leaves its integer partial sums in the shared memory of
-// the CTA that writes those tokens, which adds them up. Integer sums are exact
-// in any order, so the split does not change a bit.
 
-constexpr int kLanes = 128;           // channels of a CTA's tile
-constexpr int kBlockK = 128;          // bytes of k in a stage
-constexpr int kWTile = kLanes * kBlockK;
+constexpr int kBlockK = 128;  // bytes of k in a stage
 constexpr int kTcThreads = 192;
-
-template <int NT, int STAGES>
-struct TcSmem {
-  static constexpr int kStage = kWTile + NT * kBlockK;
-  uint8_t stage[STAGES][kStage];  // weights, then tokens; 1024-byte aligned for the swizzle
-  uint64_t full[STAGES], empty[STAGES];
-  uint64_t acc_full[2], acc_empty[2];
-  uint64_t parts, drained;
-  uint32_t tmem_base;
-  int abort;
-};
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: rows of 128
 // bytes, 8-row groups 1024 bytes apart, version 1 (sm_100), layout type 2.
@@ -138,12 +120,20 @@ __device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+template <int CTAS>
 __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
@@ -156,6 +146,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The address of another CTA's copy of a shared variable.
+__device__ __forceinline__ uint32_t remote(uint32_t local, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 struct Tile {
   uint32_t group, token0, tokens, channel0;
 };
@@ -165,9 +166,9 @@ struct TileWalk {
   const int32_t* offsets;
   uint32_t groups, m, nt, channels, channel_tiles;
   unsigned* trap;
-  uint32_t base = 0, before = 0;       // the chunk's first group, token tiles before it
-  uint32_t lo = 0, hi = 0, incl = 0;   // this lane's group: rows, token tiles up to and with it
-  uint32_t chunk = 0;                  // token tiles of the chunk
+  uint32_t base = 0, before = 0;      // the chunk's first group, token tiles before it
+  uint32_t lo = 0, hi = 0, incl = 0;  // this lane's group: rows, token tiles up to and with it
+  uint32_t chunk = 0;                 // token tiles of the chunk
 
   __device__ void load() {
     const uint32_t lane = threadIdx.x & 31, g = base + lane;
@@ -217,27 +218,92 @@ struct TcArgs {
   uint32_t m, n, k_blocks, groups, split;
 };
 
-// Writes one column (token) of a warp's 32 channels.
+// One token of a warp's 32 channels.
 template <typename T>
 __device__ __forceinline__ void put(const TcArgs& P, T* c, uint32_t token, uint32_t channel, int acc, float sb) {
   if (channel < P.n) c[(uint64_t)token * P.ldc + channel] = scaled<T>(acc, P.sa ? __ldg(P.sa + token) : 1.0f, sb);
 }
 
-template <typename T, int NT, int STAGES>
+// A warp's 32 lanes of the accumulator to C.
+template <typename T>
+__device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_t taddr, uint32_t channel, float sb) {
+  T* C = static_cast<T*>(P.C);
+  for (uint32_t j0 = 0; j0 < t.tokens; j0 += 16) {
+    int r[16];
+    tmem_ld16(taddr + j0, r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j0 + j < t.tokens) put<T>(P, C, t.token0 + j0 + j, channel, r[j], sb);
+  }
+}
+
+// ---- one CTA a tile ----------------------------------------------------------------
+//
+// Up to 128 tokens (NT) and CH channels. The MMA always has M = 128; with CH
+// below 128 the other rows of its operand are whatever shared memory holds and
+// their results are not read: a small batch is bound by reading the weights,
+// and narrower tiles spread them over more SMs.
+//
+// Where even that leaves SMs idle, k is split over a cluster of `split` CTAs:
+// each leaves its integer partial sums in the shared memory of the CTA that
+// writes those tokens, which adds them up. Integer sums are exact in any order,
+// so the split does not change a bit.
+
+// A stage holds KB blocks of k, so that one wait, one commit and one round of
+// the rings' bookkeeping (about 300 cycles in the loading lane, 140 of them a
+// wait that succeeds at once) serve KB*4 MMAs of 64 cycles each.
+template <int NT, int CH, int KB, int STAGES>
+struct TcSmem {
+  static constexpr int kWTile = CH * kBlockK, kXTile = NT * kBlockK;
+  static constexpr int kStage = KB * (kWTile + kXTile);
+  // KB blocks of weights, then of tokens; 1024-byte aligned for the swizzle.
+  // The MMA reads 128 rows of weights, in the last stage past its end.
+  uint8_t stage[STAGES][kStage];
+  uint8_t past[128 - CH > KB * NT ? (128 - CH - KB * NT) * kBlockK : 16];
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t parts, drained;
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <typename T, int NT, int CH, int KB, int STAGES>
 __global__ void __launch_bounds__(kTcThreads, 1)
     mm_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ TcArgs P) {
-  using Smem = TcSmem<NT, STAGES>;
+  using Smem = TcSmem<NT, CH, KB, STAGES>;
   constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  int* partial = reinterpret_cast<int*>(&sm + 1);  // split > 1: NT x 128 partial sums
+  int* partial = reinterpret_cast<int*>(&sm + 1);  // split > 1: NT x CH partial sums
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t split = P.split, rank = split > 1 ? blockIdx.x % split : 0;
   const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
   const uint32_t kb_lo = (uint32_t)((uint64_t)P.k_blocks * rank / split);
   const uint32_t kbs = (uint32_t)((uint64_t)P.k_blocks * (rank + 1) / split) - kb_lo;
+  volatile int* abort = &sm.abort;
 
+  TileWalk walk{P.offsets, P.groups, P.m, NT, CH, (P.n + CH - 1) / CH, P.trap};
+  walk.load();
+  Tile t;
+  bool more = walk.at(first, t);
+  uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
+
+  const uint32_t fills = (kbs + KB - 1) / KB;  // stages a tile takes
+  auto blocks_of = [&](uint32_t fill) { return min((uint32_t)KB, kbs - fill * KB); };
+  auto load = [&](uint32_t fill) {
+    const uint32_t s = it % STAGES, blocks = blocks_of(fill);
+    uint8_t* st = sm.stage[s];
+    mbar_expect_tx(&sm.full[s], blocks * (Smem::kWTile + Smem::kXTile));
+#pragma unroll
+    for (uint32_t u = 0; u < KB; ++u)
+      if (u < blocks) {
+        const int k0 = (int)(kb_lo + fill * KB + u) * kBlockK;
+        tma_load_3d(st + u * Smem::kWTile, &map_w, k0, (int)t.channel0, (int)t.group, &sm.full[s]);
+        tma_load_2d(st + KB * Smem::kWTile + u * Smem::kXTile, &map_x, k0, (int)t.token0, &sm.full[s]);
+      }
+    ++it;
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], 1);
@@ -247,11 +313,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.acc_full[b], 1);
       mbar_init(&sm.acc_empty[b], 4);
     }
-    mbar_init(&sm.parts, split * 128);
+    mbar_init(&sm.parts, split * CH);
     mbar_init(&sm.drained, 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // the first stages are on their way before the others have begun
+    if (more)
+      while (it < STAGES && it < fills) load(it);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
@@ -265,26 +334,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  volatile int* abort = &sm.abort;
 
-  TileWalk walk{P.offsets, P.groups, P.m, NT, kLanes, (P.n + kLanes - 1) / kLanes, P.trap};
-  walk.load();
-  Tile t;
-  uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
   if (warp == 0) {
     // ---- loads ----
-    for (uint64_t tile = first; walk.at(tile, t); tile += step) {
+    uint32_t fill = it;  // of the first tile, some are issued
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), fill = 0) {
       if (lane == 0)
-        for (uint32_t kb = 0; kb < kbs; ++kb, ++it) {
-          const uint32_t s = it % STAGES;
-          if (!mbar_wait(&sm.empty[s], ((it / STAGES) & 1) ^ 1, abort)) {
+        for (; fill < fills; ++fill) {
+          if (!mbar_wait(&sm.empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort)) {
             *abort = 1;
             break;
           }
-          mbar_expect_tx(&sm.full[s], Smem::kStage);
-          const int k0 = (int)(kb_lo + kb) * kBlockK;
-          tma_load_3d(sm.stage[s], &map_w, k0, (int)t.channel0, (int)t.group, &sm.full[s]);
-          tma_load_2d(sm.stage[s] + kWTile, &map_x, k0, (int)t.token0, &sm.full[s]);
+          load(fill);
         }
       __syncwarp();
       if (*abort) break;
@@ -292,23 +353,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == 1) {
     // ---- products ----
     uint32_t n = 0;
-    for (uint64_t tile = first; walk.at(tile, t); tile += step, ++n) {
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), ++n) {
       const uint32_t b = n & 1;
       if (lane == 0) {
-        const uint32_t idesc = idesc_i8(kLanes, (int)((t.tokens + 15) / 16 * 16));
+        const uint32_t idesc = idesc_i8(128, (int)((t.tokens + 15) / 16 * 16));
         if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (uint32_t kb = 0; kb < kbs && !*abort; ++kb, ++it) {
-          const uint32_t s = it % STAGES;
+        for (uint32_t fill = 0; fill < fills && !*abort; ++fill, ++it) {
+          const uint32_t s = it % STAGES, blocks = blocks_of(fill);
           if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, abort)) {
             *abort = 1;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + kWTile);
+          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + KB * Smem::kWTile);
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 32; ++kk)
-            mma_i8(tmem + b * NT, dw + kk * 2, dx + kk * 2, idesc, kb > 0 || kk > 0);
+          for (uint32_t u = 0; u < KB; ++u)
+            if (u < blocks) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < kBlockK / 32; ++kk)
+                mma_i8<1>(tmem + b * NT, dw + u * (Smem::kWTile >> 4) + kk * 2, dx + u * (Smem::kXTile >> 4) + kk * 2, idesc,
+                          fill > 0 || u > 0 || kk > 0);
+            }
           mma_commit(&sm.empty[s]);
         }
         mma_commit(&sm.acc_full[b]);
@@ -316,12 +382,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       if (*abort) break;
     }
-  } else {
+  } else if ((warp & 3) < CH / 32) {
     // ---- scales and output ----
-    T* C = static_cast<T*>(P.C);
     const int quarter = warp & 3;  // TMEM lanes 32*quarter to +31
     uint32_t n = 0;
-    for (uint64_t tile = first; walk.at(tile, t); tile += step, ++n) {
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), ++n) {
       const uint32_t b = n & 1;
       const uint32_t channel = t.channel0 + quarter * 32 + lane;
       const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
@@ -332,45 +397,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (*abort) break;  // the last commit of an aborted tile
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
-      constexpr int kTokens = NT < 16 ? NT : 16;
-      for (uint32_t j0 = 0; j0 < t.tokens; j0 += kTokens) {
-        int r[16];
-        tmem_ld16(col + j0, r);
-        if (split > 1) {
-          const uint32_t share = NT / split;
+      if (split == 1) {
+        put_tile<T>(P, t, col, channel, sb);
+      } else {
+        const uint32_t share = NT / split;
+        for (uint32_t j0 = 0; j0 < t.tokens; j0 += 16) {
+          int r[16];
+          tmem_ld16(col + j0, r);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const uint32_t at = ((rank * share + (j0 + j) % share) * kLanes + quarter * 32 + lane) * 4;
-            uint32_t to;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sa(partial) + at), "r"((j0 + j) / share));
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(r[j]) : "memory");
+            const uint32_t at = ((rank * share + (j0 + j) % share) * CH + quarter * 32 + lane) * 4;
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(sa(partial) + at, (j0 + j) / share)), "r"(r[j])
+                         : "memory");
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (j0 + j < t.tokens) put<T>(P, C, t.token0 + j0 + j, channel, r[j], sb);
         }
-      }
-      if (split > 1) {
-        for (uint32_t q = 0; q < split; ++q) {
-          uint32_t to;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sa(&sm.parts)), "r"(q));
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(to) : "memory");
-        }
+        for (uint32_t q = 0; q < split; ++q) arrive_remote(remote(sa(&sm.parts), q));
         if (!mbar_wait_cluster(&sm.parts, 0, abort)) {
           *abort = 1;
           break;
         }
-        const uint32_t share = NT / split;
         for (uint32_t j = 0; j < share && rank * share + j < t.tokens; ++j) {
           int acc = 0;
-          for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + j) * kLanes + quarter * 32 + lane];
-          put<T>(P, C, t.token0 + rank * share + j, channel, acc, sb);
+          for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + j) * CH + quarter * 32 + lane];
+          put<T>(P, static_cast<T*>(P.C), t.token0 + rank * share + j, channel, acc, sb);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+      if (lane == 0) {
+        mbar_arrive(&sm.acc_empty[b]);
+        // warps without channels arrive through the first
+        if (CH < 128 && quarter == 0)
+          for (int q = CH / 32; q < 4; ++q) mbar_arrive(&sm.acc_empty[b]);
+      }
     }
   }
 
@@ -398,6 +457,187 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
+// ---- a pair of CTAs a tile ---------------------------------------------------------
+//
+// 256 channels and up to 256 tokens: each CTA of the pair loads its 128 channels
+// and half of the tokens, and the pair's MMA (cta_group::2, issued by the first
+// CTA) reads both halves from both, so a CTA moves 32 KB a block of k where a
+// 128 x 256 tile of its own moves 48. Large products of single CTAs are bound by
+// that traffic from L2 (about 11.6 TB/s; 8192^3: 0.54 ms).
+
+constexpr int kPairStages = 3, kPairKB = 2;
+struct PairSmem {
+  static constexpr int kHalf = 128 * kBlockK;  // of channels, and of tokens
+  uint8_t stage[kPairStages][kPairKB * 2 * kHalf];
+  uint64_t full[kPairStages];   // the first CTA's: both CTAs' loads have landed
+  uint64_t empty[kPairStages];  // each CTA's own
+  uint64_t acc_full[2];         // each CTA's own
+  uint64_t acc_empty[2];        // the first CTA's: both CTAs have read the accumulator
+  uint64_t drained;
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {  // in both CTAs
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(sa(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+    mm_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                      const __grid_constant__ TcArgs P) {
+  constexpr int NT = 256;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = blockIdx.x & 1;
+  const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  volatile int* abort = &sm.abort;
+
+  TileWalk walk{P.offsets, P.groups, P.m, NT, 256, (P.n + 255) / 256, P.trap};
+  walk.load();
+  Tile t;
+  bool more = walk.at(first, t);
+  uint32_t it = 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 8);
+    }
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cg::this_cluster().sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t)) {
+      const int half = (int)((t.tokens + 31) / 32 * 16);  // tokens of each CTA
+      if (lane == 0)
+        for (uint32_t kb = 0; kb < P.k_blocks; kb += kPairKB, ++it) {
+          const uint32_t s = it % kPairStages, blocks = min((uint32_t)kPairKB, P.k_blocks - kb);
+          if (!mbar_wait(&sm.empty[s], ((it / kPairStages) & 1) ^ 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(&sm.full[s], blocks * 4 * PairSmem::kHalf);
+          const uint32_t bar = remote(sa(&sm.full[s]), 0);
+#pragma unroll
+          for (uint32_t u = 0; u < kPairKB; ++u)
+            if (u < blocks) {
+              const int k0 = (int)(kb + u) * kBlockK;
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+                  "{%2, %3, %4}], [%5];" ::"r"(sa(sm.stage[s] + 2 * u * PairSmem::kHalf)),
+                  "l"(&map_w), "r"(k0), "r"((int)(t.channel0 + rank * 128)), "r"((int)t.group), "r"(bar)
+                  : "memory");
+              asm volatile(
+                  "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+                  "{%2, %3}], [%4];" ::"r"(sa(sm.stage[s] + (2 * u + 1) * PairSmem::kHalf)),
+                  "l"(&map_x), "r"(k0), "r"((int)t.token0 + (int)rank * half), "r"(bar)
+                  : "memory");
+            }
+        }
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else if (warp == 1) {
+    // ---- products, by the first CTA ----
+    uint32_t n = 0;
+    for (uint64_t tile = first; rank == 0 && more; tile += step, more = walk.at(tile, t), ++n) {
+      const uint32_t b = n & 1;
+      if (lane == 0) {
+        const uint32_t idesc = idesc_i8(256, (int)((t.tokens + 31) / 32 * 32));
+        if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (uint32_t kb = 0; kb < P.k_blocks && !*abort; kb += kPairKB, ++it) {
+          const uint32_t s = it % kPairStages, blocks = min((uint32_t)kPairKB, P.k_blocks - kb);
+          if (!mbar_wait(&sm.full[s], (it / kPairStages) & 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + PairSmem::kHalf);
+#pragma unroll
+          for (uint32_t u = 0; u < kPairKB; ++u)
+            if (u < blocks) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < kBlockK / 32; ++kk)
+                mma_i8<2>(tmem + b * NT, dw + u * (2 * PairSmem::kHalf >> 4) + kk * 2,
+                          dx + u * (2 * PairSmem::kHalf >> 4) + kk * 2, idesc, kb > 0 || u > 0 || kk > 0);
+            }
+          pair_commit(&sm.empty[s]);
+        }
+        pair_commit(&sm.acc_full[b]);
+      }
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else {
+    // ---- scales and output ----
+    const int quarter = warp & 3;
+    uint32_t n = 0;
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), ++n) {
+      const uint32_t b = n & 1;
+      const uint32_t channel = t.channel0 + rank * 128 + quarter * 32 + lane;
+      const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
+      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+        *abort = 1;
+        break;
+      }
+      if (*abort) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_remote(remote(sa(&sm.acc_empty[b]), 0));
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cg::this_cluster().sync();
+  // A wait gave up in either CTA (its flag is read after both have stopped):
+  // what is still in flight ends before shared memory and TMEM are given back.
+  const bool stop = *abort || *(volatile int*)cg::this_cluster().map_shared_rank(&sm.abort, rank ^ 1);
+  if (stop) {
+    if (warp == 0 && lane == 0) {
+      atomicOr(P.trap, kDeviceTimeout);
+      if (rank == 0)
+        for (uint32_t i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
+          mbar_wait(&sm.full[i % kPairStages], (i / kPairStages) & 1, nullptr);
+    }
+    if (warp == 1 && lane == 0 && rank == 0) {
+      pair_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, nullptr);
+    }
+  }
+  __syncwarp();
+  cg::this_cluster().sync();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------
+
 // rows x k bytes (x matrices) in boxes of 128 bytes x box_rows.
 int make_map(CUtensorMap* map, const int8_t* base, uint64_t k, uint64_t rows, uint64_t ld, uint64_t mats, uint64_t ldm,
              int dims, uint32_t box_rows) {
@@ -407,7 +647,6 @@ int make_map(CUtensorMap* map, const int8_t* base, uint64_t k, uint64_t rows, ui
   // a stride that no access uses (one row, one matrix) may be anything: any valid one stands in
   cuuint64_t dim[3] = {k, rows, mats};
   cuuint64_t stride[2] = {rows > 1 ? ld : k16, mats > 1 ? ldm : (rows > 1 ? ld : k16) * rows};
-  if (mats <= 1) stride[1] = (stride[1] + 15) & ~15ull;
   cuuint32_t box[3] = {kBlockK, box_rows, 1}, one[3] = {1, 1, 1};
   const CUresult r =
       fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, (void*)base, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -425,21 +664,59 @@ bool tma_reads(const MapalI8Site& s, const int8_t* A, const int8_t* B) {
   return s.k > 0 && a && b && s.n * (s.n == 1 ? s.k : s.ldb) < lim;
 }
 
-template <typename T, int NT, int STAGES>
-int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, TcArgs P, uint64_t tiles) {
+// A way to cut the product: channels and tokens of a tile, parts of k; pairs
+// of CTAs have 256 channels.
+struct Cut {
+  uint32_t channels, tokens, split;
+};
+
+// Tiles of a cut: at most one part-filled token tile for each group with rows
+// (the offsets are on the device).
+uint64_t tiles_of(const MapalI8Site& s, bool grouped, const Cut& c) {
+  const uint64_t with_rows = s.groups < s.m ? s.groups : s.m;
+  const uint64_t token_tiles = grouped ? s.m / c.tokens + with_rows : (s.m + c.tokens - 1) / c.tokens;
+  return token_tiles * ((s.n + c.channels - 1) / c.channels);
+}
+
+// Cycles of a cut, from what bounds its tiles: the MMA (N/2 cycles for 128
+// channels and 32 bytes of k, 64 at least), and the loads, at up to 64 bytes a
+// cycle for an SM and 6200 for all. Tiles run in waves, each with a start and
+// an end that nothing overlaps when it is the only one.
+double cycles_of(const MapalI8Site& s, bool grouped, const Cut& c, int sms) {
+  const bool pair = c.channels == 256;
+  const double tiles = (double)tiles_of(s, grouped, c) * c.split, at_once = pair ? sms / 2 : sms;
+  const double active = tiles < at_once ? tiles : at_once, ctas = pair ? 2 * active : active;
+  const double k_blocks = (double)((s.k + kBlockK - 1) / kBlockK) / c.split;
+  const double rate = 6200.0 / ctas < 64.0 ? 6200.0 / ctas : 64.0;
+  const double load = (pair ? 256 : c.channels + c.tokens) * (double)kBlockK / rate;
+  const double tokens = s.m < c.tokens ? (double)((s.m + 15) / 16 * 16) : c.tokens;
+  const double mma = 4 * (tokens / 2 > 64 ? tokens / 2 : 64);
+  const double waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
+  return waves * (k_blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
+}
+
+int launch_maps(const MapalI8Site& s, const int8_t* A, const int8_t* B, uint32_t channels, uint32_t tokens,
+                CUtensorMap* mw, CUtensorMap* mx) {
+  MAPAL_TRY(make_map(mw, B, s.k, s.n, s.ldb, s.groups, s.ldg, 3, channels));
+  return make_map(mx, A, s.k, s.m, s.lda, 1, 0, 2, tokens);
+}
+
+template <typename T, int NT, int CH, int KB, int STAGES>
+int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, const TcArgs& P,
+              uint64_t tiles) {
+  using Smem = TcSmem<NT, CH, KB, STAGES>;
   CUtensorMap mw, mx;
-  MAPAL_TRY(make_map(&mw, B, s.k, s.n, s.ldb, s.groups, s.ldg, 3, kLanes));
-  MAPAL_TRY(make_map(&mx, A, s.k, s.m, s.lda, 1, 0, 2, NT));
-  const size_t most = sizeof(TcSmem<NT, STAGES>) + 1024 + (NT <= 64 ? NT * kLanes * 4 : 0);
-  const size_t smem = sizeof(TcSmem<NT, STAGES>) + 1024 + (P.split > 1 ? NT * kLanes * 4 : 0);
+  MAPAL_TRY(launch_maps(s, A, B, CH, NT, &mw, &mx));
+  constexpr size_t most = sizeof(Smem) + 1024 + (NT <= 64 ? NT * CH * 4 : 0);
+  static_assert(most <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
-  auto kernel = mm_i8_tc_kernel<T, NT, STAGES>;
+  auto kernel = mm_i8_tc_kernel<T, NT, CH, KB, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "matmul_i8 shared memory"));
   const uint64_t cap = P.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * P.split));
   cfg.blockDim = dim3(kTcThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(Smem) + 1024 + (P.split > 1 ? NT * CH * 4 : 0);
   cfg.stream = D.stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -448,6 +725,21 @@ int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const 
   cfg.attrs = at;
   cfg.numAttrs = P.split > 1 ? 1 : 0;
   MAPAL_CUDA(cudaLaunchKernelEx(&cfg, kernel, mw, mx, P));
+  count_launch();
+  return 0;
+}
+
+template <typename T>
+int launch_pair(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, const TcArgs& P,
+                uint64_t tiles) {
+  CUtensorMap mw, mx;
+  MAPAL_TRY(launch_maps(s, A, B, 128, 128, &mw, &mx));
+  constexpr size_t smem = sizeof(PairSmem) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  static std::atomic<uint64_t> done{0};
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)mm_i8_pair_kernel<T>, D.device, smem, "matmul_i8 shared memory"));
+  const uint64_t cap = D.prof.sm_count / 2;
+  mm_i8_pair_kernel<T><<<(unsigned)((tiles < cap ? tiles : cap) * 2), kTcThreads, smem, D.stream>>>(mw, mx, P);
   count_launch();
   return 0;
 }
@@ -466,19 +758,35 @@ int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const flo
   P.n = (uint32_t)s.n;
   P.groups = s.groups;
   P.k_blocks = (uint32_t)((s.k + kBlockK - 1) / kBlockK);
-  P.split = 1;
-  const uint64_t nt = s.m <= 16ull * s.groups ? 16 : s.m <= 32ull * s.groups ? 32 : s.m <= 64ull * s.groups ? 64 : s.m <= 128ull * s.groups ? 128 : 256;
-  // an upper bound of the tiles: every group with rows has at most one part-filled token tile
-  const uint64_t token_tiles = s.m / nt + (s.groups < s.m ? s.groups : s.m);
-  const uint64_t tiles = (offsets ? token_tiles : (s.m + nt - 1) / nt) * ((s.n + kLanes - 1) / kLanes);
-  if (nt <= 64)
-    while (P.split < 8 && tiles * P.split * 2 <= (uint64_t)D.prof.sm_count && P.split * 4 <= P.k_blocks) P.split *= 2;
-  switch (nt) {
-    case 16: return launch_tc<T, 16, 8>(D, s, A, B, P, tiles);
-    case 32: return launch_tc<T, 32, 8>(D, s, A, B, P, tiles);
-    case 64: return launch_tc<T, 64, 7>(D, s, A, B, P, tiles);
-    case 128: return launch_tc<T, 128, 6>(D, s, A, B, P, tiles);
-    default: return launch_tc<T, 256, 4>(D, s, A, B, P, tiles);
+
+  static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
+                                  {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
+  Cut best{};
+  double least = 0;
+  for (Cut c : kCuts)
+    for (c.split = 1; c.split <= 8; c.split *= 2) {
+      if (c.split > 1 && (c.tokens > 64 || c.split * 4 > P.k_blocks ||
+                          tiles_of(s, offsets, c) * c.split > (uint64_t)D.prof.sm_count))
+        break;
+      const double cy = cycles_of(s, offsets, c, D.prof.sm_count);
+      if (best.channels == 0 || cy < least) {
+        best = c;
+        least = cy;
+      }
+    }
+  P.split = best.split;
+  const uint64_t tiles = tiles_of(s, offsets, best);
+  switch (best.channels * 1000 + best.tokens) {
+    case 256256: return launch_pair<T>(D, s, A, B, P, tiles);
+    case 128128: return launch_tc<T, 128, 128, 2, 3>(D, s, A, B, P, tiles);
+    case 64128: return launch_tc<T, 128, 64, 2, 4>(D, s, A, B, P, tiles);
+    case 128064: return launch_tc<T, 64, 128, 2, 4>(D, s, A, B, P, tiles);
+    case 64064: return launch_tc<T, 64, 64, 2, 6>(D, s, A, B, P, tiles);
+    case 128032: return launch_tc<T, 32, 128, 2, 5>(D, s, A, B, P, tiles);
+    case 64032: return launch_tc<T, 32, 64, 4, 4>(D, s, A, B, P, tiles);
+    case 128016: return launch_tc<T, 16, 128, 2, 5>(D, s, A, B, P, tiles);
+    case 64016: return launch_tc<T, 16, 64, 4, 5>(D, s, A, B, P, tiles);
+    default: return launch_tc<T, 16, 32, 4, 8>(D, s, A, B, P, tiles);
   }
 }
 
