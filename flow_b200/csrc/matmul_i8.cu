@@ -218,22 +218,25 @@ struct TcArgs {
   uint32_t m, n, k_blocks, groups, split;
 };
 
-// One token of a warp's 32 channels.
-template <typename T>
-__device__ __forceinline__ void put(const TcArgs& P, T* c, uint32_t token, uint32_t channel, int acc, float sb) {
-  if (channel < P.n) c[(uint64_t)token * P.ldc + channel] = scaled<T>(acc, P.sa ? __ldg(P.sa + token) : 1.0f, sb);
-}
-
-// A warp's 32 lanes of the accumulator to C.
+// A warp's 32 lanes of the accumulator, 16 tokens at a time, to C. The tokens'
+// scales are read 32 at once and handed round by shuffles: a load for each
+// token would wait its turn behind the stores before it (90 ns a token).
 template <typename T>
 __device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_t taddr, uint32_t channel, float sb) {
-  T* C = static_cast<T*>(P.C);
+  const uint32_t lane = threadIdx.x & 31;
+  const bool in = channel < P.n;
+  T* c = static_cast<T*>(P.C) + (uint64_t)t.token0 * P.ldc + (in ? channel : 0);
+  float sv = 1.0f;
   for (uint32_t j0 = 0; j0 < t.tokens; j0 += 16) {
     int r[16];
     tmem_ld16(taddr + j0, r);
+    if (P.sa && j0 % 32 == 0) sv = j0 + lane < t.tokens ? __ldg(P.sa + t.token0 + j0 + lane) : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j0 + j < t.tokens) put<T>(P, C, t.token0 + j0 + j, channel, r[j], sb);
+    for (int j = 0; j < 16; ++j) {
+      const float s = __shfl_sync(0xffffffffu, sv, j0 % 32 + j);
+      if (in && j0 + j < t.tokens) *c = scaled<T>(r[j], s, sb);
+      c += P.ldc;
+    }
   }
 }
 
@@ -401,13 +404,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         put_tile<T>(P, t, col, channel, sb);
       } else {
         const uint32_t share = NT / split;
-        for (uint32_t j0 = 0; j0 < t.tokens; j0 += 16) {
+        for (uint32_t k0 = 0; k0 < t.tokens; k0 += 16) {
           int r[16];
-          tmem_ld16(col + j0, r);
+          tmem_ld16(col + k0, r);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const uint32_t at = ((rank * share + (j0 + j) % share) * CH + quarter * 32 + lane) * 4;
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(sa(partial) + at, (j0 + j) / share)), "r"(r[j])
+            const uint32_t at = ((rank * share + (k0 + j) % share) * CH + quarter * 32 + lane) * 4;
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(sa(partial) + at, (k0 + j) / share)), "r"(r[j])
                          : "memory");
           }
         }
@@ -416,10 +419,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           *abort = 1;
           break;
         }
-        for (uint32_t j = 0; j < share && rank * share + j < t.tokens; ++j) {
+        // at most 32 tokens a CTA: split is 2 or more and NT at most 64
+        const uint32_t j0 = rank * share;
+        const float sv = P.sa && lane < share && j0 + lane < t.tokens ? __ldg(P.sa + t.token0 + j0 + lane) : 1.0f;
+        T* c = static_cast<T*>(P.C) + (uint64_t)(t.token0 + j0) * P.ldc + channel;
+        for (uint32_t j = 0; j < share && j0 + j < t.tokens; ++j, c += P.ldc) {
           int acc = 0;
           for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + j) * CH + quarter * 32 + lane];
-          put<T>(P, static_cast<T*>(P.C), t.token0 + rank * share + j, channel, acc, sb);
+          const float s = __shfl_sync(0xffffffffu, sv, j);
+          if (channel < P.n) *c = scaled<T>(acc, s, sb);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
