@@ -8,6 +8,7 @@
 // one conversion and two multiplications, each rounded to f32.
 #include <cooperative_groups.h>
 
+#include "f32x2.cuh"
 #include "rows.cuh"
 #include "tcgen05.cuh"
 
@@ -101,13 +102,17 @@ __global__ void __launch_bounds__(kThreads) mm_i8_tile_kernel(const MapalI8Site 
 //   warp 1     allocates TMEM (two accumulators, so the next tile's products
 //              run beside this tile's output) and issues kind::i8, K32, with N
 //              the tile's tokens rounded up;
-//   warps 2-5  read the accumulator, scale and store C.
+//   the others read the accumulator, scale and store C.
 // Tiles are numbered channel tiles first, then token tiles, then groups, and a
 // persistent grid takes every gridDim-th; each warp finds a tile's group by a
 // scan over the offsets, 32 groups at a time.
 
 constexpr int kBlockK = 128;  // bytes of k in a stage
-constexpr int kTcThreads = 192;
+constexpr int kHalfTokens = 128;  // that one warp writes of a tile
+
+// Warps that write a tile of NT tokens, four (one for each quarter of the
+// lanes) for every 128 tokens.
+__host__ __device__ constexpr int out_warps(int nt) { return nt > kHalfTokens / 2 ? 8 : 4; }
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: rows of 128
 // bytes, 8-row groups 1024 bytes apart, version 1 (sm_100), layout type 2.
@@ -218,24 +223,48 @@ struct TcArgs {
   uint32_t m, n, k_blocks, groups, split;
 };
 
-// A warp's 32 lanes of the accumulator, 16 tokens at a time, to C. The tokens'
-// scales are read 32 at once and handed round by shuffles: a load for each
-// token would wait its turn behind the stores before it (90 ns a token).
+// Tokens [from, to) of a warp's 32 lanes of the accumulator, 16 at a time, to C.
+// The tokens' scales are read first, into shared memory of the warp's own
+// (`scales`): a load for each token would wait its turn behind the stores
+// before it, 90 ns a token. A warp is alone with its latencies here, so the
+// instructions a token are kept few: products on pairs of tokens, one
+// conversion for two.
 template <typename T>
-__device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_t taddr, uint32_t channel, float sb) {
+__device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_t taddr, uint32_t channel, float sb,
+                                         uint32_t from, uint32_t to, float* scales) {
   const uint32_t lane = threadIdx.x & 31;
   const bool in = channel < P.n;
-  T* c = static_cast<T*>(P.C) + (uint64_t)t.token0 * P.ldc + (in ? channel : 0);
-  float sv = 1.0f;
-  for (uint32_t j0 = 0; j0 < t.tokens; j0 += 16) {
+  to = min(to, t.tokens);
+  if (from >= to) return;
+  __syncwarp();
+  for (uint32_t j = from + lane; j < to; j += 32) scales[j - from] = P.sa ? __ldg(P.sa + t.token0 + j) : 1.0f;
+  __syncwarp();
+  T* c = static_cast<T*>(P.C) + (uint64_t)(t.token0 + from) * P.ldc + (in ? channel : 0);
+  const f2 sb2 = f2_splat(sb);
+  for (uint32_t j0 = from; j0 < to; j0 += 16, scales += 16) {
     int r[16];
     tmem_ld16(taddr + j0, r);
-    if (P.sa && j0 % 32 == 0) sv = j0 + lane < t.tokens ? __ldg(P.sa + t.token0 + j0 + lane) : 1.0f;
+    if (j0 + 16 <= to && in) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float s = __shfl_sync(0xffffffffu, sv, j0 % 32 + j);
-      if (in && j0 + j < t.tokens) *c = scaled<T>(r[j], s, sb);
-      c += P.ldc;
+      for (int j = 0; j < 16; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(scales + j);
+        const f2 v0 = f2_mul(f2_mul(f2_pack(__int2float_rn(r[j]), __int2float_rn(r[j + 1])), f2_pack(s.x, s.y)), sb2);
+        const f2 v1 = f2_mul(f2_mul(f2_pack(__int2float_rn(r[j + 2]), __int2float_rn(r[j + 3])), f2_pack(s.z, s.w)), sb2);
+        const float v[4] = {f2_lo(v0), f2_hi(v0), f2_lo(v1), f2_hi(v1)};
+        Pack<T, 4> o;
+        o.set(v);
+        T w[4];
+        memcpy(w, o.w, sizeof(w));
+        c[0] = w[0];
+        c[P.ldc] = w[1];
+        c[2 * P.ldc] = w[2];
+        c[3 * P.ldc] = w[3];
+        c += 4 * P.ldc;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j, c += P.ldc)
+        if (in && j0 + j < to) *c = scaled<T>(r[j], scales[j], sb);
     }
   }
 }
@@ -266,16 +295,18 @@ struct TcSmem {
   uint64_t full[STAGES], empty[STAGES];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t parts, drained;
+  alignas(16) float scales[out_warps(NT)][kHalfTokens];
   uint32_t tmem_base;
   int abort;
 };
 
 template <typename T, int NT, int CH, int KB, int STAGES>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     mm_i8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ TcArgs P) {
   using Smem = TcSmem<NT, CH, KB, STAGES>;
   constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+  constexpr int kOut = out_warps(NT);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   int* partial = reinterpret_cast<int*>(&sm + 1);  // split > 1: NT x CH partial sums
@@ -314,7 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
-      mbar_init(&sm.acc_empty[b], 4);
+      mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
     }
     mbar_init(&sm.parts, split * CH);
     mbar_init(&sm.drained, 1);
@@ -401,7 +432,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
       if (split == 1) {
-        put_tile<T>(P, t, col, channel, sb);
+        const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
+        put_tile<T>(P, t, col, channel, sb, from, from + NT / (kOut / 4), sm.scales[warp - 2]);
       } else {
         const uint32_t share = NT / split;
         for (uint32_t k0 = 0; k0 < t.tokens; k0 += 16) {
@@ -432,12 +464,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.acc_empty[b]);
-        // warps without channels arrive through the first
-        if (CH < 128 && quarter == 0)
-          for (int q = CH / 32; q < 4; ++q) mbar_arrive(&sm.acc_empty[b]);
-      }
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
     }
   }
 
@@ -482,6 +509,7 @@ struct PairSmem {
   uint64_t acc_full[2];         // each CTA's own
   uint64_t acc_empty[2];        // the first CTA's: both CTAs have read the accumulator
   uint64_t drained;
+  alignas(16) float scales[out_warps(256)][kHalfTokens];
   uint32_t tmem_base;
   int abort;
 };
@@ -494,7 +522,7 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {  // in both CTAs
 }
 
 template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(256), 1)
     mm_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                       const __grid_constant__ TcArgs P) {
   constexpr int NT = 256;
@@ -518,7 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
-      mbar_init(&sm.acc_empty[b], 8);
+      mbar_init(&sm.acc_empty[b], 2 * out_warps(256));
     }
     mbar_init(&sm.drained, 1);
     sm.abort = 0;
@@ -612,7 +640,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       }
       if (*abort) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb);
+      const uint32_t from = (warp - 2) / 4 * kHalfTokens;
+      put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb, from, from + kHalfTokens,
+                  sm.scales[warp - 2]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive_remote(remote(sa(&sm.acc_empty[b]), 0));
@@ -723,7 +753,7 @@ int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const 
   const uint64_t cap = P.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * P.split));
-  cfg.blockDim = dim3(kTcThreads);
+  cfg.blockDim = dim3(64 + 32 * out_warps(NT));
   cfg.dynamicSmemBytes = sizeof(Smem) + 1024 + (P.split > 1 ? NT * CH * 4 : 0);
   cfg.stream = D.stream;
   cudaLaunchAttribute at[1];
@@ -747,7 +777,7 @@ int launch_pair(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, cons
   static std::atomic<uint64_t> done{0};
   MAPAL_TRY(ensure_smem_attr(done, (const void*)mm_i8_pair_kernel<T>, D.device, smem, "matmul_i8 shared memory"));
   const uint64_t cap = D.prof.sm_count / 2;
-  mm_i8_pair_kernel<T><<<(unsigned)((tiles < cap ? tiles : cap) * 2), kTcThreads, smem, D.stream>>>(mw, mx, P);
+  mm_i8_pair_kernel<T><<<(unsigned)((tiles < cap ? tiles : cap) * 2), 64 + 32 * out_warps(256), smem, D.stream>>>(mw, mx, P);
   count_launch();
   return 0;
 }
@@ -788,7 +818,7 @@ int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const flo
     case 256256: return launch_pair<T>(D, s, A, B, P, tiles);
     case 128128: return launch_tc<T, 128, 128, 2, 3>(D, s, A, B, P, tiles);
     case 64128: return launch_tc<T, 128, 64, 2, 4>(D, s, A, B, P, tiles);
-    case 128064: return launch_tc<T, 64, 128, 2, 4>(D, s, A, B, P, tiles);
+    case 128064: return launch_tc<T, 64, 128, 2, 3>(D, s, A, B, P, tiles);
     case 64064: return launch_tc<T, 64, 64, 2, 6>(D, s, A, B, P, tiles);
     case 128032: return launch_tc<T, 32, 128, 2, 5>(D, s, A, B, P, tiles);
     case 64032: return launch_tc<T, 32, 64, 4, 4>(D, s, A, B, P, tiles);
