@@ -115,9 +115,10 @@ constexpr int kHalfTokens = 128;  // that one warp writes of a tile
 __host__ __device__ constexpr int out_warps(int nt) { return nt > kHalfTokens / 2 ? 8 : 4; }
 
 // Shared-memory matrix descriptor, K-major, 128-byte swizzle: rows of 128
-// bytes, 8-row groups 1024 bytes apart, version 1 (sm_100), layout type 2.
-__device__ __forceinline__ uint64_t desc128(const void* p) {
-  return (uint64_t)((sa(p) & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// bytes, 8-row groups `group_bytes` apart, version 1 (sm_100), layout type 2.
+__device__ __forceinline__ uint64_t desc128(const void* p, uint32_t group_bytes = 1024) {
+  return (uint64_t)((sa(p) & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(group_bytes >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
 }
 
 // D 32-bit integers, A and B signed 8-bit, both K-major.
@@ -221,24 +222,28 @@ struct TcArgs {
   unsigned* trap;
   uint64_t ldc;
   uint32_t m, n, k_blocks, groups, split;
+  uint32_t folded;  // the weights' map brings a whole stage at once (single CTAs)
 };
 
+// The scales of tokens [from, to), into shared memory of the warp's own, before
+// the accumulator is ready: a load for each token in put_tile would wait its
+// turn behind the stores before it, 90 ns a token.
+__device__ __forceinline__ void take_scales(const TcArgs& P, const Tile& t, uint32_t from, uint32_t to, float* scales) {
+  to = min(to, t.tokens);
+  __syncwarp();
+  for (uint32_t j = from + (threadIdx.x & 31); j < to; j += 32)
+    scales[j - from] = P.sa ? __ldg(P.sa + t.token0 + j) : 1.0f;
+  __syncwarp();
+}
+
 // Tokens [from, to) of a warp's 32 lanes of the accumulator, 16 at a time, to C.
-// The tokens' scales are read first, into shared memory of the warp's own
-// (`scales`): a load for each token would wait its turn behind the stores
-// before it, 90 ns a token. A warp is alone with its latencies here, so the
-// instructions a token are kept few: products on pairs of tokens, one
-// conversion for two.
+// A warp is alone with its latencies here, so the instructions a token are kept
+// few: products on pairs of tokens, one conversion for two.
 template <typename T>
 __device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_t taddr, uint32_t channel, float sb,
-                                         uint32_t from, uint32_t to, float* scales) {
-  const uint32_t lane = threadIdx.x & 31;
+                                         uint32_t from, uint32_t to, const float* scales) {
   const bool in = channel < P.n;
   to = min(to, t.tokens);
-  if (from >= to) return;
-  __syncwarp();
-  for (uint32_t j = from + lane; j < to; j += 32) scales[j - from] = P.sa ? __ldg(P.sa + t.token0 + j) : 1.0f;
-  __syncwarp();
   T* c = static_cast<T*>(P.C) + (uint64_t)(t.token0 + from) * P.ldc + (in ? channel : 0);
   const f2 sb2 = f2_splat(sb);
   for (uint32_t j0 = from; j0 < to; j0 += 16, scales += 16) {
@@ -281,6 +286,12 @@ __device__ __forceinline__ void put_tile(const TcArgs& P, const Tile& t, uint32_
 // writes those tokens, which adds them up. Integer sums are exact in any order,
 // so the split does not change a bit.
 
+// Weights come with one load a stage where k and n allow it (multiples of 128
+// and 8): the map splits k into blocks and channels into eights, so that a
+// stage lies as [eight][block][8 rows][128 bytes] and each row is read 512
+// bytes at a time, which HBM likes better than four visits of 128 (128 CTAs
+// streaming 64 rows of 4096 bytes each: 6.6 against 7.9 us).
+//
 // A stage holds KB blocks of k, so that one wait, one commit and one round of
 // the rings' bookkeeping (about 300 cycles in the loading lane, 140 of them a
 // wait that succeeds at once) serve KB*4 MMAs of 64 cycles each.
@@ -291,7 +302,7 @@ struct TcSmem {
   // KB blocks of weights, then of tokens; 1024-byte aligned for the swizzle.
   // The MMA reads 128 rows of weights, in the last stage past its end.
   uint8_t stage[STAGES][kStage];
-  uint8_t past[128 - CH > KB * NT ? (128 - CH - KB * NT) * kBlockK : 16];
+  uint8_t past[128 - CH > NT ? KB * (128 - CH - NT) * kBlockK : 16];
   uint64_t full[STAGES], empty[STAGES];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t parts, drained;
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   int* partial = reinterpret_cast<int*>(&sm + 1);  // split > 1: NT x CH partial sums
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t split = P.split, rank = split > 1 ? blockIdx.x % split : 0;
   const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
   const uint32_t kb_lo = (uint32_t)((uint64_t)P.k_blocks * rank / split);
@@ -328,17 +339,20 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   auto load = [&](uint32_t fill) {
     const uint32_t s = it % STAGES, blocks = blocks_of(fill);
     uint8_t* st = sm.stage[s];
-    mbar_expect_tx(&sm.full[s], blocks * (Smem::kWTile + Smem::kXTile));
+    const bool folded = KB > 1 && P.folded;
+    mbar_expect_tx(&sm.full[s], (folded ? KB : blocks) * Smem::kWTile + blocks * Smem::kXTile);
+    if (folded)
+      tma_load_5d(st, &map_w, 0, 0, (int)(kb_lo + fill * KB), (int)(t.channel0 / 8), (int)t.group, &sm.full[s]);
 #pragma unroll
     for (uint32_t u = 0; u < KB; ++u)
       if (u < blocks) {
         const int k0 = (int)(kb_lo + fill * KB + u) * kBlockK;
-        tma_load_3d(st + u * Smem::kWTile, &map_w, k0, (int)t.channel0, (int)t.group, &sm.full[s]);
+        if (!folded) tma_load_3d(st + u * Smem::kWTile, &map_w, k0, (int)t.channel0, (int)t.group, &sm.full[s]);
         tma_load_2d(st + KB * Smem::kWTile + u * Smem::kXTile, &map_x, k0, (int)t.token0, &sm.full[s]);
       }
     ++it;
   };
-  if (threadIdx.x == 0) {
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     // ---- loads ----
     uint32_t fill = it;  // of the first tile, some are issued
     for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), fill = 0) {
-      if (lane == 0)
+      if (elect_one())
         for (; fill < fills; ++fill) {
           if (!mbar_wait(&sm.empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort)) {
             *abort = 1;
@@ -389,7 +403,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     uint32_t n = 0;
     for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t), ++n) {
       const uint32_t b = n & 1;
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t idesc = idesc_i8(128, (int)((t.tokens + 15) / 16 * 16));
         if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -400,13 +414,15 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + KB * Smem::kWTile);
+          const uint64_t dw = desc128(sm.stage[s], P.folded ? KB * 1024 : 1024),
+                         dx = desc128(sm.stage[s] + KB * Smem::kWTile);
+          const uint32_t next = P.folded ? 1024 >> 4 : Smem::kWTile >> 4;
 #pragma unroll
           for (uint32_t u = 0; u < KB; ++u)
             if (u < blocks) {
 #pragma unroll
               for (uint32_t kk = 0; kk < kBlockK / 32; ++kk)
-                mma_i8<1>(tmem + b * NT, dw + u * (Smem::kWTile >> 4) + kk * 2, dx + u * (Smem::kXTile >> 4) + kk * 2, idesc,
+                mma_i8<1>(tmem + b * NT, dw + u * next + kk * 2, dx + u * (Smem::kXTile >> 4) + kk * 2, idesc,
                           fill > 0 || u > 0 || kk > 0);
             }
           mma_commit(&sm.empty[s]);
@@ -424,6 +440,9 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       const uint32_t b = n & 1;
       const uint32_t channel = t.channel0 + quarter * 32 + lane;
       const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
+      const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
+      float* scales = sm.scales[warp - 2];
+      if (split == 1) take_scales(P, t, from, from + NT / (kOut / 4), scales);
       if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
         *abort = 1;
         break;
@@ -432,8 +451,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
       if (split == 1) {
-        const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
-        put_tile<T>(P, t, col, channel, sb, from, from + NT / (kOut / 4), sm.scales[warp - 2]);
+        put_tile<T>(P, t, col, channel, sb, from, from + NT / (kOut / 4), scales);
       } else {
         const uint32_t share = NT / split;
         for (uint32_t k0 = 0; k0 < t.tokens; k0 += 16) {
@@ -475,12 +493,12 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     __syncthreads();
   if (*abort) {
     // a wait gave up: what is still in flight ends before shared memory and TMEM are given back
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       atomicOr(P.trap, kDeviceTimeout);
       for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
         mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1, nullptr);
     }
-    if (warp == 1 && lane == 0) {
+    if (warp == 1 && elect_one()) {
       mma_commit(&sm.drained);
       mbar_wait(&sm.drained, 0, nullptr);
     }
@@ -528,7 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   constexpr int NT = 256;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = blockIdx.x & 1;
   const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
   volatile int* abort = &sm.abort;
@@ -539,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   bool more = walk.at(first, t);
   uint32_t it = 0;
 
-  if (threadIdx.x == 0) {
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
@@ -566,7 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
     // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
     for (uint64_t tile = first; more; tile += step, more = walk.at(tile, t)) {
       const int half = (int)((t.tokens + 31) / 32 * 16);  // tokens of each CTA
-      if (lane == 0)
+      if (elect_one())
         for (uint32_t kb = 0; kb < P.k_blocks; kb += kPairKB, ++it) {
           const uint32_t s = it % kPairStages, blocks = min((uint32_t)kPairKB, P.k_blocks - kb);
           if (!mbar_wait(&sm.empty[s], ((it / kPairStages) & 1) ^ 1, abort)) {
@@ -599,7 +617,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
     uint32_t n = 0;
     for (uint64_t tile = first; rank == 0 && more; tile += step, more = walk.at(tile, t), ++n) {
       const uint32_t b = n & 1;
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t idesc = idesc_i8(256, (int)((t.tokens + 31) / 32 * 32));
         if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -634,13 +652,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
       const uint32_t b = n & 1;
       const uint32_t channel = t.channel0 + rank * 128 + quarter * 32 + lane;
       const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
+      const uint32_t from = (warp - 2) / 4 * kHalfTokens;
+      take_scales(P, t, from, from + kHalfTokens, sm.scales[warp - 2]);
       if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
         *abort = 1;
         break;
       }
       if (*abort) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t from = (warp - 2) / 4 * kHalfTokens;
       put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb, from, from + kHalfTokens,
                   sm.scales[warp - 2]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -655,13 +674,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   // what is still in flight ends before shared memory and TMEM are given back.
   const bool stop = *abort || *(volatile int*)cg::this_cluster().map_shared_rank(&sm.abort, rank ^ 1);
   if (stop) {
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       atomicOr(P.trap, kDeviceTimeout);
       if (rank == 0)
         for (uint32_t i = it > kPairStages ? it - kPairStages : 0; i < it; ++i)
           mbar_wait(&sm.full[i % kPairStages], (i / kPairStages) & 1, nullptr);
     }
-    if (warp == 1 && lane == 0 && rank == 0) {
+    if (warp == 1 && rank == 0 && elect_one()) {
       pair_commit(&sm.drained);
       mbar_wait(&sm.drained, 0, nullptr);
     }
@@ -733,18 +752,36 @@ double cycles_of(const MapalI8Site& s, bool grouped, const Cut& c, int sms) {
   return waves * (k_blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
 }
 
+// B as [group][eight channels][block of k][8][128 bytes], in boxes of
+// channels/8 x blocks.
+int make_folded_map(CUtensorMap* map, const MapalI8Site& s, const int8_t* B, uint32_t channels, uint32_t blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dim[5] = {(cuuint64_t)kBlockK, 8, s.k / kBlockK, s.n / 8, s.groups};
+  cuuint64_t stride[4] = {s.ldb, (cuuint64_t)kBlockK, 8 * s.ldb, s.groups > 1 ? s.ldg : s.n * s.ldb};
+  cuuint32_t box[5] = {(cuuint32_t)kBlockK, 8, blocks, channels / 8, 1}, one[5] = {1, 1, 1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, (void*)B, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return 0;
+}
+
 int launch_maps(const MapalI8Site& s, const int8_t* A, const int8_t* B, uint32_t channels, uint32_t tokens,
-                CUtensorMap* mw, CUtensorMap* mx) {
-  MAPAL_TRY(make_map(mw, B, s.k, s.n, s.ldb, s.groups, s.ldg, 3, channels));
+                uint32_t folded, CUtensorMap* mw, CUtensorMap* mx) {
+  if (folded)
+    MAPAL_TRY(make_folded_map(mw, s, B, channels, folded));
+  else
+    MAPAL_TRY(make_map(mw, B, s.k, s.n, s.ldb, s.groups, s.ldg, 3, channels));
   return make_map(mx, A, s.k, s.m, s.lda, 1, 0, 2, tokens);
 }
 
 template <typename T, int NT, int CH, int KB, int STAGES>
-int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, const TcArgs& P,
-              uint64_t tiles) {
+int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, TcArgs P, uint64_t tiles) {
   using Smem = TcSmem<NT, CH, KB, STAGES>;
   CUtensorMap mw, mx;
-  MAPAL_TRY(launch_maps(s, A, B, CH, NT, &mw, &mx));
+  P.folded = s.k % kBlockK == 0 && s.n % 8 == 0;
+  MAPAL_TRY(launch_maps(s, A, B, CH, NT, P.folded ? KB : 0, &mw, &mx));
   constexpr size_t most = sizeof(Smem) + 1024 + (NT <= 64 ? NT * CH * 4 : 0);
   static_assert(most <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
@@ -771,7 +808,7 @@ template <typename T>
 int launch_pair(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, const TcArgs& P,
                 uint64_t tiles) {
   CUtensorMap mw, mx;
-  MAPAL_TRY(launch_maps(s, A, B, 128, 128, &mw, &mx));
+  MAPAL_TRY(launch_maps(s, A, B, 128, 128, 0, &mw, &mx));
   constexpr size_t smem = sizeof(PairSmem) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
@@ -823,8 +860,8 @@ int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const flo
     case 128032: return launch_tc<T, 32, 128, 2, 5>(D, s, A, B, P, tiles);
     case 64032: return launch_tc<T, 32, 64, 4, 4>(D, s, A, B, P, tiles);
     case 128016: return launch_tc<T, 16, 128, 2, 5>(D, s, A, B, P, tiles);
-    case 64016: return launch_tc<T, 16, 64, 4, 5>(D, s, A, B, P, tiles);
-    default: return launch_tc<T, 16, 32, 4, 8>(D, s, A, B, P, tiles);
+    case 64016: return launch_tc<T, 16, 64, 4, 4>(D, s, A, B, P, tiles);
+    default: return launch_tc<T, 16, 32, 4, 7>(D, s, A, B, P, tiles);
   }
 }
 
