@@ -33,60 +33,6 @@ __device__ __forceinline__ void group_rows(const int32_t* offsets, uint32_t g, u
   hi = b < 0 ? lo : max(lo, min((uint32_t)b, m));
 }
 
-// Any strides and alignments: 64 x 64 tiles of C, 64 bytes of k at a time in
-// shared memory, 4 x 4 cells a thread with the 4-way byte product.
-constexpr int TM = 64, TN = 64, TK = 64, kThreads = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) mm_i8_tile_kernel(const MapalI8Site S, const int8_t* __restrict__ A,
-                                                              const float* __restrict__ sa,
-                                                              const int8_t* __restrict__ B,
-                                                              const float* __restrict__ sb,
-                                                              const int32_t* __restrict__ offsets, T* __restrict__ C,
-                                                              unsigned* trap) {
-  __shared__ __align__(16) int8_t ta[TM][TK + 4], tb[TN][TK + 4];
-  uint32_t lo = 0, hi = (uint32_t)S.m;
-  const uint32_t g = blockIdx.z;
-  if (offsets) group_rows(offsets, g, (uint32_t)S.m, trap, lo, hi);
-  const uint64_t n0 = (uint64_t)blockIdx.x * TN;
-  const int8_t* Bg = B + g * S.ldg;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (uint64_t m0 = lo + (uint64_t)blockIdx.y * TM; m0 < hi; m0 += (uint64_t)gridDim.y * TM) {
-    int acc[4][4] = {};
-    for (uint64_t k0 = 0; k0 < S.k; k0 += TK) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < TM * TK; i += kThreads) {
-        const int r = i / TK, c = i % TK;
-        const bool in = k0 + c < S.k;
-        ta[r][c] = in && m0 + r < hi ? A[(m0 + r) * S.lda + k0 + c] : (int8_t)0;
-        tb[r][c] = in && n0 + r < S.n ? Bg[(n0 + r) * S.ldb + k0 + c] : (int8_t)0;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < TK; kk += 4) {
-        int a[4], b[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          a[u] = *reinterpret_cast<const int*>(&ta[ty + 16 * u][kk]);
-          b[u] = *reinterpret_cast<const int*>(&tb[tx + 16 * u][kk]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[u][v] = __dp4a(a[u], b[v], acc[u][v]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const uint64_t i = m0 + ty + 16 * u, j = n0 + tx + 16 * v;
-        if (i < hi && j < S.n)
-          C[i * S.ldc + j] = scaled<T>(acc[u][v], sa ? sa[i] : 1.0f, sb ? sb[g * S.n + j] : 1.0f);
-      }
-  }
-}
-
 // ---- tensor cores ------------------------------------------------------------------
 //
 // The product is taken as D = B*A^T: B's rows (channels) are the M dimension
@@ -693,6 +639,301 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   }
 }
 
+// ---- operands that TMA cannot read ----------------------------------------------------
+//
+// Bases or strides off 16 bytes: eight warps bring a block of k at a time into a
+// raw ring with cp.async, as the aligned words of 16 bytes that hold it (nine
+// for a row's 128 bytes), and from there shift it into the swizzled layout. A
+// row's words are copied and read by the same eight lanes, so a warp waits for
+// nobody. Words that do not lie wholly inside the matrix are gathered byte by
+// byte. Everything else is as in the kernel of single CTAs.
+
+constexpr int kCopyThreads = 256;
+constexpr int kAnyOut = 4;  // warps that write: the copies need the registers
+
+template <int NT, int STAGES>
+struct AnySmem {
+  static constexpr int kRows = 128 + NT;  // of weights, then of tokens
+  static constexpr int kRawRow = 9 * 16;
+  uint8_t stage[STAGES][kRows * kBlockK];
+  uint8_t raw[STAGES][kRows * kRawRow];
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t drained;
+  alignas(16) float scales[kAnyOut][kHalfTokens];
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct AnyArgs {
+  const int8_t* A;
+  const int8_t* B;
+  uint64_t lda, ldb, ldg;
+  uint64_t a_bytes, b_bytes;  // from the first to the last
+  uint32_t k;
+};
+
+__device__ __forceinline__ uint4 load16(const uint8_t* p, const uint8_t* lo, const uint8_t* hi) {
+  if (p >= lo && p + 16 <= hi) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {};
+  for (int i = 0; i < 16; ++i)
+    if (p + i >= lo && p + i < hi) w[i / 4] |= (uint32_t)__ldg(p + i) << (8 * (i % 4));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Bytes sh..sh+15 of a (first) and b.
+__device__ __forceinline__ uint4 straddle(const uint4& a, const uint4& b, uint32_t sh) {
+  const bool by8 = sh & 8, by4 = sh & 4;
+  const uint32_t bits = (sh & 3) * 8;
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = by8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = by4 ? w[i + 1] : w[i];
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// One operand of a tile as a copying thread sees it: 16 bytes of each 128 of
+// every 32nd row. 32 rows are a multiple of 16 bytes whatever the stride, so
+// the shift is the same for all of a thread's rows.
+struct RowsAt {
+  const uint8_t* mine;     // the aligned word of its first row at k = 0
+  const uint8_t *lo, *hi;  // the matrix
+  uint64_t step;           // 32 rows
+  uint32_t rows, k, sh;
+  bool low;  // no word of the first block begins before the matrix
+
+  __device__ __forceinline__ void set(const uint8_t* first, uint64_t ld, uint32_t r, uint32_t len, const uint8_t* from,
+                                      const uint8_t* to) {
+    const uint8_t* p = first + (uint64_t)(threadIdx.x >> 3) * ld + (threadIdx.x & 7) * 16;
+    sh = (uint32_t)(uintptr_t)p & 15;
+    mine = p - sh;
+    lo = from;
+    hi = to;
+    step = 32 * ld;
+    rows = r;
+    k = len;
+    low = ((uintptr_t)first & 15) == 0 || first - 15 >= from;
+  }
+
+  template <int ROWS>
+  __device__ __forceinline__ void start(uint8_t* raw, uint32_t k0) const {
+    const uint32_t c = threadIdx.x & 7, r0 = threadIdx.x >> 3, at = k0 + c * 16;
+    const uint8_t* w = mine + k0;
+    uint32_t to = sa(raw + r0 * (9 * 16) + c * 16);
+    if (k0 + kBlockK + 16 <= k && (low || k0 > 0)) {
+      // every word lies in its row, give or take 15 bytes that the row or the matrix has
+#pragma unroll
+      for (int i = 0; i < ROWS / 32; ++i, w += step, to += 32 * 9 * 16)
+        if (r0 + i * 32 < rows) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(w) : "memory");
+          if (c == 7) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16), "l"(w + 16) : "memory");
+        }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < ROWS / 32; ++i, w += step, to += 32 * 9 * 16) {
+        if (r0 + i * 32 >= rows || at >= k) continue;
+        word(to, w);
+        // the next lane's word too where that lane has nothing to copy
+        if (c == 7 || at + 16 >= k) word(to + 16, w + 16);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void word(uint32_t to, const uint8_t* w) const {
+    if (w >= lo && w + 16 <= hi) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(w) : "memory");
+    } else {
+      const uint4 v = load16(w, lo, hi);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+  }
+
+  template <int ROWS>
+  __device__ __forceinline__ void shift(const uint8_t* raw, uint8_t* tile, uint32_t k0) const {
+    const uint32_t c = threadIdx.x & 7, r0 = threadIdx.x >> 3, at = k0 + c * 16;
+    raw += r0 * (9 * 16) + c * 16;
+    tile += r0 * kBlockK + ((c ^ (r0 & 7)) << 4);
+    const uint32_t left = k <= at ? 0 : k - at;
+#pragma unroll
+    for (int i = 0; i < ROWS / 32; ++i) {
+      const uint4* w = reinterpret_cast<const uint4*>(raw + i * (32 * 9 * 16));
+      uint4 v = straddle(w[0], w[1], sh);
+      if (left < 16) {  // zeros behind k
+        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+          q[j] = left >= 4 * j + 4 ? q[j] : left <= 4 * j ? 0u : q[j] & ((1u << (8 * (left - 4 * j))) - 1);
+        v = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+      *reinterpret_cast<uint4*>(tile + i * (32 * kBlockK)) = v;
+    }
+  }
+};
+
+template <typename T, int NT, int STAGES>
+__global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
+    mm_i8_any_kernel(const __grid_constant__ AnyArgs Q, const __grid_constant__ TcArgs P) {
+  using Smem = AnySmem<NT, STAGES>;
+  constexpr uint32_t kCols = 2 * NT;
+  constexpr int kOut = kAnyOut, kCopy = kCopyThreads / 32;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  volatile int* abort = &sm.abort;
+  TileWalk walk{P.offsets, P.groups, P.m, NT, 128, (P.n + 127) / 128, P.trap};
+  walk.load();
+  Tile t;
+  bool more = walk.at(blockIdx.x, t);
+  uint32_t it = 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sm.full[s], kCopyThreads);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], kOut);
+    }
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == kCopy) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
+                 "r"(kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp < kCopy) {
+    // ---- copies ----
+    const uint8_t *alo = reinterpret_cast<const uint8_t*>(Q.A), *blo = reinterpret_cast<const uint8_t*>(Q.B);
+    RowsAt w, x;
+    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, t)) {
+      w.set(blo + t.group * Q.ldg + t.channel0 * Q.ldb, Q.ldb, P.n - t.channel0, Q.k, blo, blo + Q.b_bytes);
+      x.set(alo + t.token0 * Q.lda, Q.lda, t.tokens, Q.k, alo, alo + Q.a_bytes);
+      auto start = [&](uint32_t kb) {  // one commit group a block, empty past the last
+        if (kb < P.k_blocks) {
+          uint8_t* raw = sm.raw[kb % STAGES];
+          w.start<128>(raw, kb * kBlockK);
+          x.start<NT>(raw + 128 * Smem::kRawRow, kb * kBlockK);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll 1
+      for (uint32_t kb = 0; kb < STAGES - 1; ++kb) start(kb);
+      bool gone = false;
+#pragma unroll 1
+      for (uint32_t kb = 0; kb < P.k_blocks; ++kb, ++it) {
+        start(kb + STAGES - 1);  // its slot was read a turn ago
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        const uint32_t s = it % STAGES;
+        gone = !mbar_wait(&sm.empty[s], ((it / STAGES) & 1) ^ 1, abort);
+        gone = __any_sync(0xffffffffu, gone);  // also: the warp's copies are there for all its lanes
+        if (gone) break;
+        __syncwarp();
+        const uint8_t* raw = sm.raw[kb % STAGES];
+        w.shift<128>(raw, sm.stage[s], kb * kBlockK);
+        x.shift<NT>(raw + 128 * Smem::kRawRow, sm.stage[s] + 128 * kBlockK, kb * kBlockK);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&sm.full[s]);
+        __syncwarp();
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      if (gone) *abort = 1;
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else if (warp == kCopy) {
+    // ---- products ----
+    uint32_t n = 0;
+    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, t), ++n) {
+      const uint32_t b = n & 1;
+      if (elect_one()) {
+        const uint32_t idesc = idesc_i8(128, (int)((t.tokens + 15) / 16 * 16));
+        if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (uint32_t kb = 0; kb < P.k_blocks && !*abort; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dw = desc128(sm.stage[s]), dx = desc128(sm.stage[s] + 128 * kBlockK);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            mma_i8<1>(tmem + b * NT, dw + kk * 2, dx + kk * 2, idesc, kb > 0 || kk > 0);
+          mma_commit(&sm.empty[s]);
+        }
+        mma_commit(&sm.acc_full[b]);
+      }
+      __syncwarp();
+      if (*abort) break;
+    }
+  } else {
+    // ---- scales and output ----
+    const int quarter = warp & 3, half = (warp - kCopy - 1) / 4;
+    constexpr int kShare = NT / (kOut / 4);
+    uint32_t n = 0;
+    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, t), ++n) {
+      const uint32_t b = n & 1;
+      const uint32_t channel = t.channel0 + quarter * 32 + lane;
+      const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
+      float* scales = sm.scales[warp - kCopy - 1];
+      take_scales(P, t, half * kShare, half * kShare + kShare, scales);
+      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+        *abort = 1;
+        break;
+      }
+      if (*abort) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb, half * kShare,
+                  half * kShare + kShare, scales);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (*abort) {
+    if (threadIdx.x == 0) atomicOr(P.trap, kDeviceTimeout);
+    if (warp == kCopy && elect_one()) {
+      mma_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, nullptr);
+    }
+    __syncthreads();
+  }
+  if (warp == kCopy) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+  }
+}
+
+// C where k is 0: zeros times the scales, which may not be finite.
+template <typename T>
+__global__ void __launch_bounds__(256) mm_i8_empty_kernel(const __grid_constant__ TcArgs P) {
+  TileWalk walk{P.offsets, P.groups, P.m, 32, 256, (P.n + 255) / 256, P.trap};
+  walk.load();
+  Tile t;
+  for (uint64_t tile = blockIdx.x; walk.at(tile, t); tile += gridDim.x) {
+    const uint32_t j = t.channel0 + threadIdx.x;
+    if (j >= P.n) continue;
+    const float sb = P.sb ? __ldg(P.sb + (uint64_t)t.group * P.n + j) : 1.0f;
+    for (uint32_t i = t.token0; i < t.token0 + t.tokens; ++i)
+      static_cast<T*>(P.C)[(uint64_t)i * P.ldc + j] = scaled<T>(0, P.sa ? __ldg(P.sa + i) : 1.0f, sb);
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------
 
 // rows x k bytes (x matrices) in boxes of 128 bytes x box_rows.
@@ -712,13 +953,13 @@ int make_map(CUtensorMap* map, const int8_t* base, uint64_t k, uint64_t rows, ui
   return 0;
 }
 
-// Whether TMA can read both operands where they lie.
+// Whether TMA can read both operands where they lie (k > 0).
 bool tma_reads(const MapalI8Site& s, const int8_t* A, const int8_t* B) {
   const uint64_t lim = 1ull << 39;
   const bool a = aligned16(A) && (s.m == 1 || (s.lda % 16 == 0 && s.lda < lim));
   const bool b = aligned16(B) && (s.n == 1 || (s.ldb % 16 == 0 && s.ldb < lim)) &&
                  (s.groups == 1 || (s.ldg % 16 == 0 && s.ldg < lim));
-  return s.k > 0 && a && b && s.n * (s.n == 1 ? s.k : s.ldb) < lim;
+  return a && b && s.n * (s.n == 1 ? s.k : s.ldb) < lim;
 }
 
 // A way to cut the product: channels and tokens of a tile, parts of k; pairs
@@ -736,7 +977,7 @@ uint64_t tiles_of(const MapalI8Site& s, bool grouped, const Cut& c) {
 }
 
 // Cycles of a cut, from what bounds its tiles: the MMA (N/2 cycles for 128
-// channels and 32 bytes of k, 64 at least), and the loads, at up to 64 bytes a
+// channels and 32 bytes of k, 32 + N/4 at least), and the loads, at up to 64 bytes a
 // cycle for an SM and 6200 for all. Tiles run in waves, each with a start and
 // an end that nothing overlaps when it is the only one.
 double cycles_of(const MapalI8Site& s, bool grouped, const Cut& c, int sms) {
@@ -747,7 +988,7 @@ double cycles_of(const MapalI8Site& s, bool grouped, const Cut& c, int sms) {
   const double rate = 6200.0 / ctas < 64.0 ? 6200.0 / ctas : 64.0;
   const double load = (pair ? 256 : c.channels + c.tokens) * (double)kBlockK / rate;
   const double tokens = s.m < c.tokens ? (double)((s.m + 15) / 16 * 16) : c.tokens;
-  const double mma = 4 * (tokens / 2 > 64 ? tokens / 2 : 64);
+  const double mma = 4 * (tokens / 4 + 32 > tokens / 2 ? tokens / 4 + 32 : tokens / 2);
   const double waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
   return waves * (k_blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
 }
@@ -819,8 +1060,24 @@ int launch_pair(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, cons
   return 0;
 }
 
+template <typename T, int NT, int STAGES>
+int launch_any(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, const TcArgs& P,
+               uint64_t tiles) {
+  constexpr size_t smem = sizeof(AnySmem<NT, STAGES>) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  static std::atomic<uint64_t> done{0};
+  auto kernel = mm_i8_any_kernel<T, NT, STAGES>;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "matmul_i8 shared memory"));
+  const uint64_t one = (s.n - 1) * s.ldb + s.k;
+  const AnyArgs q{A, B, s.lda, s.ldb, s.ldg, (s.m - 1) * s.lda + s.k, (s.groups - 1) * s.ldg + one, (uint32_t)s.k};
+  const uint64_t cap = D.prof.sm_count;
+  kernel<<<(unsigned)(tiles < cap ? tiles : cap), kCopyThreads + 32 * (1 + kAnyOut), smem, D.stream>>>(q, P);
+  count_launch();
+  return 0;
+}
+
 template <typename T>
-int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float* sa, const int8_t* B, const float* sb,
+int run(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float* sa, const int8_t* B, const float* sb,
            const int32_t* offsets, void* C) {
   TcArgs P{};
   P.offsets = offsets;
@@ -834,6 +1091,16 @@ int run_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const flo
   P.groups = s.groups;
   P.k_blocks = (uint32_t)((s.k + kBlockK - 1) / kBlockK);
 
+  if (s.k == 0) {
+    const uint64_t tiles = tiles_of(s, offsets, {256, 32, 1}), cap = 8ull * D.prof.sm_count;
+    mm_i8_empty_kernel<T><<<(unsigned)(tiles < cap ? tiles : cap), 256, 0, D.stream>>>(P);
+    count_launch();
+    return 0;
+  }
+  if (!tma_reads(s, A, B)) {
+    if (s.m <= 32ull * s.groups) return launch_any<T, 32, 5>(D, s, A, B, P, tiles_of(s, offsets, {128, 32, 1}));
+    return launch_any<T, 128, 3>(D, s, A, B, P, tiles_of(s, offsets, {128, 128, 1}));
+  }
   static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
                                   {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
   Cut best{};
@@ -880,17 +1147,6 @@ int check_site(const MapalI8Site* s) {
   return 0;
 }
 
-template <typename T>
-int launch_tiles(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float* sa, const int8_t* B,
-                 const float* sb, const int32_t* offsets, void* C) {
-  const uint64_t bx = (s.n + TN - 1) / TN, rows = (s.m + TM - 1) / TM;
-  const uint64_t cap = s.groups > 1 ? 64 : 65535;  // row tiles beyond the grid are walked by its blocks
-  mm_i8_tile_kernel<T><<<dim3((unsigned)bx, (unsigned)(rows < cap ? rows : cap), s.groups), kThreads, 0, D.stream>>>(
-      s, A, sa, B, sb, offsets, (T*)C, D.trap);
-  count_launch();
-  return 0;
-}
-
 }  // namespace
 
 extern "C" int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, const int8_t* A, const float* scale_a,
@@ -908,8 +1164,7 @@ extern "C" int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, co
     DeviceSlot& D = ctx->dev[0];
     auto go = [&](auto t) {
       using T = decltype(t);
-      return tma_reads(s, A, B) ? run_tc<T>(D, s, A, scale_a, B, scale_b, offsets, C)
-                                : launch_tiles<T>(D, s, A, scale_a, B, scale_b, offsets, C);
+      return run<T>(D, s, A, scale_a, B, scale_b, offsets, C);
     };
     MAPAL_TRY(s.dtype == MAPAL_DTYPE_F32   ? go(float{})
               : s.dtype == MAPAL_DTYPE_F16 ? go(__half{})
