@@ -410,7 +410,8 @@ extern "C" int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* si
     if (!offsets || (n && (!ids || !pos))) return set_error(MAPAL_ERR_INVALID, "null ids, offsets or pos");
     if (!aligned_to(ids, 4) || !aligned_to(offsets, 4) || !aligned_to(order, 4) || !aligned_to(pos, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     const uint32_t E = site->experts;
     static std::atomic<uint64_t> done{0};
@@ -452,7 +453,8 @@ extern "C" int mapal_gpu_expert_dispatch(MapalGpuCtx* ctx, const MapalExpertSite
     if (!aligned_to(x, es) || !aligned_to(xs, es) || !aligned_to(pos, 4) || !aligned_to(scale, 4) ||
         !aligned_to(scale_out, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     switch (row_width(*site, x, x, xs, xs)) {
       case 16: launch_dispatch<uint4>(D, *site, x, scale, pos, xs, scale_out); break;
@@ -473,7 +475,8 @@ static int combine_rows(MapalGpuCtx* ctx, const MapalExpertSite* site, const voi
   const int es = dtype_bytes(site->dtype);
   if (!aligned_to(h, es) || !aligned_to(y, es) || !aligned_to(pos, 4) || !aligned_to(w, 4))
     return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-  MAPAL_TRY(enter(ctx));
+  const OnDevice on(ctx);
+  MAPAL_TRY(on.rc);
   DeviceSlot& D = ctx->dev[0];
   const MapalExpertSite& s = *site;
   by_type(s, row_width(s, y, y, h, h), [&](auto t, auto v) {
@@ -508,7 +511,8 @@ extern "C" int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpert
     if (!aligned_to(h, es) || !aligned_to(dy, es) || !aligned_to(dh, es) || !aligned_to(pos, 4) || !aligned_to(w, 4) ||
         !aligned_to(dw, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     const MapalExpertSite& s = *site;
     by_type(s, row_width(s, dy, dy, h, dh), [&](auto t, auto v) {

@@ -1160,7 +1160,8 @@ extern "C" int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, co
     const int es = dtype_bytes(s.dtype);
     if (((uintptr_t)C & (es - 1)) || ((uintptr_t)scale_a & 3) || ((uintptr_t)scale_b & 3) || ((uintptr_t)offsets & 3))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     auto go = [&](auto t) {
       using T = decltype(t);

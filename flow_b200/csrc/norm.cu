@@ -62,6 +62,25 @@ __global__ void __launch_bounds__(1024)
       else
         v[j].clear();
     }
+    // with few elements a thread the weights are asked for along with the row
+    constexpr bool kAhead = EACH == 8 && sizeof(P) == 16;
+    float fw[kAhead ? 8 : 1], fb[kAhead ? 8 : 1];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i = (j * group + G.tid) * V;
+        float pw[V] = {}, pb[V] = {};
+        if (i < d) {
+          weights<TW, V>(w, i, 1.0f, pw);
+          weights<TW, V>(b, i, 0.0f, pb);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          fw[j * V + e] = pw[e];
+          fb[j * V + e] = pb[e];
+        }
+      }
+    }
     float s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -90,13 +109,21 @@ __global__ void __launch_bounds__(1024)
       const int i = (j * group + G.tid) * V;
       if (i < d) {
         if constexpr (EACH > 8) v[j].forget();
-        float f[V], fw[V], fb[V];
+        float f[V], pw[V], pb[V];
         v[j].get(f);
-        weights<TW, V>(w, i, 1.0f, fw);
-        weights<TW, V>(b, i, 0.0f, fb);
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            pw[e] = fw[j * V + e];
+            pb[e] = fb[j * V + e];
+          }
+        } else {
+          weights<TW, V>(w, i, 1.0f, pw);
+          weights<TW, V>(b, i, 0.0f, pb);
+        }
         P o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = __fmaf_rn((f[e] - mu) * rs, fw[e], fb[e]);
+        for (int e = 0; e < V; ++e) f[e] = __fmaf_rn((f[e] - mu) * rs, pw[e], pb[e]);
         o.set(f);
         st_once(reinterpret_cast<P*>(yr + i), o);
       }
@@ -749,7 +776,8 @@ extern "C" int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site,
     if (!aligned_to(x, es) || !aligned_to(y, es) || !aligned_to(w, ws) || !aligned_to(b, ws) ||
         !aligned_to(mean, 4) || !aligned_to(rstd, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(y, site->ldy * es, site->rows),
                                  align_of(nullptr, site->d * es, 2)});
     MAPAL_TRY(by_type(*site, width, w, b, [&](auto t, auto tw, auto v) {
@@ -763,7 +791,8 @@ extern "C" int mapal_gpu_layer_norm_grad_workspace(MapalGpuCtx* ctx, const Mapal
   return guarded([&]() -> int {
     MAPAL_TRY(check_norm(site));
     if (!bytes) return set_error(MAPAL_ERR_INVALID, "bytes is null");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     *bytes = grad_bytes(*site, ctx->dev[0].prof.sm_count);
     return 0;
   });
@@ -786,7 +815,8 @@ extern "C" int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* 
     if ((dw || db) && (!work || !aligned16(work)))
       return set_error(MAPAL_ERR_INVALID, "work is null or not 16-byte aligned");
     if (site->rows == 0 && !dw && !db) return 0;
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     if ((dw || db) && work_bytes < grad_bytes(*site, ctx->dev[0].prof.sm_count))
       return set_error(MAPAL_ERR_INVALID, "work is shorter than mapal_gpu_layer_norm_grad_workspace says");
     const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(dy, site->lddy * es, site->rows),

@@ -306,7 +306,8 @@ extern "C" int mapal_gpu_quantize_rows_i8(MapalGpuCtx* ctx, const MapalQuantSite
     if (!scale || (site->d && (!x || !q))) return set_error(MAPAL_ERR_INVALID, "null x, q or scale");
     if (((uintptr_t)x & (es - 1)) || ((uintptr_t)scale & 3))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
-    MAPAL_TRY(enter(ctx));
+    const OnDevice on(ctx);
+    MAPAL_TRY(on.rc);
     const DeviceSlot& D = ctx->dev[0];
     MAPAL_TRY(site->dtype == MAPAL_DTYPE_F32   ? by_width<float>(D, *site, x, q, scale)
               : site->dtype == MAPAL_DTYPE_F16 ? by_width<__half>(D, *site, x, q, scale)

@@ -169,22 +169,31 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 
 // ---- entry points -----------------------------------------------------------------
 
-// The caller's current device is put back when an entry point returns.
-struct DeviceGuard {
-  int prev = -1;
-  DeviceGuard() {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+// The context's first device is current while this lives; the caller's current
+// device is put back after. Nothing is set where the two are the same, which
+// spares a small call two of its driver calls.
+struct OnDevice {
+  int prev = -1, rc;
+  explicit OnDevice(MapalGpuCtx* ctx) {
+    int cur = -1;
+    if (ctx && cudaGetDevice(&cur) == cudaSuccess && cur == ctx->dev[0].device) {
+      rc = 0;
+      return;
+    }
+    prev = cur;
+    rc = enter(ctx);
   }
-  ~DeviceGuard() {
+  ~OnDevice() {
     if (prev >= 0) cudaSetDevice(prev);
   }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
 };
 
 // No C++ exception leaves an entry point (the error text is a std::string).
 template <typename F>
 int guarded(F&& f) noexcept {
   try {
-    DeviceGuard g;
     return f();
   } catch (...) {
     return MAPAL_ERR_NOMEM;
