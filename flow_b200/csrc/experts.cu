@@ -25,9 +25,24 @@ constexpr uint32_t kSortBlocks = 8;  // at most, in the cluster
 constexpr int kThreads = 256;
 constexpr int kSortUnroll = 8;  // ids in flight for each lane
 
+// Lanes (of those with ok) that have the same id, which has `bits` bits: a
+// ballot for each bit. match.any answers the same question some eight times
+// slower when the ids differ (2^20 slots of 64 experts: 254 us with it).
+__device__ __forceinline__ uint32_t same_id(int32_t id, bool ok, int bits) {
+  uint32_t same = __ballot_sync(0xffffffffu, ok);
+  for (int b0 = 0; b0 < bits; b0 += 4)
+#pragma unroll
+    for (int b = b0; b < b0 + 4; ++b) {  // a bit that no id has changes nothing
+      const bool one = (id >> b) & 1;
+      const uint32_t ones = __ballot_sync(0xffffffffu, ok && one);
+      same &= one ? ones : ~ones;
+    }
+  return same;
+}
+
 // One cluster sorts all slots, each warp a contiguous run of them in order.
 // First walk: every warp counts its run's experts in its own row of shared
-// counters (lanes with the same expert found with match.any, so a counter has
+// counters (lanes with the same expert are found with ballots, so a counter has
 // one writer). Then counts become starting places: over warps in the block,
 // over blocks through distributed shared memory, over experts by a block scan.
 // Second walk: a slot's place is its expert's counter plus the lanes before it
@@ -46,6 +61,7 @@ __global__ void __launch_bounds__(kSortThreads)
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
   const uint32_t lt = (1u << lane) - 1;
+  const int bits = 32 - __clz(E - 1);
   const uint64_t lo64 = (uint64_t)(rank * warps + warp) * chunk;
   const uint32_t lo = (uint32_t)(lo64 < n ? lo64 : n), hi = (uint32_t)(lo64 + chunk < n ? lo64 + chunk : n);
   uint32_t* mine = cnt + warp * E;
@@ -69,7 +85,7 @@ __global__ void __launch_bounds__(kSortThreads)
       if (i0 + u * 32 >= hi) break;
       const bool ok = (uint32_t)id[u] < E;
       bad |= !ok && id[u] != -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, ok ? id[u] : -1);
+      const uint32_t same = same_id(id[u], ok, bits);
       if (ok && (same & lt) == 0) mine[id[u]] += __popc(same);
       __syncwarp();
     }
@@ -135,7 +151,7 @@ __global__ void __launch_bounds__(kSortThreads)
       if (i0 + u * 32 >= hi) break;
       const uint32_t i = i0 + u * 32 + lane;
       const bool ok = (uint32_t)id[u] < E;
-      const uint32_t same = __match_any_sync(0xffffffffu, ok ? id[u] : -1);
+      const uint32_t same = same_id(id[u], ok, bits);
       int32_t p = -1;
       if (ok) {
         p = (int32_t)(start[id[u]] + mine[id[u]] + __popc(same & lt));
@@ -417,11 +433,13 @@ extern "C" int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* si
     static std::atomic<uint64_t> done{0};
     MAPAL_TRY(ensure_smem_attr(done, (const void*)expert_sort_kernel, D.device,
                                (size_t)(kSortWarps + 2) * kMaxExperts * sizeof(uint32_t), "expert_sort shared memory"));
-    // About 64 slots a warp (a few warps sort a generated batch), then up to
-    // 8 blocks of 32 warps.
+    // About 64 slots a warp: a few warps of one block sort a generated batch,
+    // 8 blocks more (1024 slots of 64 experts 4 us either way, 4096: 8 and 5).
     const uint64_t want = (n + 63) / 64;
-    const unsigned blocks = want <= 2 * kSortWarps ? 1 : want <= 4 * kSortWarps ? 2 : want <= 8 * kSortWarps ? 4 : 8;
-    const uint32_t warps = (uint32_t)(want < 4 ? 4 : want < kSortWarps ? want : kSortWarps);
+    const unsigned blocks = n <= 1024 ? 1 : kSortBlocks;
+    const uint64_t share = (want + blocks - 1) / blocks;
+    const uint64_t least = E / 64 < 4 ? 4 : E / 64;  // an expert is a thread's when places are counted
+    const uint32_t warps = (uint32_t)(share > kSortWarps ? kSortWarps : share > least ? share : least);
     const uint64_t all = (uint64_t)blocks * warps;
     const uint32_t chunk = (uint32_t)(((n + all - 1) / all + 31) / 32 * 32);
     const size_t smem = (size_t)(warps + 2) * E * sizeof(uint32_t);
