@@ -358,6 +358,7 @@ int check_site(const MapalExpertSite* s, bool rows_arrays, bool bytes_too) {
   if (!rows_arrays) return 0;
   const int es = dtype_bytes(s->dtype);
   if (es == 0 || (es == 1 && !bytes_too)) return set_error(MAPAL_ERR_INVALID, "the element type is not one this call takes");
+  if (s->d > 0x7fffffffull) return set_error(MAPAL_ERR_INVALID, "rows of 2^31 elements or more");
   if (s->rows > 0x7fffffffull) return set_error(MAPAL_ERR_INVALID, "2^31 sorted rows or more");
   if (!rows_ok(s->tokens, s->d, s->ldt, es) || !rows_ok(s->rows, s->d, s->ldr, es))
     return set_error(MAPAL_ERR_INVALID, "a row stride is shorter than a row, or too long");

@@ -1021,7 +1021,7 @@ template <typename T, int NT, int CH, int KB, int STAGES>
 int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const int8_t* B, TcArgs P, uint64_t tiles) {
   using Smem = TcSmem<NT, CH, KB, STAGES>;
   CUtensorMap mw, mx;
-  P.folded = s.k % kBlockK == 0 && s.n % 8 == 0;
+  P.folded = s.k % kBlockK == 0 && s.n % 8 == 0 && s.ldb < (1ull << 36);
   MAPAL_TRY(launch_maps(s, A, B, CH, NT, P.folded ? KB : 0, &mw, &mx));
   constexpr size_t most = sizeof(Smem) + 1024 + (NT <= 64 ? NT * CH * 4 : 0);
   static_assert(most <= 227 * 1024, "shared memory of a CTA");
@@ -1138,7 +1138,8 @@ int check_site(const MapalI8Site* s) {
   if (es < 2) return set_error(MAPAL_ERR_INVALID, "C is f32, f16 or bf16");
   if (s->groups == 0 || s->groups > 65535) return set_error(MAPAL_ERR_INVALID, "1 to 65535 groups");
   if (s->k >= 131072) return set_error(MAPAL_ERR_UNSUPPORTED, "k of 131072 or more: a sum could leave 32 bits");
-  if (s->m > 0x7fffffffull || s->n > 0x7fffffffull) return set_error(MAPAL_ERR_UNSUPPORTED, "m or n of 2^31 or more");
+  // a tile's last row or channel is counted in 32 bits
+  if (s->m > 0x7fffff00ull || s->n > 0x7fffff00ull) return set_error(MAPAL_ERR_UNSUPPORTED, "m or n over 2^31 - 256");
   if (!rows_ok(s->m, s->k, s->lda, 1) || !rows_ok(s->n, s->k, s->ldb, 1) || !rows_ok(s->m, s->n, s->ldc, es))
     return set_error(MAPAL_ERR_INVALID, "a row stride is shorter than a row, or too long");
   const uint64_t one = s->n ? (s->n - 1) * s->ldb + s->k : 0;

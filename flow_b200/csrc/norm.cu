@@ -773,6 +773,8 @@ extern "C" int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site,
       return set_error(MAPAL_ERR_INVALID, "a row stride is shorter than a row, or too long");
     if (site->rows == 0) return 0;
     if (!x || !y) return set_error(MAPAL_ERR_INVALID, "null x or y");
+    if (x == y && site->rows > 1 && site->ldx != site->ldy)
+      return set_error(MAPAL_ERR_INVALID, "y is x, but not at the same stride");
     if (!aligned_to(x, es) || !aligned_to(y, es) || !aligned_to(w, ws) || !aligned_to(b, ws) ||
         !aligned_to(mean, 4) || !aligned_to(rstd, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
@@ -809,6 +811,8 @@ extern "C" int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* 
       return set_error(MAPAL_ERR_INVALID, "a row stride is shorter than a row, or too long");
     if (site->rows && (!x || !mean || !rstd || !dy || !dx))
       return set_error(MAPAL_ERR_INVALID, "null x, mean, rstd, dy or dx");
+    if (site->rows > 1 && ((dx == dy && site->lddx != site->lddy) || (dx == x && site->lddx != site->ldx)))
+      return set_error(MAPAL_ERR_INVALID, "dx is dy or x, but not at the same stride");
     if (!aligned_to(x, es) || !aligned_to(dy, es) || !aligned_to(dx, es) || !aligned_to(w, ws) ||
         !aligned_to(mean, 4) || !aligned_to(rstd, 4) || !aligned_to(dw, 4) || !aligned_to(db, 4))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");

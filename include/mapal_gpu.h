@@ -519,14 +519,15 @@ int mapal_gpu_layer_norm_grad_workspace(MapalGpuCtx* ctx, const MapalNormSite* s
  * device, so they are the same on every run. `work` is scratch of at least
  * the stated bytes, 16-byte aligned, used until the call's work has finished:
  * calls that may overlap need one each (NULL when both dw and db are).
- * dx may be dy itself. rows = 0 writes zeros to dw and db. */
+ * dx may be dy or x itself (same pointer and stride). rows = 0 writes zeros to
+ * dw and db. */
 int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* site, const void* x, const void* w,
                               const float* mean, const float* rstd, const void* dy, void* dx, float* dw, float* db,
                               void* work, uint64_t work_bytes);
 
 /* Tokens that go to k of `experts` each. Token arrays (x, y, dy, dx) have
  * `tokens` rows at stride ldt, sorted arrays (xs, h, dh, dxs) `rows` rows at
- * stride ldr. tokens*k < 2^31, experts <= 1024. */
+ * stride ldr. tokens*k, rows and d < 2^31, experts <= 1024. */
 typedef struct MapalExpertSite {
   uint64_t tokens;
   uint64_t d;
@@ -552,8 +553,8 @@ int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* site, const i
 /* xs[pos[t*k + j]] = x[t], and where scale is given (one float a token, the
  * scales of 8-bit rows) scale_out[pos[t*k + j]] = scale[t]. A negative pos is
  * skipped, one at or above site->rows traps index_oob and is skipped; rows
- * that no pos names are left as they were. Two slots with the same place give
- * that row either token's values. */
+ * that no pos names are left as they were. Two slots with the same place leave
+ * pieces of both tokens' rows there. */
 int mapal_gpu_expert_dispatch(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* x, const float* scale,
                               const int32_t* pos, void* xs, float* scale_out);
 
@@ -606,7 +607,8 @@ typedef struct MapalI8Site {
 } MapalI8Site;
 
 /* C[i, j] = (sum over k of A[i, k]*B[g][j, k]) * scale_a[i] * scale_b[g*n + j],
- * the sum exact in 32-bit integers (k < 131072), converted to f32 and
+ * the sum exact in 32-bit integers (k < 131072; m and n up to 2^31 - 256, at
+ * most 65535 groups), converted to f32 and
  * multiplied by scale_a, then by scale_b, each rounded to f32 (NULL scales:
  * 1). offsets NULL: groups is 1 and every row belongs to it. Otherwise rows
  * offsets[g] to offsets[g + 1] (groups + 1 values on the device, as

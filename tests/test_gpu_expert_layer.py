@@ -72,8 +72,10 @@ def test_serving_pass(tokens, k, experts, d, n, drop):
 @pytest.mark.parametrize("tokens,k,experts,d,drop", [(5, 2, 4, 33, 0), (120, 3, 9, 260, 11)])
 def test_training_step(tokens, k, experts, d, drop):
     """y = combine(scale_e * dispatch(norm(x))), with one scale an expert as its stand-in, and all gradients
-    against autograd in f64. Bounds: f32's half step times the roundings along each path (about 60 for the
-    norm's sums, k + 4 for the experts' way) relative to the largest entry of the result's row."""
+    against autograd in f64. Each operator's own error bound is tested in its file; this is about the whole: a
+    wrong place, a missing term or weight is off by the entries' own size, while rounding stays at (roundings
+    along the path)*2^-24 of the terms, which a row of d entries holds below sqrt(d) times its largest entry
+    (their 2-norm), plus 1 for the entries of size 1 that the inputs are drawn with."""
     with fb.Context((0,), sync=False) as ctx:
         rows = tokens * k
         x = torch.randn(tokens, d, device="cuda")
@@ -109,5 +111,4 @@ def test_training_step(tokens, k, experts, d, drop):
         for got, want, n in ((y, Y.detach(), 80), (dgate, G.grad, 100), (dx, X.grad, 200), (dw, W.grad, 200 + tokens),
                              (db, B.grad, 100 + tokens)):
             size = want.abs().amax() if want.dim() == 1 else want.abs().amax(1, keepdim=True)
-            # sums of terms that cancel: a term is at most a few times the row's largest entry times sqrt(d)
             assert_within(got, want, (n * U32 * (d ** 0.5) * (size + 1)).expand(want.shape), "gradient")

@@ -198,15 +198,38 @@ def test_combine_and_gradients(ctx, dtype, tokens, k, experts, d, pad, offset, d
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_without_weights_and_in_place(ctx, dtype):
-    L = Layer(ctx, 50, 3, 9, 136, dtype, 0.2)
+@pytest.mark.parametrize("tokens,k,d", [(1500, 3, 200), (1300, 5, 1031), (1201, 4, 2048), (1190, 9, 72)])
+def test_many_tokens(ctx, dtype, tokens, k, d):
+    test_combine_and_gradients(ctx, dtype, tokens, k, 30, d, 0, 0, 0.1)
+
+
+def test_more_rows_than_a_grid_has_blocks(ctx):
+    n = (1 << 20) + 1111
+    pos = torch.randperm(n, device="cuda").to(torch.int32)
+    site = fb.expert_site(n, 1, 4, 3, "float32")
+    x, w = randn((n, 3), torch.float32, 1), randn((n, 1), torch.float32, 2)
+    xs, y, dh, dw = (torch.empty(n, 3, device="cuda") for _ in range(4))
+    dw = torch.empty(n, 1, device="cuda")
+    ctx.expert_dispatch(site, x, pos, xs)
+    assert torch.equal(xs[pos.long()], x)
+    ctx.expert_combine(site, xs, None, pos, y)
+    assert torch.equal(y, x)
+    ctx.expert_combine_grad(site, xs, w, pos, y, dh, dw)
+    assert torch.equal(dh[pos.long()], w * x)
+    assert_within(dw[:, 0], (x.double() ** 2).sum(1), 17 * U32 * (x.double() ** 2).sum(1), "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [50, 1400])
+def test_without_weights_and_in_place(ctx, dtype, tokens):
+    L = Layer(ctx, tokens, 3, 9, 136, dtype, 0.2)
     h, y, dx, dy = L.R(3), L.T(), L.T(), L.T(4)
     ctx.expert_combine(L.site, h.t, None, L.pos, y.t)
     ctx.expert_dispatch_grad(L.site, h.t, L.pos, dx.t)
     assert torch.equal(y.t, dx.t)
-    dh, dw, dw2 = L.R(), torch.empty(50, 3, device="cuda"), torch.empty(50, 3, device="cuda")
+    dh, dw, dw2 = L.R(), torch.empty(tokens, 3, device="cuda"), torch.empty(tokens, 3, device="cuda")
     ctx.expert_combine_grad(L.site, h.t, None, L.pos, dy.t, dh.t, dw)
-    ones = torch.ones(50, 3, device="cuda")
+    ones = torch.ones(tokens, 3, device="cuda")
     dh2 = L.R()
     ctx.expert_combine_grad(L.site, h.t, ones, L.pos, dy.t, dh2.t, None)
     assert torch.equal(dh.t, dh2.t)

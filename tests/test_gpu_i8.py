@@ -57,6 +57,13 @@ def test_quantize(ctx, dtype, rows, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,d", [(90000, 64), (19000, 260), (9000, 1024), (5100, 1021), (5003, 1030), (2000, 4096), (1201, 5001),
+                                    (700, 8192), (350, 16384), (320, 16001)])
+def test_quantize_many_rows(ctx, dtype, rows, d):
+    check_quant(ctx, rows_of(rows, d, dtype, rows + d))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (4, 4), (16, 0), (7, 3), (8, 8)])
 @pytest.mark.parametrize("d", [40, 1000, 4096])
 def test_quantize_strides(ctx, dtype, pad, offset, d):
@@ -136,6 +143,35 @@ SHAPES = [(1, 1, 1), (1, 7, 16), (2, 3, 5), (1, 128, 128), (1, 4096, 512), (3, 2
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_product(ctx, dtype, m, n, k):
     check_mm(ctx, m, n, k, dtype)
+
+
+# shapes that between them take every tile (channels x tokens) and splits of k over 1, 2, 4 and 8 blocks
+CUTS = [(1, 32, 5520), (1, 4752, 32), (3, 2360, 8624), (97, 80, 5952), (944, 72, 48), (18, 2360, 10112), (117, 80, 6208),
+        (2070, 72, 32), (603, 416, 9984), (623, 144, 6320), (168, 144, 6480), (66, 5176, 32), (1, 9528, 32),
+        (1, 2392, 9824), (1, 1168, 6512), (17, 9808, 32), (21, 2424, 9024), (66, 456, 7008), (33, 9656, 32),
+        (407, 664, 11024), (311, 456, 7712), (278, 200, 7328), (65, 13336, 32), (66, 8288, 32), (2500, 1000, 400),
+        (5, 8192, 1024), (30, 4096, 896), (60, 8192, 384), (2100, 2056, 256)]
+
+
+@pytest.mark.parametrize("m,n,k", CUTS)
+def test_product_every_tile(ctx, m, n, k):
+    check_mm(ctx, m, n, k, torch.bfloat16)
+    check_mm(ctx, m, n, k, torch.float32, pads=(16, 32, 1))
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 1009), (700, 260, 517), (2, 129, 4097), (1, 1, 300), (129, 1, 200), (1, 700, 77)])
+@pytest.mark.parametrize("pads,offsets", [((0, 0, 0), (0, 0, 0)), ((1, 2, 0), (3, 7, 0)), ((5, 0, 0), (0, 9, 0)), ((16, 8, 0), (0, 0, 0))])
+def test_product_unaligned(ctx, m, n, k, pads, offsets):
+    check_mm(ctx, m, n, k, torch.bfloat16, pads, offsets)
+
+
+def test_product_at_the_very_ends_of_its_buffers(ctx):
+    """Unaligned operands that begin and end with their allocations (the loads of aligned words stay inside)."""
+    for m, n, k in ((5, 130, 333), (150, 131, 1001)):
+        A, B = i8((m, k), 1), i8((n, k), 2)
+        C = torch.empty(m, n, device="cuda")
+        ctx.matmul_i8(fb.matmul_i8_site(m, n, k, "float32"), A, None, B, None, C)
+        assert torch.equal(C, plain(A, None, B, None, torch.float32))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -221,6 +257,15 @@ def test_grouped(ctx, dtype, counts, n, k):
                                                  ((1, 0, 0), 0, 130, 1), ((0, 3, 0), 5, 2, 2), ((16, 16, 0), 8, 1, 1)])
 def test_grouped_strides_and_rows_in_no_group(ctx, counts, pads, gap, first, tail):
     check_grouped(ctx, counts, 130, 272, torch.bfloat16, tail, pads, gap, first)
+
+
+@pytest.mark.parametrize("g,m,n,k", [(2, 1, 32, 32), (60, 257, 40, 32), (60, 272, 72, 32), (60, 2514, 32, 32), (16, 2156, 136, 80),
+                                     (60, 57, 136, 32), (60, 335, 136, 32), (60, 537, 136, 32), (16, 64, 1080, 32),
+                                     (60, 1104, 136, 32), (3, 2000, 520, 256), (16, 3000, 264, 384)])
+def test_grouped_every_tile(ctx, g, m, n, k):
+    r = torch.Generator().manual_seed(m)
+    counts = torch.bincount(torch.multinomial(torch.rand(g, generator=r), m, replacement=True, generator=r), minlength=g)
+    check_grouped(ctx, counts.tolist(), n, k, torch.bfloat16)
 
 
 def test_many_groups(ctx):

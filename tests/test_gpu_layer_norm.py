@@ -170,6 +170,27 @@ def test_row_counts(ctx, rows, d):
     assert not dw.any() and not db.any()  # sums over no rows
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,d,pad", [(80000, 64, 0), (76003, 63, 1), (40001, 128, 0), (39000, 127, 0), (20000, 256, 8), (16500, 300, 0),
+                                        (9001, 600, 0), (5003, 1021, 3), (4903, 1024, 0), (2500, 2050, 0), (1203, 4096, 0),
+                                        (1001, 5000, 0), (603, 8192, 0), (450, 12000, 0), (303, 16384, 0), (310, 16003, 0)])
+def test_many_rows(ctx, rows, d, pad, dtype):
+    check(ctx, rows, d, dtype, dtype, pad=pad)
+
+
+@pytest.mark.parametrize("rows,d", [(80001, 64), (5003, 1021), (5003, 1024), (1203, 4096), (603, 8192), (303, 16384)])
+def test_many_rows_in_place(ctx, rows, d):
+    x, dy = rows_of(rows, d, torch.bfloat16, 5), rows_of(rows, d, torch.bfloat16, 6)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    mean, rstd, dw, db = run(ctx, x, None, None, y, dy, dx)
+    site = fb.norm_site(rows, d, x.dtype, eps=EPS)
+    work = torch.empty(ctx.layer_norm_grad_workspace(site), dtype=torch.uint8, device="cuda")
+    dw2, db2 = torch.empty_like(dw), torch.empty_like(db)
+    ctx.layer_norm_grad(site, x, None, mean, rstd, dy, dy, dw2, db2, work)
+    ctx.layer_norm(site, x, None, None, x)
+    assert torch.equal(dy, dx) and torch.equal(dw, dw2) and torch.equal(db, db2) and torch.equal(x, y)
+
+
 def test_in_place(ctx):
     for d in (40, 1023, 4096, 20001, 70000):
         x, dy = rows_of(9, d, torch.float32, 5), rows_of(9, d, torch.float32, 6)
@@ -180,8 +201,12 @@ def test_in_place(ctx):
         work = torch.empty(ctx.layer_norm_grad_workspace(site), dtype=torch.uint8, device="cuda")
         dw2, db2 = torch.empty_like(dw), torch.empty_like(db)
         ctx.layer_norm_grad(site, x, w, mean, rstd, dy, dy, dw2, db2, work)
+        assert torch.equal(dy, dx) and torch.equal(dw, dw2) and torch.equal(db, db2)
+        x2, dy = x.clone(), rows_of(9, d, torch.float32, 6)
+        ctx.layer_norm_grad(site, x2, w, mean, rstd, dy, x2, dw2, db2, work)
+        assert torch.equal(x2, dx) and torch.equal(dw, dw2) and torch.equal(db, db2)
         ctx.layer_norm(site, x, w, None, x)
-        assert torch.equal(dy, dx) and torch.equal(dw, dw2) and torch.equal(db, db2) and torch.equal(x, y)
+        assert torch.equal(x, y)
 
 
 def test_either_weight_gradient_alone(ctx):

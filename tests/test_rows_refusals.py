@@ -29,11 +29,11 @@ def with_(site, **kw):
 ACCEPTED = (INVALID, "ctx is null")
 
 
-def norm(site, x=P, w=P, b=P, y=P, mean=P, rstd=P):
+def norm(site, x=P, w=P, b=P, y=2 * P, mean=P, rstd=P):
     return call("layer_norm", site, x, w, b, y, mean, rstd)
 
 
-def norm_grad(site, x=P, w=P, mean=P, rstd=P, dy=P, dx=P, dw=P, db=P, work=P, n=1 << 30):
+def norm_grad(site, x=P, w=P, mean=P, rstd=P, dy=2 * P, dx=3 * P, dw=P, db=P, work=P, n=1 << 30):
     return call("layer_norm_grad", site, x, w, mean, rstd, dy, dx, dw, db, work, n)
 
 
@@ -74,6 +74,11 @@ def test_layer_norm_refuses_pointers():
         assert "not aligned" in norm_grad(s, **kw)[1]
     for kw in (dict(lddy=4), dict(lddx=4)):
         assert "stride" in norm_grad(with_(fb.norm_site(3, 5, "float32"), **kw))[1]
+    assert "same stride" in norm(with_(fb.norm_site(3, 5, "float32"), ldy=6), x=P, y=P)[1]
+    assert norm(with_(fb.norm_site(3, 5, "float32"), ldy=5), x=P, y=P) == ACCEPTED
+    assert "same stride" in norm_grad(with_(fb.norm_site(3, 5, "float32"), lddx=6), x=2 * P, dy=P, dx=P)[1]
+    assert norm_grad(s, x=2 * P, dy=P, dx=P) == ACCEPTED
+    assert "same stride" in norm_grad(with_(fb.norm_site(3, 5, "float32"), lddx=6), x=P, dy=2 * P, dx=P)[1]
     # one row has no stride
     assert norm(with_(fb.norm_site(1, 5, "float32"), ldx=0, ldy=0)) == ACCEPTED
     assert call("layer_norm_grad_workspace", s, None) == (INVALID, "bytes is null")
@@ -106,8 +111,8 @@ def test_experts_refuse_record(change, rc, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(dtype=7), "type"), (dict(rows=1 << 31), "sorted rows"), (dict(ldt=4), "stride"), (dict(ldr=4), "stride"),
-    (dict(d=1 << 62), "stride"),
+    (dict(dtype=7), "type"), (dict(rows=1 << 31), "sorted rows"), (dict(d=1 << 31, ldt=1 << 31, ldr=1 << 31), "2^31 elements"), (dict(ldt=4), "stride"), (dict(ldr=4), "stride"),
+    (dict(ldt=1 << 61), "stride"),
 ])
 def test_expert_rows_refuse_record(change, text):
     for name, n in (("expert_dispatch", 5), ("expert_combine", 4), ("expert_dispatch_grad", 3),
@@ -167,6 +172,7 @@ def test_matmul_i8_refusals():
     for kw, rc, text in ((dict(dtype=3), INVALID, "C is f32"), (dict(groups=0), INVALID, "groups"),
                          (dict(groups=1 << 17), INVALID, "groups"), (dict(k=131072, lda=131072, ldb=131072), UNSUPPORTED, "32 bits"),
                          (dict(m=1 << 31), UNSUPPORTED, "2^31"), (dict(n=1 << 31, ldc=1 << 31), UNSUPPORTED, "2^31"),
+                         (dict(m=0x7fffff01), UNSUPPORTED, "2^31"),
                          (dict(lda=4), INVALID, "stride"), (dict(ldb=4), INVALID, "stride"), (dict(ldc=3), INVALID, "stride"),
                          (dict(groups=2, ldg=19), INVALID, "between groups")):
         got, msg = call("matmul_i8", mm(**kw), P, P, P, P, P, P)
