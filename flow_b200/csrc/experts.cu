@@ -73,9 +73,11 @@ __global__ void __launch_bounds__(kSortThreads)
       id[u] = i < hi ? __ldg(ids + i) : -1;
     }
   };
+  for (uint32_t e = lane; e < E; e += 32) mine[e] = 0;
+  grid_wait();
+  grid_go();
   int32_t id[kSortUnroll];
   load(id, lo);
-  for (uint32_t e = lane; e < E; e += 32) mine[e] = 0;
   __syncwarp();
   bool bad = false;
   for (uint32_t i0 = lo; i0 < hi; i0 += 32 * kSortUnroll) {
@@ -199,6 +201,8 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const U* __restri
                                                                float* __restrict__ scale_out, Pieces Q, uint32_t k,
                                                                uint64_t units, uint64_t ldt, uint64_t ldr,
                                                                uint64_t rows, unsigned* trap) {
+  grid_wait();
+  grid_go();
   for (uint64_t item = blockIdx.x; item < Q.items; item += gridDim.x) {
     const uint64_t t = item / Q.pieces;
     const uint32_t piece = (uint32_t)(item % Q.pieces);
@@ -226,6 +230,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const T* __restric
                                                               Pieces Q, uint32_t k, uint64_t d, uint64_t ldt,
                                                               uint64_t ldr, uint64_t rows, unsigned* trap) {
   using P = Pack<T, V>;
+  grid_wait();
+  grid_go();
   for (uint64_t item = blockIdx.x; item < Q.items; item += gridDim.x) {
     const uint64_t t = item / Q.pieces;
     const uint64_t i0 = ((item % Q.pieces) * (kRowThreads * NV) + threadIdx.x) * V;
@@ -280,6 +286,8 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* h, cons
   const uint32_t turns = (k + SLOTS - 1) / SLOTS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int par = 0;
+  grid_wait();
+  grid_go();
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x, par ^= 1) {
     const uint64_t t = item / turns;
     const uint32_t j0 = (uint32_t)(item % turns) * SLOTS;
@@ -380,19 +388,19 @@ Pieces pieces_of(uint64_t tokens, uint64_t accesses, int nv) {
 }
 
 template <typename U>
-void launch_dispatch(const DeviceSlot& D, const MapalExpertSite& s, const void* x, const float* scale, const int32_t* pos,
+int launch_dispatch(const DeviceSlot& D, const MapalExpertSite& s, const void* x, const float* scale, const int32_t* pos,
                      void* xs, float* scale_out) {
   const uint64_t es = dtype_bytes(s.dtype), u = sizeof(U);
   constexpr int NV = sizeof(U) == 16 ? 2 : 4;
   const Pieces q = pieces_of(s.tokens, s.d * es / u, NV);
-  dispatch_kernel<U, NV><<<(unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0, D.stream>>>(
-      (const U*)x, scale, pos, (U*)xs, scale_out, q, s.k, s.d * es / u, s.ldt * es / u, s.ldr * es / u, s.rows, D.trap);
-  count_launch();
+  return launch_rows(dispatch_kernel<U, NV>, (unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0,
+                     D.stream, 1, (const U*)x, scale, pos, (U*)xs, scale_out, q, s.k, s.d * es / u, s.ldt * es / u,
+                     s.ldr * es / u, s.rows, D.trap);
 }
 
 // f(T, V) for the site's type and the widest access that the arrays allow.
 template <typename F>
-void by_type(const MapalExpertSite& s, int width, F&& f) {
+int by_type(const MapalExpertSite& s, int width, F&& f) {
   using std::integral_constant;
   if (s.dtype == MAPAL_DTYPE_F32) {
     if (width >= 16) return f(float{}, integral_constant<int, 4>{});
@@ -444,19 +452,8 @@ extern "C" int mapal_gpu_expert_sort(MapalGpuCtx* ctx, const MapalExpertSite* si
     const uint64_t all = (uint64_t)blocks * warps;
     const uint32_t chunk = (uint32_t)(((n + all - 1) / all + 31) / 32 * 32);
     const size_t smem = (size_t)(warps + 2) * E * sizeof(uint32_t);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = D.stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = blocks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = blocks > 1 ? 1 : 0;
-    MAPAL_CUDA(cudaLaunchKernelEx(&cfg, expert_sort_kernel, ids, (uint32_t)n, E, chunk, offsets, order, pos, D.trap));
-    count_launch();
+    MAPAL_TRY(launch_rows(expert_sort_kernel, blocks, (int)warps * 32, smem, D.stream, blocks, ids, (uint32_t)n, E, chunk,
+                          offsets, order, pos, D.trap));
     return finish(ctx, 0, true);
   });
 }
@@ -476,11 +473,11 @@ extern "C" int mapal_gpu_expert_dispatch(MapalGpuCtx* ctx, const MapalExpertSite
     MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     switch (row_width(*site, x, x, xs, xs)) {
-      case 16: launch_dispatch<uint4>(D, *site, x, scale, pos, xs, scale_out); break;
-      case 8: launch_dispatch<uint2>(D, *site, x, scale, pos, xs, scale_out); break;
-      case 4: launch_dispatch<uint32_t>(D, *site, x, scale, pos, xs, scale_out); break;
-      case 2: launch_dispatch<uint16_t>(D, *site, x, scale, pos, xs, scale_out); break;
-      default: launch_dispatch<uint8_t>(D, *site, x, scale, pos, xs, scale_out); break;
+      case 16: MAPAL_TRY(launch_dispatch<uint4>(D, *site, x, scale, pos, xs, scale_out)); break;
+      case 8: MAPAL_TRY(launch_dispatch<uint2>(D, *site, x, scale, pos, xs, scale_out)); break;
+      case 4: MAPAL_TRY(launch_dispatch<uint32_t>(D, *site, x, scale, pos, xs, scale_out)); break;
+      case 2: MAPAL_TRY(launch_dispatch<uint16_t>(D, *site, x, scale, pos, xs, scale_out)); break;
+      default: MAPAL_TRY(launch_dispatch<uint8_t>(D, *site, x, scale, pos, xs, scale_out)); break;
     }
     return finish(ctx, 0, true);
   });
@@ -498,14 +495,13 @@ static int combine_rows(MapalGpuCtx* ctx, const MapalExpertSite* site, const voi
   MAPAL_TRY(on.rc);
   DeviceSlot& D = ctx->dev[0];
   const MapalExpertSite& s = *site;
-  by_type(s, row_width(s, y, y, h, h), [&](auto t, auto v) {
+  MAPAL_TRY(by_type(s, row_width(s, y, y, h, h), [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = v.value, NV = V * sizeof(T) == 16 ? 1 : 4;
     const Pieces q = pieces_of(s.tokens, s.d / V, NV);
-    combine_kernel<T, V, NV><<<(unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0, D.stream>>>(
-        (const T*)h, w, pos, (T*)y, q, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
-    count_launch();
-  });
+    return launch_rows(combine_kernel<T, V, NV>, (unsigned)(q.items < kMostBlocks ? q.items : kMostBlocks), kRowThreads, 0,
+                       D.stream, 1, (const T*)h, w, pos, (T*)y, q, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
+  }));
   return finish(ctx, 0, true);
 }
 
@@ -534,7 +530,7 @@ extern "C" int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpert
     MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     const MapalExpertSite& s = *site;
-    by_type(s, row_width(s, dy, dy, h, dh), [&](auto t, auto v) {
+    MAPAL_TRY(by_type(s, row_width(s, dy, dy, h, dh), [&](auto t, auto v) {
       using T = decltype(t);
       constexpr int V = v.value;
       const uint64_t wide = (s.d / V + 31) / 32 * 32;
@@ -543,10 +539,9 @@ extern "C" int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpert
       const bool few = s.tokens < 8ull * D.prof.sm_count;
       const uint64_t items = s.tokens * (few ? s.k : (s.k + kAtOnce - 1) / kAtOnce);
       auto kernel = few ? combine_grad_kernel<T, V, 1> : combine_grad_kernel<T, V, kAtOnce>;
-      kernel<<<(unsigned)(items < kMostBlocks ? items : kMostBlocks), threads, 0, D.stream>>>(
-          (const T*)h, w, pos, (const T*)dy, (T*)dh, dw, items, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
-      count_launch();
-    });
+      return launch_rows(kernel, (unsigned)(items < kMostBlocks ? items : kMostBlocks), (int)threads, 0, D.stream, 1,
+                         (const T*)h, w, pos, (const T*)dy, (T*)dh, dw, items, s.k, s.d, s.ldt, s.ldr, s.rows, D.trap);
+    }));
     return finish(ctx, 0, true);
   });
 }

@@ -274,6 +274,23 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   const uint32_t kbs = (uint32_t)((uint64_t)P.k_blocks * (rank + 1) / split) - kb_lo;
   volatile int* abort = &sm.abort;
 
+  if (warp == 0 && elect_one()) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
+    }
+    mbar_init(&sm.parts, split * CH);
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  grid_wait();
+  grid_go();
   TileWalk walk{P.offsets, P.groups, P.m, NT, CH, (P.n + CH - 1) / CH, P.trap};
   walk.load();
   Tile t;
@@ -298,24 +315,9 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       }
     ++it;
   };
-  if (warp == 0 && elect_one()) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&sm.acc_full[b], 1);
-      mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
-    }
-    mbar_init(&sm.parts, split * CH);
-    mbar_init(&sm.drained, 1);
-    sm.abort = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    // the first stages are on their way before the others have begun
-    if (more)
-      while (it < STAGES && it < fills) load(it);
-  }
+  // the first stages are on their way before the others have begun
+  if (warp == 0 && more && elect_one())
+    while (it < STAGES && it < fills) load(it);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
                  "r"(kCols));
@@ -497,12 +499,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
   volatile int* abort = &sm.abort;
 
-  TileWalk walk{P.offsets, P.groups, P.m, NT, 256, (P.n + 255) / 256, P.trap};
-  walk.load();
-  Tile t;
-  bool more = walk.at(first, t);
-  uint32_t it = 0;
-
   if (warp == 0 && elect_one()) {
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&sm.full[s], 1);
@@ -525,6 +521,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   cg::this_cluster().sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
+  grid_wait();
+  grid_go();
+  TileWalk walk{P.offsets, P.groups, P.m, NT, 256, (P.n + 255) / 256, P.trap};
+  walk.load();
+  Tile t;
+  bool more = walk.at(first, t);
+  uint32_t it = 0;
+
 
   if (warp == 0) {
     // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
@@ -782,11 +786,6 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   volatile int* abort = &sm.abort;
-  TileWalk walk{P.offsets, P.groups, P.m, NT, 128, (P.n + 127) / 128, P.trap};
-  walk.load();
-  Tile t;
-  bool more = walk.at(blockIdx.x, t);
-  uint32_t it = 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], kCopyThreads);
@@ -810,6 +809,13 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
+  grid_wait();
+  grid_go();
+  TileWalk walk{P.offsets, P.groups, P.m, NT, 128, (P.n + 127) / 128, P.trap};
+  walk.load();
+  Tile t;
+  bool more = walk.at(blockIdx.x, t);
+  uint32_t it = 0;
 
   if (warp < kCopy) {
     // ---- copies ----
@@ -922,6 +928,8 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
 // C where k is 0: zeros times the scales, which may not be finite.
 template <typename T>
 __global__ void __launch_bounds__(256) mm_i8_empty_kernel(const __grid_constant__ TcArgs P) {
+  grid_wait();
+  grid_go();
   TileWalk walk{P.offsets, P.groups, P.m, 32, 256, (P.n + 255) / 256, P.trap};
   walk.load();
   Tile t;
@@ -1029,20 +1037,8 @@ int launch_tc(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const 
   auto kernel = mm_i8_tc_kernel<T, NT, CH, KB, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "matmul_i8 shared memory"));
   const uint64_t cap = P.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < cap ? tiles : cap) * P.split));
-  cfg.blockDim = dim3(64 + 32 * out_warps(NT));
-  cfg.dynamicSmemBytes = sizeof(Smem) + 1024 + (P.split > 1 ? NT * CH * 4 : 0);
-  cfg.stream = D.stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = P.split;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = P.split > 1 ? 1 : 0;
-  MAPAL_CUDA(cudaLaunchKernelEx(&cfg, kernel, mw, mx, P));
-  count_launch();
-  return 0;
+  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * P.split), 64 + 32 * out_warps(NT),
+                     sizeof(Smem) + 1024 + (P.split > 1 ? NT * CH * 4 : 0), D.stream, P.split, mw, mx, P);
 }
 
 template <typename T>
@@ -1055,9 +1051,8 @@ int launch_pair(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, cons
   static std::atomic<uint64_t> done{0};
   MAPAL_TRY(ensure_smem_attr(done, (const void*)mm_i8_pair_kernel<T>, D.device, smem, "matmul_i8 shared memory"));
   const uint64_t cap = D.prof.sm_count / 2;
-  mm_i8_pair_kernel<T><<<(unsigned)((tiles < cap ? tiles : cap) * 2), 64 + 32 * out_warps(256), smem, D.stream>>>(mw, mx, P);
-  count_launch();
-  return 0;
+  return launch_rows(mm_i8_pair_kernel<T>, (unsigned)((tiles < cap ? tiles : cap) * 2), 64 + 32 * out_warps(256), smem,
+                     D.stream, 1, mw, mx, P);
 }
 
 template <typename T, int NT, int STAGES>
@@ -1071,9 +1066,8 @@ int launch_any(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const
   const uint64_t one = (s.n - 1) * s.ldb + s.k;
   const AnyArgs q{A, B, s.lda, s.ldb, s.ldg, (s.m - 1) * s.lda + s.k, (s.groups - 1) * s.ldg + one, (uint32_t)s.k};
   const uint64_t cap = D.prof.sm_count;
-  kernel<<<(unsigned)(tiles < cap ? tiles : cap), kCopyThreads + 32 * (1 + kAnyOut), smem, D.stream>>>(q, P);
-  count_launch();
-  return 0;
+  return launch_rows(kernel, (unsigned)(tiles < cap ? tiles : cap), kCopyThreads + 32 * (1 + kAnyOut), smem, D.stream, 1, q,
+                     P);
 }
 
 template <typename T>
@@ -1093,9 +1087,7 @@ int run(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float*
 
   if (s.k == 0) {
     const uint64_t tiles = tiles_of(s, offsets, {256, 32, 1}), cap = 8ull * D.prof.sm_count;
-    mm_i8_empty_kernel<T><<<(unsigned)(tiles < cap ? tiles : cap), 256, 0, D.stream>>>(P);
-    count_launch();
-    return 0;
+    return launch_rows(mm_i8_empty_kernel<T>, (unsigned)(tiles < cap ? tiles : cap), 256, 0, D.stream, 1, P);
   }
   if (!tma_reads(s, A, B)) {
     if (s.m <= 32ull * s.groups) return launch_any<T, 32, 5>(D, s, A, B, P, tiles_of(s, offsets, {128, 32, 1}));

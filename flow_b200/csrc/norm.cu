@@ -48,6 +48,8 @@ __global__ void __launch_bounds__(1024)
   constexpr int NV = EACH / V;
   __shared__ float red[32][2][32];  // at most 32 groups
   const Group<false> G(group);
+  grid_wait();
+  grid_go();
   const uint64_t stride = (uint64_t)gridDim.x * (blockDim.x / group);
   const int d = (int)S.d;
   const float n = (float)d;
@@ -173,6 +175,8 @@ __global__ void __launch_bounds__(kFlow, 1)
       }
     ring.commit();
   };
+  grid_wait();
+  grid_go();
 #pragma unroll
   for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
   f2 fw[EACH / 2], fb[EACH / 2];
@@ -314,6 +318,8 @@ __global__ void __launch_bounds__(kFlow, 1)
       }
     ring.commit();
   };
+  grid_wait();
+  grid_go();
 #pragma unroll
   for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
   float nmu[ROWS], nrs[ROWS];
@@ -459,6 +465,8 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const MapalNormSite
   __shared__ float red[2][32];
   const int64_t d = (int64_t)S.d;
   const float n = (float)S.d;
+  grid_wait();
+  grid_go();
   for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x) {
     const T* xr = x + r * S.ldx;
     T* yr = y + r * S.ldy;
@@ -506,6 +514,8 @@ __global__ void __launch_bounds__(kThreads) norm_grad_rows_kernel(const MapalNor
   __shared__ float red[2][2][32];
   const int64_t d = (int64_t)S.d;
   const float n = (float)S.d;
+  grid_wait();
+  grid_go();
   int par = 0;
   for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x, par ^= 1) {
     const T* xr = x + r * S.ldx;
@@ -549,6 +559,8 @@ __global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const MapalNor
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const uint64_t c = ((uint64_t)blockIdx.x * 32 + lane) * V;
   float aw[V] = {}, ab[V] = {};
+  grid_wait();
+  grid_go();
   if (c < S.d)
     for (uint64_t r = blockIdx.y * 8ull + sub; r < S.rows; r += parts * 8ull) {
       const Pack<T, V> p = ld_once(reinterpret_cast<const Pack<T, V>*>(x + r * S.ldx + c));
@@ -590,6 +602,8 @@ __global__ void __launch_bounds__(1024) norm_grad_join_kernel(const float* __res
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;  // 0..d: dw, d..2d: db
   float a = 0.0f;
+  grid_wait();
+  grid_go();
   if (c < 2 * d) {
 #pragma unroll 10
     for (uint32_t p = sub; p < parts; p += 32) a += __ldcs(work + 2ull * p * d + c);
@@ -628,15 +642,15 @@ uint64_t grad_bytes(const MapalNormSite& s, int sms) { return grad_parts(s, sms)
 unsigned row_blocks(const MapalNormSite& s, int sms) { return (unsigned)(s.rows < 8ull * sms ? s.rows : 8ull * sms); }
 
 template <typename T, typename TW, int V, int EACH>
-void launch_held(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
+int launch_held(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                  float* mean, float* rstd) {
   const int group = (int)((s.d + 32 * EACH - 1) / (32 * EACH)) * 32;
   // one row a block while that leaves no SM with two
   const int threads = group >= 256 || s.rows <= (uint64_t)D.prof.sm_count ? group : 256 / group * group;
   const uint64_t want = (s.rows + threads / group - 1) / (threads / group),
                  cap = (uint64_t)D.prof.sm_count * (1024 / threads);
-  norm_held_kernel<T, TW, V, EACH><<<(unsigned)(want < cap ? want : cap), threads, 0, D.stream>>>(
-      s, (const T*)x, w, b, (T*)y, mean, rstd, group);
+  return launch_rows(norm_held_kernel<T, TW, V, EACH>, (unsigned)(want < cap ? want : cap), threads, 0, D.stream, 1, s,
+                     (const T*)x, w, b, (T*)y, mean, rstd, group);
 }
 
 template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
@@ -647,8 +661,7 @@ int launch_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
   auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS, SUB>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "layer_norm shared memory"));
   const Plan p = flow_plan(s.rows, s.d, D.prof.sm_count, EACH, ROWS);
-  kernel<<<p.blocks, p.threads, smem, D.stream>>>(s, (const T*)x, w, b, (T*)y, mean, rstd, p.group);
-  return 0;
+  return launch_rows(kernel, p.blocks, p.threads, smem, D.stream, 1, s, (const T*)x, w, b, (T*)y, mean, rstd, p.group);
 }
 
 template <typename T, typename TW, int V>
@@ -664,22 +677,20 @@ int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
   // against 60 us, 60000 x 1024 45 against 54; f32 and narrow accesses do not.
   constexpr uint64_t kNarrow = sizeof(T) * V == 16 && sizeof(T) == 2 ? 512 : 4096;
   if (s.d <= 128 && many)
-    MAPAL_TRY((launch_flow<T, TW, V, 8, 4, true>(D, s, x, w, b, y, mean, rstd)));
+    return launch_flow<T, TW, V, 8, 4, true>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= kNarrow && many)
-    MAPAL_TRY((launch_flow<T, TW, V, 8, 4, false>(D, s, x, w, b, y, mean, rstd)));
+    return launch_flow<T, TW, V, 8, 4, false>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= kMostFlow && many)
-    MAPAL_TRY((launch_flow<T, TW, V, 16, 2, false>(D, s, x, w, b, y, mean, rstd)));
+    return launch_flow<T, TW, V, 16, 2, false>(D, s, x, w, b, y, mean, rstd);
   else if (V > 1 && s.d <= 2 * kMostFlow && many)
-    MAPAL_TRY((launch_flow<T, TW, V, kLong, 32 / kLong, false>(D, s, x, w, b, y, mean, rstd)));
+    return launch_flow<T, TW, V, kLong, 32 / kLong, false>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= 1024 * 8)
-    launch_held<T, TW, V, 8>(D, s, x, w, b, y, mean, rstd);
+    return launch_held<T, TW, V, 8>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= 1024 * kMid)
-    launch_held<T, TW, V, kMid>(D, s, x, w, b, y, mean, rstd);
+    return launch_held<T, TW, V, kMid>(D, s, x, w, b, y, mean, rstd);
   else
-    norm_rows_kernel<T, TW, V><<<row_blocks(s, D.prof.sm_count), kThreads, 0, D.stream>>>(s, (const T*)x, w, b, (T*)y,
-                                                                                         mean, rstd);
-  count_launch();
-  return 0;
+    return launch_rows(norm_rows_kernel<T, TW, V>, row_blocks(s, D.prof.sm_count), kThreads, 0, D.stream, 1, s,
+                       (const T*)x, w, b, (T*)y, mean, rstd);
 }
 
 template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
@@ -693,10 +704,8 @@ int launch_grad_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x,
   const size_t sums = p.threads > p.group ? 2 * s.d * sizeof(float) : 0;  // at most 32 KB: d <= 4096
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, ring > 32768 ? ring : 32768,
                              "layer_norm_grad shared memory"));
-  kernel<<<p.blocks, p.threads, ring > sums ? ring : sums, D.stream>>>(s, (const T*)x, w, mean, rstd, (const T*)dy, (T*)dx, work,
-                                                         p.group);
-  count_launch();
-  return 0;
+  return launch_rows(kernel, p.blocks, p.threads, ring > sums ? ring : sums, D.stream, 1, s, (const T*)x, w, mean, rstd,
+                     (const T*)dy, (T*)dx, work, p.group);
 }
 
 template <typename T, typename TW, int V>
@@ -717,19 +726,15 @@ int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x,
     MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1, false>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (work) {
     // before dx is written, which may be dy
-    norm_grad_cols_kernel<T, V><<<dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0, D.stream>>>(
-        s, (const T*)x, mean, rstd, (const T*)dy, work, parts);
-    count_launch();
+    MAPAL_TRY(launch_rows(norm_grad_cols_kernel<T, V>, dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0,
+                          D.stream, 1, s, (const T*)x, mean, rstd, (const T*)dy, work, parts));
   }
-  if (work) {
-    norm_grad_join_kernel<<<(unsigned)((2 * s.d + 31) / 32), 1024, 0, D.stream>>>(work, s.d, parts, dw, db);
-    count_launch();
-  }
-  if (!flow && s.rows) {
-    norm_grad_rows_kernel<T, TW, V><<<row_blocks(s, sms), kThreads, 0, D.stream>>>(s, (const T*)x, w, mean, rstd,
-                                                                                  (const T*)dy, (T*)dx);
-    count_launch();
-  }
+  if (work)
+    MAPAL_TRY(launch_rows(norm_grad_join_kernel, (unsigned)((2 * s.d + 31) / 32), 1024, 0, D.stream, 1, work, s.d, parts, dw,
+                          db));
+  if (!flow && s.rows)
+    MAPAL_TRY(launch_rows(norm_grad_rows_kernel<T, TW, V>, row_blocks(s, sms), kThreads, 0, D.stream, 1, s, (const T*)x, w,
+                          mean, rstd, (const T*)dy, (T*)dx));
   return 0;
 }
 

@@ -147,6 +147,8 @@ __global__ void __launch_bounds__(kFlow, 1) quant_flow_kernel(const MapalQuantSi
       }
     ring.commit();
   };
+  grid_wait();
+  grid_go();
 #pragma unroll
   for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
   for (int par = 0; r < S.rows; r += step, par ^= 1) {
@@ -202,6 +204,8 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const MapalQuantSite S
   __shared__ uint32_t red[2][32];
   const int64_t d = (int64_t)S.d, step = (int64_t)blockDim.x * V;
   int par = 0;
+  grid_wait();
+  grid_go();
   for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x, par ^= 1) {
     const T* xr = x + r * S.ldx;
     P v[NV];
@@ -250,8 +254,7 @@ int launch_flow(const DeviceSlot& D, const MapalQuantSite& s, const T* x, int8_t
   const int group = (int)((s.d + 32 * EACH - 1) / (32 * EACH)) * 32, threads = kFlow / group * group;
   const uint64_t turn = (uint64_t)(threads / group) * ROWS, want = (s.rows + turn - 1) / turn;
   const uint64_t cap = D.prof.sm_count;
-  kernel<<<(unsigned)(want < cap ? want : cap), threads, smem, D.stream>>>(s, x, q, scale, group);
-  return 0;
+  return launch_rows(kernel, (unsigned)(want < cap ? want : cap), threads, smem, D.stream, 1, s, x, q, scale, group);
 }
 
 template <typename T, int V>
@@ -261,20 +264,15 @@ int launch_quant(const DeviceSlot& D, const MapalQuantSite& s, const void* from,
   const bool many = s.rows * s.d >= 64ull * kFlow * D.prof.sm_count;
   const uint64_t cap = 8ull * D.prof.sm_count;
   const unsigned blocks = (unsigned)(s.rows < cap ? s.rows : cap);
-  if (many && s.d <= 1024)
-    MAPAL_TRY((launch_flow<T, V, 8, 4>(D, s, x, q, scale)));
-  else if (many && s.d <= 8192)
-    MAPAL_TRY((launch_flow<T, V, 16, 2>(D, s, x, q, scale)));
-  else if (many && s.d <= 16384)
-    MAPAL_TRY((launch_flow<T, V, 32, 1>(D, s, x, q, scale)));
-  else if (s.d <= 8192)
-    quant_rows_kernel<T, V, 8><<<blocks, (unsigned)((s.d + 255) / 256 * 32 + (s.d == 0 ? 32 : 0)), 0, D.stream>>>(s, x, q, scale);
-  else if (s.d <= 32768)
-    quant_rows_kernel<T, V, 32><<<blocks, (unsigned)((s.d + 1023) / 1024 * 32), 0, D.stream>>>(s, x, q, scale);
-  else
-    quant_rows_kernel<T, V, 0><<<blocks, 1024, 0, D.stream>>>(s, x, q, scale);
-  count_launch();
-  return 0;
+  if (many && s.d <= 1024) return launch_flow<T, V, 8, 4>(D, s, x, q, scale);
+  if (many && s.d <= 8192) return launch_flow<T, V, 16, 2>(D, s, x, q, scale);
+  if (many && s.d <= 16384) return launch_flow<T, V, 32, 1>(D, s, x, q, scale);
+  if (s.d <= 8192)
+    return launch_rows(quant_rows_kernel<T, V, 8>, blocks, s.d ? (int)((s.d + 255) / 256 * 32) : 32, 0, D.stream, 1, s, x, q,
+                       scale);
+  if (s.d <= 32768)
+    return launch_rows(quant_rows_kernel<T, V, 32>, blocks, (int)((s.d + 1023) / 1024 * 32), 0, D.stream, 1, s, x, q, scale);
+  return launch_rows(quant_rows_kernel<T, V, 0>, blocks, 1024, 0, D.stream, 1, s, x, q, scale);
 }
 
 // The widest access that x's rows, q's rows and a row's length allow.
