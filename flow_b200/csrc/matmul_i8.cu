@@ -23,16 +23,6 @@ __device__ __forceinline__ T scaled(int acc, float sa, float sb) {
   return from_f32<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc), sa), sb));
 }
 
-// Group g's rows [lo, hi), clamped to [0, m] and ascending; raises the trap
-// where the offsets are not.
-__device__ __forceinline__ void group_rows(const int32_t* offsets, uint32_t g, uint32_t m, unsigned* trap, uint32_t& lo,
-                                           uint32_t& hi) {
-  const int32_t a = __ldg(offsets + g), b = __ldg(offsets + g + 1);
-  if (a < 0 || b < a || (uint32_t)b > m) atomicMax(trap, kTrapOob);
-  lo = a < 0 ? 0u : min((uint32_t)a, m);
-  hi = b < 0 ? lo : max(lo, min((uint32_t)b, m));
-}
-
 // ---- tensor cores ------------------------------------------------------------------
 //
 // The product is taken as D = B*A^T: B's rows (channels) are the M dimension
@@ -121,16 +111,25 @@ struct TileWalk {
   uint32_t base = 0, before = 0;      // the chunk's first group, token tiles before it
   uint32_t lo = 0, hi = 0, incl = 0;  // this lane's group: rows, token tiles up to and with it
   uint32_t chunk = 0;                 // token tiles of the chunk
+  uint32_t least = 0;                 // once an offset was bad: the largest so far
+  bool broken = false;
 
   __device__ void load() {
     const uint32_t lane = threadIdx.x & 31, g = base + lane;
     lo = hi = 0;
+    bool bad = false;
     if (g < groups) {
-      if (offsets)
-        group_rows(offsets, g, m, trap, lo, hi);
-      else
+      if (offsets) {
+        const int32_t a = __ldg(offsets + g), b = __ldg(offsets + g + 1);
+        bad = a < 0 || b < a || (uint32_t)b > m;
+        lo = (uint32_t)max(a, 0);
+        hi = (uint32_t)max(b, 0);
+      } else {
         hi = m;
+      }
     }
+    broken = __any_sync(0xffffffffu, bad || broken);
+    if (broken) raise(bad);
     incl = (hi - lo + nt - 1) / nt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -138,6 +137,24 @@ struct TileWalk {
       if (lane >= o) incl += up;
     }
     chunk = __shfl_sync(0xffffffffu, incl, 31);
+  }
+
+  // Bad offsets: each becomes the largest up to it, at most m, so that groups
+  // still do not share rows and there are no more tiles than rows allow.
+  __device__ __forceinline__ void raise(bool bad) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (bad) atomicMax(trap, kTrapOob);
+    lo = min(lo, m);
+    hi = max(lo, min(hi, m));
+    uint32_t top = hi;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane >= o) top = max(top, up);
+    }
+    const uint32_t below = __shfl_up_sync(0xffffffffu, top, 1);
+    lo = max(lo, max(least, lane ? below : 0u));
+    hi = max(lo, hi);
+    least = max(least, __shfl_sync(0xffffffffu, top, 31));
   }
 
   __device__ bool at(uint64_t tile, Tile& t) {

@@ -614,7 +614,7 @@ typedef struct MapalI8Site {
  * offsets[g] to offsets[g + 1] (groups + 1 values on the device, as
  * mapal_gpu_expert_sort writes them) belong to g; rows of C in no group are
  * left as they were. Offsets that descend or leave [0, m] trap index_oob and
- * are taken as if clamped. k = 0 gives zeros times the scales. */
+ * are taken as the largest up to them, clamped to [0, m]. k = 0 gives zeros times the scales. */
 int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, const int8_t* A, const float* scale_a,
                         const int8_t* B, const float* scale_b, const int32_t* offsets, void* C);
 

@@ -287,6 +287,33 @@ def test_bad_offsets_trap_and_stay_inside(ctx, off, k):
     assert torch.equal(C.t[:5], plain(A[:5], None, B[0], None, torch.float32))
 
 
+@pytest.mark.parametrize("off", [[0, 5, 3, 20], [0, 4, 8, 21], [-1, 4, 8, 20], [0, 1 << 30, 8, 20], [0, 9, -9, 12], [3, 2, 1, 15],
+                                 [0, 3, 9] + [7] * 60 + [11, 10, 20]])
+@pytest.mark.parametrize("k", [64, 61, 4096])
+def test_bad_offsets_still_give_each_row_to_one_group(ctx, off, k):
+    """An offset counts as the largest up to it, clamped; k = 4096 is split over a cluster."""
+    g = len(off) - 1
+    A, B, C = i8((20, k), 1), i8((g, 140, k), 2), torch.full((20, 140), 5.0, device="cuda")
+    site = fb.matmul_i8_site(20, 140, k, "float32", groups=g)
+    with pytest.raises(fb.MapalTrap, match="index_oob"):
+        ctx.matmul_i8(site, A, None, B, None, C, offsets=torch.tensor(off, dtype=torch.int32, device="cuda"))
+    want, top = torch.full_like(C, 5.0), [min(max(0, max(off[:i + 1])), 20) for i in range(len(off))]
+    for e in range(g):
+        if top[e + 1] > top[e]:
+            want[top[e]:top[e + 1]] = plain(A[top[e]:top[e + 1]], None, B[e], None, torch.float32)
+    assert torch.equal(C, want)
+
+
+def test_offsets_that_go_up_and_down_cost_no_more_work(ctx):
+    """Each of 4000 groups would otherwise claim all rows; the first takes them."""
+    m, n, k, g = 2000, 256, 256, 4000
+    A, B, C = i8((m, k), 1), i8((g, n, k), 2), torch.zeros(m, n, device="cuda")
+    off = torch.tensor([0, m] * (g // 2) + [m], dtype=torch.int32, device="cuda")
+    with pytest.raises(fb.MapalTrap, match="index_oob"):
+        ctx.matmul_i8(fb.matmul_i8_site(m, n, k, "float32", groups=g), A, None, B, None, C, offsets=off)
+    assert torch.equal(C, plain(A, None, B[0], None, torch.float32))
+
+
 @pytest.mark.parametrize("m", [3, 300])
 def test_captured_replayed_and_two_contexts(ctx, m):
     A, B, sa, sb = i8((m, 512), 1), i8((2, 300, 512), 2), f32(m, 3), f32((2, 300), 4)
