@@ -39,6 +39,9 @@ __device__ __forceinline__ T scaled(int acc, float sa, float sb) {
 //              run beside this tile's output) and issues kind::i8, K32, with N
 //              the tile's tokens rounded up;
 //   the others read the accumulator, scale and store C.
+// TMEM is taken after grid_wait: no kernel holds it while it waits for the one
+// before it, which may still have to take its own. A wait that gave up ends its
+// whole warp together (any_of), since every step of a tile is a warp's.
 // Tiles are numbered channel tiles first, then token tiles, then groups, and a
 // persistent grid takes every gridDim-th; each warp finds a tile's group by a
 // scan over the offsets, 32 groups at a time.
@@ -98,6 +101,8 @@ __device__ __forceinline__ uint32_t remote(uint32_t local, uint32_t rank) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+
+__device__ __forceinline__ bool any_of(bool p) { return __any_sync(0xffffffffu, p); }
 
 struct Tile {
   uint32_t group, token0, tokens, channel0;
@@ -360,8 +365,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
           }
           load(fill);
         }
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else if (warp == 1) {
     // ---- products ----
@@ -394,8 +398,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
         }
         mma_commit(&sm.acc_full[b]);
       }
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else if ((warp & 3) < CH / 32) {
     // ---- scales and output ----
@@ -408,11 +411,10 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
       float* scales = sm.scales[warp - 2];
       if (split == 1) take_scales(P, t, from, from + NT / (kOut / 4), scales);
-      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {  // *abort: its commit was an aborted tile's
         *abort = 1;
         break;
       }
-      if (*abort) break;  // the last commit of an aborted tile
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
       if (split == 1) {
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
           }
         }
         for (uint32_t q = 0; q < split; ++q) arrive_remote(remote(sa(&sm.parts), q));
-        if (!mbar_wait_cluster(&sm.parts, 0, abort)) {
+        if (any_of(!mbar_wait_cluster(&sm.parts, 0, abort))) {
           *abort = 1;
           break;
         }
@@ -481,7 +483,9 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
 // and half of the tokens, and the pair's MMA (cta_group::2, issued by the first
 // CTA) reads both halves from both, so a CTA moves 32 KB a block of k where a
 // 128 x 256 tile of its own moves 48. Large products of single CTAs are bound by
-// that traffic from L2 (about 11.6 TB/s; 8192^3: 0.54 ms).
+// that traffic from L2 (about 11.6 TB/s): 8192^3 0.54 ms, where pairs take 0.39
+// and are bound by the tensor pipe (84% of its cycles, measured on 2048 x 8192 x
+// 8192) and, back to back, by the power limit (0.43 ms).
 
 constexpr int kPairStages = 3, kPairKB = 2;
 struct PairSmem {
@@ -530,6 +534,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  grid_wait();
+  grid_go();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -538,8 +544,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
   cg::this_cluster().sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  grid_wait();
-  grid_go();
   TileWalk walk{P.offsets, P.groups, P.m, NT, 256, (P.n + 255) / 256, P.trap};
   walk.load();
   Tile t;
@@ -576,8 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
                   : "memory");
             }
         }
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else if (warp == 1) {
     // ---- products, by the first CTA ----
@@ -608,8 +611,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
         }
         pair_commit(&sm.acc_full[b]);
       }
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else {
     // ---- scales and output ----
@@ -621,11 +623,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
       const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
       const uint32_t from = (warp - 2) / 4 * kHalfTokens;
       take_scales(P, t, from, from + kHalfTokens, sm.scales[warp - 2]);
-      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
         *abort = 1;
         break;
       }
-      if (*abort) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb, from, from + kHalfTokens,
                   sm.scales[warp - 2]);
@@ -817,6 +818,8 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  grid_wait();
+  grid_go();
   if (warp == kCopy) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
                  "r"(kCols));
@@ -826,8 +829,6 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  grid_wait();
-  grid_go();
   TileWalk walk{P.offsets, P.groups, P.m, NT, 128, (P.n + 127) / 128, P.trap};
   walk.load();
   Tile t;
@@ -858,7 +859,7 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         const uint32_t s = it % STAGES;
         gone = !mbar_wait(&sm.empty[s], ((it / STAGES) & 1) ^ 1, abort);
-        gone = __any_sync(0xffffffffu, gone);  // also: the warp's copies are there for all its lanes
+        gone = any_of(gone);  // also: the warp's copies are there for all its lanes
         if (gone) break;
         __syncwarp();
         const uint8_t* raw = sm.raw[kb % STAGES];
@@ -871,8 +872,7 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
       if (gone) *abort = 1;
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else if (warp == kCopy) {
     // ---- products ----
@@ -898,8 +898,7 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
         }
         mma_commit(&sm.acc_full[b]);
       }
-      __syncwarp();
-      if (*abort) break;
+      if (any_of(*abort)) break;
     }
   } else {
     // ---- scales and output ----
@@ -912,11 +911,10 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
       const float sb = P.sb && channel < P.n ? __ldg(P.sb + (uint64_t)t.group * P.n + channel) : 1.0f;
       float* scales = sm.scales[warp - kCopy - 1];
       take_scales(P, t, half * kShare, half * kShare + kShare, scales);
-      if (!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort)) {
+      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
         *abort = 1;
         break;
       }
-      if (*abort) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       put_tile<T>(P, t, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, channel, sb, half * kShare,
                   half * kShare + kShare, scales);

@@ -4,7 +4,8 @@
 // a = max|x|, scale = a/127, q = clamp(rint(x*(127/a)), -127, 127). The
 // maximum is taken over the bit patterns of |x| as integers, which order as
 // the values do with infinity and then NaN above them, so one reduction finds
-// the maximum and whether the row is finite.//
+// the maximum and whether the row is finite.
+//
 // Bound by HBM (an element's bytes and one), so a row is read once and held in
 // registers as it came, and the instructions an element are kept few: the
 // maximum of 16-bit types is taken on pairs, one redux instruction joins a
