@@ -104,16 +104,17 @@ def _span(rows: int, cols: int, ld: int) -> int:
     return (rows - 1) * ld + cols if rows and cols else 0
 
 
-def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0):
+def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0, ldg: int = 0):
     """Address of a device buffer of a row-wise operator: None, an int address taken as given, or a torch tensor,
-    which must be of the record's type, on the context's device, with `need` elements from its first."""
+    which must be of the record's type, on the context's device, with `need` elements from its first. A view must lie
+    as the record says: rows at stride `ld` (matrices at `ldg`), whatever dimensions they are counted by."""
     if (t.__class__ is _tensor and t.dtype is _dtypes[code] and t.get_device() == device and t.numel() >= need
             and t.is_contiguous()):
         return t.data_ptr()
-    return t if t is None else _buf_checked(t, code, need, device, what, ld)
+    return t if t is None else _buf_checked(t, code, need, device, what, ld, ldg)
 
 
-def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int) -> int:
+def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int, ldg: int) -> int:
     global _tensor
     if isinstance(t, int):
         return t
@@ -129,8 +130,18 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int) -> in
         if t.numel() and t.dim():
             if t.stride(-1) != 1 and t.size(-1) > 1:
                 raise ValueError(f"{what}: the elements of a row must be contiguous")
-            if ld and t.dim() > 1 and t.size(-2) > 1 and t.stride(-2) != ld:
-                raise ValueError(f"{what} has row stride {t.stride(-2)}, the record says {ld}")
+            if not ld and not t.is_contiguous():
+                raise ValueError(f"{what} must be contiguous")
+            step = ld  # of the dimensions from the last but one on, while they count rows
+            for i in range(t.dim() - 2, -1, -1):
+                if t.size(i) == 1 or not ld:
+                    continue
+                if ldg and i == 0 and t.dim() == 3:
+                    step = ldg
+                if t.stride(i) != step:
+                    raise ValueError(f"{what} has row stride {t.stride(i)}, the record says {ld}" if step == ld else
+                                     f"{what} has stride {t.stride(i)} in dimension {i}, the record says {step}")
+                step *= t.size(i)
         have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
         if have < need:
             raise ValueError(f"{what} holds {have} elements, the record needs {need}")
@@ -423,7 +434,7 @@ class Context:
         _check(_native.load().mapal_gpu_matmul_i8(
             self._h, site, _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),
             _buf(scale_a, 0, m, dev, "scale_a"),
-            _buf(B, 3, _span(groups, _span(n, k, ldb), site.ldg), dev, "B", ldb),
+            _buf(B, 3, _span(groups, _span(n, k, ldb), site.ldg), dev, "B", ldb, site.ldg),
             _buf(scale_b, 0, groups * n, dev, "scale_b"), _buf(offsets, 4, groups + 1, dev, "offsets"),
             _buf(C, site.dtype, _span(m, n, site.ldc), dev, "C", site.ldc)))
 

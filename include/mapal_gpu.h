@@ -478,7 +478,8 @@ int mapal_gpu_matmul_f32_sharded(MapalGpuCtx* ctx, const MapalTileSite* site,
  * are contiguous. Any alignment of a type is accepted, 16-byte aligned rows
  * are the fast ones. Arithmetic is f32 (exact 32-bit integers for the 8-bit
  * product); values are rounded to a 16-bit type once, on writing. Outputs do
- * not depend on timing: no floating-point atomics. */
+ * not depend on timing: no floating-point atomics. An output overlaps no
+ * other array of its call except where a call says so. */
 #define MAPAL_DTYPE_F32 0
 #define MAPAL_DTYPE_F16 1
 #define MAPAL_DTYPE_BF16 2
@@ -571,7 +572,8 @@ int mapal_gpu_expert_dispatch_grad(MapalGpuCtx* ctx, const MapalExpertSite* site
 /* The gradient of combine: dh[pos[t*k + j]] = w[t*k + j]*dy[t] and
  * dw[t*k + j] = <dy[t], h[pos[t*k + j]]> (0 for a slot without a place).
  * w NULL: 1; dw may be NULL. Rows of dh that no pos names are left as they
- * were. dh may be h itself. */
+ * were. dh may be h itself. Two slots with the same place leave one's or the
+ * other's pieces in dh, and where dh is h the dot products of both undefined. */
 int mapal_gpu_expert_combine_grad(MapalGpuCtx* ctx, const MapalExpertSite* site, const void* h, const float* w,
                                   const int32_t* pos, const void* dy, void* dh, float* dw);
 

@@ -242,3 +242,47 @@ def test_wrapper_refuses_other_arguments(ctx):
         ctx.layer_norm_grad(fb.norm_site(3, 4, "float32"), 64, None, 64, 64, 64, 64, 64, 64, torch.zeros(9))
     with pytest.raises(ValueError, match="no element type"):
         fb.norm_site(3, 5, torch.float64)
+
+
+BATCH = torch.zeros(4, 6, 5)  # 4 sequences of 6 tokens
+
+
+@pytest.mark.parametrize("x,rows,ld,text", [
+    (BATCH[:, :3], 12, 0, "stride 30 in dimension 0, the record says 15"),  # a padded batch is not evenly spaced rows
+    (BATCH[:, :, :4], 24, 5, None), (BATCH[1:, :, :4], 18, 5, None), (BATCH[:, 2], 4, 30, None),
+    (BATCH[:, 2], 4, 0, "row stride 30"), (BATCH[:, 2:3], 4, 30, None), (BATCH[:, 2:3], 4, 5, "row stride 30"),
+    (BATCH[::2], 12, 0, "stride 60 in dimension 0, the record says 30"), (BATCH.transpose(0, 1), 24, 0, "row stride 30"),
+    (BATCH.view(4, 2, 3, 5)[:, :, :2], 16, 0, "stride 15 in dimension 1, the record says 10"),
+])
+def test_wrapper_takes_views_as_they_lie(ctx, x, rows, ld, text):
+    d = x.shape[-1]
+    site = fb.norm_site(rows, d, "float32", ldx=ld)
+    with pytest.raises(ValueError if text else fb.MapalInfraError, match=text or "ctx is null"):
+        ctx.layer_norm(site, x, None, None, torch.zeros(rows, d))
+
+
+def test_wrapper_refuses_views_of_what_has_no_stride(ctx):
+    e, x, ids = fb.expert_site(6, 2, 4, 5, "float32"), torch.zeros(6, 5), torch.zeros(12, dtype=torch.int32)
+    wide = torch.zeros(6, 8, dtype=torch.int32)[:, :2]  # the first 2 of 8
+    with pytest.raises(ValueError, match="ids must be contiguous"):
+        ctx.expert_sort(e, wide, ids, ids, ids)
+    with pytest.raises(ValueError, match="pos must be contiguous"):
+        ctx.expert_dispatch(e, x, wide, torch.zeros(12, 5))
+    with pytest.raises(ValueError, match="w must be contiguous"):
+        ctx.expert_combine(e, torch.zeros(12, 5), torch.zeros(6, 8)[:, :2], ids, x)
+    with pytest.raises(ValueError, match="scale_out must be contiguous|elements of a row"):
+        ctx.expert_dispatch(e, x, ids, torch.zeros(12, 5), scale=torch.zeros(6), scale_out=torch.zeros(24)[::2])
+
+
+def test_wrapper_checks_the_stride_between_matrices(ctx):
+    a, f, off = torch.zeros(3, 5, dtype=torch.int8), torch.zeros(12), torch.zeros(3, dtype=torch.int32)
+    b = torch.zeros(4, 3, 8, dtype=torch.int8)
+    c = torch.zeros(3, 3)
+    run = lambda B, **kw: ctx.matmul_i8(fb.matmul_i8_site(3, 3, 5, "float32", groups=2, **kw), a, f, B, f, c, offsets=off)
+    for B, kw in ((b[:2, :, :5], dict(ldb=8, ldg=24)), (b[::2, :, :5], dict(ldb=8, ldg=48)), (b[1:3, :, 3:], dict(ldb=8))):
+        with pytest.raises(fb.MapalInfraError, match="ctx is null"):
+            run(B, **kw)
+    with pytest.raises(ValueError, match="stride 48 in dimension 0, the record says 24"):
+        run(b[::2, :, :5], ldb=8)
+    with pytest.raises(ValueError, match="row stride 8"):
+        run(b[:2, :, :5])
