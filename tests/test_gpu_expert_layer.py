@@ -112,3 +112,76 @@ def test_training_step(tokens, k, experts, d, drop):
                              (db, B.grad, 100 + tokens)):
             size = want.abs().amax() if want.dim() == 1 else want.abs().amax(1, keepdim=True)
             assert_within(got, want, (n * U32 * (d ** 0.5) * (size + 1)).expand(want.shape), "gradient")
+
+
+class Served:
+    """The serving pass over inputs of its own, its calls on one stream or with the sort on another beside the
+    norm and the quantising, joined before the rows move."""
+
+    def __init__(self, tokens, k, experts, d, n, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+        bf, rows = torch.bfloat16, tokens * k
+        self.x, self.w, self.b = r(tokens, d).to(bf), r(d).to(bf), r(d).to(bf)
+        self.ids, self.gate = routed(tokens, k, experts, seed)
+        self.bq = torch.randint(-127, 128, (experts, n, d), generator=g, device="cuda").to(torch.int8)
+        self.bs = r(experts, n)
+        e = lambda *s, t=torch.float32: torch.empty(*s, dtype=t, device="cuda")  # noqa: E731
+        self.off, self.pos = e(experts + 1, t=torch.int32), e(rows, t=torch.int32)
+        self.normed, self.q, self.s = e(tokens, d, t=bf), e(tokens, d, t=torch.int8), e(tokens)
+        self.qs, self.ss, self.h, self.out = e(rows, d, t=torch.int8), e(rows), e(rows, n, t=bf), e(tokens, n, t=bf)
+        self.ns, self.qsite = fb.norm_site(tokens, d, bf), fb.quant_site(tokens, d, bf)
+        self.moved = fb.expert_site(tokens, k, experts, d, torch.int8)
+        self.mm = fb.matmul_i8_site(rows, n, d, bf, groups=experts)
+        self.back = fb.expert_site(tokens, k, experts, n, bf)
+
+    def run(self, ctx, main, side=None):
+        side = side or main
+        if side is not main:
+            side.wait_stream(main)
+        ctx.set_stream(side.cuda_stream)
+        ctx.expert_sort(self.moved, self.ids, self.off, None, self.pos)
+        ctx.set_stream(main.cuda_stream)
+        ctx.layer_norm(self.ns, self.x, self.w, self.b, self.normed)
+        ctx.quantize_rows_i8(self.qsite, self.normed, self.q, self.s)
+        if side is not main:
+            main.wait_stream(side)
+        ctx.expert_dispatch(self.moved, self.q, self.pos, self.qs, self.s, self.ss)
+        ctx.matmul_i8(self.mm, self.qs, self.ss, self.bq, self.bs, self.h, offsets=self.off)
+        ctx.expert_combine(self.back, self.h, self.gate, self.pos, self.out)
+
+
+@pytest.mark.parametrize("tokens,k,experts,d,n", [(3, 2, 8, 256, 128), (700, 4, 16, 1024, 520)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_two_streams_that_join(tokens, k, experts, d, n, captured):
+    """Sort beside norm on a second stream, joined by an event: run after run in a row, without a wait on the host,
+    each over the buffers of the run before, with other inputs, gives what the calls one by one give."""
+    with fb.Context((0,), sync=False) as ctx:
+        steps = [Served(tokens, k, experts, d, n, i) for i in range(4)]
+        main, side = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        want = []
+        for s in steps:
+            s.run(ctx, main)
+            ctx.synchronize()
+            want.append(s.out.clone())
+        torch.cuda.synchronize()
+        s, outs = Served(tokens, k, experts, d, n, 0), [torch.empty_like(want[0]) for _ in range(40)]
+        g = torch.cuda.CUDAGraph()
+        if captured:
+            with torch.cuda.graph(g, stream=main):
+                s.run(ctx, main, side)
+        with torch.cuda.stream(main):
+            for i, out in enumerate(outs):
+                for name in ("x", "w", "b", "ids", "gate", "bq", "bs"):
+                    getattr(s, name).copy_(getattr(steps[i % 4], name))
+                if captured:
+                    g.replay()
+                else:
+                    s.run(ctx, main, side)
+                out.copy_(s.out)
+        torch.cuda.synchronize()
+        ctx.synchronize()
+        for i, out in enumerate(outs):
+            assert torch.equal(out, want[i % 4]), f"run {i}"
+        del g
