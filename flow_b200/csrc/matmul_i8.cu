@@ -703,19 +703,6 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p, const uint8_t* lo, con
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Bytes sh..sh+15 of a (first) and b.
-__device__ __forceinline__ uint4 straddle(const uint4& a, const uint4& b, uint32_t sh) {
-  const bool by8 = sh & 8, by4 = sh & 4;
-  const uint32_t bits = (sh & 3) * 8;
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) w[i] = by8 ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) w[i] = by4 ? w[i + 1] : w[i];
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
-}
-
 // One operand of a tile as a copying thread sees it: 16 bytes of each 128 of
 // every 32nd row. 32 rows are a multiple of 16 bytes whatever the stride, so
 // the shift is the same for all of a thread's rows.

@@ -30,6 +30,19 @@ __device__ __forceinline__ void weights(const void* w, int64_t i, float none, fl
   }
 }
 
+// The same for columns i to i + V - 1 of d, which need not be aligned or all
+// exist; zeros for those that do not.
+template <typename TW, int V>
+__device__ __forceinline__ void weights_at(const void* w, int i, int d, float none, float (&out)[V]) {
+  if (i >= 0 && i + V <= d && i % V == 0) {
+    weights<TW, V>(w, i, none, out);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      out[e] = i + e < 0 || i + e >= d ? 0.0f : w ? to_f32(__ldg(static_cast<const TW*>(w) + i + e)) : none;
+  }
+}
+
 __device__ __forceinline__ float inv_std(float var, float eps) { return __fdiv_rn(1.0f, __fsqrt_rn(var + eps)); }
 
 
@@ -148,37 +161,53 @@ __global__ void __launch_bounds__(1024)
 
 __device__ __forceinline__ float f2_sum(f2 v) { return f2_lo(v) + f2_hi(v); }
 
-template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB, int EDGE>
 __global__ void __launch_bounds__(kFlow, 1)
     norm_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const void* __restrict__ b, T* y,
-                     float* __restrict__ mean, float* __restrict__ rstd, int group) {
-  using R = Ring<T, V, EACH, ROWS, 1>;
+                     float* __restrict__ mean, float* __restrict__ rstd, int group, uint32_t period) {
+  using R = std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 1, SUB, EDGE == 2>, Ring<T, V, EACH, ROWS, 1>>;
   using P = Pack<T, V>;
   constexpr int NV = EACH / V;
   __shared__ float sets[kMostGroups][2][4][16];
   extern __shared__ __align__(16) uint8_t dyn[];
-  R ring(dyn);
   const Group<SUB> G(group);
+  R ring(dyn, G);
   auto* red = sets[SUB || group == 32 ? 0 : G.id];
-  const int groups = blockDim.x / group, d = (int)S.d;
-  const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
-  uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
+  const Turns<SUB, EDGE, ROWS> mine(G, period, S.rows);
+  uint64_t rows = mine.rows, ldx = mine.stride(S.ldx), ldy = mine.stride(S.ldy);
+  uint64_t r = mine.first;
+  const int d = (int)S.d, shift = mine.template shift<T>(S.ldy), shift_x = mine.template shift<T>(S.ldx);
+  const std::conditional_t<EDGE != 0, Input<V, NV>, Whole> in(group, G.tid, d, shift_x, shift);
+  const std::conditional_t<EDGE != 0, Mine<V, NV>, Whole> part(group, G.tid, shift, d + shift);
+  const std::conditional_t<EDGE != 0, Masks<P, V, NV>, Whole> keep(part);
+  x = mine.at(x, S.ldx) - shift_x + (G.tid - in.back) * V;
+  y = mine.at(y, S.ldy) - shift + G.tid * V;
+  mean = mine.at(mean, 1);
+  rstd = mine.at(rstd, 1);
+  if constexpr (EDGE != 0) {
+    pin(x), pin(y);
+    pin(rows), pin(ldx), pin(ldy);
+  }
   const float n = (float)d;
   auto start = [&](int st, uint64_t row) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k)
-      if (row + k < S.rows) {
-        const T* from = x + (row + k) * S.ldx + G.tid * V;
+      if (row + k < rows) {
+        const T* from = x + (row + k) * ldx;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if ((j * group + G.tid) * V < d) ring.copy(st, k * NV + j, from + j * group * V);
+        for (int j = 0; j < NV; ++j) {
+          if constexpr (EDGE != 0)
+            ring.bring(st, k * NV + j, from + j * group * V, in.left[j]);
+          else if ((j * group + G.tid) * V < d)
+            ring.copy(st, k * NV + j, from + j * group * V);
+        }
       }
     ring.commit();
   };
   grid_wait();
   grid_go();
 #pragma unroll
-  for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
+  for (int k = 0; k < R::kStages; ++k) start(k, r + k * mine.step);
   f2 fw[EACH / 2], fb[EACH / 2];
   {
     float a[EACH], c[EACH];
@@ -186,7 +215,10 @@ __global__ void __launch_bounds__(kFlow, 1)
     for (int j = 0; j < NV; ++j) {
       const int i = (j * group + G.tid) * V;
       float pa[V] = {}, pc[V] = {};
-      if (i < d) {
+      if constexpr (EDGE != 0) {
+        weights_at<TW, V>(w, i - shift, d, 1.0f, pa);
+        weights_at<TW, V>(b, i - shift, d, 0.0f, pc);
+      } else if (i < d) {
         weights<TW, V>(w, i, 1.0f, pa);
         weights<TW, V>(b, i, 0.0f, pc);
       }
@@ -202,7 +234,7 @@ __global__ void __launch_bounds__(kFlow, 1)
       fb[u] = f2_pack(c[2 * u], c[2 * u + 1]);
     }
   }
-  for (; r < S.rows; r += step) {
+  for (; r < rows; r += mine.step) {
     ring.wait();
     f2 v[ROWS][EACH / 2];
     float s[ROWS], q[ROWS];
@@ -212,10 +244,14 @@ __global__ void __launch_bounds__(kFlow, 1)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         P p;
-        if ((j * group + G.tid) * V < d && r + k < S.rows)
+        if constexpr (EDGE != 0) {
+          p = ring.take(k * NV + j, in.by);
+          keep(p, j);
+        } else if ((j * group + G.tid) * V < d && r + k < rows) {
           p = ring.take(k * NV + j);
-        else
+        } else {
           p.clear();
+        }
         float g[V];
         p.get(g);
 #pragma unroll
@@ -230,8 +266,9 @@ __global__ void __launch_bounds__(kFlow, 1)
       s[k] = f2_sum(t);
     }
     G.sums(s, red[0]);
-    start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
-    ring.next();
+    if constexpr (EDGE != 0) ring.taken();
+    start(ring.stage, r + R::kStages * mine.step);  // this turn's slots have been read
+    ring.next_stage();
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       s[k] = __fdiv_rn(s[k], n);
@@ -239,8 +276,16 @@ __global__ void __launch_bounds__(kFlow, 1)
 #pragma unroll
       for (int u = 0; u < EACH / 2; ++u) v[k][u] = f2_add(v[k][u], m);
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if ((j * group + G.tid) * V >= d) {  // no elements here
+      for (int j = 0; j < NV; ++j) {
+        if constexpr (EDGE != 0) {
+          const uint32_t own = part.at(j);
+          if (own != part.kAll)
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+              f2& u = v[k][(j * V + e) / 2];
+              u = f2_pack(own & (1u << e) ? f2_lo(u) : 0.0f, own & (2u << e) ? f2_hi(u) : 0.0f);
+            }
+        } else if ((j * group + G.tid) * V >= d) {  // no elements here
           if constexpr (V > 1) {
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) v[k][j * (V / 2) + e] = f2_splat(0.0f);
@@ -248,6 +293,7 @@ __global__ void __launch_bounds__(kFlow, 1)
             v[k][j / 2] = j % 2 ? f2_pack(f2_lo(v[k][j / 2]), 0.0f) : f2_pack(0.0f, f2_hi(v[k][j / 2]));
           }
         }
+      }
       f2 t = f2_splat(0.0f);
 #pragma unroll
       for (int u = 0; u < EACH / 2; ++u) t = f2_fma(v[k][u], v[k][u], t);
@@ -257,7 +303,7 @@ __global__ void __launch_bounds__(kFlow, 1)
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       const float rs = inv_std(__fdiv_rn(q[k], n), S.eps);
-      if (r + k >= S.rows) break;
+      if (r + k >= rows) break;
       const f2 m = f2_splat(rs);
       float f[EACH];
 #pragma unroll
@@ -266,7 +312,7 @@ __global__ void __launch_bounds__(kFlow, 1)
         f[2 * u] = f2_lo(o);
         f[2 * u + 1] = f2_hi(o);
       }
-      T* to = y + (r + k) * S.ldy + G.tid * V;
+      T* to = y + (r + k) * ldy;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         float g[V];
@@ -274,11 +320,18 @@ __global__ void __launch_bounds__(kFlow, 1)
         for (int e = 0; e < V; ++e) g[e] = f[j * V + e];
         P p;
         p.set(g);
-        if ((j * group + G.tid) * V < d) st_once(reinterpret_cast<P*>(to + j * group * V), p);
+        if constexpr (EDGE != 0) {
+          if (part.at(j) == part.kAll)
+            st_once(reinterpret_cast<P*>(to + j * group * V), p);
+          else
+            st_part(to + j * group * V, p, part.at(j));
+        } else if ((j * group + G.tid) * V < d) {
+          st_once(reinterpret_cast<P*>(to + j * group * V), p);
+        }
       }
       if (G.tid == 0) {
-        if (mean) mean[r + k] = s[k];
-        if (rstd) rstd[r + k] = rs;
+        if (mean) mean[(r + k) * mine.period] = s[k];
+        if (rstd) rstd[(r + k) * mine.period] = rs;
       }
     }
   }
@@ -286,49 +339,69 @@ __global__ void __launch_bounds__(kFlow, 1)
 
 // The gradient: dx, and where work is given this block's sums of dy*h and dy
 // as rows 2*block and 2*block + 1 of it (the groups add theirs in order).
-template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB, int EDGE>
 __global__ void __launch_bounds__(kFlow, 1)
     norm_grad_flow_kernel(const MapalNormSite S, const T* x, const void* __restrict__ w, const float* __restrict__ mean,
-                          const float* __restrict__ rstd, const T* dy, T* dx, float* __restrict__ work, int group) {
-  using R = Ring<T, V, EACH, ROWS, 2>;
+                          const float* __restrict__ rstd, const T* dy, T* dx, float* __restrict__ work, int group,
+                          uint32_t period) {
+  using R = std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 2, SUB, EDGE == 2>, Ring<T, V, EACH, ROWS, 2>>;
   using P = Pack<T, V>;
   constexpr int NV = EACH / V, H = EACH / 2;
   __shared__ float sets[kMostGroups][2][2 * ROWS][16];
   extern __shared__ __align__(16) uint8_t dyn[];
-  R ring(dyn);
   float* sums = reinterpret_cast<float*>(dyn);  // 2*d floats, when the ring is done
   const Group<SUB> G(group);
+  R ring(dyn, G);
   auto* red = sets[SUB || group == 32 ? 0 : G.id];
-  const int groups = blockDim.x / group, d = (int)S.d;
-  const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
-  uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
+  const Turns<SUB, EDGE, ROWS> mine(G, period, S.rows);
+  uint64_t rows = mine.rows, ldx = mine.stride(S.ldx), lddy = mine.stride(S.lddy), lddx = mine.stride(S.lddx);
+  uint64_t r = mine.first;
+  const int d = (int)S.d, shift = mine.template shift<T>(S.lddx);
+  const int shift_x = mine.template shift<T>(S.ldx), shift_y = mine.template shift<T>(S.lddy);
+  using In = std::conditional_t<EDGE != 0, Input<V, NV>, Whole>;
+  const In ix(group, G.tid, d, shift_x, shift), iy(group, G.tid, d, shift_y, shift);
+  const std::conditional_t<EDGE != 0, Mine<V, NV>, Whole> part(group, G.tid, shift, d + shift);
+  const std::conditional_t<EDGE != 0, Masks<P, V, NV>, Whole> keep(part);
+  x = mine.at(x, S.ldx) - shift_x + (G.tid - ix.back) * V;
+  dy = mine.at(dy, S.lddy) - shift_y + (G.tid - iy.back) * V;
+  dx = mine.at(dx, S.lddx) - shift + G.tid * V;
+  mean = mine.at(mean, 1);
+  rstd = mine.at(rstd, 1);
+  if constexpr (EDGE != 0) {
+    pin(x), pin(dy), pin(dx);
+    pin(rows), pin(ldx), pin(lddy), pin(lddx);
+  }
   const float inv_n = __fdiv_rn(1.0f, (float)d);
   auto start = [&](int st, uint64_t row) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k)
-      if (row + k < S.rows) {
-        const T* from = x + (row + k) * S.ldx + G.tid * V;
-        const T* from2 = dy + (row + k) * S.lddy + G.tid * V;
+      if (row + k < rows) {
+        const T* from = x + (row + k) * ldx;
+        const T* from2 = dy + (row + k) * lddy;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if ((j * group + G.tid) * V < d) {
+        for (int j = 0; j < NV; ++j) {
+          if constexpr (EDGE != 0) {
+            ring.bring(st, k * NV + j, from + j * group * V, ix.left[j]);
+            ring.bring(st, (ROWS + k) * NV + j, from2 + j * group * V, iy.left[j]);
+          } else if ((j * group + G.tid) * V < d) {
             ring.copy(st, k * NV + j, from + j * group * V);
             ring.copy(st, (ROWS + k) * NV + j, from2 + j * group * V);
           }
+        }
       }
     ring.commit();
   };
   grid_wait();
   grid_go();
 #pragma unroll
-  for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
+  for (int k = 0; k < R::kStages; ++k) start(k, r + k * mine.step);
   float nmu[ROWS], nrs[ROWS];
   auto stats = [&](uint64_t row) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const bool in = row + k < S.rows;
-      nmu[k] = in ? __ldg(mean + row + k) : 0.0f;
-      nrs[k] = in ? __ldg(rstd + row + k) : 0.0f;
+      const bool in = row + k < rows;
+      nmu[k] = in ? __ldg(mean + (row + k) * mine.period) : 0.0f;
+      nrs[k] = in ? __ldg(rstd + (row + k) * mine.period) : 0.0f;
     }
   };
   stats(r);
@@ -339,7 +412,10 @@ __global__ void __launch_bounds__(kFlow, 1)
     for (int j = 0; j < NV; ++j) {
       const int i = (j * group + G.tid) * V;
       float pa[V] = {};
-      if (i < d) weights<TW, V>(w, i, 1.0f, pa);
+      if constexpr (EDGE != 0)
+        weights_at<TW, V>(w, i - shift, d, 1.0f, pa);
+      else if (i < d)
+        weights<TW, V>(w, i, 1.0f, pa);
 #pragma unroll
       for (int e = 0; e < V; ++e) a[j * V + e] = pa[e];
     }
@@ -350,7 +426,7 @@ __global__ void __launch_bounds__(kFlow, 1)
     }
   }
   int par = 0;
-  for (; r < S.rows; r += step, par ^= 1) {
+  for (; r < rows; r += mine.step, par ^= 1) {
     ring.wait();
     f2 h[ROWS][H], g[ROWS][H];
     float c[2 * ROWS], rs[ROWS];
@@ -360,7 +436,16 @@ __global__ void __launch_bounds__(kFlow, 1)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         P px, py;
-        if ((j * group + G.tid) * V < d && r + k < S.rows) {
+        if constexpr (EDGE != 0) {
+          px = ring.take(k * NV + j, ix.by);
+          py = ring.take((ROWS + k) * NV + j, iy.by);
+          keep(px, j);
+          keep(py, j);
+          if (r + k >= rows) {  // they are added to the sums over rows
+            px.clear();
+            py.clear();
+          }
+        } else if ((j * group + G.tid) * V < d && r + k < rows) {
           px = ring.take(k * NV + j);
           py = ring.take((ROWS + k) * NV + j);
         } else {
@@ -392,13 +477,14 @@ __global__ void __launch_bounds__(kFlow, 1)
       c[2 * k] = f2_sum(c1);
       c[2 * k + 1] = f2_sum(c2);
     }
-    stats(r + step);
+    stats(r + mine.step);
     G.sums(c, red[par]);
-    start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
-    ring.next();
+    if constexpr (EDGE != 0) ring.taken();
+    start(ring.stage, r + R::kStages * mine.step);  // this turn's slots have been read
+    ring.next_stage();
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      if (r + k >= S.rows) break;
+      if (r + k >= rows) break;
       const f2 c1 = f2_splat(-c[2 * k] * inv_n), c2 = f2_splat(-c[2 * k + 1] * inv_n), sc = f2_splat(rs[k]);
       float f[EACH];
 #pragma unroll
@@ -407,7 +493,7 @@ __global__ void __launch_bounds__(kFlow, 1)
         f[2 * u] = f2_lo(o);
         f[2 * u + 1] = f2_hi(o);
       }
-      T* to = dx + (r + k) * S.lddx + G.tid * V;
+      T* to = dx + (r + k) * lddx;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         float o[V];
@@ -415,7 +501,14 @@ __global__ void __launch_bounds__(kFlow, 1)
         for (int e = 0; e < V; ++e) o[e] = f[j * V + e];
         P p;
         p.set(o);
-        if ((j * group + G.tid) * V < d) st_once(reinterpret_cast<P*>(to + j * group * V), p);
+        if constexpr (EDGE != 0) {
+          if (part.at(j) == part.kAll)
+            st_once(reinterpret_cast<P*>(to + j * group * V), p);
+          else
+            st_part(to + j * group * V, p, part.at(j));
+        } else if ((j * group + G.tid) * V < d) {
+          st_once(reinterpret_cast<P*>(to + j * group * V), p);
+        }
       }
     }
   }
@@ -430,7 +523,7 @@ __global__ void __launch_bounds__(kFlow, 1)
         ab[u] = f2_add(ab[u], __shfl_xor_sync(0xffffffffu, ab[u], o));
       }
   }
-  const int turns = SUB ? blockDim.x / 32 : groups;
+  const int turns = blockDim.x / (SUB ? 32 : group);
   const int turn = !SUB ? G.id : (int)(threadIdx.x % 32) < group ? (int)(threadIdx.x / 32) : -1;
   float* out = work + 2ull * blockIdx.x * S.d;
   __syncthreads();  // every group has taken its last rows out of the ring
@@ -439,10 +532,12 @@ __global__ void __launch_bounds__(kFlow, 1)
       const bool first = k == 0, last = k == turns - 1;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int i = (j * group + G.tid) * V;
+        const int i = (j * group + G.tid) * V - shift;
         if (i >= d) continue;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
+          if constexpr (EDGE != 0)
+            if (!(part.at(j) & (1u << e))) continue;
           const int u = j * V + e;
           const float a = u % 2 ? f2_hi(aw[u / 2]) : f2_lo(aw[u / 2]), c = u % 2 ? f2_hi(ab[u / 2]) : f2_lo(ab[u / 2]);
           (last ? out : sums)[i + e] = first ? a : sums[i + e] + a;
@@ -631,9 +726,10 @@ int check_norm(const MapalNormSite* s) {
   return 0;
 }
 
-// Partial sums that the gradient's scratch has room for: a block each.
+// Partial sums that the gradient's scratch has room for: a block each (up to 7
+// more than rows, so that their number suits every period).
 uint32_t grad_parts(const MapalNormSite& s, int sms) {
-  const uint64_t want = s.d <= kMostFlow ? s.rows : (s.rows + 7) / 8, cap = s.d <= kMostFlow ? sms : 2ull * sms;
+  const uint64_t want = s.d <= kMostFlow ? s.rows + 7 : (s.rows + 7) / 8, cap = s.d <= kMostFlow ? sms : 2ull * sms;
   return (uint32_t)(want < 1 ? 1 : want < cap ? want : cap);
 }
 
@@ -653,18 +749,21 @@ int launch_held(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
                      (const T*)x, w, b, (T*)y, mean, rstd, group);
 }
 
-template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB, int EDGE = 0>
 int launch_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                 float* mean, float* rstd) {
-  constexpr size_t smem = Ring<T, V, EACH, ROWS, 1>::kBytes;
+  constexpr size_t smem =
+      std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 1, SUB, EDGE == 2>, Ring<T, V, EACH, ROWS, 1>>::kBytes;
   static std::atomic<uint64_t> done{0};
-  auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS, SUB>;
+  auto kernel = norm_flow_kernel<T, TW, V, EACH, ROWS, SUB, EDGE>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "layer_norm shared memory"));
-  const Plan p = flow_plan(s.rows, s.d, D.prof.sm_count, EACH, ROWS);
-  return launch_rows(kernel, p.blocks, p.threads, smem, D.stream, 1, s, (const T*)x, w, b, (T*)y, mean, rstd, p.group);
+  const uint32_t period = EDGE ? edge_period(s.rows, {s.ldx, s.ldy}, V) : 1;
+  const Plan p = flow_plan(s.rows, EDGE ? s.d + V - 1 : s.d, D.prof.sm_count, EACH, ROWS, period);
+  return launch_rows(kernel, p.blocks, p.threads, smem, D.stream, 1, s, (const T*)x, w, b, (T*)y, mean, rstd, p.group,
+                     period);
 }
 
-template <typename T, typename TW, int V>
+template <typename T, typename TW, int V, int EDGE>
 int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const void* b, void* y,
                 float* mean, float* rstd) {
   constexpr int kMid = V == 1 ? 16 : 32;
@@ -676,7 +775,16 @@ int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
   // half the warps at each barrier) from 512 columns on: 16384 x 4096 bf16 52
   // against 60 us, 60000 x 1024 45 against 54; f32 and narrow accesses do not.
   constexpr uint64_t kNarrow = sizeof(T) * V == 16 && sizeof(T) == 2 ? 512 : 4096;
-  if (s.d <= 128 && many)
+  if constexpr (EDGE != 0) {
+    const uint64_t span = s.d + V - 1;
+    if (span <= 128) return launch_flow<T, TW, V, 8, 4, true, EDGE>(D, s, x, w, b, y, mean, rstd);
+    // whichever has more rows at once, which is what a span just over a whole
+    // number of warps decides (60000 x 1021: 93 us, with 16 columns a thread 100)
+    const uint64_t wide = rows_at_once(span, 16, 2), narrow = span <= 4096 ? rows_at_once(span, 8, 4) : 0;
+    if (span <= kNarrow ? narrow >= wide : narrow > wide)
+      return launch_flow<T, TW, V, 8, 4, false, EDGE>(D, s, x, w, b, y, mean, rstd);
+    return launch_flow<T, TW, V, 16, 2, false, EDGE>(D, s, x, w, b, y, mean, rstd);
+  } else if (s.d <= 128 && many)
     return launch_flow<T, TW, V, 8, 4, true>(D, s, x, w, b, y, mean, rstd);
   else if (s.d <= kNarrow && many)
     return launch_flow<T, TW, V, 8, 4, false>(D, s, x, w, b, y, mean, rstd);
@@ -693,22 +801,24 @@ int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
                        (const T*)x, w, b, (T*)y, mean, rstd);
 }
 
-template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB>
+template <typename T, typename TW, int V, int EACH, int ROWS, bool SUB, int EDGE>
 int launch_grad_flow(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
                      const float* rstd, const void* dy, void* dx, float* work, uint32_t& parts) {
-  constexpr size_t ring = Ring<T, V, EACH, ROWS, 2>::kBytes;
+  constexpr size_t ring =
+      std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 2, SUB, EDGE == 2>, Ring<T, V, EACH, ROWS, 2>>::kBytes;
   static std::atomic<uint64_t> done{0};
-  auto kernel = norm_grad_flow_kernel<T, TW, V, EACH, ROWS, SUB>;
-  const Plan p = flow_plan(s.rows, s.d, D.prof.sm_count, EACH, ROWS);
+  auto kernel = norm_grad_flow_kernel<T, TW, V, EACH, ROWS, SUB, EDGE>;
+  const uint32_t period = EDGE ? edge_period(s.rows, {s.ldx, s.lddy, s.lddx}, V) : 1;
+  const Plan p = flow_plan(s.rows, EDGE ? s.d + V - 1 : s.d, D.prof.sm_count, EACH, ROWS, period);
   parts = p.blocks;
   const size_t sums = p.threads > p.group ? 2 * s.d * sizeof(float) : 0;  // at most 32 KB: d <= 4096
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, ring > 32768 ? ring : 32768,
                              "layer_norm_grad shared memory"));
   return launch_rows(kernel, p.blocks, p.threads, ring > sums ? ring : sums, D.stream, 1, s, (const T*)x, w, mean, rstd,
-                     (const T*)dy, (T*)dx, work, p.group);
+                     (const T*)dy, (T*)dx, work, p.group, period);
 }
 
-template <typename T, typename TW, int V>
+template <typename T, typename TW, int V, int EDGE>
 int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x, const void* w, const float* mean,
                      const float* rstd, const void* dy, void* dx, float* dw, float* db, float* work) {
   const int sms = D.prof.sm_count;
@@ -718,12 +828,13 @@ int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x,
   // as in the forward pass, but more registers hang on a column: 16384 x 4096
   // bf16 75 against 77 us, 60000 x 1024 73 against 69
   constexpr uint64_t kNarrow = sizeof(T) * V == 16 && sizeof(T) == 2 ? 2048 : 4096;
-  if (flow && s.d <= 128) {
-    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, true>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
-  } else if (flow && s.d <= kNarrow) {
-    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, false>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
+  const uint64_t span = EDGE ? s.d + V - 1 : s.d;
+  if (flow && span <= 128) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, true, EDGE>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
+  } else if (flow && (EDGE ? span <= 4096 && rows_at_once(span, 8, 2) >= rows_at_once(span, 16, 1) : span <= kNarrow)) {
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, false, EDGE>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (flow) {
-    MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1, false>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
+    MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1, false, EDGE>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (work) {
     // before dx is written, which may be dy
     MAPAL_TRY(launch_rows(norm_grad_cols_kernel<T, V>, dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0,
@@ -738,13 +849,25 @@ int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x,
   return 0;
 }
 
-// f(T, TW, V) for the site's types and the widest access (16, 4 or an element's
-// bytes) that a row is a multiple of and all arrays' rows begin at.
+// f(T, TW, V, EDGE) for the site's types and the widest access (16, 4 or an
+// element's bytes) that a row is a multiple of and all arrays' rows begin at;
+// edge (1 or 2): 16 bytes whatever the rows are, instead of single elements.
+// Pairs of 16-bit elements do without (30000 x 2046 bf16 74 and 101 us, with it
+// 75 and 137).
 template <typename F>
-int by_type(const MapalNormSite& s, int width, const void* w, const void* b, F&& f) {
+int by_type(const MapalNormSite& s, int width, int edge, const void* w, const void* b, F&& f0) {
   using std::integral_constant;
   const int ww = align_of(w, 0, 1) < align_of(b, 0, 1) ? align_of(w, 0, 1) : align_of(b, 0, 1);
   const int ws = dtype_bytes(s.wtype);
+  if (width >= (s.dtype == MAPAL_DTYPE_F32 ? 16 : 4) || ww < 16) edge = 0;
+  auto f = [&](auto t, auto tw, auto v) {
+    if constexpr (v.value * sizeof(t) == 16) {
+      if (edge == 1) return f0(t, tw, v, integral_constant<int, 1>{});
+      if (edge == 2) return f0(t, tw, v, integral_constant<int, 2>{});
+    }
+    return f0(t, tw, v, integral_constant<int, 0>{});
+  };
+  if (edge) width = 16;
   if (s.dtype == MAPAL_DTYPE_F32) {
     if (width >= 16 && ww >= 16) return f(float{}, float{}, integral_constant<int, 4>{});
     return f(float{}, float{}, integral_constant<int, 1>{});
@@ -757,6 +880,18 @@ int by_type(const MapalNormSite& s, int width, const void* w, const void* b, F&&
   const bool wide = s.wtype == MAPAL_DTYPE_F32;
   if (s.dtype == MAPAL_DTYPE_F16) return wide ? half(__half{}, float{}) : half(__half{}, __half{});
   return wide ? half(__nv_bfloat16{}, float{}) : half(__nv_bfloat16{}, __nv_bfloat16{});
+}
+
+// Whether the kernels for rows at odd places take these (arrays that begin at
+// a 16-byte boundary, rows that fit), and which: 1 where the inputs' rows begin
+// as the output's do, 2 where they are shifted.
+template <typename... A>
+int edge_rows(const MapalNormSite& s, std::initializer_list<uint64_t> ins, uint64_t out, A... arrays) {
+  const uint64_t v = 16 / dtype_bytes(s.dtype);
+  if (s.d + v - 1 > (uint64_t)kMostFlow || !(aligned16(arrays) && ...)) return 0;
+  for (const uint64_t ld : ins)
+    if (s.rows > 1 && (ld - out) % v != 0) return 2;
+  return 1;
 }
 
 int narrowest(std::initializer_list<int> widths) {
@@ -787,8 +922,11 @@ extern "C" int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site,
     MAPAL_TRY(on.rc);
     const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(y, site->ldy * es, site->rows),
                                  align_of(nullptr, site->d * es, 2)});
-    MAPAL_TRY(by_type(*site, width, w, b, [&](auto t, auto tw, auto v) {
-      return launch_norm<decltype(t), decltype(tw), v.value>(ctx->dev[0], *site, x, w, b, y, mean, rstd);
+    const DeviceSlot& D = ctx->dev[0];
+    const bool few = site->rows * site->d < kEdgeTurns * kFlow * D.prof.sm_count;
+    const int edge = few ? 0 : edge_rows(*site, {site->ldx}, site->ldy, x, y);
+    MAPAL_TRY(by_type(*site, width, edge, w, b, [&](auto t, auto tw, auto v, auto e) {
+      return launch_norm<decltype(t), decltype(tw), v.value, e.value>(D, *site, x, w, b, y, mean, rstd);
     }));
     return finish(ctx, 0, false);
   });
@@ -830,9 +968,13 @@ extern "C" int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* 
       return set_error(MAPAL_ERR_INVALID, "work is shorter than mapal_gpu_layer_norm_grad_workspace says");
     const int width = narrowest({align_of(x, site->ldx * es, site->rows), align_of(dy, site->lddy * es, site->rows),
                                  align_of(dx, site->lddx * es, site->rows), align_of(nullptr, site->d * es, 2)});
-    MAPAL_TRY(by_type(*site, width, w, w, [&](auto t, auto tw, auto v) {
-      return launch_norm_grad<decltype(t), decltype(tw), v.value>(ctx->dev[0], *site, x, w, mean, rstd, dy, dx, dw, db,
-                                                                  (float*)work);
+    // a few longer rows have more threads one by one (300 x 4091 bf16 11.4 us, 13.8)
+    const DeviceSlot& D = ctx->dev[0];
+    const bool few = site->d > 2040 && site->rows * site->d < 64ull * kFlow * D.prof.sm_count;
+    const int edge = few ? 0 : edge_rows(*site, {site->ldx, site->lddy}, site->lddx, x, dy, dx);
+    MAPAL_TRY(by_type(*site, width, edge, w, w, [&](auto t, auto tw, auto v, auto e) {
+      return launch_norm_grad<decltype(t), decltype(tw), v.value, e.value>(D, *site, x, w, mean, rstd, dy, dx, dw,
+                                                                            db, (float*)work);
     }));
     return finish(ctx, 0, false);
   });

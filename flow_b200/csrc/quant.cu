@@ -123,36 +123,50 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
 
 // ROWS rows at a time through the ring, a group of warps with EACH elements a
 // thread: rows that fit in a block's registers.
-template <typename T, int V, int EACH, int ROWS>
-__global__ void __launch_bounds__(kFlow, 1) quant_flow_kernel(const MapalQuantSite S, const T* __restrict__ x,
-                                                              int8_t* __restrict__ q, float* __restrict__ scale,
-                                                              int group) {
-  using R = Ring<T, V, EACH, ROWS, 1>;
+template <typename T, int V, int EACH, int ROWS, int EDGE>
+__global__ void __launch_bounds__(kFlow, 1) quant_flow_kernel(const MapalQuantSite S, const T* x, int8_t* q, float* scale,
+                                                              int group, uint32_t period) {
+  using R = std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 1, false, EDGE == 2>, Ring<T, V, EACH, ROWS, 1>>;
   using P = Pack<T, V>;
   constexpr int NV = EACH / V;
   __shared__ uint32_t sets[kFlow / 32][2][ROWS][16];
   extern __shared__ __align__(16) uint8_t dyn[];
-  R ring(dyn);
   const Group<false> G(group);
-  const int groups = blockDim.x / group, d = (int)S.d, lane = threadIdx.x & 31, warps = group / 32;
-  const uint64_t step = (uint64_t)gridDim.x * groups * ROWS;
-  uint64_t r = ((uint64_t)blockIdx.x * groups + G.id) * ROWS;
+  R ring(dyn, G);
+  const int d = (int)S.d, lane = threadIdx.x & 31, warps = group / 32;
+  const Turns<false, EDGE, ROWS> mine(G, period, S.rows);
+  uint64_t rows = mine.rows, ldx = mine.stride(S.ldx), ldq = mine.stride(S.ldq), r = mine.first;
+  const int shift = mine.template shift<T>(S.ldq), shift_x = mine.template shift<T>(S.ldx);
+  const std::conditional_t<EDGE != 0, Input<V, NV>, Whole> in(group, G.tid, d, shift_x, shift);
+  const std::conditional_t<EDGE != 0, Mine<V, NV>, Whole> part(group, G.tid, shift, d + shift);
+  const std::conditional_t<EDGE != 0, Masks<P, V, NV>, Whole> keep(part);
+  x = mine.at(x, S.ldx) - shift_x + (G.tid - in.back) * V;
+  q = mine.at(q, S.ldq) - shift + G.tid * V;
+  scale = mine.at(scale, 1);
+  if constexpr (EDGE != 0) {
+    pin(x), pin(q), pin(scale);
+    pin(rows), pin(ldx), pin(ldq);
+  }
   auto start = [&](int st, uint64_t row) {
 #pragma unroll
     for (int k = 0; k < ROWS; ++k)
-      if (row + k < S.rows) {
-        const T* from = x + (row + k) * S.ldx + G.tid * V;
+      if (row + k < rows) {
+        const T* from = x + (row + k) * ldx;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if ((j * group + G.tid) * V < d) ring.copy(st, k * NV + j, from + j * group * V);
+        for (int j = 0; j < NV; ++j) {
+          if constexpr (EDGE != 0)
+            ring.bring(st, k * NV + j, from + j * group * V, in.left[j]);
+          else if ((j * group + G.tid) * V < d)
+            ring.copy(st, k * NV + j, from + j * group * V);
+        }
       }
     ring.commit();
   };
   grid_wait();
   grid_go();
 #pragma unroll
-  for (int k = 0; k < R::kStages; ++k) start(k, r + k * step);
-  for (int par = 0; r < S.rows; r += step, par ^= 1) {
+  for (int k = 0; k < R::kStages; ++k) start(k, r + k * mine.step);
+  for (int par = 0; r < rows; r += mine.step, par ^= 1) {
     ring.wait();
     P v[ROWS][NV];
     uint32_t most[ROWS];
@@ -161,16 +175,21 @@ __global__ void __launch_bounds__(kFlow, 1) quant_flow_kernel(const MapalQuantSi
       Most<T> m;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if ((j * group + G.tid) * V < d && r + k < S.rows)
+        if constexpr (EDGE != 0) {
+          v[k][j] = ring.take(k * NV + j, in.by);
+          keep(v[k][j], j);
+        } else if ((j * group + G.tid) * V < d && r + k < rows) {
           v[k][j] = ring.take(k * NV + j);
-        else
+        } else {
           v[k][j].clear();
+        }
         m.add(v[k][j]);
       }
       most[k] = __reduce_max_sync(0xffffffffu, m.bits());
     }
-    start(ring.stage, r + R::kStages * step);  // this turn's slots have been read
-    ring.next();
+    if constexpr (EDGE != 0) ring.taken();
+    start(ring.stage, r + R::kStages * mine.step);  // this turn's slots have been read
+    ring.next_stage();
     if (warps > 1) {
       auto* red = sets[G.id][par];
       if (lane == 0)
@@ -182,16 +201,26 @@ __global__ void __launch_bounds__(kFlow, 1) quant_flow_kernel(const MapalQuantSi
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      if (r + k >= S.rows) break;
+      if (r + k >= rows) break;
       const RowScale rs = row_scale(float_bits<T>(most[k]));
-      int8_t* to = q + (r + k) * S.ldq + G.tid * V;
+      int8_t* to = q + (r + k) * ldq;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         uint32_t o[V >= 4 ? V / 4 : 1];
         quantize<T, V>(v[k][j], rs.inv, o);
-        if ((j * group + G.tid) * V < d) put<V>(to + j * group * V, o);
+        if constexpr (EDGE != 0) {
+          if (part.at(j) == part.kAll) {
+            put<V>(to + j * group * V, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (part.at(j) & (1u << e)) to[j * group * V + e] = (int8_t)(o[e / 4] >> (8 * (e % 4)));
+          }
+        } else if ((j * group + G.tid) * V < d) {
+          put<V>(to + j * group * V, o);
+        }
       }
-      if (G.tid == 0) scale[r + k] = rs.scale;
+      if (G.tid == 0) scale[(r + k) * mine.period] = rs.scale;
     }
   }
 }
@@ -246,16 +275,25 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const MapalQuantSite S
   }
 }
 
-template <typename T, int V, int EACH, int ROWS>
+template <typename T, int V, int EACH, int ROWS, int EDGE = 0>
 int launch_flow(const DeviceSlot& D, const MapalQuantSite& s, const T* x, int8_t* q, float* scale) {
-  constexpr size_t smem = Ring<T, V, EACH, ROWS, 1>::kBytes;
+  constexpr size_t smem =
+      std::conditional_t<EDGE != 0, EdgeRing<T, EACH, ROWS, 1, false, EDGE == 2>, Ring<T, V, EACH, ROWS, 1>>::kBytes;
   static std::atomic<uint64_t> done{0};
-  auto kernel = quant_flow_kernel<T, V, EACH, ROWS>;
+  auto kernel = quant_flow_kernel<T, V, EACH, ROWS, EDGE>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "quantize_rows shared memory"));
-  const int group = (int)((s.d + 32 * EACH - 1) / (32 * EACH)) * 32, threads = kFlow / group * group;
-  const uint64_t turn = (uint64_t)(threads / group) * ROWS, want = (s.rows + turn - 1) / turn;
-  const uint64_t cap = D.prof.sm_count;
-  return launch_rows(kernel, (unsigned)(want < cap ? want : cap), threads, smem, D.stream, 1, s, x, q, scale, group);
+  const uint32_t period = EDGE ? edge_period(s.rows, {s.ldx, s.ldq}, V) : 1;
+  const Plan p = flow_plan<false>(s.rows, EDGE ? s.d + V - 1 : s.d, D.prof.sm_count, EACH, ROWS, period);
+  return launch_rows(kernel, p.blocks, p.threads, smem, D.stream, 1, s, x, q, scale, p.group, period);
+}
+
+// Many rows at odd places.
+template <typename T, int V, int EDGE>
+int launch_edge(const DeviceSlot& D, const MapalQuantSite& s, const T* x, int8_t* q, float* scale) {
+  const uint64_t span = s.d + V - 1;
+  if (span <= 1024) return launch_flow<T, V, 8, 4, EDGE>(D, s, x, q, scale);
+  if (span <= 8192) return launch_flow<T, V, 16, 2, EDGE>(D, s, x, q, scale);
+  return launch_flow<T, V, 32, 1, EDGE>(D, s, x, q, scale);
 }
 
 template <typename T, int V>
@@ -281,11 +319,14 @@ template <typename T>
 int by_width(const DeviceSlot& D, const MapalQuantSite& s, const void* x, int8_t* q, float* scale) {
   const int xw = align_of(x, s.ldx * sizeof(T), s.rows), qw = align_of(q, s.ldq, s.rows), dw = align_of(nullptr, s.d, 2);
   auto fits = [&](int v) { return xw >= v * (int)sizeof(T) && qw >= v && dw >= v; };
-  if constexpr (sizeof(T) == 4) {
-    if (fits(4)) return launch_quant<T, 4>(D, s, x, q, scale);
-  } else {
-    if (fits(8)) return launch_quant<T, 8>(D, s, x, q, scale);
+  constexpr int V = 16 / sizeof(T);
+  if (fits(V)) return launch_quant<T, V>(D, s, x, q, scale);
+  if constexpr (sizeof(T) == 2)
     if (fits(2)) return launch_quant<T, 2>(D, s, x, q, scale);
+  if (s.d + V - 1 <= 16384 && s.rows * s.d >= kEdgeTurns * kFlow * D.prof.sm_count && aligned16(x) &&
+      align_of(q, 0, 1) >= V) {
+    if (s.rows > 1 && (s.ldx - s.ldq) % V != 0) return launch_edge<T, V, 2>(D, s, (const T*)x, q, scale);
+    return launch_edge<T, V, 1>(D, s, (const T*)x, q, scale);
   }
   return launch_quant<T, 1>(D, s, x, q, scale);
 }

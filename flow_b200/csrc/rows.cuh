@@ -100,6 +100,18 @@ struct alignas(sizeof(T) * V) Pack {
     for (int i = 0; i < (W == 0 ? 1 : W); ++i) w[i] = 0;
   }
 
+  // Zeros for the elements whose bits are not in m.
+  __device__ __forceinline__ void keep(uint32_t m) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = m & (1u << i) ? w[i] : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        w[i] &= (m & (1u << (2 * i)) ? 0xffffu : 0u) | (m & (2u << (2 * i)) ? 0xffff0000u : 0u);
+    }
+  }
+
   // Hides where the bits come from, so that a later use converts them again
   // instead of keeping the floats of an earlier one in registers.
   __device__ __forceinline__ void forget() {
@@ -138,6 +150,29 @@ __device__ __forceinline__ void st_once(P* p, const P& r) {
     static_assert(sizeof(P) == 2, "packs of 2, 4 or 16 bytes");
     __stcs(reinterpret_cast<unsigned short*>(p), r.w[0]);
   }
+}
+
+// The elements of a pack whose bits are in m, one by one.
+template <typename T, int V>
+__device__ __forceinline__ void st_part(T* p, const Pack<T, V>& r, uint32_t m) {
+  T v[V];
+  memcpy(v, r.w, sizeof(v));
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (m & (1u << e)) p[e] = v[e];
+}
+
+// Bytes sh..sh+15 of a (first) and b.
+__device__ __forceinline__ uint4 straddle(const uint4& a, const uint4& b, uint32_t sh) {
+  const bool by8 = sh & 8, by4 = sh & 4;
+  const uint32_t bits = (sh & 3) * 8;
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = by8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = by4 ? w[i + 1] : w[i];
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
 inline int dtype_bytes(int dtype) {

@@ -64,6 +64,18 @@ def test_quantize_many_rows(ctx, dtype, rows, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("xpad,pad", [(0, 0), (1, 1), (3, 0), (0, 7), (2, 6), (5, 13), (7, 8), (8, 4)])
+@pytest.mark.parametrize("rows,d", [(40001, 57), (20003, 121), (9003, 1013), (4507, 1025), (2205, 2043), (1203, 4093), (603, 8185),
+                                    (603, 8187), (301, 16369)])
+def test_quantize_rows_at_odd_places(ctx, rows, d, xpad, pad, dtype):
+    """Rows that begin and end inside an access; every third holds NaN and infinities, which share accesses with
+    the rows beside it."""
+    x = rows_of(rows, d, dtype, rows + d)
+    x[1::3, :9], x[1::3, -9:] = float("nan"), float("inf")
+    check_quant(ctx, Guarded(rows, d, dtype, xpad).put(x).t, pad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (4, 4), (16, 0), (7, 3), (8, 8)])
 @pytest.mark.parametrize("d", [40, 1000, 4096])
 def test_quantize_strides(ctx, dtype, pad, offset, d):

@@ -178,7 +178,61 @@ def test_many_rows(ctx, rows, d, pad, dtype):
     check(ctx, rows, d, dtype, dtype, pad=pad)
 
 
-@pytest.mark.parametrize("rows,d", [(80001, 64), (5003, 1021), (5003, 1024), (1203, 4096), (603, 8192), (303, 16384)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad", [0, 1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("rows,d", [(90001, 57), (60007, 121), (60003, 122), (22001, 249), (9003, 505), (4507, 1025), (2205, 2043),
+                                    (1207, 4089), (1203, 4093), (603, 8185)])
+def test_rows_at_odd_places(ctx, rows, d, pad, dtype):
+    """Rows that begin and end inside an access of 16 bytes: strides of every kind, neither the rows beside them
+    nor the gaps between them written."""
+    check(ctx, rows, d, dtype, torch.float32 if pad % 2 else dtype, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 15, 17, 149, 600])
+@pytest.mark.parametrize("d,pad", [(1, 0), (9, 0), (60, 1), (121, 0), (1021, 2), (8187, 0)])
+def test_gradient_of_a_few_rows_at_odd_places(ctx, rows, d, pad, dtype):
+    check(ctx, rows, d, dtype, dtype, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,d", [(40001, 61), (4507, 1027)])
+def test_values_beside_a_row_do_not_reach_it(ctx, dtype, rows, d):
+    """Every other row holds NaN and infinities, which share accesses with the rows beside them."""
+    x, dy = rows_of(rows, d, dtype, 3), rows_of(rows, d, dtype, 4)
+    x[1::2, :7], x[1::2, -7:] = float("nan"), float("inf")
+    dy[1::2] = float("nan")
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    mean, rstd, _, _ = run(ctx, x, None, None, y, dy, dx)
+    assert torch.isnan(y[1::2]).all() and torch.isnan(dx[1::2]).all()
+    x, dy, mean, rstd = x[::2], dy[::2], mean[::2], rstd[::2]
+    want, _, _, err, _, _ = formula(x, None, None)
+    assert_within(y[::2], want, err + out_error(want, dtype) * 1.01, "y")
+    want, _, _, err, _, _ = grad_formula(x, None, mean, rstd, dy)
+    assert_within(dx[::2], want, err + out_error(want, dtype) * 1.01, "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("strides", [(1021, 1029, 1037, 1021), (1024, 1021, 1021, 1024), (1022, 1026, 1022, 1030), (1021, 1022, 1023, 1024)])
+def test_arrays_of_different_strides(ctx, dtype, strides):
+    """Equal in where their rows begin, and not."""
+    rows, d = 5003, 1021
+    bufs = [torch.full((rows, ld), 7.0, device="cuda").to(dtype) for ld in strides]
+    x, y, dy, dx = (b[:, :d] for b in bufs)
+    x.copy_(rows_of(rows, d, dtype, 1))
+    dy.copy_(rows_of(rows, d, dtype, 2))
+    mean, rstd, dw, db = run(ctx, x, None, None, y, dy, dx, ldx=strides[0], ldy=strides[1], lddy=strides[2], lddx=strides[3])
+    want, _, _, err, _, _ = formula(x, None, None)
+    assert_within(y, want, err + out_error(want, dtype) * 1.01, "y")
+    want, gw, gb, err, gw_err, gb_err = grad_formula(x, None, mean, rstd, dy)
+    assert_within(dx, want, err + out_error(want, dtype) * 1.01, "dx")
+    assert_within(dw, gw, gw_err, "dw")
+    assert_within(db, gb, gb_err, "db")
+    for b in bufs:
+        assert (b[:, d:] == 7).all()
+
+
+@pytest.mark.parametrize("rows,d", [(80001, 64), (70001, 59), (1203, 4093), (5003, 1021), (5003, 1024), (1203, 4096), (603, 8192), (303, 16384)])
 def test_many_rows_in_place(ctx, rows, d):
     x, dy = rows_of(rows, d, torch.bfloat16, 5), rows_of(rows, d, torch.bfloat16, 6)
     y, dx = torch.empty_like(x), torch.empty_like(x)
