@@ -645,6 +645,93 @@ __global__ void __launch_bounds__(kThreads) norm_grad_rows_kernel(const MapalNor
   }
 }
 
+// dx of rows that a block's registers hold as they were read, EACH elements of
+// x and of dy a thread, with the weights in shared memory (f32 weights of 16384
+// columns do not stay in L1 beside the rows: 300 us for 8000 rows of bf16). Two
+// blocks an SM hide each other's barriers. 8000 x 16384 bf16 156 us, the kernel
+// above 396.
+template <typename T, typename TW, int V, int EACH>
+__global__ void __launch_bounds__(1024) norm_grad_held_kernel(const MapalNormSite S, const T* x, const TW* w,
+                                                              const float* mean, const float* rstd, const T* dy, T* dx) {
+  using P = Pack<T, V>;
+  constexpr int NV = EACH / V;
+  __shared__ float red[2][2][32];
+  extern __shared__ __align__(16) uint8_t dyn[];  // d weights
+  const int d = (int)S.d, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const float n = (float)d;
+  int par = 0;
+  grid_wait();
+  grid_go();
+  if (w) {
+    using U = Pack<TW, (V * sizeof(TW) > 16 ? 16 / sizeof(TW) : V)>;
+    constexpr int kU = sizeof(U) / sizeof(TW);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < d / kU; i += blockDim.x) reinterpret_cast<U*>(dyn)[i] = reinterpret_cast<const U*>(w)[i];
+    w = reinterpret_cast<const TW*>(dyn);
+    __syncthreads();
+  }
+  for (uint64_t r = blockIdx.x; r < S.rows; r += gridDim.x, par ^= 1) {
+    P a[NV], b[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * blockDim.x + threadIdx.x) * V;
+      if (i < d) {
+        a[j] = ld_once(reinterpret_cast<const P*>(x + r * S.ldx + i));
+        b[j] = ld_once(reinterpret_cast<const P*>(dy + r * S.lddy + i));
+      } else {
+        a[j].clear();
+        b[j].clear();
+      }
+    }
+    const float mu = __ldg(mean + r), rs = __ldg(rstd + r);
+    float c1 = 0.0f, c2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * blockDim.x + threadIdx.x) * V;
+      if (i < d) {
+        float fx[V], fy[V], fw[V];
+        a[j].get(fx);
+        b[j].get(fy);
+        weights<TW, V>(w, i, 1.0f, fw);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float g = fy[e] * fw[e];
+          c1 += g;
+          c2 = __fmaf_rn(g, (fx[e] - mu) * rs, c2);
+        }
+      }
+      asm volatile("" ::: "memory");  // keeps the weights' loads from piling up in registers
+    }
+    c1 = warp_sum(c1);
+    c2 = warp_sum(c2);
+    if (lane == 0) {
+      red[par][0][warp] = c1;
+      red[par][1][warp] = c2;
+    }
+    __syncthreads();
+    c1 = __fdiv_rn(warp_sum(lane < warps ? red[par][0][lane] : 0.0f), n);
+    c2 = __fdiv_rn(warp_sum(lane < warps ? red[par][1][lane] : 0.0f), n);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = (j * blockDim.x + threadIdx.x) * V;
+      if (i < d) {
+        a[j].forget();
+        b[j].forget();
+        float fx[V], fy[V], fw[V];
+        a[j].get(fx);
+        b[j].get(fy);
+        weights<TW, V>(w, i, 1.0f, fw);
+        P o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) fx[e] = __fmaf_rn(-((fx[e] - mu) * rs), c2, fy[e] * fw[e] - c1) * rs;
+        o.set(fx);
+        st_once(reinterpret_cast<P*>(dx + r * S.lddx + i), o);
+      }
+      asm volatile("" ::: "memory");
+    }
+  }
+}
+
 // dw and db over rows p*8 + sub, then every parts*8-th: part p's sums of 32*V columns.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const MapalNormSite S, const T* x, const float* mean,
@@ -727,9 +814,11 @@ int check_norm(const MapalNormSite* s) {
 }
 
 // Partial sums that the gradient's scratch has room for: a block each (up to 7
-// more than rows, so that their number suits every period).
+// more than rows, so that their number suits every period), and for longer rows
+// as many as give 16 blocks an SM or more.
 uint32_t grad_parts(const MapalNormSite& s, int sms) {
-  const uint64_t want = s.d <= kMostFlow ? s.rows + 7 : (s.rows + 7) / 8, cap = s.d <= kMostFlow ? sms : 2ull * sms;
+  const uint64_t want = s.d <= kMostFlow ? s.rows + 7 : (s.rows + 7) / 8,
+                 cap = s.d <= kMostFlow ? sms : (16ull * sms * 256 + s.d - 1) / s.d;
   return (uint32_t)(want < 1 ? 1 : want < cap ? want : cap);
 }
 
@@ -843,7 +932,16 @@ int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x,
   if (work)
     MAPAL_TRY(launch_rows(norm_grad_join_kernel, (unsigned)((2 * s.d + 31) / 32), 1024, 0, D.stream, 1, work, s.d, parts, dw,
                           db));
-  if (!flow && s.rows)
+  constexpr int kHeld = sizeof(T) * V == 16 && sizeof(T) == 2 ? 32 : 16;
+  if (!flow && s.rows && s.d <= 1024 * kHeld) {
+    const int threads = (int)((s.d + 32 * kHeld - 1) / (32 * kHeld)) * 32;
+    static std::atomic<uint64_t> done{0};
+    MAPAL_TRY(ensure_smem_attr(done, (const void*)norm_grad_held_kernel<T, TW, V, kHeld>, D.device, 1024 * kHeld * sizeof(TW),
+                               "layer_norm_grad shared memory"));
+    const uint64_t cap = (uint64_t)sms * (1024 / threads);
+    MAPAL_TRY(launch_rows(norm_grad_held_kernel<T, TW, V, kHeld>, (unsigned)(s.rows < cap ? s.rows : cap), threads,
+                          w ? s.d * sizeof(TW) : 0, D.stream, 1, s, (const T*)x, (const TW*)w, mean, rstd, (const T*)dy, (T*)dx));
+  } else if (!flow && s.rows)
     MAPAL_TRY(launch_rows(norm_grad_rows_kernel<T, TW, V>, row_blocks(s, sms), kThreads, 0, D.stream, 1, s, (const T*)x, w,
                           mean, rstd, (const T*)dy, (T*)dx));
   return 0;
