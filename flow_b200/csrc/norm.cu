@@ -867,6 +867,7 @@ int launch_norm(const DeviceSlot& D, const MapalNormSite& s, const void* x, cons
   if constexpr (EDGE != 0) {
     const uint64_t span = s.d + V - 1;
     if (span <= 128) return launch_flow<T, TW, V, 8, 4, true, EDGE>(D, s, x, w, b, y, mean, rstd);
+    if (span > kMostFlow) return launch_flow<T, TW, V, 32, 1, false, EDGE>(D, s, x, w, b, y, mean, rstd);
     // whichever has more rows at once, which is what a span just over a whole
     // number of warps decides (60000 x 1021: 93 us, with 16 columns a thread 100)
     const uint64_t wide = rows_at_once(span, 16, 2), narrow = span <= 4096 ? rows_at_once(span, 8, 4) : 0;
@@ -984,9 +985,9 @@ int by_type(const MapalNormSite& s, int width, int edge, const void* w, const vo
 // a 16-byte boundary, rows that fit), and which: 1 where the inputs' rows begin
 // as the output's do, 2 where they are shifted.
 template <typename... A>
-int edge_rows(const MapalNormSite& s, std::initializer_list<uint64_t> ins, uint64_t out, A... arrays) {
+int edge_rows(const MapalNormSite& s, uint64_t most, std::initializer_list<uint64_t> ins, uint64_t out, A... arrays) {
   const uint64_t v = 16 / dtype_bytes(s.dtype);
-  if (s.d + v - 1 > (uint64_t)kMostFlow || !(aligned16(arrays) && ...)) return 0;
+  if (s.d + v - 1 > most || !(aligned16(arrays) && ...)) return 0;
   for (const uint64_t ld : ins)
     if (s.rows > 1 && (ld - out) % v != 0) return 2;
   return 1;
@@ -1022,7 +1023,7 @@ extern "C" int mapal_gpu_layer_norm(MapalGpuCtx* ctx, const MapalNormSite* site,
                                  align_of(nullptr, site->d * es, 2)});
     const DeviceSlot& D = ctx->dev[0];
     const bool few = site->rows * site->d < kEdgeTurns * kFlow * D.prof.sm_count;
-    const int edge = few ? 0 : edge_rows(*site, {site->ldx}, site->ldy, x, y);
+    const int edge = few ? 0 : edge_rows(*site, 2 * kMostFlow, {site->ldx}, site->ldy, x, y);
     MAPAL_TRY(by_type(*site, width, edge, w, b, [&](auto t, auto tw, auto v, auto e) {
       return launch_norm<decltype(t), decltype(tw), v.value, e.value>(D, *site, x, w, b, y, mean, rstd);
     }));
@@ -1069,7 +1070,7 @@ extern "C" int mapal_gpu_layer_norm_grad(MapalGpuCtx* ctx, const MapalNormSite* 
     // a few longer rows have more threads one by one (300 x 4091 bf16 11.4 us, 13.8)
     const DeviceSlot& D = ctx->dev[0];
     const bool few = site->d > 2040 && site->rows * site->d < 64ull * kFlow * D.prof.sm_count;
-    const int edge = few ? 0 : edge_rows(*site, {site->ldx, site->lddy}, site->lddx, x, dy, dx);
+    const int edge = few ? 0 : edge_rows(*site, kMostFlow, {site->ldx, site->lddy}, site->lddx, x, dy, dx);
     MAPAL_TRY(by_type(*site, width, edge, w, w, [&](auto t, auto tw, auto v, auto e) {
       return launch_norm_grad<decltype(t), decltype(tw), v.value, e.value>(D, *site, x, w, mean, rstd, dy, dx, dw,
                                                                             db, (float*)work);

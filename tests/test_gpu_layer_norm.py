@@ -181,7 +181,7 @@ def test_many_rows(ctx, rows, d, pad, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pad", [0, 1, 2, 3, 4, 5, 6, 7, 8])
 @pytest.mark.parametrize("rows,d", [(90001, 57), (60007, 121), (60003, 122), (22001, 249), (9003, 505), (4507, 1025), (2205, 2043),
-                                    (1207, 4089), (1203, 4093), (603, 8185)])
+                                    (1207, 4089), (1203, 4093), (603, 8185), (303, 8187), (203, 12001), (151, 16377)])
 def test_rows_at_odd_places(ctx, rows, d, pad, dtype):
     """Rows that begin and end inside an access of 16 bytes: strides of every kind, neither the rows beside them
     nor the gaps between them written."""
