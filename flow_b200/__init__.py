@@ -99,6 +99,31 @@ _tensor = None  # torch.Tensor, and torch dtypes by MAPAL_DTYPE_* (4: int32), fr
 _dtypes: list = [None] * 5
 
 
+class _Direct:
+    """The row-wise operators without ctypes (flow_b200/_rows.so, binding/rows_py.cpp): each of its functions takes a
+    method's arguments and answers the status, or None for anything but plain tensors that pass the method's checks.
+    Bound when the first tensor is checked, since it is built against torch; until then every answer is None."""
+
+    def __init__(self):
+        none = lambda *a: None  # noqa: E731
+        for name in self.NAMES:
+            setattr(self, name, none)
+
+    NAMES = ("layer_norm", "layer_norm_grad", "expert_sort", "expert_dispatch", "expert_combine",
+             "expert_dispatch_grad", "expert_combine_grad", "quantize_rows_i8", "matmul_i8")
+
+    def bind(self):
+        from . import _rows
+        L = _native.load()
+        _rows.bind(tuple(ctypes.cast(getattr(L, "mapal_gpu_" + n), ctypes.c_void_p).value for n in self.NAMES),
+                   (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site))
+        for name in self.NAMES:
+            setattr(self, name, getattr(_rows, name))
+
+
+_direct = _Direct()
+
+
 def _span(rows: int, cols: int, ld: int) -> int:
     """Elements from the first to the last of rows x cols at row stride ld."""
     return (rows - 1) * ld + cols if rows and cols else 0
@@ -122,6 +147,7 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int, ldg: 
         import torch
         _dtypes[:] = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.int32
         _tensor = torch.Tensor
+        _direct.bind()
     if not 0 <= code < len(_dtypes) or t.dtype is not _dtypes[code]:
         raise ValueError(f"{what} is {t.dtype}, the record says {_dtypes[code] if 0 <= code < len(_dtypes) else code}")
     if t.get_device() != device:
@@ -351,6 +377,11 @@ class Context:
     # ---- rows of a model's layer (local device 0) --------------------------------------
     def layer_norm(self, site: NormSite, x, w, b, y, mean=None, rstd=None) -> None:
         """y = (x - mean(x)) / sqrt(var(x) + eps) * w + b for each row; mean and rstd for the gradient."""
+        rc = _direct.layer_norm(self._h, self.devices[0], site, x, w, b, y, mean, rstd)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, rows, d, t, ldx, ldy = self.devices[0], site.rows, site.d, site.dtype, site.ldx, site.ldy
         _check(_native.load().mapal_gpu_layer_norm(
             self._h, site, _buf(x, t, _span(rows, d, ldx), dev, "x", ldx),
@@ -367,6 +398,11 @@ class Context:
     def layer_norm_grad(self, site: NormSite, x, w, mean, rstd, dy, dx, dw, db, work) -> None:
         """dx, dw and db (f32; either may be None) of layer_norm. `work`: a CUDA buffer of at least
         layer_norm_grad_workspace(site) bytes, its own for calls that may overlap."""
+        rc = _direct.layer_norm_grad(self._h, self.devices[0], site, x, w, mean, rstd, dy, dx, dw, db, work)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
         if work is not None and work.get_device() != dev:
             raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
@@ -381,6 +417,11 @@ class Context:
     def expert_sort(self, site: ExpertSite, ids, offsets, order, pos) -> None:
         """Slots sorted by expert, stably: offsets (experts + 1), order (place -> slot; may be None) and pos
         (slot -> place, -1 where ids is -1), all int32."""
+        rc = _direct.expert_sort(self._h, self.devices[0], site, ids, offsets, order, pos)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, n = self.devices[0], site.tokens * site.k
         _check(_native.load().mapal_gpu_expert_sort(
             self._h, site, _buf(ids, 4, n, dev, "ids"),
@@ -389,6 +430,11 @@ class Context:
 
     def expert_dispatch(self, site: ExpertSite, x, pos, xs, scale=None, scale_out=None) -> None:
         """xs[pos[t, j]] = x[t], and scale_out likewise from scale (the scales of 8-bit rows)."""
+        rc = _direct.expert_dispatch(self._h, self.devices[0], site, x, pos, xs, scale, scale_out)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_dispatch(
             self._h, site, _buf(x, t, _span(tokens, d, site.ldt), dev, "x", site.ldt),
@@ -398,6 +444,11 @@ class Context:
 
     def expert_combine(self, site: ExpertSite, h, w, pos, y) -> None:
         """y[t] = sum over j of w[t, j] * h[pos[t, j]] (w None: 1)."""
+        rc = _direct.expert_combine(self._h, self.devices[0], site, h, w, pos, y)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_combine(
             self._h, site, _buf(h, t, _span(site.rows, d, site.ldr), dev, "h", site.ldr),
@@ -406,6 +457,11 @@ class Context:
 
     def expert_dispatch_grad(self, site: ExpertSite, dxs, pos, dx) -> None:
         """dx[t] = sum over j of dxs[pos[t, j]]."""
+        rc = _direct.expert_dispatch_grad(self._h, self.devices[0], site, dxs, pos, dx)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_dispatch_grad(
             self._h, site, _buf(dxs, t, _span(site.rows, d, site.ldr), dev, "dxs", site.ldr),
@@ -413,6 +469,11 @@ class Context:
 
     def expert_combine_grad(self, site: ExpertSite, h, w, pos, dy, dh, dw) -> None:
         """dh[pos[t, j]] = w[t, j] * dy[t] and dw[t, j] = <dy[t], h[pos[t, j]]> (dw may be None)."""
+        rc = _direct.expert_combine_grad(self._h, self.devices[0], site, h, w, pos, dy, dh, dw)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, t, d, tokens, n = self.devices[0], site.dtype, site.d, site.tokens, site.tokens * site.k
         sorted_span = _span(site.rows, d, site.ldr)
         _check(_native.load().mapal_gpu_expert_combine_grad(
@@ -422,6 +483,11 @@ class Context:
 
     def quantize_rows_i8(self, site: QuantSite, x, q, scale) -> None:
         """scale = max|x|/127 and q = x/scale rounded to int8, for each row."""
+        rc = _direct.quantize_rows_i8(self._h, self.devices[0], site, x, q, scale)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, rows, d = self.devices[0], site.rows, site.d
         _check(_native.load().mapal_gpu_quantize_rows_i8(
             self._h, site, _buf(x, site.dtype, _span(rows, d, site.ldx), dev, "x", site.ldx),
@@ -430,6 +496,11 @@ class Context:
     def matmul_i8(self, site: I8Site, A, scale_a, B, scale_b, C, offsets=None) -> None:
         """C[i] = (A[i] . B[g]^T) * scale_a[i] * scale_b[g] with exact integer sums; rows offsets[g] to
         offsets[g + 1] belong to g (offsets None: one matrix for all rows)."""
+        rc = _direct.matmul_i8(self._h, self.devices[0], site, A, scale_a, B, scale_b, C, offsets)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return
         dev, m, n, k, groups, ldb = self.devices[0], site.m, site.n, site.k, site.groups, site.ldb
         _check(_native.load().mapal_gpu_matmul_i8(
             self._h, site, _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),

@@ -6,7 +6,9 @@
 Each .cu / .cpp under flow_b200/csrc compiles to an object in
 flow_b200/_build; objects are rebuilt when their source or any header
 changed. nvcc links the CUDA runtime statically, so the library depends on
-the driver only; NCCL is bound at run time with dlopen.
+the driver only; NCCL is bound at run time with dlopen. flow_b200/_rows.so
+(binding/rows_py.cpp) lets the row-wise operators be called with torch tensors
+without ctypes; it is built against the installed torch's headers.
 """
 from __future__ import annotations
 
@@ -25,6 +27,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libmapal_gpu.so")
 DRIVER_SRC = os.path.join(HERE, "driver", "mapal_run.cpp")
 DRIVER = os.path.join(HERE, "mapal-run")
+ROWS_SRC = os.path.join(HERE, "binding", "rows_py.cpp")
+ROWS = os.path.join(HERE, "_rows.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -fmad=false: no multiply and add is ever contracted into an FMA (the
@@ -86,6 +90,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     build_driver(force)
+    build_rows(force)
     if verbose:
         print(LIB)
         print(DRIVER)
@@ -108,6 +113,32 @@ def build_driver(force: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"driver link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     return DRIVER
+
+
+def build_rows(force: bool = False) -> str:
+    """Compile the torch binding of the row-wise operators (flow_b200/_rows.so)."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    stamp = os.path.join(BUILD, "rows.txt")
+    made_for = f"{torch.__version__} {sys.version}"
+    same = os.path.exists(stamp) and open(stamp).read() == made_for
+    if not force and same and os.path.exists(ROWS) and os.path.getmtime(ROWS) >= max(os.path.getmtime(ROWS_SRC),
+                                                                                     _headers_mtime()):
+        return ROWS
+    cmd = ["g++"] + CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-shared",
+                                 "-isystem", os.path.join(root, "include"), "-isystem",
+                                 os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem",
+                                 sysconfig.get_path("include"), ROWS_SRC, "-o", ROWS, "-L", os.path.join(root, "lib"),
+                                 "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(made_for)
+    return ROWS
 
 
 def main() -> int:

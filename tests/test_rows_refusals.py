@@ -286,3 +286,52 @@ def test_wrapper_checks_the_stride_between_matrices(ctx):
         run(b[::2, :, :5], ldb=8)
     with pytest.raises(ValueError, match="row stride 8"):
         run(b[:2, :, :5])
+
+
+# ---- the calls without ctypes --------------------------------------------------------------------
+
+
+def test_direct_calls_take_what_the_methods_take(ctx):
+    """Plain tensors go through, as the refusal of the C entry shows; everything else is left to the method."""
+    i, f = torch.zeros(12, dtype=torch.int32), torch.zeros(64)
+    z = lambda *s: torch.zeros(*s)  # noqa: E731
+    with pytest.raises(fb.MapalInfraError, match="ctx is null"):
+        ctx.layer_norm(fb.norm_site(3, 5, "float32"), z(3, 5), None, None, z(3, 5))  # binds them
+    D, h = fb._direct, ctypes.c_void_p()
+    n, e, q = fb.norm_site(3, 5, "float32"), fb.expert_site(6, 2, 4, 5, "float32"), fb.quant_site(3, 5, "float32")
+    m = fb.matmul_i8_site(3, 4, 5, "float32", groups=2)
+    i8 = lambda *s: torch.zeros(*s, dtype=torch.int8)  # noqa: E731
+    calls = {
+        "layer_norm": (n, [z(3, 5), z(5), z(5), z(3, 5), z(3), z(3)]),
+        "layer_norm_grad": (n, [z(3, 5), z(5), z(3), z(3), z(3, 5), z(3, 5), z(5), z(5), z(64)]),
+        "expert_sort": (e, [i, i[:5].clone(), i, i]),
+        "expert_dispatch": (e, [z(6, 5), i, z(12, 5), z(6), z(12)]),
+        "expert_combine": (e, [z(12, 5), z(12), i, z(6, 5)]),
+        "expert_dispatch_grad": (e, [z(12, 5), i, z(6, 5)]),
+        "expert_combine_grad": (e, [z(12, 5), z(12), i, z(6, 5), z(12, 5), z(12)]),
+        "quantize_rows_i8": (q, [z(3, 5), i8(3, 5), z(3)]),
+        "matmul_i8": (m, [i8(3, 5), z(3), i8(2, 4, 5), z(2, 4), z(3, 4), i[:3].clone()]),
+    }
+    assert set(calls) == set(fb._Direct.NAMES)
+    for name, (site, args) in calls.items():
+        call = getattr(D, name)
+        # the C entry refuses the null context, or an address that is not as aligned as CPU memory happens to be
+        assert call(h, -1, site, *args) == INVALID, name
+        assert "null" in fb.lib().mapal_gpu_last_error().decode() or "align" in fb.lib().mapal_gpu_last_error().decode()
+        assert call(h, 0, site, *args) is None  # another device
+        assert call(None, -1, site, *args) is None and call(h, -1, None, *args) is None
+        assert call(h, -1, q if site is not q else n, *args) is None  # another record
+        assert call(h, -1, site, *args[:-1]) is None and call() is None
+        for k, t in enumerate(args):
+            for bad in (t.data_ptr(), "x", t.double(), t.flatten()[:-1]):
+                if name == "layer_norm_grad" and k == 8 and not isinstance(bad, (int, str)):
+                    continue  # scratch of any type; its length is the entry's to check
+                assert call(h, -1, site, *args[:k], bad, *args[k + 1:]) is None, (name, k)
+            wide = torch.stack([t, t], -1)[..., 0]  # every second element
+            if t.numel() > 1:
+                assert call(h, -1, site, *args[:k], wide, *args[k + 1:]) is None, (name, k)
+    # the record is read on every call
+    n.rows = 4
+    assert D.layer_norm(h, -1, n, *calls["layer_norm"][1]) is None
+    n.rows, n.d = 1, 4
+    assert D.layer_norm(h, -1, n, *calls["layer_norm"][1]) == INVALID
