@@ -663,14 +663,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * out_warps(
 
 // ---- operands that TMA cannot read ----------------------------------------------------
 //
-// Bases or strides off 16 bytes: eight warps bring a block of k at a time into a
+// Bases or strides off 16 bytes: sixteen warps bring a block of k at a time into a
 // raw ring with cp.async, as the aligned words of 16 bytes that hold it (nine
 // for a row's 128 bytes), and from there shift it into the swizzled layout. A
 // row's words are copied and read by the same eight lanes, so a warp waits for
 // nobody. Words that do not lie wholly inside the matrix are gathered byte by
 // byte. Everything else is as in the kernel of single CTAs.
 
-constexpr int kCopyThreads = 256;
+constexpr int kCopyThreads = 512;  // 4096 x 8192 x 4097: 0.55 ms, with 256 0.71
+constexpr int kCopyRows = kCopyThreads / 8;  // at a time
 constexpr int kAnyOut = 4;  // warps that write: the copies need the registers
 
 template <int NT, int STAGES>
@@ -704,12 +705,12 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p, const uint8_t* lo, con
 }
 
 // One operand of a tile as a copying thread sees it: 16 bytes of each 128 of
-// every 32nd row. 32 rows are a multiple of 16 bytes whatever the stride, so
-// the shift is the same for all of a thread's rows.
+// every kCopyRows-th row, which is a multiple of 16 bytes on whatever the
+// stride, so the shift is the same for all of a thread's rows.
 struct RowsAt {
   const uint8_t* mine;     // the aligned word of its first row at k = 0
   const uint8_t *lo, *hi;  // the matrix
-  uint64_t step;           // 32 rows
+  uint64_t step;           // kCopyRows rows
   uint32_t rows, k, sh;
   bool low;  // no word of the first block begins before the matrix
 
@@ -720,7 +721,7 @@ struct RowsAt {
     mine = p - sh;
     lo = from;
     hi = to;
-    step = 32 * ld;
+    step = kCopyRows * ld;
     rows = r;
     k = len;
     low = ((uintptr_t)first & 15) == 0 || first - 15 >= from;
@@ -734,15 +735,15 @@ struct RowsAt {
     if (k0 + kBlockK + 16 <= k && (low || k0 > 0)) {
       // every word lies in its row, give or take 15 bytes that the row or the matrix has
 #pragma unroll
-      for (int i = 0; i < ROWS / 32; ++i, w += step, to += 32 * 9 * 16)
-        if (r0 + i * 32 < rows) {
+      for (int i = 0; i < (ROWS + kCopyRows - 1) / kCopyRows; ++i, w += step, to += kCopyRows * 9 * 16)
+        if (r0 + i * kCopyRows < rows) {
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(w) : "memory");
           if (c == 7) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16), "l"(w + 16) : "memory");
         }
     } else {
 #pragma unroll 1
-      for (int i = 0; i < ROWS / 32; ++i, w += step, to += 32 * 9 * 16) {
-        if (r0 + i * 32 >= rows || at >= k) continue;
+      for (int i = 0; i < (ROWS + kCopyRows - 1) / kCopyRows; ++i, w += step, to += kCopyRows * 9 * 16) {
+        if (r0 + i * kCopyRows >= rows || at >= k) continue;
         word(to, w);
         // the next lane's word too where that lane has nothing to copy
         if (c == 7 || at + 16 >= k) word(to + 16, w + 16);
@@ -766,8 +767,9 @@ struct RowsAt {
     tile += r0 * kBlockK + ((c ^ (r0 & 7)) << 4);
     const uint32_t left = k <= at ? 0 : k - at;
 #pragma unroll
-    for (int i = 0; i < ROWS / 32; ++i) {
-      const uint4* w = reinterpret_cast<const uint4*>(raw + i * (32 * 9 * 16));
+    for (int i = 0; i < (ROWS + kCopyRows - 1) / kCopyRows; ++i) {
+      if (ROWS % kCopyRows && r0 + i * kCopyRows >= ROWS) break;
+      const uint4* w = reinterpret_cast<const uint4*>(raw + i * (kCopyRows * 9 * 16));
       uint4 v = straddle(w[0], w[1], sh);
       if (left < 16) {  // zeros behind k
         uint32_t q[4] = {v.x, v.y, v.z, v.w};
@@ -776,7 +778,7 @@ struct RowsAt {
           q[j] = left >= 4 * j + 4 ? q[j] : left <= 4 * j ? 0u : q[j] & ((1u << (8 * (left - 4 * j))) - 1);
         v = make_uint4(q[0], q[1], q[2], q[3]);
       }
-      *reinterpret_cast<uint4*>(tile + i * (32 * kBlockK)) = v;
+      *reinterpret_cast<uint4*>(tile + i * (kCopyRows * kBlockK)) = v;
     }
   }
 };
@@ -1093,7 +1095,8 @@ int run(const DeviceSlot& D, const MapalI8Site& s, const int8_t* A, const float*
   }
   if (!tma_reads(s, A, B)) {
     // the rows that an SM brings for a block of k, over its waves of tiles (81 x
-    // 2299 x 1073: 19.7 us with 18 tiles of 128 tokens, 14.1 with 54 of 32)
+    // 2299 x 1073: 19.7 us with 18 tiles of 128 tokens, 14.1 with 54 of 32, both
+    // with 256 copying threads)
     const uint64_t few = tiles_of(s, offsets, {128, 32, 1}), wide = tiles_of(s, offsets, {128, 128, 1});
     const uint64_t sms = D.prof.sm_count;
     if ((few + sms - 1) / sms * (128 + 32) <= (wide + sms - 1) / sms * (128 + 128)) return launch_any<T, 32, 5>(D, s, A, B, P, few);
