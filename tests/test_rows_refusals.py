@@ -330,6 +330,13 @@ def test_direct_calls_take_what_the_methods_take(ctx):
             wide = torch.stack([t, t], -1)[..., 0]  # every second element
             if t.numel() > 1:
                 assert call(h, -1, site, *args[:k], wide, *args[k + 1:]) is None, (name, k)
+    # matrices at the record's stride go through, others are left to the method
+    s = fb.norm_site(3, 5, "float32", ldx=8, ldy=7)
+    x, y = torch.zeros(3, 8), torch.zeros(3, 7)
+    for a, b, ok in ((x[:, :5], y[:, 1:6], True), (x[:, 1:6], y[:, 2:], True), (x[:, :5], z(3, 9)[:, :5], False),
+                     (x[:, :5].t(), y[:, :5], False), (x[:2, :5], y[:, :5], True), (x[1:, :5], y[:, :5], False),
+                     (x[:1, :5], y[:, :5], False), (x.view(3, 2, 4)[:, :, :3], y[:, :5], False)):
+        assert (D.layer_norm(h, -1, s, a, None, None, b, None, None) is not None) is ok
     # the record is read on every call
     n.rows = 4
     assert D.layer_norm(h, -1, n, *calls["layer_norm"][1]) is None
