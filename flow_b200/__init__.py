@@ -113,8 +113,11 @@ class _Direct:
              "expert_dispatch_grad", "expert_combine_grad", "quantize_rows_i8", "matmul_i8")
 
     def bind(self):
-        from . import _rows
         L = _native.load()
+        try:
+            from . import _rows
+        except ImportError as e:
+            raise MapalInfraError(ERR_INVALID, f"flow_b200/_rows.so: {e}; build it with: python -m flow_b200.build") from e
         _rows.bind(tuple(ctypes.cast(getattr(L, "mapal_gpu_" + n), ctypes.c_void_p).value for n in self.NAMES),
                    (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site))
         for name in self.NAMES:
@@ -146,8 +149,8 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int, ldg: 
     if _tensor is None:
         import torch
         _dtypes[:] = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.int32
-        _tensor = torch.Tensor
         _direct.bind()
+        _tensor = torch.Tensor
     if not 0 <= code < len(_dtypes) or t.dtype is not _dtypes[code]:
         raise ValueError(f"{what} is {t.dtype}, the record says {_dtypes[code] if 0 <= code < len(_dtypes) else code}")
     if t.get_device() != device:

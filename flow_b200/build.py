@@ -116,9 +116,12 @@ def build_driver(force: bool = False) -> str:
 
 
 def build_rows(force: bool = False) -> str:
-    """Compile the torch binding of the row-wise operators (flow_b200/_rows.so)."""
+    """Compile the torch binding of the row-wise operators (flow_b200/_rows.so); without torch there is none."""
+    import importlib.util
     import sysconfig
 
+    if importlib.util.find_spec("torch") is None:
+        return ""
     import torch
 
     root = os.path.dirname(torch.__file__)
