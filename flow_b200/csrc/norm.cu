@@ -732,7 +732,8 @@ __global__ void __launch_bounds__(1024) norm_grad_held_kernel(const MapalNormSit
   }
 }
 
-// dw and db over rows p*8 + sub, then every parts*8-th: part p's sums of 32*V columns.
+// dw and db over rows p*8 + sub, then every parts*8-th: part p's sums of 32*V
+// columns. A row is a whole number of packs (V divides d).
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const MapalNormSite S, const T* x, const float* mean,
                                                                   const float* rstd, const T* dy, float* work,
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(kThreads) norm_grad_cols_kernel(const MapalNor
   }
 }
 
-// dw and db from the parts' sums: 32 runs of parts in order, then the runs.
+// dw and db from the parts' sums: 32 runs of parts in order, then the runs. No parts: zeros.
 __global__ void __launch_bounds__(1024) norm_grad_join_kernel(const float* __restrict__ work, uint64_t d,
                                                                   uint32_t parts, float* dw, float* db) {
   __shared__ float red[32][33];
@@ -925,26 +926,33 @@ int launch_norm_grad(const DeviceSlot& D, const MapalNormSite& s, const void* x,
     MAPAL_TRY((launch_grad_flow<T, TW, V, 8, 2, false, EDGE>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
   } else if (flow) {
     MAPAL_TRY((launch_grad_flow<T, TW, V, 16, 1, false, EDGE>(D, s, x, w, mean, rstd, dy, dx, work, parts)));
-  } else if (work) {
-    // before dx is written, which may be dy
-    MAPAL_TRY(launch_rows(norm_grad_cols_kernel<T, V>, dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads, 0,
-                          D.stream, 1, s, (const T*)x, mean, rstd, (const T*)dy, work, parts));
+  } else if (s.rows == 0) {
+    parts = 0;  // sums over no rows: the join writes zeros and reads nothing
+  } else if constexpr (EDGE == 0) {
+    // rows of more than kMostFlow elements, which are whole accesses (V divides d): edge_rows takes none of them
+    if (work)  // before dx is written, which may be dy
+      MAPAL_TRY(launch_rows(norm_grad_cols_kernel<T, V>, dim3((unsigned)((s.d + 32 * V - 1) / (32 * V)), parts), kThreads,
+                            0, D.stream, 1, s, (const T*)x, mean, rstd, (const T*)dy, work, parts));
   }
   if (work)
     MAPAL_TRY(launch_rows(norm_grad_join_kernel, (unsigned)((2 * s.d + 31) / 32), 1024, 0, D.stream, 1, work, s.d, parts, dw,
                           db));
-  constexpr int kHeld = sizeof(T) * V == 16 && sizeof(T) == 2 ? 32 : 16;
-  if (!flow && s.rows && s.d <= 1024 * kHeld) {
-    const int threads = (int)((s.d + 32 * kHeld - 1) / (32 * kHeld)) * 32;
-    static std::atomic<uint64_t> done{0};
-    MAPAL_TRY(ensure_smem_attr(done, (const void*)norm_grad_held_kernel<T, TW, V, kHeld>, D.device, 1024 * kHeld * sizeof(TW),
-                               "layer_norm_grad shared memory"));
-    const uint64_t cap = (uint64_t)sms * (1024 / threads);
-    MAPAL_TRY(launch_rows(norm_grad_held_kernel<T, TW, V, kHeld>, (unsigned)(s.rows < cap ? s.rows : cap), threads,
-                          w ? s.d * sizeof(TW) : 0, D.stream, 1, s, (const T*)x, (const TW*)w, mean, rstd, (const T*)dy, (T*)dx));
-  } else if (!flow && s.rows)
-    MAPAL_TRY(launch_rows(norm_grad_rows_kernel<T, TW, V>, row_blocks(s, sms), kThreads, 0, D.stream, 1, s, (const T*)x, w,
-                          mean, rstd, (const T*)dy, (T*)dx));
+  if constexpr (EDGE == 0) {
+    constexpr int kHeld = sizeof(T) * V == 16 && sizeof(T) == 2 ? 32 : 16;
+    if (!flow && s.rows && s.d <= 1024 * kHeld) {
+      const int threads = (int)((s.d + 32 * kHeld - 1) / (32 * kHeld)) * 32;
+      static std::atomic<uint64_t> done{0};
+      MAPAL_TRY(ensure_smem_attr(done, (const void*)norm_grad_held_kernel<T, TW, V, kHeld>, D.device,
+                                 1024 * kHeld * sizeof(TW), "layer_norm_grad shared memory"));
+      const uint64_t cap = (uint64_t)sms * (1024 / threads);
+      MAPAL_TRY(launch_rows(norm_grad_held_kernel<T, TW, V, kHeld>, (unsigned)(s.rows < cap ? s.rows : cap), threads,
+                            w ? s.d * sizeof(TW) : 0, D.stream, 1, s, (const T*)x, (const TW*)w, mean, rstd, (const T*)dy,
+                            (T*)dx));
+    } else if (!flow && s.rows) {
+      MAPAL_TRY(launch_rows(norm_grad_rows_kernel<T, TW, V>, row_blocks(s, sms), kThreads, 0, D.stream, 1, s, (const T*)x,
+                            w, mean, rstd, (const T*)dy, (T*)dx));
+    }
+  }
   return 0;
 }
 
