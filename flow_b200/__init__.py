@@ -95,6 +95,7 @@ def _arr(ptrs: Sequence) -> ctypes.Array:
     return (ctypes.c_void_p * len(ptrs))(*[_ptr(p) for p in ptrs])
 
 
+_SHORT = 1 << 16  # of a direct call: not a status, see binding/rows_py.cpp
 _tensor = None  # torch.Tensor, and torch dtypes by MAPAL_DTYPE_* (4: int32), from the first tensor on
 _dtypes: list = [None] * 5
 
@@ -132,17 +133,28 @@ def _span(rows: int, cols: int, ld: int) -> int:
     return (rows - 1) * ld + cols if rows and cols else 0
 
 
-def _buf(t, code: int, need: int, device: int, what: str, ld: int = 0, ldg: int = 0):
+def _buf(t, code: int, n: int, device: int, what: str):
     """Address of a device buffer of a row-wise operator: None, an int address taken as given, or a torch tensor,
-    which must be of the record's type, on the context's device, with `need` elements from its first. A view must lie
-    as the record says: rows at stride `ld` (matrices at `ldg`), whatever dimensions they are counted by."""
+    which must be of the record's type, on the context's device, contiguous, with `n` elements of its own."""
+    if (t.__class__ is _tensor and t.dtype is _dtypes[code] and t.get_device() == device and t.numel() >= n
+            and t.is_contiguous()):
+        return t.data_ptr()
+    return t if t is None else _buf_checked(t, code, n, device, what, 1, n, 0, 1, 0)
+
+
+def _mat(t, code: int, rows: int, cols: int, ld: int, device: int, what: str, groups: int = 1, ldg: int = 0):
+    """The same of rows x cols elements at row stride `ld` (`groups` matrices at `ldg`). A view must lie as the
+    record says, whatever dimensions its rows are counted by, and hold all of the record's rows and columns itself:
+    what lies behind a slice in its storage is not the call's."""
+    need = _span(groups, _span(rows, cols, ld), ldg)
     if (t.__class__ is _tensor and t.dtype is _dtypes[code] and t.get_device() == device and t.numel() >= need
             and t.is_contiguous()):
         return t.data_ptr()
-    return t if t is None else _buf_checked(t, code, need, device, what, ld, ldg)
+    return t if t is None else _buf_checked(t, code, need, device, what, rows, cols, ld, groups, ldg)
 
 
-def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int, ldg: int) -> int:
+def _buf_checked(t, code: int, need: int, device: int, what: str, rows: int, cols: int, ld: int, groups: int,
+                 ldg: int) -> int:
     global _tensor
     if isinstance(t, int):
         return t
@@ -171,10 +183,28 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, ld: int, ldg: 
                     raise ValueError(f"{what} has row stride {t.stride(i)}, the record says {ld}" if step == ld else
                                      f"{what} has stride {t.stride(i)} in dimension {i}, the record says {step}")
                 step *= t.size(i)
-        have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-        if have < need:
-            raise ValueError(f"{what} holds {have} elements, the record needs {need}")
+        if t.is_contiguous():
+            raise ValueError(f"{what} holds {t.numel()} elements, the record needs {need}")
+        if need:
+            _check_extent(t, what, rows, cols, ld, groups, ldg)
     return t.data_ptr()
+
+
+def _check_extent(t, what: str, rows: int, cols: int, ld: int, groups: int, ldg: int) -> None:
+    """Whether a view of evenly spaced rows holds the record's."""
+    if ldg and t.dim() == 3:
+        have = t.size(0), t.size(1), t.size(2)
+        if have[0] < groups or have[1] < rows or have[2] < cols:
+            raise ValueError(f"{what} holds {have[0]} matrices of {have[1]} x {have[2]} elements, the record needs "
+                             f"{groups} of {rows} x {cols}")
+        return
+    if groups > 1:
+        if ldg % ld:
+            raise ValueError(f"{what}: matrices {ldg} elements apart are not among its rows at stride {ld}")
+        rows += (groups - 1) * (ldg // ld)
+    have = t.numel() // t.size(-1)
+    if have < rows or t.size(-1) < cols:
+        raise ValueError(f"{what} holds {have} rows of {t.size(-1)} elements, the record needs {rows} of {cols}")
 
 
 def _u64s(vals: Sequence[int]) -> ctypes.Array:
@@ -381,15 +411,15 @@ class Context:
     def layer_norm(self, site: NormSite, x, w, b, y, mean=None, rstd=None) -> None:
         """y = (x - mean(x)) / sqrt(var(x) + eps) * w + b for each row; mean and rstd for the gradient."""
         rc = _direct.layer_norm(self._h, self.devices[0], site, x, w, b, y, mean, rstd)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, rows, d, t, ldx, ldy = self.devices[0], site.rows, site.d, site.dtype, site.ldx, site.ldy
         _check(_native.load().mapal_gpu_layer_norm(
-            self._h, site, _buf(x, t, _span(rows, d, ldx), dev, "x", ldx),
+            self._h, site, _mat(x, t, rows, d, ldx, dev, "x"),
             _buf(w, site.wtype, d, dev, "w"), _buf(b, site.wtype, d, dev, "b"),
-            _buf(y, t, _span(rows, d, ldy), dev, "y", ldy), _buf(mean, 0, rows, dev, "mean"),
+            _mat(y, t, rows, d, ldy, dev, "y"), _buf(mean, 0, rows, dev, "mean"),
             _buf(rstd, 0, rows, dev, "rstd")))
 
     def layer_norm_grad_workspace(self, site: NormSite) -> int:
@@ -402,7 +432,7 @@ class Context:
         """dx, dw and db (f32; either may be None) of layer_norm. `work`: a CUDA buffer of at least
         layer_norm_grad_workspace(site) bytes, its own for calls that may overlap."""
         rc = _direct.layer_norm_grad(self._h, self.devices[0], site, x, w, mean, rstd, dy, dx, dw, db, work)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
@@ -410,10 +440,10 @@ class Context:
         if work is not None and work.get_device() != dev:
             raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
         _check(_native.load().mapal_gpu_layer_norm_grad(
-            self._h, site, _buf(x, t, _span(rows, d, site.ldx), dev, "x", site.ldx),
+            self._h, site, _mat(x, t, rows, d, site.ldx, dev, "x"),
             _buf(w, site.wtype, d, dev, "w"), _buf(mean, 0, rows, dev, "mean"), _buf(rstd, 0, rows, dev, "rstd"),
-            _buf(dy, t, _span(rows, d, site.lddy), dev, "dy", site.lddy),
-            _buf(dx, t, _span(rows, d, site.lddx), dev, "dx", site.lddx), _buf(dw, 0, d, dev, "dw"),
+            _mat(dy, t, rows, d, site.lddy, dev, "dy"),
+            _mat(dx, t, rows, d, site.lddx, dev, "dx"), _buf(dw, 0, d, dev, "dw"),
             _buf(db, 0, d, dev, "db"), 0 if work is None else work.data_ptr(),
             0 if work is None else work.numel() * work.element_size()))
 
@@ -421,7 +451,7 @@ class Context:
         """Slots sorted by expert, stably: offsets (experts + 1), order (place -> slot; may be None) and pos
         (slot -> place, -1 where ids is -1), all int32."""
         rc = _direct.expert_sort(self._h, self.devices[0], site, ids, offsets, order, pos)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
@@ -434,83 +464,82 @@ class Context:
     def expert_dispatch(self, site: ExpertSite, x, pos, xs, scale=None, scale_out=None) -> None:
         """xs[pos[t, j]] = x[t], and scale_out likewise from scale (the scales of 8-bit rows)."""
         rc = _direct.expert_dispatch(self._h, self.devices[0], site, x, pos, xs, scale, scale_out)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_dispatch(
-            self._h, site, _buf(x, t, _span(tokens, d, site.ldt), dev, "x", site.ldt),
+            self._h, site, _mat(x, t, tokens, d, site.ldt, dev, "x"),
             _buf(scale, 0, tokens, dev, "scale"), _buf(pos, 4, tokens * site.k, dev, "pos"),
-            _buf(xs, t, _span(site.rows, d, site.ldr), dev, "xs", site.ldr),
+            _mat(xs, t, site.rows, d, site.ldr, dev, "xs"),
             _buf(scale_out, 0, site.rows, dev, "scale_out")))
 
     def expert_combine(self, site: ExpertSite, h, w, pos, y) -> None:
         """y[t] = sum over j of w[t, j] * h[pos[t, j]] (w None: 1)."""
         rc = _direct.expert_combine(self._h, self.devices[0], site, h, w, pos, y)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_combine(
-            self._h, site, _buf(h, t, _span(site.rows, d, site.ldr), dev, "h", site.ldr),
+            self._h, site, _mat(h, t, site.rows, d, site.ldr, dev, "h"),
             _buf(w, 0, tokens * site.k, dev, "w"), _buf(pos, 4, tokens * site.k, dev, "pos"),
-            _buf(y, t, _span(tokens, d, site.ldt), dev, "y", site.ldt)))
+            _mat(y, t, tokens, d, site.ldt, dev, "y")))
 
     def expert_dispatch_grad(self, site: ExpertSite, dxs, pos, dx) -> None:
         """dx[t] = sum over j of dxs[pos[t, j]]."""
         rc = _direct.expert_dispatch_grad(self._h, self.devices[0], site, dxs, pos, dx)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, t, d, tokens = self.devices[0], site.dtype, site.d, site.tokens
         _check(_native.load().mapal_gpu_expert_dispatch_grad(
-            self._h, site, _buf(dxs, t, _span(site.rows, d, site.ldr), dev, "dxs", site.ldr),
-            _buf(pos, 4, tokens * site.k, dev, "pos"), _buf(dx, t, _span(tokens, d, site.ldt), dev, "dx", site.ldt)))
+            self._h, site, _mat(dxs, t, site.rows, d, site.ldr, dev, "dxs"),
+            _buf(pos, 4, tokens * site.k, dev, "pos"), _mat(dx, t, tokens, d, site.ldt, dev, "dx")))
 
     def expert_combine_grad(self, site: ExpertSite, h, w, pos, dy, dh, dw) -> None:
         """dh[pos[t, j]] = w[t, j] * dy[t] and dw[t, j] = <dy[t], h[pos[t, j]]> (dw may be None)."""
         rc = _direct.expert_combine_grad(self._h, self.devices[0], site, h, w, pos, dy, dh, dw)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, t, d, tokens, n = self.devices[0], site.dtype, site.d, site.tokens, site.tokens * site.k
-        sorted_span = _span(site.rows, d, site.ldr)
         _check(_native.load().mapal_gpu_expert_combine_grad(
-            self._h, site, _buf(h, t, sorted_span, dev, "h", site.ldr), _buf(w, 0, n, dev, "w"),
-            _buf(pos, 4, n, dev, "pos"), _buf(dy, t, _span(tokens, d, site.ldt), dev, "dy", site.ldt),
-            _buf(dh, t, sorted_span, dev, "dh", site.ldr), _buf(dw, 0, n, dev, "dw")))
+            self._h, site, _mat(h, t, site.rows, d, site.ldr, dev, "h"), _buf(w, 0, n, dev, "w"),
+            _buf(pos, 4, n, dev, "pos"), _mat(dy, t, tokens, d, site.ldt, dev, "dy"),
+            _mat(dh, t, site.rows, d, site.ldr, dev, "dh"), _buf(dw, 0, n, dev, "dw")))
 
     def quantize_rows_i8(self, site: QuantSite, x, q, scale) -> None:
         """scale = max|x|/127 and q = x/scale rounded to int8, for each row."""
         rc = _direct.quantize_rows_i8(self._h, self.devices[0], site, x, q, scale)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, rows, d = self.devices[0], site.rows, site.d
         _check(_native.load().mapal_gpu_quantize_rows_i8(
-            self._h, site, _buf(x, site.dtype, _span(rows, d, site.ldx), dev, "x", site.ldx),
-            _buf(q, 3, _span(rows, d, site.ldq), dev, "q", site.ldq), _buf(scale, 0, rows, dev, "scale")))
+            self._h, site, _mat(x, site.dtype, rows, d, site.ldx, dev, "x"),
+            _mat(q, 3, rows, d, site.ldq, dev, "q"), _buf(scale, 0, rows, dev, "scale")))
 
     def matmul_i8(self, site: I8Site, A, scale_a, B, scale_b, C, offsets=None) -> None:
         """C[i] = (A[i] . B[g]^T) * scale_a[i] * scale_b[g] with exact integer sums; rows offsets[g] to
         offsets[g + 1] belong to g (offsets None: one matrix for all rows)."""
         rc = _direct.matmul_i8(self._h, self.devices[0], site, A, scale_a, B, scale_b, C, offsets)
-        if rc is not None:
+        if rc is not None and rc != _SHORT:
             if rc:
                 _check(rc)
             return
         dev, m, n, k, groups, ldb = self.devices[0], site.m, site.n, site.k, site.groups, site.ldb
         _check(_native.load().mapal_gpu_matmul_i8(
-            self._h, site, _buf(A, 3, _span(m, k, site.lda), dev, "A", site.lda),
+            self._h, site, _mat(A, 3, m, k, site.lda, dev, "A"),
             _buf(scale_a, 0, m, dev, "scale_a"),
-            _buf(B, 3, _span(groups, _span(n, k, ldb), site.ldg), dev, "B", ldb, site.ldg),
+            _mat(B, 3, n, k, ldb, dev, "B", groups, site.ldg),
             _buf(scale_b, 0, groups * n, dev, "scale_b"), _buf(offsets, 4, groups + 1, dev, "offsets"),
-            _buf(C, site.dtype, _span(m, n, site.ldc), dev, "C", site.ldc)))
+            _mat(C, site.dtype, m, n, site.ldc, dev, "C")))
 
     # ---- sharded sites (one buffer per local device) --------------------------------
     def saxpy_sharded(self, a: float, xs, y0s, outs) -> None:
