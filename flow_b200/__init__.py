@@ -429,7 +429,7 @@ class Context:
         return n.value
 
     def layer_norm_grad(self, site: NormSite, x, w, mean, rstd, dy, dx, dw, db, work) -> None:
-        """dx, dw and db (f32; either may be None) of layer_norm. `work`: a CUDA buffer of at least
+        """dx, dw and db (f32; either may be None) of layer_norm. `work`: a contiguous CUDA buffer of at least
         layer_norm_grad_workspace(site) bytes, its own for calls that may overlap."""
         rc = _direct.layer_norm_grad(self._h, self.devices[0], site, x, w, mean, rstd, dy, dx, dw, db, work)
         if rc is not None and rc != _SHORT:
@@ -439,6 +439,8 @@ class Context:
         dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
         if work is not None and work.get_device() != dev:
             raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
+        if work is not None and not work.is_contiguous():  # its bytes would not be numel() elements in a row
+            raise ValueError("work must be contiguous")
         _check(_native.load().mapal_gpu_layer_norm_grad(
             self._h, site, _mat(x, t, rows, d, site.ldx, dev, "x"),
             _buf(w, site.wtype, d, dev, "w"), _buf(mean, 0, rows, dev, "mean"), _buf(rstd, 0, rows, dev, "rstd"),

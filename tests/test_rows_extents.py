@@ -133,3 +133,21 @@ def test_a_record_of_nothing_takes_any_slice(ctx):
     x = torch.zeros(4, 8)[:, :5]
     with pytest.raises(fb.MapalInfraError, match="ctx is null"):
         ctx.expert_combine(fb.expert_site(3, 2, 4, 5, F, rows=0, ldr=8), x[:, :3], None, torch.zeros(6, dtype=I), torch.zeros(3, 5))
+
+
+@pytest.mark.parametrize("work", [
+    torch.empty(1, dtype=torch.uint8).expand(1 << 20),  # a megabyte by its shape, a byte in memory
+    torch.empty(1 << 20)[::2],
+    torch.empty(64, 4096)[:, :1024],  # the other columns are the caller's
+    torch.empty(64, 64).t()[:32],
+])
+@pytest.mark.parametrize("direct", [True, False])
+def test_scratch_is_contiguous(ctx, work, direct):
+    """Through the direct call, which leaves it to the method, and where an address sends the call there at once."""
+    x, mean = torch.zeros(3, 5), torch.zeros(3)
+    site = fb.norm_site(3, 5, F)
+    with pytest.raises(ValueError, match="work must be contiguous"):
+        ctx.layer_norm_grad(site, x if direct else x.data_ptr(), None, mean, mean, x, x, torch.zeros(5), None, work)
+    with pytest.raises(fb.MapalInfraError, match="ctx is null"):
+        ctx.layer_norm_grad(site, x if direct else x.data_ptr(), None, mean, mean, x, x, torch.zeros(5), None,
+                            torch.empty(work.shape))
