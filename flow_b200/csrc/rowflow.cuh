@@ -123,7 +123,11 @@ struct Ring {
 // thread's own aligned word and the next thread's. Where a row begins goes
 // round with the rows, so a unit (a group, or a warp of several) takes rows of
 // one class modulo `period`, which begin alike: its columns, weights and sums
-// over rows stay as they are. What is left is instructions. Layer norm and its
+// over rows stay as they are. What is left is instructions and their latencies:
+// at 60000 x 1021 the 15 warps of an SM fill 55 (forward) and 57 % (gradient) of
+// the issue slots and wait for results of their own and at the sums' barriers,
+// with HBM at 24 and 37 % of its peak; rows to 8 bits, 16384 x 8191: 9 warps,
+// 46 % and 43 %. Layer norm and its
 // gradient, bf16: 60000 x 1021 93 and 112 us, element by element 104 and 182;
 // 30000 x 2047 77 and 138, 109 and 188; 12000 x 5001 83 and 165, 169 and 794.
 // Rows to 8 bits: 16384 x 8191 101 us, with shifted words 133, one by one 187.
