@@ -21,14 +21,15 @@ import ctypes
 from typing import Sequence
 
 from . import _native
-from .records import (DTYPES, ExpertSite, ExprOp, GpuProfile, I8Site, KSplit, MoveSite, NormSite, QuantSite, TileRead,
-                      TileSite, conv2d_site, expert_site, fir_site, matmul_i8_site, matmul_site, norm_site, program,
-                      quant_site, transpose_site)
+from .records import (DTYPES, ExpertSite, ExprOp, GpuProfile, I8Site, KSplit, MoveSite, NormSite, ProductSite, QuantSite,
+                      TileRead, TileSite, conv2d_site, expert_site, fir_site, matmul_i8_site, matmul_site, norm_site,
+                      product_site, program, quant_site, transpose_site)
 
 __all__ = [
     "Context", "MapalTrap", "MapalInfraError", "Unsupported", "TileSite", "TileRead", "KSplit",
     "MoveSite", "GpuProfile", "matmul_site", "fir_site", "conv2d_site", "transpose_site",
     "NormSite", "ExpertSite", "QuantSite", "I8Site", "norm_site", "expert_site", "quant_site", "matmul_i8_site",
+    "ProductSite", "product_site",
     "STRICT", "TF32X3", "U11", "U01", "OP_ADD", "OP_SUB", "OP_MUL", "OP_DIV", "OP_MOD",
     "shard_range", "render_f32", "render_f64", "lib",
 ]
@@ -107,11 +108,12 @@ class _Direct:
 
     def __init__(self):
         none = lambda *a: None  # noqa: E731
-        for name in self.NAMES:
+        for name in self.NAMES + self.TRAINING:
             setattr(self, name, none)
 
     NAMES = ("layer_norm", "layer_norm_grad", "expert_sort", "expert_dispatch", "expert_combine",
              "expert_dispatch_grad", "expert_combine_grad", "quantize_rows_i8", "matmul_i8")
+    TRAINING = ("product", "product_grad")
 
     def bind(self):
         L = _native.load()
@@ -119,9 +121,9 @@ class _Direct:
             from . import _rows
         except ImportError as e:
             raise MapalInfraError(ERR_INVALID, f"flow_b200/_rows.so: {e}; build it with: python -m flow_b200.build") from e
-        _rows.bind(tuple(ctypes.cast(getattr(L, "mapal_gpu_" + n), ctypes.c_void_p).value for n in self.NAMES),
-                   (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site))
-        for name in self.NAMES:
+        _rows.bind(tuple(ctypes.cast(getattr(L, "mapal_gpu_" + n), ctypes.c_void_p).value for n in self.NAMES + self.TRAINING),
+                   (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site, ProductSite))
+        for name in self.NAMES + self.TRAINING:
             setattr(self, name, getattr(_rows, name))
 
 
@@ -542,6 +544,32 @@ class Context:
             _mat(B, 3, n, k, ldb, dev, "B", groups, site.ldg),
             _buf(scale_b, 0, groups * n, dev, "scale_b"), _buf(offsets, 4, groups + 1, dev, "offsets"),
             _mat(C, site.dtype, m, n, site.ldc, dev, "C")))
+
+    def product(self, site: ProductSite, x, w, y, offsets=None) -> None:
+        """y[i] = w[g] . x[i] in 16-bit floats with f32 sums; rows offsets[g] to offsets[g + 1] belong to g (offsets
+        None: one matrix for all rows)."""
+        rc = _direct.product(self._h, self.devices[0], site, x, w, y, offsets)
+        if rc is not None and rc != _SHORT:
+            if rc:
+                _check(rc)
+            return
+        dev, m, n, k, groups, t = self.devices[0], site.m, site.n, site.k, site.groups, site.dtype
+        _check(_native.load().mapal_gpu_product(
+            self._h, site, _mat(x, t, m, k, site.ldx, dev, "x"), _mat(w, t, n, k, site.ldw, dev, "w", groups, site.ldg),
+            _buf(offsets, 4, groups + 1, dev, "offsets"), _mat(y, site.ytype, m, n, site.ldy, dev, "y")))
+
+    def product_grad(self, site: ProductSite, x, w, dy, dx, dw, offsets=None) -> None:
+        """dx[i] = w[g]^T . dy[i] and dw[g] = the sum over g's rows of dy[i]^T . x[i]; either may be None."""
+        rc = _direct.product_grad(self._h, self.devices[0], site, x, w, dy, dx, dw, offsets)
+        if rc is not None and rc != _SHORT:
+            if rc:
+                _check(rc)
+            return
+        dev, m, n, k, groups, t = self.devices[0], site.m, site.n, site.k, site.groups, site.dtype
+        _check(_native.load().mapal_gpu_product_grad(
+            self._h, site, _mat(x, t, m, k, site.ldx, dev, "x"), _mat(w, t, n, k, site.ldw, dev, "w", groups, site.ldg),
+            _buf(offsets, 4, groups + 1, dev, "offsets"), _mat(dy, t, m, n, site.lddy, dev, "dy"),
+            _mat(dx, t, m, k, site.lddx, dev, "dx"), _mat(dw, site.dwtype, n, k, site.lddw, dev, "dw", groups, site.lddg)))
 
     # ---- sharded sites (one buffer per local device) --------------------------------
     def saxpy_sharded(self, a: float, xs, y0s, outs) -> None:

@@ -30,8 +30,10 @@ struct Library {
   decltype(&mapal_gpu_expert_combine_grad) expert_combine_grad;
   decltype(&mapal_gpu_quantize_rows_i8) quantize_rows_i8;
   decltype(&mapal_gpu_matmul_i8) matmul_i8;
+  decltype(&mapal_gpu_product) product;
+  decltype(&mapal_gpu_product_grad) product_grad;
 } lib;
-enum { kHandle, kNorm, kExpert, kQuant, kI8, kTypes };
+enum { kHandle, kNorm, kExpert, kQuant, kI8, kProduct, kTypes };
 PyObject* types[kTypes];  // the ctypes classes, kept for good
 
 constexpr int kI32 = 4;          // beside MAPAL_DTYPE_*
@@ -243,13 +245,39 @@ PyObject* matmul_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {  // A, scale_
   });
 }
 
-// bind(addresses of the nine entries in Library's order, the five classes in order)
+PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, w, y, offsets
+  return guarded([&] {
+    MapalProductSite s{};
+    Call c(a, n, 4, kProduct, &s);
+    const void* x = c.at(0, s.dtype, s.m, s.k, s.ldx);
+    const void* w = c.at(1, s.dtype, span(s.groups, span(s.n, s.k, s.ldw), s.ldg));
+    void* y = c.at(2, s.ytype, s.m, s.n, s.ldy);
+    const int32_t* offsets = c.at<int32_t>(3, kI32, (uint64_t)s.groups + 1);
+    return c.run([&] { return lib.product(c.ctx, &s, x, w, offsets, y); });
+  });
+}
+
+PyObject* product_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, w, dy, dx, dw, offsets
+  return guarded([&] {
+    MapalProductSite s{};
+    Call c(a, n, 6, kProduct, &s);
+    const void* x = c.at(0, s.dtype, s.m, s.k, s.ldx);
+    const void* w = c.at(1, s.dtype, span(s.groups, span(s.n, s.k, s.ldw), s.ldg));
+    const void* dy = c.at(2, s.dtype, s.m, s.n, s.lddy);
+    void* dx = c.at(3, s.dtype, s.m, s.k, s.lddx);
+    void* dw = c.at(4, s.dwtype, span(s.groups, span(s.n, s.k, s.lddw), s.lddg));
+    const int32_t* offsets = c.at<int32_t>(5, kI32, (uint64_t)s.groups + 1);
+    return c.run([&] { return lib.product_grad(c.ctx, &s, x, w, offsets, dy, dx, dw); });
+  });
+}
+
+// bind(addresses of the entries in Library's order, the classes in order)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *entries, *classes;
   if (!PyArg_ParseTuple(args, "O!O!", &PyTuple_Type, &entries, &PyTuple_Type, &classes)) return nullptr;
   void* f[sizeof(Library) / sizeof(void*)];
   if (PyTuple_GET_SIZE(entries) != (Py_ssize_t)(sizeof(f) / sizeof(f[0])) || PyTuple_GET_SIZE(classes) != kTypes) {
-    PyErr_SetString(PyExc_ValueError, "nine entries and five classes");
+    PyErr_SetString(PyExc_ValueError, "entries or classes of another number");
     return nullptr;
   }
   for (size_t i = 0; i < sizeof(f) / sizeof(f[0]); ++i) {
@@ -279,6 +307,8 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          FAST(expert_combine_grad),
                          FAST(quantize_rows_i8),
                          FAST(matmul_i8),
+                         FAST(product),
+                         FAST(product_grad),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -194,6 +194,15 @@ class I8Site(ctypes.Structure):
                 ("groups", ctypes.c_uint32), ("dtype", ctypes.c_int32)]
 
 
+class ProductSite(ctypes.Structure):
+    """A product in 16-bit floats, of one matrix or one per group of rows (MapalProductSite)."""
+    _fields_ = [("m", ctypes.c_uint64), ("n", ctypes.c_uint64), ("k", ctypes.c_uint64), ("ldx", ctypes.c_uint64),
+                ("ldw", ctypes.c_uint64), ("ldg", ctypes.c_uint64), ("ldy", ctypes.c_uint64),
+                ("lddy", ctypes.c_uint64), ("lddx", ctypes.c_uint64), ("lddw", ctypes.c_uint64),
+                ("lddg", ctypes.c_uint64), ("groups", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+                ("ytype", ctypes.c_int32), ("dwtype", ctypes.c_int32)]
+
+
 def norm_site(rows: int, d: int, dtype, wdtype=None, eps: float = 1e-5, ldx: int = 0, ldy: int = 0, lddy: int = 0,
               lddx: int = 0) -> NormSite:
     """rows x d elements of `dtype`, w and b of `wdtype` (default: the same); strides 0: contiguous rows."""
@@ -218,3 +227,13 @@ def matmul_i8_site(m: int, n: int, k: int, dtype, groups: int = 1, lda: int = 0,
     """C (m x n, of `dtype`) from A (m x k) and `groups` matrices B (n x k); strides 0: contiguous."""
     ldb = ldb or k
     return I8Site(m, n, k, lda or k, ldb, ldg or n * ldb, ldc or n, groups, dtype_code(dtype))
+
+
+def product_site(m: int, n: int, k: int, dtype, groups: int = 1, ldx: int = 0, ldw: int = 0, ldg: int = 0, ldy: int = 0,
+                 lddy: int = 0, lddx: int = 0, lddw: int = 0, lddg: int = 0, ytype=None, dwtype=None) -> ProductSite:
+    """Y (m x n) from X (m x k) and `groups` matrices W (n x k) of `dtype`; Y of `ytype` and dW of `dwtype` (default:
+    the same); strides 0: contiguous."""
+    code, ldw, lddw = dtype_code(dtype), ldw or k, lddw or k
+    return ProductSite(m, n, k, ldx or k, ldw, ldg or n * ldw, ldy or n, lddy or n, lddx or k, lddw, lddg or n * lddw,
+                       groups, code, code if ytype is None else dtype_code(ytype),
+                       code if dwtype is None else dtype_code(dwtype))

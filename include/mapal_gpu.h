@@ -620,6 +620,48 @@ typedef struct MapalI8Site {
 int mapal_gpu_matmul_i8(MapalGpuCtx* ctx, const MapalI8Site* site, const int8_t* A, const float* scale_a,
                         const int8_t* B, const float* scale_b, const int32_t* offsets, void* C);
 
+/* A product in 16-bit floats: X is m x k, W holds `groups` matrices of n x k (a
+ * weight's rows are its output channels, contiguous along k), Y is m x n. With
+ * several groups the rows of X and Y are sorted by group. m, n and k up to
+ * 2^31 - 256, at most 65535 groups. */
+typedef struct MapalProductSite {
+  uint64_t m;
+  uint64_t n;
+  uint64_t k;
+  uint64_t ldx;
+  uint64_t ldw;
+  uint64_t ldg;  /* from one of W's matrices to the next */
+  uint64_t ldy;
+  uint64_t lddy; /* the gradients' */
+  uint64_t lddx;
+  uint64_t lddw;
+  uint64_t lddg;
+  uint32_t groups;
+  int32_t dtype;  /* X, W, dY, dX: MAPAL_DTYPE_F16 or MAPAL_DTYPE_BF16 */
+  int32_t ytype;  /* Y: dtype or MAPAL_DTYPE_F32 */
+  int32_t dwtype; /* dW: dtype or MAPAL_DTYPE_F32 */
+} MapalProductSite;
+
+/* Y[i, j] = sum over t of X[i, t]*W[g][j, t], the products exact, the sum in f32
+ * on the tensor cores, in an order fixed by the record and the device. offsets
+ * NULL: groups is 1 and every row belongs to it. Otherwise rows offsets[g] to
+ * offsets[g + 1] (groups + 1 values on the device, as mapal_gpu_expert_sort
+ * writes them) belong to g; rows of Y in no group are left as they were.
+ * Offsets that descend or leave [0, m] trap index_oob and are taken as the
+ * largest up to them, clamped to [0, m]. k = 0 gives zeros. */
+int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site, const void* x, const void* w,
+                      const int32_t* offsets, void* y);
+
+/* The gradients of mapal_gpu_product:
+ *   dX[i, t] = sum over j of dY[i, j]*W[g][j, t],
+ *   dW[g][j, t] = sum over the rows i of g of dY[i, j]*X[i, t],
+ * written (not added to). dx (m x k) or dw (groups of n x k) may be NULL, then
+ * w or x is not read. Rows of dX in no group are left as they were; a group
+ * without rows has a dW of zeros. Bad offsets trap index_oob; dW[g] is then
+ * the sum over its range's rows that exist. */
+int mapal_gpu_product_grad(MapalGpuCtx* ctx, const MapalProductSite* site, const void* x, const void* w,
+                           const int32_t* offsets, const void* dy, void* dx, void* dw);
+
 /* ---- measurement --------------------------------------------------------------
  * No counterpart in the reference: the roofline of MAPAL_MATMUL_TF32X3.
  * Issues the 3xTF32 GEMM's own tensor-core instruction (tcgen05.mma M128 N256,
