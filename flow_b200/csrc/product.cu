@@ -251,34 +251,24 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
 
 // ---- host ------------------------------------------------------------------------------
 
-// Tiles of `nt` columns and `ch` lanes: at most one part-filled column tile for
-// each group with rows (the offsets are on the device).
-template <int MODE>
-uint64_t tiles_of(const ProductArgs& P, uint32_t nt, uint32_t ch) {
-  const uint64_t lane_tiles = (P.lanes + ch - 1) / ch;
-  if (MODE == kGradW) return (uint64_t)P.groups * ((P.cols + nt - 1) / nt) * lane_tiles;
-  const uint64_t with_rows = P.groups < P.m ? P.groups : P.m;
-  const uint64_t col_tiles = P.offsets ? P.m / nt + with_rows : (P.m + nt - 1) / nt;
-  return col_tiles * lane_tiles * P.parts;
-}
-
 template <int MODE, typename T, int NT, int STAGES>
-int launch_any(const DeviceSlot& D, const AnyOperand& A, const AnyOperand& B, const ProductArgs& P,
-               const StoreTile<MODE, T, false>& out) {
+int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T, false>& out) {
   constexpr size_t smem = sizeof(AnySmem<NT, STAGES>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
   auto kernel = product_any_kernel<MODE, T, NT, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "product shared memory"));
-  const uint64_t tiles = tiles_of<MODE>(P, NT, 128), cap = D.prof.sm_count;
+  const AnyOperand A{static_cast<const uint8_t*>(o.a), 2 * o.lda, 2 * o.ldga};
+  const AnyOperand B{static_cast<const uint8_t*>(o.b), 2 * o.ldb, 0};
+  const uint64_t tiles = product_tiles(MODE, P, NT, 128), cap = D.prof.sm_count;
   return launch_rows(kernel, (unsigned)(tiles < cap ? tiles : cap), kCopyThreads + 32 * (1 + kAnyOut), smem, D.stream, 1, A,
                      B, P, out);
 }
 
 template <int MODE, typename T>
-int run(const DeviceSlot& D, const AnyOperand& A, const AnyOperand& B, const ProductArgs& P,
-        const StoreTile<MODE, T, false>& out) {
-  return launch_any<MODE, T, 128, 4>(D, A, B, P, out);
+int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T, false>& out) {
+  if (tma_reads(MODE, P, o)) return launch_product_pair<MODE>(D, o, P, out);
+  return launch_any<MODE, T, 128, 4>(D, o, P, out);
 }
 
 int check_site(const MapalProductSite* s) {
@@ -321,20 +311,16 @@ ProductArgs args_of(const DeviceSlot& D, const MapalProductSite& s, const int32_
   return P;
 }
 
-AnyOperand operand(const void* base, uint64_t ld, uint64_t ldg) {
-  return {static_cast<const uint8_t*>(base), 2 * ld, 2 * ldg};
-}
-
 template <int MODE>
-int by_type(const DeviceSlot& D, const AnyOperand& A, const AnyOperand& B, const ProductArgs& P, int dtype, void* out,
-            uint64_t ld, uint64_t ldg) {
+int by_type(const DeviceSlot& D, const Operands& o, const ProductArgs& P, int dtype, void* out, uint64_t ld, uint64_t ldg) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    return run<MODE, T>(D, A, B, P, StoreTile<MODE, T, false>{static_cast<T*>(out), nullptr, ld, ldg, 0});
+    return run<MODE, T>(D, o, P, StoreTile<MODE, T, false>{static_cast<T*>(out), nullptr, ld, ldg, 0});
   };
   if (dtype == MAPAL_DTYPE_F16) return go(__half{});
-  if (dtype == MAPAL_DTYPE_BF16) return go(__nv_bfloat16{});
-  return go(float{});
+  if constexpr (MODE != kGradX)  // dX is of the rows' type
+    if (dtype == MAPAL_DTYPE_F32) return go(float{});
+  return go(__nv_bfloat16{});
 }
 
 }  // namespace
@@ -358,7 +344,7 @@ extern "C" int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site,
     ProductArgs P = args_of(D, s, offsets);
     P.lanes = (uint32_t)s.n;
     P.depth = (uint32_t)s.k;
-    MAPAL_TRY(by_type<kForward>(D, operand(w, s.ldw, s.ldg), operand(x, s.ldx, 0), P, s.ytype, y, s.ldy, 0));
+    MAPAL_TRY(by_type<kForward>(D, {w, x, s.ldw, s.ldg, s.ldx, s.n, s.k, s.k}, P, s.ytype, y, s.ldy, 0));
     return finish(ctx, 0, true);
   });
 }
@@ -391,12 +377,12 @@ extern "C" int mapal_gpu_product_grad(MapalGpuCtx* ctx, const MapalProductSite* 
     P.lanes = (uint32_t)s.k;
     if (do_x) {
       P.depth = (uint32_t)s.n;
-      MAPAL_TRY(by_type<kGradX>(D, operand(w, s.ldw, s.ldg), operand(dy, s.lddy, 0), P, s.dtype, dx, s.lddx, 0));
+      MAPAL_TRY(by_type<kGradX>(D, {w, dy, s.ldw, s.ldg, s.lddy, s.n, s.k, s.n}, P, s.dtype, dx, s.lddx, 0));
     }
     if (do_w) {
       P.depth = 0;
       P.cols = (uint32_t)s.n;
-      MAPAL_TRY(by_type<kGradW>(D, operand(x, s.ldx, 0), operand(dy, s.lddy, 0), P, s.dwtype, dw, s.lddw, s.lddg));
+      MAPAL_TRY(by_type<kGradW>(D, {x, dy, s.ldx, 0, s.lddy, s.m, s.k, s.n}, P, s.dwtype, dw, s.lddw, s.lddg));
     }
     return finish(ctx, 0, true);
   });

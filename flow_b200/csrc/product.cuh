@@ -218,3 +218,331 @@ struct StoreTile {
     }
   }
 };
+
+// ---- a pair of CTAs a tile ---------------------------------------------------------------
+//
+// 256 lanes by up to 256 columns: each CTA of the pair loads its 128 lanes of A and
+// half of B's columns, and the pair's MMA (cta_group::2, issued by the first CTA)
+// reads both halves from both, so a CTA moves 32 KB a block of t where a 128 x 256
+// tile of its own moves 48. Persistent; two accumulators in tensor memory, so that
+// a tile's output runs beside the next one's products.
+//
+// grad w: the last block of a group's rows may hold rows of the next group. Such a
+// block is counted by a barrier of its own (landed); a warp clears the rows behind
+// the group's last up to the next 16 (the MMA's step) in both operands, since zero
+// times NaN is not zero, and lets the products go on (fixed).
+
+constexpr int kPairStages = 3, kPairKB = 2, kPairTokens = 256, kPairOut = 8;
+
+struct PairSmem {
+  static constexpr int kHalf = 128 * 128;  // bytes of a block of lanes, and of columns
+  uint8_t stage[kPairStages][kPairKB * 2 * kHalf];
+  uint64_t full[kPairStages];    // the first CTA's: both CTAs' loads have landed
+  uint64_t empty[kPairStages];   // each CTA's own
+  uint64_t landed[kPairStages];  // each CTA's own: a last block to clear
+  uint64_t fixed[kPairStages];   // the first CTA's: cleared in both
+  uint64_t acc_full[2];          // each CTA's own
+  uint64_t acc_empty[2];         // the first CTA's: both CTAs have read the accumulator
+  uint64_t drained;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr size_t kPairSmem = sizeof(PairSmem) + 1024;
+static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
+constexpr int pair_threads(int mode) { return 64 + 32 * kPairOut + (mode == kGradW ? 32 : 0); }
+
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(sa(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(sa(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// A CTA's 128 lanes and its half of the columns of one block of t. W's map has the
+// groups as its third dimension.
+template <int MODE>
+__device__ __forceinline__ void pair_load_block(uint8_t* a, const CUtensorMap* map_a, const CUtensorMap* map_b, const Job& j,
+                                                int t, int lane0, int col0, uint32_t bar) {
+  uint8_t* b = a + PairSmem::kHalf;
+  constexpr int kChunk = kStepK * 128;  // 64 lanes or columns of an MN-major block
+  if constexpr (MODE == kForward) {
+    pair_load_3d(a, map_a, t, lane0, (int)j.group, bar);
+    pair_load_2d(b, map_b, t, col0, bar);
+  } else if constexpr (MODE == kGradX) {
+    pair_load_3d(a, map_a, lane0, t, (int)j.group, bar);
+    pair_load_3d(a + kChunk, map_a, lane0 + 64, t, (int)j.group, bar);
+    pair_load_2d(b, map_b, t, col0, bar);
+  } else {
+    pair_load_2d(a, map_a, lane0, t, bar);
+    pair_load_2d(a + kChunk, map_a, lane0 + 64, t, bar);
+    pair_load_2d(b, map_b, col0, t, bar);
+    pair_load_2d(b + kChunk, map_b, col0 + 64, t, bar);
+  }
+}
+
+template <int MODE, typename Out>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 1)
+    product_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ ProductArgs P, const __grid_constant__ Out out) {
+  namespace cg = cooperative_groups;
+  constexpr int NT = kPairTokens;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const uint32_t rank = blockIdx.x & 1;
+  const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  volatile int* abort = &sm.abort;
+
+  if (warp == 0 && elect_one()) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+      mbar_init(&sm.landed[s], 1);
+      mbar_init(&sm.fixed[s], 2);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 2 * kPairOut);
+    }
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  grid_wait();
+  grid_go();
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cg::this_cluster().sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+  JobWalk<MODE> walk(P, NT, 256);
+  Job j;
+  bool more = walk.at(first, j);
+  uint32_t it = 0;      // stages taken
+  uint32_t fixes = 0;   // a bit a stage: the parity of its next clearing
+
+  auto blocks_of = [](const Job& q) { return (q.depth + kStepK - 1) / kStepK; };
+  // whether the last block holds rows that are not the group's
+  auto to_fix = [&](const Job& q) { return MODE == kGradW && (q.depth & 15) && q.t0 + q.depth < P.m; };
+
+  if (warp == 0) {
+    // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j)) {
+      const uint32_t blocks = blocks_of(j), half = (j.cols + 31) / 32 * 16;  // columns of each CTA
+      const bool fix = to_fix(j);
+      const int lane0 = (int)(j.lane0 + rank * 128), col0 = (int)(j.col0 + rank * half);
+      if (elect_one())
+        for (uint32_t kb = 0; kb < blocks; kb += kPairKB, ++it) {
+          const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
+          if (!mbar_wait(&sm.empty[s], ((it / kPairStages) & 1) ^ 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          const bool last = fix && kb + here == blocks;
+          if (rank == 0) mbar_expect_tx(&sm.full[s], (here - last) * 4 * PairSmem::kHalf);
+          if (last) {
+            mbar_expect_tx(&sm.landed[s], 2 * PairSmem::kHalf);
+            fixes ^= 1u << s;
+          }
+          const uint32_t bar = remote(sa(&sm.full[s]), 0);
+#pragma unroll
+          for (uint32_t u = 0; u < kPairKB; ++u)
+            if (u < here)
+              pair_load_block<MODE>(sm.stage[s] + 2 * u * PairSmem::kHalf, &map_a, &map_b, j, (int)(j.t0 + (kb + u) * kStepK),
+                                    lane0, col0, last && u + 1 == here ? remote(sa(&sm.landed[s]), rank) : bar);
+        }
+      if (any_of(*abort)) break;
+    }
+  } else if (warp == 1) {
+    // ---- products, by the first CTA ----
+    uint32_t n = 0;
+    for (uint64_t tile = first; rank == 0 && more; tile += step, more = walk.at(tile, j), ++n) {
+      const uint32_t b = n & 1, blocks = blocks_of(j);
+      const bool fix = to_fix(j);
+      if (elect_one()) {
+        const uint32_t idesc = idesc_f16<MODE>(P.bf16, 256, (int)((j.cols + 31) / 32 * 32));
+        if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (uint32_t kb = 0; kb < blocks && !*abort; kb += kPairKB, ++it) {
+          const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
+          bool ok = mbar_wait(&sm.full[s], (it / kPairStages) & 1, abort);
+          if (fix && kb + here == blocks) {
+            ok = ok && mbar_wait_cluster(&sm.fixed[s], (fixes >> s) & 1, abort);
+            fixes ^= 1u << s;
+          }
+          if (!ok) {
+            *abort = 1;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t da = operand_desc<MODE != kForward>(sm.stage[s]),
+                         db = operand_desc<MODE == kGradW>(sm.stage[s] + PairSmem::kHalf);
+#pragma unroll
+          for (uint32_t u = 0; u < kPairKB; ++u)
+            if (u < here) {
+              // grad w: no step behind the group's rows
+              const uint32_t left = j.depth - (kb + u) * kStepK;
+#pragma unroll
+              for (uint32_t kk = 0; kk < kStepK / 16; ++kk)
+                if (MODE != kGradW || kk * 16 < left)
+                  mma_f16<2>(tmem + b * NT, da + u * (2 * PairSmem::kHalf >> 4) + kk * operand_step<MODE != kForward>(),
+                             db + u * (2 * PairSmem::kHalf >> 4) + kk * operand_step<MODE == kGradW>(), idesc,
+                             kb > 0 || u > 0 || kk > 0);
+            }
+          pair_commit(&sm.empty[s]);
+        }
+        pair_commit(&sm.acc_full[b]);
+      }
+      if (any_of(*abort)) break;
+    }
+  } else if (MODE == kGradW && warp == 2 + kPairOut) {
+    // ---- last blocks: rows behind the group's become zeros ----
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j)) {
+      const uint32_t blocks = blocks_of(j), fills = (blocks + kPairKB - 1) / kPairKB;
+      it += fills;
+      if (!to_fix(j)) continue;
+      const uint32_t s = (it - 1) % kPairStages;
+      if (any_of(!mbar_wait(&sm.landed[s], (fixes >> s) & 1, abort))) {
+        *abort = 1;
+        break;
+      }
+      fixes ^= 1u << s;
+      const uint32_t rows = j.depth - (blocks - 1) * kStepK, to = (rows + 15) / 16 * 16;
+      uint8_t* block = sm.stage[s] + (blocks - 1) % kPairKB * (2 * PairSmem::kHalf);
+      for (uint32_t chunk = 0; chunk < 4; ++chunk)
+        for (uint32_t i = rows * 8 + lane; i < to * 8; i += 32)
+          *reinterpret_cast<uint4*>(block + chunk * (kStepK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_remote(remote(sa(&sm.fixed[s]), 0));
+    }
+  } else {
+    // ---- output ----
+    const int quarter = warp & 3;
+    const uint32_t from = (warp - 2) / 4 * kHalfTokens;
+    uint32_t n = 0;
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+      const uint32_t b = n & 1;
+      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
+        *abort = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      out.put(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + rank * 128 + quarter * 32 + lane, from,
+              from + kHalfTokens);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_remote(remote(sa(&sm.acc_empty[b]), 0));
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cg::this_cluster().sync();
+  // A wait gave up in either CTA (its flag is read after both have stopped):
+  // what is still in flight ends before shared memory and TMEM are given back.
+  const bool stop = *abort || *(volatile int*)cg::this_cluster().map_shared_rank(&sm.abort, rank ^ 1);
+  if (stop) {
+    if (warp == 0 && elect_one()) {
+      atomicOr(P.trap, kDeviceTimeout);
+      // every stage's last use, in the first CTA for both, and each CTA's own blocks to clear
+      for (uint32_t i = it > kPairStages ? it - kPairStages : 0; i < it; ++i) {
+        if (rank == 0) mbar_wait(&sm.full[i % kPairStages], (i / kPairStages) & 1, nullptr);
+      }
+      if (MODE == kGradW)
+        for (int s = 0; s < kPairStages; ++s) mbar_wait(&sm.landed[s], ((fixes >> s) & 1) ^ 1, nullptr);
+    }
+    if (warp == 1 && rank == 0 && elect_one()) {
+      pair_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, nullptr);
+    }
+  }
+  __syncwarp();
+  cg::this_cluster().sync();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------
+
+// Tiles of `nt` columns and `ch` lanes: at most one part-filled column tile for
+// each group with rows (the offsets are on the device).
+inline uint64_t product_tiles(int mode, const ProductArgs& P, uint32_t nt, uint32_t ch) {
+  const uint64_t lane_tiles = (P.lanes + ch - 1) / ch;
+  if (mode == kGradW) return (uint64_t)P.groups * ((P.cols + nt - 1) / nt) * lane_tiles;
+  const uint64_t with_rows = P.groups < P.m ? P.groups : P.m;
+  const uint64_t col_tiles = P.offsets ? P.m / nt + with_rows : (P.m + nt - 1) / nt;
+  return col_tiles * lane_tiles * P.parts;
+}
+
+// Whether TMA can read rows x cols 16-bit elements at stride ld (`mats` of them at ldm).
+inline bool tma_reads16(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t mats, uint64_t ldm) {
+  const uint64_t lim = 1ull << 38;
+  return rows && cols && aligned16(p) && (rows == 1 || (ld % 8 == 0 && ld < lim)) &&
+         (mats == 1 || (ldm % 8 == 0 && ldm < lim)) && rows * (rows == 1 ? cols : ld) < lim;
+}
+
+// rows x cols elements (mats matrices of them) in boxes of 64 elements x box_rows.
+inline int product_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t mats,
+                       uint64_t ldm, int dims, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const uint64_t c8 = (cols + 7) & ~7ull;
+  // a stride that no access uses (one row, one matrix) may be anything: any valid one stands in
+  const uint64_t row = rows > 1 ? ld : c8;
+  cuuint64_t dim[3] = {cols, rows, mats};
+  cuuint64_t stride[2] = {2 * row, 2 * (mats > 1 ? ldm : row * rows)};
+  cuuint32_t box[3] = {(cuuint32_t)kStepK, box_rows, 1}, one[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, dims, const_cast<void*>(base), dim, stride, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return 0;
+}
+
+// The two operands of a product as they lie in memory, strides in elements: A is W
+// (n x k matrices, ldga apart) or, grad w, X; B is X, dY or dY.
+struct Operands {
+  const void* a;
+  const void* b;
+  uint64_t lda, ldga, ldb;
+  uint64_t rows, a_cols, b_cols;  // rows and columns of one of A's matrices, columns of B
+};
+
+inline bool tma_reads(int mode, const ProductArgs& P, const Operands& o) {
+  return tma_reads16(o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga) &&
+         tma_reads16(o.b, P.m, o.b_cols, o.ldb, 1, 0);
+}
+
+// The maps of tiles of `lanes` and `cols`; an MN-major operand comes in boxes of 64 x 64.
+inline int product_maps(int mode, const ProductArgs& P, const Operands& o, uint32_t lanes, uint32_t cols, CUtensorMap* ma,
+                        CUtensorMap* mb) {
+  MAPAL_TRY(product_map(ma, o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga, mode == kGradW ? 2 : 3,
+                        mode == kForward ? lanes : kStepK));
+  return product_map(mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, mode == kGradW ? kStepK : cols);
+}
+
+template <int MODE, typename Out>
+int launch_product_pair(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Out& out) {
+  CUtensorMap ma, mb;
+  MAPAL_TRY(product_maps(MODE, P, o, 128, 128, &ma, &mb));
+  static std::atomic<uint64_t> done{0};
+  auto kernel = product_pair_kernel<MODE, Out>;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, kPairSmem, "product shared memory"));
+  const uint64_t tiles = product_tiles(MODE, P, kPairTokens, 256), cap = D.prof.sm_count / 2;
+  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * 2), pair_threads(MODE), kPairSmem, D.stream, 1, ma, mb,
+                     P, out);
+}
