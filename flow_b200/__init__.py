@@ -21,15 +21,16 @@ import ctypes
 from typing import Sequence
 
 from . import _native
-from .records import (DTYPES, ExpertSite, ExprOp, GpuProfile, I8Site, KSplit, MoveSite, NormSite, ProductSite, QuantSite,
-                      TileRead, TileSite, conv2d_site, expert_site, fir_site, matmul_i8_site, matmul_site, norm_site,
-                      product_site, program, quant_site, transpose_site)
+from .records import (DTYPES, DropoutSite, ExpertSite, ExprOp, GpuProfile, I8Site, KSplit, LossSite, MoveSite, NormSite,
+                      ProductSite, QuantSite, TileRead, TileSite, conv2d_site, dropout_site, expert_site, fir_site,
+                      loss_site, matmul_i8_site, matmul_site, norm_site, product_site, program, quant_site,
+                      transpose_site)
 
 __all__ = [
     "Context", "MapalTrap", "MapalInfraError", "Unsupported", "TileSite", "TileRead", "KSplit",
     "MoveSite", "GpuProfile", "matmul_site", "fir_site", "conv2d_site", "transpose_site",
     "NormSite", "ExpertSite", "QuantSite", "I8Site", "norm_site", "expert_site", "quant_site", "matmul_i8_site",
-    "ProductSite", "product_site",
+    "ProductSite", "LossSite", "DropoutSite", "product_site", "loss_site", "dropout_site",
     "STRICT", "TF32X3", "U11", "U01", "OP_ADD", "OP_SUB", "OP_MUL", "OP_DIV", "OP_MOD",
     "shard_range", "render_f32", "render_f64", "lib",
 ]
@@ -97,8 +98,8 @@ def _arr(ptrs: Sequence) -> ctypes.Array:
 
 
 _SHORT = 1 << 16  # of a direct call: not a status, see binding/rows_py.cpp
-_tensor = None  # torch.Tensor, and torch dtypes by MAPAL_DTYPE_* (4: int32), from the first tensor on
-_dtypes: list = [None] * 5
+_tensor = None  # torch.Tensor, and torch dtypes by MAPAL_DTYPE_* (4: int32, 5: int64), from the first tensor on
+_dtypes: list = [None] * 6
 
 
 class _Direct:
@@ -113,7 +114,7 @@ class _Direct:
 
     NAMES = ("layer_norm", "layer_norm_grad", "expert_sort", "expert_dispatch", "expert_combine",
              "expert_dispatch_grad", "expert_combine_grad", "quantize_rows_i8", "matmul_i8")
-    TRAINING = ("product", "product_grad")
+    TRAINING = ("product", "product_grad", "linear_loss", "linear_loss_grad", "dropout")
 
     def bind(self):
         L = _native.load()
@@ -122,7 +123,8 @@ class _Direct:
         except ImportError as e:
             raise MapalInfraError(ERR_INVALID, f"flow_b200/_rows.so: {e}; build it with: python -m flow_b200.build") from e
         _rows.bind(tuple(ctypes.cast(getattr(L, "mapal_gpu_" + n), ctypes.c_void_p).value for n in self.NAMES + self.TRAINING),
-                   (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site, ProductSite))
+                   (ctypes.c_void_p, NormSite, ExpertSite, QuantSite, I8Site, ProductSite, LossSite,
+                    DropoutSite))
         for name in self.NAMES + self.TRAINING:
             setattr(self, name, getattr(_rows, name))
 
@@ -162,7 +164,7 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, rows: int, col
         return t
     if _tensor is None:
         import torch
-        _dtypes[:] = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.int32
+        _dtypes[:] = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.int32, torch.int64
         _direct.bind()
         _tensor = torch.Tensor
     if not 0 <= code < len(_dtypes) or t.dtype is not _dtypes[code]:
@@ -190,6 +192,17 @@ def _buf_checked(t, code: int, need: int, device: int, what: str, rows: int, col
         if need:
             _check_extent(t, what, rows, cols, ld, groups, ldg)
     return t.data_ptr()
+
+
+def _work(work, dev: int) -> tuple[int, int]:
+    """Address and bytes of a scratch tensor of any type."""
+    if work is None:
+        return 0, 0
+    if work.get_device() != dev:
+        raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
+    if not work.is_contiguous():  # its bytes would not be numel() elements in a row
+        raise ValueError("work must be contiguous")
+    return work.data_ptr(), work.numel() * work.element_size()
 
 
 def _check_extent(t, what: str, rows: int, cols: int, ld: int, groups: int, ldg: int) -> None:
@@ -439,17 +452,13 @@ class Context:
                 _check(rc)
             return
         dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
-        if work is not None and work.get_device() != dev:
-            raise ValueError(f"work is on {work.device}, the context drives cuda:{dev}")
-        if work is not None and not work.is_contiguous():  # its bytes would not be numel() elements in a row
-            raise ValueError("work must be contiguous")
+        at, n = _work(work, dev)
         _check(_native.load().mapal_gpu_layer_norm_grad(
             self._h, site, _mat(x, t, rows, d, site.ldx, dev, "x"),
             _buf(w, site.wtype, d, dev, "w"), _buf(mean, 0, rows, dev, "mean"), _buf(rstd, 0, rows, dev, "rstd"),
             _mat(dy, t, rows, d, site.lddy, dev, "dy"),
             _mat(dx, t, rows, d, site.lddx, dev, "dx"), _buf(dw, 0, d, dev, "dw"),
-            _buf(db, 0, d, dev, "db"), 0 if work is None else work.data_ptr(),
-            0 if work is None else work.numel() * work.element_size()))
+            _buf(db, 0, d, dev, "db"), at, n))
 
     def expert_sort(self, site: ExpertSite, ids, offsets, order, pos) -> None:
         """Slots sorted by expert, stably: offsets (experts + 1), order (place -> slot; may be None) and pos
@@ -570,6 +579,59 @@ class Context:
             self._h, site, _mat(x, t, m, k, site.ldx, dev, "x"), _mat(w, t, n, k, site.ldw, dev, "w", groups, site.ldg),
             _buf(offsets, 4, groups + 1, dev, "offsets"), _mat(dy, t, m, n, site.lddy, dev, "dy"),
             _mat(dx, t, m, k, site.lddx, dev, "dx"), _mat(dw, site.dwtype, n, k, site.lddw, dev, "dw", groups, site.lddg)))
+
+    def linear_loss_workspace(self, site: LossSite, w=None, grad: bool = True) -> int:
+        """Bytes of scratch that linear_loss takes, or (grad) that serve its gradient too. `w`: the weights that the
+        calls will be given, where they may lie off a 16-byte boundary."""
+        n = ctypes.c_uint64()
+        _check(_native.load().mapal_gpu_linear_loss_workspace(self._h, site, _ptr(w), 1 if grad else 0, ctypes.byref(n)))
+        return n.value
+
+    def linear_loss(self, site: LossSite, h, w, targets, loss, lse, work) -> None:
+        """loss[i] = lse[i] - <h[i], w[targets[i]]> with lse[i] the log of the summed exponentials of <h[i], w[v]> over
+        the vocabulary, both f32 (lse may be None); 0 where the target is -1. `work`: a contiguous CUDA buffer of at
+        least linear_loss_workspace(site) bytes, its own for calls that may overlap."""
+        rc = _direct.linear_loss(self._h, self.devices[0], site, h, w, targets, loss, lse, work)
+        if rc is not None and rc != _SHORT:
+            if rc:
+                _check(rc)
+            return
+        dev, rows, vocab, d, t = self.devices[0], site.rows, site.vocab, site.d, site.dtype
+        at, n = _work(work, dev)
+        _check(_native.load().mapal_gpu_linear_loss(
+            self._h, site, _mat(h, t, rows, d, site.ldh, dev, "h"), _mat(w, t, vocab, d, site.ldw, dev, "w"),
+            _buf(targets, 4, rows, dev, "targets"), _buf(loss, 0, rows, dev, "loss"), _buf(lse, 0, rows, dev, "lse"),
+            at, n))
+
+    def linear_loss_grad(self, site: LossSite, h, w, targets, lse, dloss, dh, dw, work) -> None:
+        """dh and dw (either may be None) of linear_loss from its lse and the loss's gradient, one f32 a row (None:
+        1)."""
+        rc = _direct.linear_loss_grad(self._h, self.devices[0], site, h, w, targets, lse, dloss, dh, dw, work)
+        if rc is not None and rc != _SHORT:
+            if rc:
+                _check(rc)
+            return
+        dev, rows, vocab, d, t = self.devices[0], site.rows, site.vocab, site.d, site.dtype
+        at, n = _work(work, dev)
+        _check(_native.load().mapal_gpu_linear_loss_grad(
+            self._h, site, _mat(h, t, rows, d, site.ldh, dev, "h"), _mat(w, t, vocab, d, site.ldw, dev, "w"),
+            _buf(targets, 4, rows, dev, "targets"), _buf(lse, 0, rows, dev, "lse"),
+            _buf(dloss, 0, rows, dev, "dloss"), _mat(dh, t, rows, d, site.lddh, dev, "dh"),
+            _mat(dw, t, vocab, d, site.lddw, dev, "dw"), at, n))
+
+    def dropout(self, site: DropoutSite, x, residual, y, rng) -> None:
+        """y = residual + x/(1 - p) where the generator keeps the element, residual alone elsewhere (residual None: 0).
+        `rng`: two int64 on the device, the key and the place in its stream; a call's mask depends on these, the row
+        and the column alone, so the gradient is the same call on dy without a residual."""
+        rc = _direct.dropout(self._h, self.devices[0], site, x, residual, y, rng)
+        if rc is not None and rc != _SHORT:
+            if rc:
+                _check(rc)
+            return
+        dev, rows, d, t = self.devices[0], site.rows, site.d, site.dtype
+        _check(_native.load().mapal_gpu_dropout(
+            self._h, site, _mat(x, t, rows, d, site.ldx, dev, "x"), _mat(residual, t, rows, d, site.ldr, dev, "residual"),
+            _buf(rng, 5, 2, dev, "rng"), _mat(y, t, rows, d, site.ldy, dev, "y")))
 
     # ---- sharded sites (one buffer per local device) --------------------------------
     def saxpy_sharded(self, a: float, xs, y0s, outs) -> None:

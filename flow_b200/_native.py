@@ -8,7 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 
-from .records import ExpertSite, ExprOp, GpuProfile, I8Site, MoveSite, NormSite, ProductSite, QuantSite, TileSite
+from .records import (DropoutSite, ExpertSite, ExprOp, GpuProfile, I8Site, LossSite, MoveSite, NormSite, ProductSite,
+                      QuantSite, TileSite)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmapal_gpu.so")
 
@@ -80,6 +81,10 @@ SIGNATURES: dict[str, tuple] = {
     "mapal_gpu_matmul_i8": (_int, [_vp, _c.POINTER(I8Site), _vp, _vp, _vp, _vp, _vp, _vp]),
     "mapal_gpu_product": (_int, [_vp, _c.POINTER(ProductSite), _vp, _vp, _vp, _vp]),
     "mapal_gpu_product_grad": (_int, [_vp, _c.POINTER(ProductSite), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mapal_gpu_linear_loss_workspace": (_int, [_vp, _c.POINTER(LossSite), _vp, _int, _pu64]),
+    "mapal_gpu_linear_loss": (_int, [_vp, _c.POINTER(LossSite), _vp, _vp, _vp, _vp, _vp, _vp, _u64]),
+    "mapal_gpu_linear_loss_grad": (_int, [_vp, _c.POINTER(LossSite), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64]),
+    "mapal_gpu_dropout": (_int, [_vp, _c.POINTER(DropoutSite), _vp, _vp, _vp, _vp]),
     "mapal_gpu_probe_mma_peak": (_int, [_vp, _int, _c.c_uint32, _c.POINTER(_c.c_double)]),
     "mapal_gpu_probe_launch_floor": (_int, [_vp, _int, _vp, _u64, _vp]),
     # mapal-rt re-exports (include/mapal_rt.h)

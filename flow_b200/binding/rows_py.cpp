@@ -32,11 +32,14 @@ struct Library {
   decltype(&mapal_gpu_matmul_i8) matmul_i8;
   decltype(&mapal_gpu_product) product;
   decltype(&mapal_gpu_product_grad) product_grad;
+  decltype(&mapal_gpu_linear_loss) linear_loss;
+  decltype(&mapal_gpu_linear_loss_grad) linear_loss_grad;
+  decltype(&mapal_gpu_dropout) dropout;
 } lib;
-enum { kHandle, kNorm, kExpert, kQuant, kI8, kProduct, kTypes };
+enum { kHandle, kNorm, kExpert, kQuant, kI8, kProduct, kLoss, kDropout, kTypes };
 PyObject* types[kTypes];  // the ctypes classes, kept for good
 
-constexpr int kI32 = 4;          // beside MAPAL_DTYPE_*
+constexpr int kI32 = 4, kI64 = 5;  // beside MAPAL_DTYPE_*
 constexpr int kShort = 1 << 16;  // beside the statuses; flow_b200._SHORT
 
 uint64_t span(uint64_t rows, uint64_t cols, uint64_t ld) { return rows && cols ? (rows - 1) * ld + cols : 0; }
@@ -80,8 +83,8 @@ struct Call {
   void* address(int i, int code, uint64_t need, uint64_t rows, uint64_t cols, uint64_t ld) {
     PyObject* o = args[3 + i];
     if (!ok || o == Py_None) return nullptr;
-    static constexpr at::ScalarType kOf[] = {at::kFloat, at::kHalf, at::kBFloat16, at::kChar, at::kInt};
-    if (!THPVariable_Check(o) || code < 0 || code > kI32) {
+    static constexpr at::ScalarType kOf[] = {at::kFloat, at::kHalf, at::kBFloat16, at::kChar, at::kInt, at::kLong};
+    if (!THPVariable_Check(o) || code < 0 || code > kI64) {
       ok = false;
       return nullptr;
     }
@@ -271,6 +274,44 @@ PyObject* product_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, w, 
   });
 }
 
+PyObject* linear_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {  // h, w, targets, loss, lse, work
+  return guarded([&] {
+    MapalLossSite s{};
+    Call c(a, n, 6, kLoss, &s);
+    const void *h = c.at(0, s.dtype, s.rows, s.d, s.ldh), *w = c.at(1, s.dtype, s.vocab, s.d, s.ldw);
+    const int32_t* targets = c.at<int32_t>(2, kI32, s.rows);
+    float *loss = c.at<float>(3, 0, s.rows), *lse = c.at<float>(4, 0, s.rows);
+    uint64_t bytes;
+    void* work = c.bytes(5, &bytes);
+    return c.run([&] { return lib.linear_loss(c.ctx, &s, h, w, targets, loss, lse, work, bytes); });
+  });
+}
+
+PyObject* linear_loss_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {  // h, w, targets, lse, dloss, dh, dw, work
+  return guarded([&] {
+    MapalLossSite s{};
+    Call c(a, n, 8, kLoss, &s);
+    const void *h = c.at(0, s.dtype, s.rows, s.d, s.ldh), *w = c.at(1, s.dtype, s.vocab, s.d, s.ldw);
+    const int32_t* targets = c.at<int32_t>(2, kI32, s.rows);
+    const float *lse = c.at<float>(3, 0, s.rows), *dloss = c.at<float>(4, 0, s.rows);
+    void *dh = c.at(5, s.dtype, s.rows, s.d, s.lddh), *dw = c.at(6, s.dtype, s.vocab, s.d, s.lddw);
+    uint64_t bytes;
+    void* work = c.bytes(7, &bytes);
+    return c.run([&] { return lib.linear_loss_grad(c.ctx, &s, h, w, targets, lse, dloss, dh, dw, work, bytes); });
+  });
+}
+
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, residual, y, rng
+  return guarded([&] {
+    MapalDropoutSite s{};
+    Call c(a, n, 4, kDropout, &s);
+    const void *x = c.at(0, s.dtype, s.rows, s.d, s.ldx), *residual = c.at(1, s.dtype, s.rows, s.d, s.ldr);
+    void* y = c.at(2, s.dtype, s.rows, s.d, s.ldy);
+    const uint64_t* rng = c.at<uint64_t>(3, kI64, 2);
+    return c.run([&] { return lib.dropout(c.ctx, &s, x, residual, rng, y); });
+  });
+}
+
 // bind(addresses of the entries in Library's order, the classes in order)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *entries, *classes;
@@ -309,6 +350,9 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          FAST(matmul_i8),
                          FAST(product),
                          FAST(product_grad),
+                         FAST(linear_loss),
+                         FAST(linear_loss_grad),
+                         FAST(dropout),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -113,7 +113,7 @@ struct Lines {
 template <int MODE, typename T, int NT, int STAGES>
 __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
     product_any_kernel(const AnyOperand A, const AnyOperand B, const __grid_constant__ ProductArgs P,
-                       const StoreTile<MODE, T, false> out) {
+                       const StoreTile<MODE, T> out) {
   using Smem = AnySmem<NT, STAGES>;
   constexpr uint32_t kCols = 2 * NT;
   constexpr int kCopy = kCopyThreads / 32;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
 // ---- host ------------------------------------------------------------------------------
 
 template <int MODE, typename T, int NT, int STAGES>
-int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T, false>& out) {
+int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T>& out) {
   constexpr size_t smem = sizeof(AnySmem<NT, STAGES>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
@@ -266,7 +266,7 @@ int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, con
 }
 
 template <int MODE, typename T>
-int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T, false>& out) {
+int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T>& out) {
   if (tma_reads(MODE, P, o)) return launch_product_pair<MODE>(D, o, P, out);
   return launch_any<MODE, T, 128, 4>(D, o, P, out);
 }
@@ -315,7 +315,7 @@ template <int MODE>
 int by_type(const DeviceSlot& D, const Operands& o, const ProductArgs& P, int dtype, void* out, uint64_t ld, uint64_t ldg) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    return run<MODE, T>(D, o, P, StoreTile<MODE, T, false>{static_cast<T*>(out), nullptr, ld, ldg, 0});
+    return run<MODE, T>(D, o, P, StoreTile<MODE, T>{static_cast<T*>(out), ld, ldg});
   };
   if (dtype == MAPAL_DTYPE_F16) return go(__half{});
   if constexpr (MODE != kGradX)  // dX is of the rows' type

@@ -33,6 +33,7 @@ struct ProductArgs {
   unsigned* trap;
   uint32_t groups, m;
   uint32_t lanes;  // extent of the lanes' dimension
+  const int32_t* lane_count;  // where not null: how many of them count, on the device
   uint32_t cols;   // grad w: extent of the columns' dimension (n)
   uint32_t depth;  // forward, grad x: extent of t
   uint32_t parts;  // forward, grad x: t cut into so many parts, each with its own output
@@ -54,15 +55,18 @@ struct JobWalk {
   TileWalk tiles;
   uint32_t nt, ch, lane_tiles, per_part;
 
-  __device__ JobWalk(const ProductArgs& p, uint32_t nt_, uint32_t ch_)
-      : P(p), tiles{p.offsets, p.groups, p.m, nt_, ch_, (p.lanes + ch_ - 1) / ch_, p.trap}, nt(nt_), ch(ch_) {
-    lane_tiles = (p.lanes + ch_ - 1) / ch_;
+  __device__ JobWalk(const ProductArgs& p, uint32_t nt_, uint32_t ch_) : P(p), nt(nt_), ch(ch_) {
+    uint32_t lanes = p.lanes;
+    if (p.lane_count) lanes = min(lanes, (uint32_t)max(__ldg(p.lane_count), 0));
+    lane_tiles = (lanes + ch_ - 1) / ch_;
+    tiles = TileWalk{p.offsets, p.groups, p.m, nt_, ch_, lane_tiles, p.trap};
     const uint32_t blocks = (p.depth + kStepK - 1) / kStepK;
     per_part = p.parts > 1 ? (blocks + p.parts - 1) / p.parts * kStepK : p.depth;
     if constexpr (MODE != kGradW) tiles.load();
   }
 
   __device__ bool at(uint64_t tile, Job& j) {
+    if (lane_tiles == 0) return false;
     if constexpr (MODE == kGradW) {
       const uint32_t col_tiles = (P.cols + nt - 1) / nt;
       const uint64_t per = (uint64_t)col_tiles * lane_tiles;
@@ -89,10 +93,10 @@ struct JobWalk {
       // parts run slowest: the tiles of one part share the operands' blocks
       uint32_t part = 0;
       if (P.parts > 1) {  // one group of all rows
-        const uint64_t per = (uint64_t)((P.m + nt - 1) / nt) * lane_tiles;
+        const uint64_t per = (uint64_t)tiles.chunk * lane_tiles;
+        if (tile >= per * P.parts) return false;
         part = (uint32_t)(tile / per);
         tile %= per;
-        if (part >= P.parts) return false;
       }
       Tile t;
       if (!tiles.at(tile, t)) return false;
@@ -159,61 +163,50 @@ __device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&f)[16]) {
 
 // ---- writing a tile --------------------------------------------------------------------
 
+// Sixteen columns of 32 lanes, one a lane, to 16 rows of memory: one conversion for two.
+template <typename T>
+__device__ __forceinline__ void put16(T* c, uint64_t ld, const float (&f)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float v[4] = {f[i], f[i + 1], f[i + 2], f[i + 3]};
+    Pack<T, 4> o;
+    o.set(v);
+    T w[4];
+    memcpy(w, o.w, sizeof(w));
+    c[0] = w[0];
+    c[ld] = w[1];
+    c[2 * ld] = w[2];
+    c[3 * ld] = w[3];
+    c += 4 * ld;
+  }
+}
+
 // The output as it lies in memory: column j of a job at row (grad w: row of the
-// group's matrix), lanes along the row. ADD: the f32 sums so far, at the same
-// places, are added first (a product taken in pieces of t).
-template <int MODE, typename T, bool ADD>
+// group's matrix), lanes along the row.
+template <int MODE, typename T>
 struct StoreTile {
   T* out;
-  const float* sums;
-  uint64_t ld, ldg, ldp;  // rows, groups' matrices, parts
+  uint64_t ld, ldg;  // rows, groups' matrices
 
   // Columns [from, to) of the 32 lanes of a warp, of which this thread has `lane`.
   __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane, uint32_t from,
                                       uint32_t to) const {
     const bool in = lane < P.lanes, zero = j.depth == 0;
     to = min(to, j.cols);
-    const uint64_t at = (MODE == kGradW ? (uint64_t)j.group * ldg : (uint64_t)j.part * ldp) +
-                        (uint64_t)(j.col0 + from) * ld + (in ? lane : 0);
-    T* c = out + at;
-    const float* s = ADD ? sums + at : nullptr;
-    for (uint32_t j0 = from; j0 < to; j0 += 16) {
+    T* c = out + (MODE == kGradW ? (uint64_t)j.group * ldg : 0) + (uint64_t)(j.col0 + from) * ld + (in ? lane : 0);
+    for (uint32_t j0 = from; j0 < to; j0 += 16, c += 16 * ld) {
       float f[16];
-      if (ADD) {
-        float g[16];
+      tmem_ld16f(taddr + j0, f);
+      if (zero) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = in && j0 + i < to ? s[i * ld] : 0.0f;
-        tmem_ld16f(taddr + j0, f);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = g[i] + (zero ? 0.0f : f[i]);
-        s += 16 * ld;
-      } else {
-        tmem_ld16f(taddr + j0, f);
-        if (zero) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = 0.0f;
-        }
+        for (int i = 0; i < 16; ++i) f[i] = 0.0f;
       }
       if (j0 + 16 <= to) {
-        if (in) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float v[4] = {f[i], f[i + 1], f[i + 2], f[i + 3]};
-            Pack<T, 4> o;
-            o.set(v);
-            T w[4];
-            memcpy(w, o.w, sizeof(w));
-            c[0] = w[0];
-            c[ld] = w[1];
-            c[2 * ld] = w[2];
-            c[3 * ld] = w[3];
-            c += 4 * ld;
-          }
-        }
+        if (in) put16(c, ld, f);
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i, c += ld)
-          if (in && j0 + i < to) *c = from_f32<T>(f[i]);
+        for (int i = 0; i < 16; ++i)
+          if (in && j0 + i < to) c[i * ld] = from_f32<T>(f[i]);
       }
     }
   }

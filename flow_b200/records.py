@@ -203,6 +203,20 @@ class ProductSite(ctypes.Structure):
                 ("ytype", ctypes.c_int32), ("dwtype", ctypes.c_int32)]
 
 
+class LossSite(ctypes.Structure):
+    """Rows before a vocabulary's logits (MapalLossSite)."""
+    _fields_ = [("rows", ctypes.c_uint64), ("vocab", ctypes.c_uint64), ("d", ctypes.c_uint64), ("ldh", ctypes.c_uint64),
+                ("ldw", ctypes.c_uint64), ("lddh", ctypes.c_uint64), ("lddw", ctypes.c_uint64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class DropoutSite(ctypes.Structure):
+    """Rows to drop elements of (MapalDropoutSite)."""
+    _fields_ = [("rows", ctypes.c_uint64), ("d", ctypes.c_uint64), ("ldx", ctypes.c_uint64), ("ldr", ctypes.c_uint64),
+                ("ldy", ctypes.c_uint64), ("p", ctypes.c_double), ("dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 def norm_site(rows: int, d: int, dtype, wdtype=None, eps: float = 1e-5, ldx: int = 0, ldy: int = 0, lddy: int = 0,
               lddx: int = 0) -> NormSite:
     """rows x d elements of `dtype`, w and b of `wdtype` (default: the same); strides 0: contiguous rows."""
@@ -237,3 +251,13 @@ def product_site(m: int, n: int, k: int, dtype, groups: int = 1, ldx: int = 0, l
     return ProductSite(m, n, k, ldx or k, ldw, ldg or n * ldw, ldy or n, lddy or n, lddx or k, lddw, lddg or n * lddw,
                        groups, code, code if ytype is None else dtype_code(ytype),
                        code if dwtype is None else dtype_code(dwtype))
+
+
+def loss_site(rows: int, vocab: int, d: int, dtype, ldh: int = 0, ldw: int = 0, lddh: int = 0, lddw: int = 0) -> LossSite:
+    """rows x d before a vocabulary's weights (vocab x d) of `dtype`; strides 0: contiguous rows."""
+    return LossSite(rows, vocab, d, ldh or d, ldw or d, lddh or d, lddw or d, dtype_code(dtype), 0)
+
+
+def dropout_site(rows: int, d: int, dtype, p: float, ldx: int = 0, ldr: int = 0, ldy: int = 0) -> DropoutSite:
+    """rows x d elements of `dtype`, dropped with probability p; strides (of x, residual, y) 0: contiguous rows."""
+    return DropoutSite(rows, d, ldx or d, ldr or d, ldy or d, p, dtype_code(dtype), 0)

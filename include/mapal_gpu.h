@@ -662,6 +662,77 @@ int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site, const void
 int mapal_gpu_product_grad(MapalGpuCtx* ctx, const MapalProductSite* site, const void* x, const void* w,
                            const int32_t* offsets, const void* dy, void* dx, void* dw);
 
+/* Rows before a vocabulary's logits: H is rows x d, W is vocab x d. */
+typedef struct MapalLossSite {
+  uint64_t rows;
+  uint64_t vocab;
+  uint64_t d;
+  uint64_t ldh;
+  uint64_t ldw;
+  uint64_t lddh; /* the gradients' */
+  uint64_t lddw;
+  int32_t dtype; /* H, W, dH, dW: MAPAL_DTYPE_F16 or MAPAL_DTYPE_BF16 */
+  int32_t reserved;
+} MapalLossSite;
+
+/* Bytes of scratch that mapal_gpu_linear_loss takes for this site on this
+ * context's device (grad 0), or that serve both it and its gradient (grad 1).
+ * w: the weights that the calls will be given; NULL stands for any on a 16-byte
+ * boundary. Weights elsewhere, or at a stride that 8 does not divide, are copied
+ * a piece at a time and take more. */
+int mapal_gpu_linear_loss_workspace(MapalGpuCtx* ctx, const MapalLossSite* site, const void* w, int grad,
+                                    uint64_t* bytes);
+
+/* Softmax cross entropy of the logits l[i, v] = <H[i], W[v]>, which are never
+ * in memory: with lse[i] = log(sum over v of exp(l[i, v])) and target t,
+ * loss[i] = lse[i] - l[i, t]. Logits are f32 (products exact, sums on the
+ * tensor cores, the target's by itself), and the loss of a target that is
+ * nearly certain is the others' share, not what is left of two large numbers.
+ * targets: one of [0, vocab) a row; -1: the row has none, its loss and lse are
+ * 0 and its H is not read. Any other target traps index_oob; its row is
+ * treated as one without. lse may be NULL (the gradient needs it). `work` is
+ * scratch of at least the stated bytes, 16-byte aligned, used until the
+ * call's work has finished: calls that may overlap need one each. */
+int mapal_gpu_linear_loss(MapalGpuCtx* ctx, const MapalLossSite* site, const void* h, const void* w,
+                          const int32_t* targets, float* loss, float* lse, void* work, uint64_t work_bytes);
+
+/* The gradient of mapal_gpu_linear_loss from its h, w, targets and lse: with
+ * dl[i, v] = dloss[i]*(exp(l[i, v] - lse[i]) - (v == t)) (dloss NULL: 1),
+ *   dH[i] = sum over v of dl[i, v]*W[v],  dW[v] = sum over i of dl[i, v]*H[i],
+ * written (not added to); either may be NULL. dl is taken for a piece of the
+ * vocabulary at a time and rounded to the rows' type, f16 after a power of two
+ * that keeps a mean's small gradients in its range; sums are f32. A row without
+ * a target has a dH of zeros and adds nothing to dW, whatever it holds. */
+int mapal_gpu_linear_loss_grad(MapalGpuCtx* ctx, const MapalLossSite* site, const void* h, const void* w,
+                               const int32_t* targets, const float* lse, const float* dloss, void* dh, void* dw,
+                               void* work, uint64_t work_bytes);
+
+/* Rows of `d` elements to drop some of. rows and d < 2^31. */
+typedef struct MapalDropoutSite {
+  uint64_t rows;
+  uint64_t d;
+  uint64_t ldx;
+  uint64_t ldr; /* residual */
+  uint64_t ldy;
+  double p;      /* the share that is dropped, 0 to 1 */
+  int32_t dtype; /* x, residual, y: f32, f16 or bf16 */
+  int32_t reserved;
+} MapalDropoutSite;
+
+/* y = residual + keep*x*scale (residual NULL: 0), with T = p*65536 rounded,
+ * scale = 65536/(65536 - T) and keep = (bits >= T) for 16 random bits an
+ * element: what is dropped is 0 whatever x holds, and p = 1 drops all. The
+ * bits are Philox 4x32-10's (Salmon, Moraes, Dror and Shaw, 2011): rng, two
+ * 64-bit words on the device, are the key and a place in its stream, and eight
+ * elements from column 8*c on of row r take the words of the counter
+ * (c, r, low word of the place, high word of the place), the low half of a
+ * word first. No mask is stored: it depends on rng, row and column alone, so the
+ * gradient of x is the same call on the gradient of y without a residual, and
+ * a graph's replays differ as rng does. y may be x or residual (same pointer
+ * and stride). */
+int mapal_gpu_dropout(MapalGpuCtx* ctx, const MapalDropoutSite* site, const void* x, const void* residual,
+                      const uint64_t* rng, void* y);
+
 /* ---- measurement --------------------------------------------------------------
  * No counterpart in the reference: the roofline of MAPAL_MATMUL_TF32X3.
  * Issues the 3xTF32 GEMM's own tensor-core instruction (tcgen05.mma M128 N256,
