@@ -249,6 +249,259 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   }
 }
 
+// ---- a CTA a tile ------------------------------------------------------------------------
+//
+// Forward and grad x of a few rows: up to 128 columns (NT) and CH lanes. The MMA
+// always has M = 128; with CH below 128 the other rows of its operand are whatever
+// shared memory holds and their results are not read: few rows are bound by reading
+// the weights, and narrower tiles spread them over more SMs.
+//
+// Where even that leaves SMs idle, t is split over a cluster of `split` CTAs: each
+// leaves its f32 partial sums in the shared memory of the CTA that writes those
+// columns, which adds them up in the CTAs' order.
+//
+// A stage holds KB blocks of t. Forward weights come with one load a stage where k
+// and n allow it (multiples of 64 and 8): the map splits k into blocks and channels
+// into eights, so that a stage lies as [eight][block][8 rows][128 bytes] and each row
+// is read KB*128 bytes at a time. Grad x takes 64 lanes by KB*64 steps with a load.
+
+template <int NT, int CH, int KB, int STAGES>
+struct TileSmem {
+  static constexpr int kATile = CH * 128, kBTile = NT * 128;
+  static constexpr int kStage = KB * (kATile + kBTile);
+  // KB blocks of A, then of B; 1024-byte aligned for the swizzle. The MMA reads 128
+  // lanes of A, in the last stage past its end.
+  uint8_t stage[STAGES][kStage];
+  uint8_t past[128 - CH > NT ? KB * (128 - CH - NT) * 128 : 16];
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t parts, drained;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct TileArgs {
+  void* out;
+  uint64_t ld;
+  int32_t otype;
+  uint32_t split;
+  uint32_t folded;  // forward: A's map brings a whole stage at once
+};
+
+// f(typed pointer) for the output's type.
+template <typename F>
+__device__ __forceinline__ void with_type(const TileArgs& O, F&& f) {
+  if (O.otype == MAPAL_DTYPE_BF16)
+    f(static_cast<__nv_bfloat16*>(O.out));
+  else if (O.otype == MAPAL_DTYPE_F16)
+    f(static_cast<__half*>(O.out));
+  else
+    f(static_cast<float*>(O.out));
+}
+
+template <int MODE, int NT, int CH, int KB, int STAGES>
+__global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
+    product_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ ProductArgs P, const __grid_constant__ TileArgs O) {
+  using Smem = TileSmem<NT, CH, KB, STAGES>;
+  constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+  constexpr int kOut = out_warps(NT);
+  constexpr bool MN = MODE != kForward;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* partial = reinterpret_cast<float*>(&sm + 1);  // split > 1: NT x CH partial sums
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const uint32_t split = O.split, rank = split > 1 ? blockIdx.x % split : 0;
+  const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
+  const uint32_t k_blocks = (P.depth + kStepK - 1) / kStepK;
+  const uint32_t kb_lo = (uint32_t)((uint64_t)k_blocks * rank / split);
+  const uint32_t kbs = (uint32_t)((uint64_t)k_blocks * (rank + 1) / split) - kb_lo;
+  volatile int* abort = &sm.abort;
+
+  if (warp == 0 && elect_one()) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
+    }
+    mbar_init(&sm.parts, split * CH);
+    mbar_init(&sm.drained, 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  grid_wait();
+  grid_go();
+  JobWalk<MODE> walk(P, NT, CH);
+  Job j;
+  bool more = walk.at(first, j);
+  uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
+
+  const uint32_t fills = (kbs + KB - 1) / KB;  // stages a tile takes
+  auto blocks_of = [&](uint32_t fill) { return min((uint32_t)KB, kbs - fill * KB); };
+  const bool folded = !MN && KB > 1 && O.folded;
+  auto load = [&](uint32_t fill) {
+    const uint32_t s = it % STAGES, blocks = blocks_of(fill);
+    uint8_t* st = sm.stage[s];
+    const int t0 = (int)(kb_lo + fill * KB) * kStepK;
+    mbar_expect_tx(&sm.full[s], (MN || folded ? KB : blocks) * Smem::kATile + blocks * Smem::kBTile);
+    if (MN) {
+#pragma unroll
+      for (int c = 0; c < CH / 64; ++c)
+        tma_load_3d(st + c * (KB * kStepK * 128), &map_a, (int)j.lane0 + c * 64, t0, (int)j.group, &sm.full[s]);
+    } else if (folded) {
+      tma_load_5d(st, &map_a, 0, 0, (int)(kb_lo + fill * KB), (int)(j.lane0 / 8), (int)j.group, &sm.full[s]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < KB; ++u)
+      if (u < blocks) {
+        const int t = t0 + (int)u * kStepK;
+        if (!MN && !folded) tma_load_3d(st + u * Smem::kATile, &map_a, t, (int)j.lane0, (int)j.group, &sm.full[s]);
+        tma_load_2d(st + KB * Smem::kATile + u * Smem::kBTile, &map_b, t, (int)j.col0, &sm.full[s]);
+      }
+    ++it;
+  };
+  // the first stages are on their way before the others have begun
+  if (warp == 0 && more && elect_one())
+    while (it < STAGES && it < fills) load(it);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&sm.tmem_base)),
+                 "r"(kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if (split > 1)
+    cg::this_cluster().sync();  // the others' barriers are there before any arrival
+  else
+    __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ---- loads ----
+    uint32_t fill = it;  // of the first tile, some are issued
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), fill = 0) {
+      if (elect_one())
+        for (; fill < fills; ++fill) {
+          if (!mbar_wait(&sm.empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          load(fill);
+        }
+      if (any_of(*abort)) break;
+    }
+  } else if (warp == 1) {
+    // ---- products ----
+    uint32_t n = 0;
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+      const uint32_t b = n & 1;
+      if (elect_one()) {
+        const uint32_t idesc = idesc_f16<MODE>(P.bf16, 128, (int)((j.cols + 15) / 16 * 16));
+        if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (uint32_t fill = 0; fill < fills && !*abort; ++fill, ++it) {
+          const uint32_t s = it % STAGES, blocks = blocks_of(fill);
+          if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, abort)) {
+            *abort = 1;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t da = MN ? desc_mn(sm.stage[s], KB * kStepK * 128) : desc128(sm.stage[s], folded ? KB * 1024 : 1024),
+                         db = desc128(sm.stage[s] + KB * Smem::kATile);
+          const uint32_t next = (MN ? kStepK * 128 : folded ? 1024 : Smem::kATile) >> 4;
+#pragma unroll
+          for (uint32_t u = 0; u < KB; ++u)
+            if (u < blocks) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < kStepK / 16; ++kk)
+                mma_f16<1>(tmem + b * NT, da + u * next + kk * operand_step<MN>(), db + u * (Smem::kBTile >> 4) + kk * 2,
+                           idesc, fill > 0 || u > 0 || kk > 0);
+            }
+          mma_commit(&sm.empty[s]);
+        }
+        mma_commit(&sm.acc_full[b]);
+      }
+      if (any_of(*abort)) break;
+    }
+  } else if ((warp & 3) < CH / 32) {
+    // ---- output ----
+    const int quarter = warp & 3;  // TMEM lanes 32*quarter to +31
+    uint32_t n = 0;
+    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+      const uint32_t b = n & 1, at = j.lane0 + quarter * 32 + lane;
+      const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
+      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {  // *abort: its commit was an aborted tile's
+        *abort = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
+      if (split == 1) {
+        with_type(O, [&](auto* out) {
+          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, 0}.put(P, j, col, at, from, from + NT / (kOut / 4));
+        });
+      } else {
+        const uint32_t share = NT / split;
+        for (uint32_t k0 = 0; k0 < j.cols; k0 += 16) {
+          float r[16];
+          tmem_ld16f(col + k0, r);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t to = ((rank * share + (k0 + i) % share) * CH + quarter * 32 + lane) * 4;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(sa(partial) + to, (k0 + i) / share)), "f"(r[i])
+                         : "memory");
+          }
+        }
+        for (uint32_t q = 0; q < split; ++q) arrive_remote(remote(sa(&sm.parts), q));
+        if (any_of(!mbar_wait_cluster(&sm.parts, 0, abort))) {
+          *abort = 1;
+          break;
+        }
+        const uint32_t j0 = rank * share;
+        with_type(O, [&](auto* out) {
+          using T = std::remove_pointer_t<decltype(out)>;
+          T* c = out + (uint64_t)(j.col0 + j0) * O.ld + at;
+          for (uint32_t i = 0; i < share && j0 + i < j.cols; ++i, c += O.ld) {
+            float acc = 0.0f;
+            for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + i) * CH + quarter * 32 + lane];
+            if (at < P.lanes) *c = from_f32<T>(acc);
+          }
+        });
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if (split > 1)
+    cg::this_cluster().sync();  // nobody leaves while another may still write here
+  else
+    __syncthreads();
+  if (*abort) {
+    // a wait gave up: what is still in flight ends before shared memory and TMEM are given back
+    if (warp == 0 && elect_one()) {
+      atomicOr(P.trap, kDeviceTimeout);
+      for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+        mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1, nullptr);
+    }
+    if (warp == 1 && elect_one()) {
+      mma_commit(&sm.drained);
+      mbar_wait(&sm.drained, 0, nullptr);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------
 
 template <int MODE, typename T, int NT, int STAGES>
@@ -265,10 +518,102 @@ int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, con
                      B, P, out);
 }
 
+// A way to cut the product: lanes and columns of a tile, parts of t; pairs of CTAs
+// have 256 lanes.
+struct Cut {
+  uint32_t lanes, cols, split;
+};
+
+// Cycles of a cut, from what bounds its tiles: the MMA (N/2 cycles for 128 lanes and
+// 16 steps of t, 32 + N/4 at least), and the loads, at up to 64 bytes a cycle for
+// an SM and 6200 for all. Tiles run in waves, each with a start and an end that
+// nothing overlaps when it is the only one. It ranks cuts; see the 8-bit products
+// for how far it is from a time.
+double cycles_of(int mode, const ProductArgs& P, const Cut& c, int sms) {
+  const bool pair = c.lanes == 256;
+  const double tiles = (double)product_tiles(mode, P, c.cols, c.lanes) * c.split, at_once = pair ? sms / 2 : sms;
+  const double active = tiles < at_once ? tiles : at_once, ctas = pair ? 2 * active : active;
+  const double blocks = (double)((P.depth + kStepK - 1) / kStepK) / c.split;
+  const double rate = 6200.0 / ctas < 64.0 ? 6200.0 / ctas : 64.0;
+  const double load = (pair ? 256 : c.lanes + c.cols) * 128.0 / rate;
+  const double cols = P.m < c.cols ? (double)((P.m + 15) / 16 * 16) : c.cols;
+  const double mma = 4 * (cols / 4 + 32 > cols / 2 ? cols / 4 + 32 : cols / 2);
+  const double waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
+  return waves * (blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
+}
+
+// W as [group][eight channels][block of k][8][64], in boxes of lanes/8 x blocks.
+int folded_map(CUtensorMap* map, const ProductArgs& P, const Operands& o, uint32_t lanes, uint32_t blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dim[5] = {(cuuint64_t)kStepK, 8, o.a_cols / kStepK, o.rows / 8, P.groups};
+  cuuint64_t stride[4] = {2 * o.lda, 128, 16 * o.lda, 2 * (P.groups > 1 ? o.ldga : o.rows * o.lda)};
+  cuuint32_t box[5] = {(cuuint32_t)kStepK, 8, blocks, lanes / 8, 1}, one[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, const_cast<void*>(o.a), dim, stride, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return 0;
+}
+
+template <int MODE, int NT, int CH, int KB, int STAGES>
+int launch_tile(const DeviceSlot& D, const Operands& o, const ProductArgs& P, TileArgs O) {
+  using Smem = TileSmem<NT, CH, KB, STAGES>;
+  CUtensorMap ma, mb;
+  O.folded = MODE == kForward && KB > 1 && o.a_cols % kStepK == 0 && o.rows % 8 == 0 && o.lda < (1ull << 35);
+  if (O.folded)
+    MAPAL_TRY(folded_map(&ma, P, o, CH, KB));
+  else
+    MAPAL_TRY(product_map(&ma, o.a, o.rows, o.a_cols, o.lda, P.groups, o.ldga, 3, MODE == kForward ? CH : KB * kStepK));
+  MAPAL_TRY(product_map(&mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, NT));
+  constexpr size_t most = sizeof(Smem) + 1024 + (NT <= 64 ? NT * CH * 4 : 0);
+  static_assert(most <= 227 * 1024, "shared memory of a CTA");
+  static std::atomic<uint64_t> done{0};
+  auto kernel = product_tile_kernel<MODE, NT, CH, KB, STAGES>;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "product shared memory"));
+  const uint64_t tiles = product_tiles(MODE, P, NT, CH), cap = O.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
+  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * O.split), 64 + 32 * out_warps(NT),
+                     sizeof(Smem) + 1024 + (O.split > 1 ? NT * CH * 4 : 0), D.stream, O.split, ma, mb, P, O);
+}
+
 template <int MODE, typename T>
-int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T>& out) {
-  if (tma_reads(MODE, P, o)) return launch_product_pair<MODE>(D, o, P, out);
-  return launch_any<MODE, T, 128, 4>(D, o, P, out);
+int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T>& out, int otype) {
+  if (!tma_reads(MODE, P, o)) return launch_any<MODE, T, 128, 4>(D, o, P, out);
+  if constexpr (MODE != kGradW) {
+    static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
+                                    {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
+    const uint32_t blocks = (P.depth + kStepK - 1) / kStepK;
+    Cut best{};
+    double least = 0;
+    for (Cut c : kCuts) {
+      if (MODE == kGradX && c.lanes == 32) continue;  // an MN-major line is 64 lanes
+      for (c.split = 1; c.split <= 8; c.split *= 2) {
+        if (c.split > 1 && (c.cols > 64 || c.split * 4 > blocks ||
+                            product_tiles(MODE, P, c.cols, c.lanes) * c.split > (uint64_t)D.prof.sm_count))
+          break;
+        const double cy = cycles_of(MODE, P, c, D.prof.sm_count);
+        if (best.lanes == 0 || cy < least) {
+          best = c;
+          least = cy;
+        }
+      }
+    }
+    const TileArgs O{out.out, out.ld, otype, best.split, 0};
+    switch (best.lanes * 1000 + best.cols) {
+      case 256256: break;
+      case 128128: return launch_tile<MODE, 128, 128, 2, 3>(D, o, P, O);
+      case 64128: return launch_tile<MODE, 128, 64, 2, 4>(D, o, P, O);
+      case 128064: return launch_tile<MODE, 64, 128, 2, 3>(D, o, P, O);
+      case 64064: return launch_tile<MODE, 64, 64, 2, 6>(D, o, P, O);
+      case 128032: return launch_tile<MODE, 32, 128, 2, 5>(D, o, P, O);
+      case 64032: return launch_tile<MODE, 32, 64, 4, 4>(D, o, P, O);
+      case 128016: return launch_tile<MODE, 16, 128, 2, 5>(D, o, P, O);
+      case 64016: return launch_tile<MODE, 16, 64, 4, 4>(D, o, P, O);
+      default:
+        if constexpr (MODE == kForward) return launch_tile<MODE, 16, 32, 4, 7>(D, o, P, O);
+    }
+  }
+  return launch_product_pair<MODE>(D, o, P, out);
 }
 
 int check_site(const MapalProductSite* s) {
@@ -315,7 +660,7 @@ template <int MODE>
 int by_type(const DeviceSlot& D, const Operands& o, const ProductArgs& P, int dtype, void* out, uint64_t ld, uint64_t ldg) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    return run<MODE, T>(D, o, P, StoreTile<MODE, T>{static_cast<T*>(out), ld, ldg});
+    return run<MODE, T>(D, o, P, StoreTile<MODE, T>{static_cast<T*>(out), ld, ldg}, dtype);
   };
   if (dtype == MAPAL_DTYPE_F16) return go(__half{});
   if constexpr (MODE != kGradX)  // dX is of the rows' type
