@@ -185,8 +185,9 @@ struct SumTile {
   const int32_t* target;
   uint32_t v0, part0;
 
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane, uint32_t from,
-                                      uint32_t to) const {
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
+                                      uint32_t to, uint8_t* scratch) const {
+    const uint32_t lane = lane0 + (threadIdx.x & 31);
     const bool in = lane < P.lanes;
     const uint32_t end = min(to, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;  // the target's column of this tile
@@ -313,8 +314,9 @@ struct GradientTile {
   const unsigned* most;
   uint32_t v0;
 
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane, uint32_t from,
-                                      uint32_t to) const {
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
+                                      uint32_t to, uint8_t* scratch) const {
+    const uint32_t lane = lane0 + (threadIdx.x & 31);
     const bool in = lane < (uint32_t)__ldg(P.lane_count);
     to = min(to, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;
@@ -356,13 +358,29 @@ struct SumsTile {
   const int32_t* place;
   const unsigned* most;  // where not null, the values are divided by dl's scale
   uint64_t ld, lds, ldp;  // rows of out and of sums, parts
+  bool wide;              // see StoreTile
 
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane, uint32_t from,
-                                      uint32_t to) const {
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
+                                      uint32_t to, uint8_t* scratch) const {
+    const uint32_t lane = lane0 + (threadIdx.x & 31);
     const bool in = lane < P.lanes, zero = j.depth == 0;
     const uint32_t l = in ? lane : 0;
     to = min(to, j.cols);
     const float down = scale_down(most);
+    if constexpr (sizeof(T) == 2 && !ADD) {
+      if (wide) {
+        auto row = [&](uint32_t col) {
+          const uint64_t r = j.col0 + col;
+          return out + (place ? (uint64_t)__ldg(place + r) : r) * ld + lane0;
+        };
+        const int left = (int)(P.lanes - lane0);
+        if (most)
+          put_turned<T, true>(taddr, from, to, left, zero, down, scratch, row);
+        else
+          put_turned<T, false>(taddr, from, to, left, zero, 1.0f, scratch, row);
+        return;
+      }
+    }
     for (uint32_t j0 = from; j0 < to; j0 += 16) {
       const uint32_t n = min(16u, to - j0);
       float g[16];
@@ -602,7 +620,7 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
     P.lanes = (uint32_t)s.d;
     if (dw) {
       P.cols = n;
-      const SumsTile<T, false> out{static_cast<T*>(dw) + v0 * s.lddw, nullptr, nullptr, c.q.most, s.lddw, 0, 0};
+      const SumsTile<T, false> out{static_cast<T*>(dw) + v0 * s.lddw, nullptr, nullptr, c.q.most, s.lddw, 0, 0, aligned16(dw) && s.lddw % 8 == 0};
       MAPAL_TRY(launch_product_pair<kGradW>(c.D, {c.q.h, dl, p.ld, 0, p.piece, s.rows, s.d, n}, P, out));
     }
     if (dh) {
@@ -610,15 +628,16 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
       P.parts = p.parts;
       const Operands o{from, dl, ldw, 0, p.piece, n, s.d, n};
       T* to = static_cast<T*>(dh);
+      const bool wide = aligned16(dh) && s.lddh % 8 == 0;
       if (p.parts == 1 && i + 1 == p.pieces) {
         if (p.pieces == 1)
-          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, false>{to, nullptr, c.q.list, c.q.most, s.lddh, 0, 0}));
+          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, false>{to, nullptr, c.q.list, c.q.most, s.lddh, 0, 0, wide}));
         else
-          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, true>{to, sums, c.q.list, c.q.most, s.lddh, s.d, 0}));
+          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, true>{to, sums, c.q.list, c.q.most, s.lddh, s.d, 0, false}));
       } else if (i == 0) {
-        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, false>{sums, nullptr, nullptr, nullptr, s.d, 0, ldp}));
+        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, false>{sums, nullptr, nullptr, nullptr, s.d, 0, ldp, false}));
       } else {
-        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, true>{sums, sums, nullptr, nullptr, s.d, s.d, ldp}));
+        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, true>{sums, sums, nullptr, nullptr, s.d, s.d, ldp, false}));
       }
     }
   }

@@ -146,16 +146,16 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  JobWalk<MODE> walk(P, NT, 128);
+  JobWalk<MODE, NT, 128> walk(P, blockIdx.x, gridDim.x);
   Job j;
-  bool more = walk.at(blockIdx.x, j);
+  bool more = walk.now(j);
   uint32_t it = 0;
 
   if (warp < kCopy) {
     // ---- copies ----
     Lines<MODE != kForward, 128> la;
     Lines<MODE == kGradW, NT> lb;
-    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, j)) {
+    for (; more; more = walk.next(j)) {
       // (lane, t) and (col, t) of the operands: K-major ones run along t
       const uint8_t* a = A.base + (MODE == kGradW ? 0 : j.group * A.ldg);
       a += MODE == kForward ? j.lane0 * A.ld + 2ull * j.t0 : j.t0 * A.ld + 2ull * j.lane0;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
   } else if (warp == kCopy) {
     // ---- products ----
     uint32_t n = 0;
-    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, j), ++n) {
+    for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1, blocks = (j.depth + kStepK - 1) / kStepK;
       if (elect_one()) {
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 128, (int)((j.cols + 15) / 16 * 16));
@@ -219,14 +219,14 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
     // ---- output ----
     const int quarter = warp & 3;
     uint32_t n = 0;
-    for (uint64_t tile = blockIdx.x; more; tile += gridDim.x, more = walk.at(tile, j), ++n) {
+    for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1;
       if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
         *abort = 1;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      out.put(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + quarter * 32 + lane, 0, NT);
+      out.put_plain(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + quarter * 32, 0, NT);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
@@ -276,6 +276,7 @@ struct TileSmem {
   uint64_t full[STAGES], empty[STAGES];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t parts, drained;
+  alignas(16) uint8_t scratch[out_warps(NT)][kOutScratch];
   uint32_t tmem_base;
   int abort;
 };
@@ -285,6 +286,7 @@ struct TileArgs {
   uint64_t ld;
   int32_t otype;
   uint32_t split;
+  uint32_t wide;    // see StoreTile
   uint32_t folded;  // forward: A's map brings a whole stage at once
 };
 
@@ -319,6 +321,8 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   volatile int* abort = &sm.abort;
 
   if (warp == 0 && elect_one()) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
@@ -335,9 +339,9 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   }
   grid_wait();
   grid_go();
-  JobWalk<MODE> walk(P, NT, CH);
+  JobWalk<MODE, NT, CH> walk(P, first, step);
   Job j;
-  bool more = walk.at(first, j);
+  bool more = walk.now(j);
   uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
 
   const uint32_t fills = (kbs + KB - 1) / KB;  // stages a tile takes
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   if (warp == 0) {
     // ---- loads ----
     uint32_t fill = it;  // of the first tile, some are issued
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), fill = 0) {
+    for (; more; more = walk.next(j), fill = 0) {
       if (elect_one())
         for (; fill < fills; ++fill) {
           if (!mbar_wait(&sm.empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort)) {
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   } else if (warp == 1) {
     // ---- products ----
     uint32_t n = 0;
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+    for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1;
       if (elect_one()) {
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 128, (int)((j.cols + 15) / 16 * 16));
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     // ---- output ----
     const int quarter = warp & 3;  // TMEM lanes 32*quarter to +31
     uint32_t n = 0;
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+    for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1, at = j.lane0 + quarter * 32 + lane;
       const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
       if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {  // *abort: its commit was an aborted tile's
@@ -442,7 +446,8 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
       if (split == 1) {
         with_type(O, [&](auto* out) {
-          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, 0}.put(P, j, col, at, from, from + NT / (kOut / 4));
+          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, 0, O.wide != 0}.put(
+              P, j, col, j.lane0 + quarter * 32, from, from + NT / (kOut / 4), sm.scratch[warp - 2]);
         });
       } else {
         const uint32_t share = NT / split;
@@ -598,7 +603,7 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
         }
       }
     }
-    const TileArgs O{out.out, out.ld, otype, best.split, 0};
+    const TileArgs O{out.out, out.ld, otype, best.split, out.wide, 0};
     switch (best.lanes * 1000 + best.cols) {
       case 256256: break;
       case 128128: return launch_tile<MODE, 128, 128, 2, 3>(D, o, P, O);
@@ -660,7 +665,9 @@ template <int MODE>
 int by_type(const DeviceSlot& D, const Operands& o, const ProductArgs& P, int dtype, void* out, uint64_t ld, uint64_t ldg) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    return run<MODE, T>(D, o, P, StoreTile<MODE, T>{static_cast<T*>(out), ld, ldg}, dtype);
+    const uint64_t rows = MODE == kGradW ? P.cols : P.m;
+    const bool wide = aligned16(out) && (rows == 1 || ld % 8 == 0) && (MODE != kGradW || P.groups == 1 || ldg % 8 == 0);
+    return run<MODE, T>(D, o, P, StoreTile<MODE, T>{static_cast<T*>(out), ld, ldg, wide}, dtype);
   };
   if (dtype == MAPAL_DTYPE_F16) return go(__half{});
   if constexpr (MODE != kGradX)  // dX is of the rows' type

@@ -46,69 +46,113 @@ struct Job {
   uint32_t part;
 };
 
-// A warp's walk over the jobs of tiles of NT columns and CH lanes; every lane
-// gets the answer. Lanes run fastest, so that the tiles in flight share their
-// columns' operand.
-template <int MODE>
+// A warp's walk over every step-th job of tiles of NT columns and CH lanes; every
+// lane gets the answers. Lanes run fastest, so that the tiles in flight share their
+// columns' operand. Divisions are made once: one by one, the 64-bit ones of a tile's
+// number took a lone warp 1200 cycles a tile, as long as four blocks' products.
+template <int MODE, int NT, int CH>
 struct JobWalk {
   const ProductArgs& P;
   TileWalk tiles;
-  uint32_t nt, ch, lane_tiles, per_part;
+  uint32_t lane_tiles, per_part;
+  uint64_t outer;               // column tiles (forward, grad x: of all parts) before this one
+  uint32_t inner;               // its lane tile
+  uint64_t d_outer;             // of a step
+  uint32_t d_inner;
+  uint32_t col_tiles, col, group, d_col, d_group;  // grad w: outer, divided by the column tiles of a matrix
+  uint32_t lo, hi;
 
-  __device__ JobWalk(const ProductArgs& p, uint32_t nt_, uint32_t ch_) : P(p), nt(nt_), ch(ch_) {
+  __device__ JobWalk(const ProductArgs& p, uint64_t first, uint64_t step) : P(p) {
     uint32_t lanes = p.lanes;
     if (p.lane_count) lanes = min(lanes, (uint32_t)max(__ldg(p.lane_count), 0));
-    lane_tiles = (lanes + ch_ - 1) / ch_;
-    tiles = TileWalk{p.offsets, p.groups, p.m, nt_, ch_, lane_tiles, p.trap};
-    const uint32_t blocks = (p.depth + kStepK - 1) / kStepK;
-    per_part = p.parts > 1 ? (blocks + p.parts - 1) / p.parts * kStepK : p.depth;
-    if constexpr (MODE != kGradW) tiles.load();
+    lane_tiles = (lanes + CH - 1) / CH;
+    const uint32_t by = max(lane_tiles, 1u);
+    if (((first | step) >> 32) == 0) {
+      outer = (uint32_t)first / by;
+      d_outer = (uint32_t)step / by;
+    } else {
+      outer = first / by;
+      d_outer = step / by;
+    }
+    inner = (uint32_t)(first - outer * by);
+    d_inner = (uint32_t)(step - d_outer * by);
+    if constexpr (MODE == kGradW) {
+      // at most 2^32 column tiles of all matrices: 65535 of 2^23
+      col_tiles = (p.cols + NT - 1) / NT;
+      group = (uint32_t)(outer / col_tiles);
+      col = (uint32_t)(outer - (uint64_t)group * col_tiles);
+      d_group = (uint32_t)(d_outer / col_tiles);
+      d_col = (uint32_t)(d_outer - (uint64_t)d_group * col_tiles);
+      range();
+    } else {
+      tiles = TileWalk{p.offsets, p.groups, p.m, NT, CH, lane_tiles, p.trap};
+      tiles.load();
+      const uint32_t blocks = (p.depth + kStepK - 1) / kStepK;
+      per_part = p.parts > 1 ? (blocks + p.parts - 1) / p.parts * kStepK : p.depth;
+    }
   }
 
-  __device__ bool at(uint64_t tile, Job& j) {
+  // grad w: the group's rows.
+  __device__ __forceinline__ void range() {
+    lo = 0, hi = P.m;
+    if (P.offsets && group < P.groups) {
+      const int32_t a = __ldg(P.offsets + group), b = __ldg(P.offsets + group + 1);
+      const bool bad = a < 0 || b < a || (uint32_t)b > P.m;
+      if (bad && (threadIdx.x & 31) == 0) atomicMax(P.trap, kTrapOob);
+      lo = min((uint32_t)max(a, 0), P.m);
+      hi = max(lo, min((uint32_t)max(b, 0), P.m));
+    }
+  }
+
+  __device__ __forceinline__ bool now(Job& j) {
     if (lane_tiles == 0) return false;
+    j.lane0 = inner * CH;
+    j.part = 0;
     if constexpr (MODE == kGradW) {
-      const uint32_t col_tiles = (P.cols + nt - 1) / nt;
-      const uint64_t per = (uint64_t)col_tiles * lane_tiles;
-      const uint64_t g = tile / per;
-      if (g >= P.groups) return false;
-      const uint32_t in = (uint32_t)(tile % per);  // at most 2^32 tiles a matrix, checked on the host
-      j.group = (uint32_t)g;
-      j.col0 = in / lane_tiles * nt;
-      j.cols = min(nt, P.cols - j.col0);
-      j.lane0 = in % lane_tiles * ch;
-      j.part = 0;
-      uint32_t lo = 0, hi = P.m;
-      if (P.offsets) {
-        const int32_t a = __ldg(P.offsets + g), b = __ldg(P.offsets + g + 1);
-        const bool bad = a < 0 || b < a || (uint32_t)b > P.m;
-        if (bad && (threadIdx.x & 31) == 0) atomicMax(P.trap, kTrapOob);
-        lo = min((uint32_t)max(a, 0), P.m);
-        hi = max(lo, min((uint32_t)max(b, 0), P.m));
-      }
+      if (group >= P.groups) return false;
+      j.group = group;
+      j.col0 = col * NT;
+      j.cols = min((uint32_t)NT, P.cols - j.col0);
       j.t0 = lo;
       j.depth = hi - lo;
-      return true;
     } else {
-      // parts run slowest: the tiles of one part share the operands' blocks
-      uint32_t part = 0;
-      if (P.parts > 1) {  // one group of all rows
-        const uint64_t per = (uint64_t)tiles.chunk * lane_tiles;
-        if (tile >= per * P.parts) return false;
-        part = (uint32_t)(tile / per);
-        tile %= per;
+      // parts (of one group of all rows) run slowest: the tiles of one share the operands' blocks
+      uint64_t at = outer;
+      if (P.parts > 1) {
+        if (at >= (uint64_t)tiles.chunk * P.parts) return false;
+        j.part = (uint32_t)(at / tiles.chunk);
+        at -= (uint64_t)j.part * tiles.chunk;
       }
       Tile t;
-      if (!tiles.at(tile, t)) return false;
+      if (!tiles.find(at, t)) return false;
       j.group = t.group;
       j.col0 = t.token0;
       j.cols = t.tokens;
-      j.lane0 = t.channel0;
-      j.part = part;
-      j.t0 = min(part * per_part, P.depth);
+      j.t0 = min(j.part * per_part, P.depth);
       j.depth = min(per_part, P.depth - j.t0);
-      return true;
     }
+    return true;
+  }
+
+  __device__ __forceinline__ bool next(Job& j) {
+    inner += d_inner;
+    const uint32_t carry = inner >= lane_tiles;
+    inner -= carry ? lane_tiles : 0;
+    if constexpr (MODE == kGradW) {
+      col += d_col + carry;
+      uint32_t g = group + d_group;
+      if (col >= col_tiles) {
+        col -= col_tiles;
+        ++g;
+      }
+      if (g != group) {
+        group = g;
+        range();
+      }
+    } else {
+      outer += d_outer + carry;
+    }
+    return now(j);
   }
 };
 
@@ -181,19 +225,128 @@ __device__ __forceinline__ void put16(T* c, uint64_t ld, const float (&f)[16]) {
   }
 }
 
+// 16 lanes by 32 columns of tensor memory as fragments: of every 8 columns a thread
+// gets two neighbours of lane t/4 and the same of lane t/4 + 8.
+__device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, float (&f)[16]) {
+  int r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = __int_as_float(r[i]);
+}
+
+constexpr int kOutScratch = 32 * 64;  // bytes of shared memory that a writing warp needs
+
+// Columns [from, to) of a warp's 32 lanes, of which `left` exist, as 16-bit values: 32
+// columns at a time are turned in shared memory (stmatrix, transposed) so that a
+// thread writes 8 lanes of a column at once, row(j) + 8*its part; every row is
+// 16-byte aligned. Elements written one by one keep a warp 32 stores for what
+// takes 4 here: the weights' gradient of 256 rows over 64 matrices of 1024 x 2048,
+// which is writing, 100 us with them.
+template <typename T, bool SCALE, typename Row>
+__device__ __forceinline__ void put_turned(uint32_t taddr, uint32_t from, uint32_t to, int left, bool zero, float factor,
+                                           uint8_t* scratch, Row&& row) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t put = sa(scratch) + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+  const uint32_t get = (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  const int have = left - (int)(lane & 3) * 8;  // of this thread's 8 lanes
+  float f[2][16];
+  auto load = [&](uint32_t j0) {
+    tmem_ld16x32(taddr + j0, f[0]);
+    tmem_ld16x32(taddr + (16u << 16) + j0, f[1]);
+  };
+  if (zero) {  // sums over nothing
+    for (uint32_t j0 = from; j0 < to; j0 += 8) {
+      const uint32_t col = j0 + (lane >> 2);
+      if (col < to)
+        for (int e = 0; e < min(8, have); ++e) row(col)[(lane & 3) * 8 + e] = from_f32<T>(0.0f);
+    }
+    return;
+  }
+  if (from < to) load(from);
+  for (uint32_t j0 = from; j0 < to; j0 += 32) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(f[0][i]), "+f"(f[1][i]));
+    uint32_t w[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // lanes t/4 and t/4 + 8 of both halves
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = SCALE ? f[h][4 * q + e] * factor : f[h][4 * q + e];
+        Pack<T, 4> o;
+        o.set(v);
+        w[q][2 * h] = o.w[0], w[q][2 * h + 1] = o.w[1];
+      }
+    if (j0 + 32 < to) load(j0 + 32);  // beside the stores
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + q * 512),
+                   "r"(w[q][0]), "r"(w[q][1]), "r"(w[q][2]), "r"(w[q][3])
+                   : "memory");
+    __syncwarp();
+    Pack<T, 8> o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(scratch + i * 512 + get);
+      o[i].w[0] = v.x, o[i].w[1] = v.y, o[i].w[2] = v.z, o[i].w[3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t col = j0 + i * 8 + (lane >> 2);
+      if (col < to && have > 0) {
+        T* c = row(col) + (lane & 3) * 8;
+        if (have >= 8)
+          *reinterpret_cast<Pack<T, 8>*>(c) = o[i];
+        else
+          st_part(c, o[i], (1u << have) - 1);
+      }
+    }
+    __syncwarp();
+  }
+}
+
 // The output as it lies in memory: column j of a job at row (grad w: row of the
-// group's matrix), lanes along the row.
+// group's matrix), lanes along the row. wide: 16-bit rows on 16-byte boundaries.
 template <int MODE, typename T>
 struct StoreTile {
   T* out;
   uint64_t ld, ldg;  // rows, groups' matrices
+  bool wide;
 
-  // Columns [from, to) of the 32 lanes of a warp, of which this thread has `lane`.
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane, uint32_t from,
-                                      uint32_t to) const {
-    const bool in = lane < P.lanes, zero = j.depth == 0;
+  __device__ __forceinline__ T* at(const Job& j, uint32_t lane0) const {
+    return out + (MODE == kGradW ? (uint64_t)j.group * ldg : 0) + (uint64_t)j.col0 * ld + lane0;
+  }
+
+  // Columns [from, to) of the 32 lanes of a warp from lane0 on.
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
+                                      uint32_t to, uint8_t* scratch) const {
+    if constexpr (sizeof(T) == 2) {
+      if (wide) {
+        T* c = at(j, lane0);
+        put_turned<T, false>(taddr, from, min(to, j.cols), (int)(P.lanes - lane0), j.depth == 0, 1.0f, scratch,
+                             [&](uint32_t col) { return c + col * ld; });
+        return;
+      }
+    }
+    put_plain(P, j, taddr, lane0, from, to);
+  }
+
+  // The same, element by element.
+  __device__ __forceinline__ void put_plain(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0,
+                                            uint32_t from, uint32_t to) const {
+    const bool zero = j.depth == 0;
     to = min(to, j.cols);
-    T* c = out + (MODE == kGradW ? (uint64_t)j.group * ldg : 0) + (uint64_t)(j.col0 + from) * ld + (in ? lane : 0);
+    T* c = at(j, lane0);
+    const uint32_t lane = threadIdx.x & 31;
+    const bool in = lane0 + lane < P.lanes;
+    c += from * ld + (in ? lane : 0);
     for (uint32_t j0 = from; j0 < to; j0 += 16, c += 16 * ld) {
       float f[16];
       tmem_ld16f(taddr + j0, f);
@@ -237,12 +390,19 @@ struct PairSmem {
   uint64_t acc_full[2];          // each CTA's own
   uint64_t acc_empty[2];         // the first CTA's: both CTAs have read the accumulator
   uint64_t drained;
+  alignas(16) uint8_t scratch[kPairOut][kOutScratch];
   uint32_t tmem_base;
   int abort;
 };
 constexpr size_t kPairSmem = sizeof(PairSmem) + 1024;
 static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
 constexpr int pair_threads(int mode) { return 64 + 32 * kPairOut + (mode == kGradW ? 32 : 0); }
+
+// An arrival at another CTA's barrier that orders nothing but the tensor memory read
+// before it (tcgen05.fence): a release would first wait for the tile's stores.
+__device__ __forceinline__ void arrive_remote_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
@@ -293,8 +453,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
   const uint32_t rank = blockIdx.x & 1;
   const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
   volatile int* abort = &sm.abort;
+  auto give_up = [&]() {  // both CTAs stop
+    *abort = 1;
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(sa(&sm.abort), rank ^ 1)), "r"(1) : "memory");
+  };
 
   if (warp == 0 && elect_one()) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
@@ -317,12 +483,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  cg::this_cluster().sync();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  JobWalk<MODE, NT, 256> walk(P, first, step);  // while the other CTA gets here
+  Job j;
+  bool more = walk.now(j);
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  JobWalk<MODE> walk(P, NT, 256);
-  Job j;
-  bool more = walk.at(first, j);
   uint32_t it = 0;      // stages taken
   uint32_t fixes = 0;   // a bit a stage: the parity of its next clearing
 
@@ -332,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
 
   if (warp == 0) {
     // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j)) {
+    for (; more; more = walk.next(j)) {
       const uint32_t blocks = blocks_of(j), half = (j.cols + 31) / 32 * 16;  // columns of each CTA
       const bool fix = to_fix(j);
       const int lane0 = (int)(j.lane0 + rank * 128), col0 = (int)(j.col0 + rank * half);
@@ -340,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
         for (uint32_t kb = 0; kb < blocks; kb += kPairKB, ++it) {
           const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
           if (!mbar_wait(&sm.empty[s], ((it / kPairStages) & 1) ^ 1, abort)) {
-            *abort = 1;
+            give_up();
             break;
           }
           const bool last = fix && kb + here == blocks;
@@ -361,12 +528,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
   } else if (warp == 1) {
     // ---- products, by the first CTA ----
     uint32_t n = 0;
-    for (uint64_t tile = first; rank == 0 && more; tile += step, more = walk.at(tile, j), ++n) {
+    for (; rank == 0 && more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1, blocks = blocks_of(j);
       const bool fix = to_fix(j);
       if (elect_one()) {
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 256, (int)((j.cols + 31) / 32 * 32));
-        if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
+        if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) give_up();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         for (uint32_t kb = 0; kb < blocks && !*abort; kb += kPairKB, ++it) {
           const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
@@ -376,7 +543,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
             fixes ^= 1u << s;
           }
           if (!ok) {
-            *abort = 1;
+            give_up();
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -402,13 +569,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
     }
   } else if (MODE == kGradW && warp == 2 + kPairOut) {
     // ---- last blocks: rows behind the group's become zeros ----
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j)) {
+    for (; more; more = walk.next(j)) {
       const uint32_t blocks = blocks_of(j), fills = (blocks + kPairKB - 1) / kPairKB;
       it += fills;
       if (!to_fix(j)) continue;
       const uint32_t s = (it - 1) % kPairStages;
       if (any_of(!mbar_wait(&sm.landed[s], (fixes >> s) & 1, abort))) {
-        *abort = 1;
+        give_up();
         break;
       }
       fixes ^= 1u << s;
@@ -426,27 +593,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
     const int quarter = warp & 3;
     const uint32_t from = (warp - 2) / 4 * kHalfTokens;
     uint32_t n = 0;
-    for (uint64_t tile = first; more; tile += step, more = walk.at(tile, j), ++n) {
+    for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1;
       if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
-        *abort = 1;
+        give_up();
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      out.put(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + rank * 128 + quarter * 32 + lane, from,
-              from + kHalfTokens);
+      out.put(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + rank * 128 + quarter * 32, from,
+              from + kHalfTokens, sm.scratch[warp - 2]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_remote(remote(sa(&sm.acc_empty[b]), 0));
+      if (lane == 0) arrive_remote_relaxed(remote(sa(&sm.acc_empty[b]), 0));
     }
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   cg::this_cluster().sync();
-  // A wait gave up in either CTA (its flag is read after both have stopped):
-  // what is still in flight ends before shared memory and TMEM are given back.
-  const bool stop = *abort || *(volatile int*)cg::this_cluster().map_shared_rank(&sm.abort, rank ^ 1);
+  const bool stop = *abort;  // a wait gave up in either CTA, which told the other
   if (stop) {
+    // what is still in flight ends before shared memory and TMEM are given back
     if (warp == 0 && elect_one()) {
       atomicOr(P.trap, kDeviceTimeout);
       // every stage's last use, in the first CTA for both, and each CTA's own blocks to clear
@@ -462,7 +628,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
     }
   }
   __syncwarp();
-  cg::this_cluster().sync();
+  if (stop) cg::this_cluster().sync();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));

@@ -59,6 +59,7 @@ __device__ __forceinline__ uint64_t now_ns() {
 // Bounded wait on a phase: false when kWaitLimitNs ran out, or (abort given)
 // when another role has aborted.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
+  if (mbar_try(b, parity)) return true;  // without a look at the timer, which takes some 200 cycles
   const uint64_t t0 = now_ns();
   for (uint32_t i = 0;; ++i) {
     if (mbar_try(b, parity)) return true;
@@ -72,7 +73,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile
 // The same for a barrier that other CTAs of the cluster arrive at: what they
 // wrote before their arrivals is visible after the wait.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort) {
-  const uint64_t t0 = now_ns();
+  uint64_t t0 = 0;
   for (uint32_t i = 0;; ++i) {
     uint32_t ok;
     asm volatile(
@@ -83,6 +84,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* b, uint32_t parity, 
         : "r"(sa(b)), "r"(parity)
         : "memory");
     if (ok) return true;
+    if (i == 0) t0 = now_ns();
     if ((i & 255) == 255) {
       if (abort && *abort) return false;
       if (now_ns() - t0 > kWaitLimitNs) return false;
@@ -118,6 +120,11 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sa(bar))
                : "memory");
+}
+
+// Brings a tensor map near the TMA unit ahead of its first load.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // The driver's cuTensorMapEncodeTiled, looked up once (a function-local

@@ -104,7 +104,12 @@ struct TileWalk {
   }
 
   __device__ bool at(uint64_t tile, Tile& t) {
-    const uint64_t token_tile = tile / channel_tiles;
+    t.channel0 = (uint32_t)(tile % channel_tiles) * channels;
+    return find(tile / channel_tiles, t);
+  }
+
+  // The group and tokens of a token tile.
+  __device__ __forceinline__ bool find(uint64_t token_tile, Tile& t) {
     while (token_tile >= (uint64_t)before + chunk) {
       base += 32;
       if (base >= groups) return false;
@@ -118,7 +123,6 @@ struct TileWalk {
     t.group = base + src;
     t.token0 = glo + (want - first) * nt;
     t.tokens = min(nt, ghi - t.token0);
-    t.channel0 = (uint32_t)(tile % channel_tiles) * channels;
     return true;
   }
 };
