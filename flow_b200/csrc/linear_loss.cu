@@ -564,7 +564,7 @@ struct Call {
     P.lanes = (uint32_t)s.rows;
     P.lane_count = q.count + 1;
     P.depth = (uint32_t)s.d;
-    return launch_product_pair<kForward>(D, {q.h, w, p.ld, 0, ldw, s.rows, s.d, s.d}, P, out);
+    return launch_product_pair<kForward, false, false>(D, {q.h, w, p.ld, 0, ldw, s.rows, s.d, s.d}, P, out);
   }
 };
 
@@ -621,7 +621,7 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
     if (dw) {
       P.cols = n;
       const SumsTile<T, false> out{static_cast<T*>(dw) + v0 * s.lddw, nullptr, nullptr, c.q.most, s.lddw, 0, 0, aligned16(dw) && s.lddw % 8 == 0};
-      MAPAL_TRY(launch_product_pair<kGradW>(c.D, {c.q.h, dl, p.ld, 0, p.piece, s.rows, s.d, n}, P, out));
+      MAPAL_TRY((launch_product_pair<kGradW, false, false>(c.D, {c.q.h, dl, p.ld, 0, p.piece, s.rows, s.d, n}, P, out)));
     }
     if (dh) {
       P.depth = n;
@@ -631,13 +631,13 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
       const bool wide = aligned16(dh) && s.lddh % 8 == 0;
       if (p.parts == 1 && i + 1 == p.pieces) {
         if (p.pieces == 1)
-          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, false>{to, nullptr, c.q.list, c.q.most, s.lddh, 0, 0, wide}));
+          MAPAL_TRY((launch_product_pair<kGradX, false, false>(c.D, o, P, SumsTile<T, false>{to, nullptr, c.q.list, c.q.most, s.lddh, 0, 0, wide})));
         else
-          MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<T, true>{to, sums, c.q.list, c.q.most, s.lddh, s.d, 0, false}));
+          MAPAL_TRY((launch_product_pair<kGradX, false, false>(c.D, o, P, SumsTile<T, true>{to, sums, c.q.list, c.q.most, s.lddh, s.d, 0, false})));
       } else if (i == 0) {
-        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, false>{sums, nullptr, nullptr, nullptr, s.d, 0, ldp, false}));
+        MAPAL_TRY((launch_product_pair<kGradX, false, false>(c.D, o, P, SumsTile<float, false>{sums, nullptr, nullptr, nullptr, s.d, 0, ldp, false})));
       } else {
-        MAPAL_TRY(launch_product_pair<kGradX>(c.D, o, P, SumsTile<float, true>{sums, sums, nullptr, nullptr, s.d, s.d, ldp, false}));
+        MAPAL_TRY((launch_product_pair<kGradX, false, false>(c.D, o, P, SumsTile<float, true>{sums, sums, nullptr, nullptr, s.d, s.d, ldp, false})));
       }
     }
   }

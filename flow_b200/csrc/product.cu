@@ -1,21 +1,106 @@
 // product.cu — products in 16-bit floats with one matrix or one per group of rows,
 // and their gradients (mapal_gpu_product*). No counterpart in the reference.
+#include <cstdlib>
 #include "product.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace {
 
-// ---- any operands ----------------------------------------------------------------------
+// ---- operands that TMA cannot read ---------------------------------------------------------
 //
-// One CTA a tile of 128 lanes by NT columns. Copying warps bring a block of t at
-// a time into the swizzled layout of shared memory, from operands at any place and
-// stride: both layouts are lines of 128 bytes (a K-major line is a lane's or
-// column's 64 steps of t, an MN-major one 64 lanes or columns at one step), so
-// one loop serves all three products. Steps behind the group's last are zeros in
-// both operands.
+// Bases or strides off 16 bytes: copying warps bring such an operand's block of t into
+// the layout that TMA would have given it. Both layouts are lines of 128 bytes (a
+// K-major line is a lane's or column's 64 steps of t, an MN-major one 64 lanes or
+// columns at one step), so one loop serves all products. A thread has 16 bytes of
+// every 32nd line: lines so far apart, and a line's next blocks, begin at the same
+// place in an aligned word of 16 bytes, so its shift is the same for a whole tile. It
+// loads the two aligned words that hold its bytes, a block ahead, and shifts them on
+// the way to shared memory. What does not exist is zeros, steps behind a group's last
+// among them.
 
-constexpr int kCopyThreads = 512;
+struct CopyOperand {
+  const uint8_t* base;
+  uint64_t ld, ldg;  // bytes
+};
+
+constexpr int kCopyThreads = 256;
+
+template <bool MN, int LINES>
+struct Lines {
+  static constexpr int kTurns = (LINES * 8 + kCopyThreads - 1) / kCopyThreads;
+  const uint8_t* at;  // the aligned word of this thread's first line at the block's t
+  uint64_t ld;
+  uint32_t sh;
+  int32_t lines;  // K-major: lines from this thread's first on; MN-major: steps of t from its first on
+  int32_t width;  // elements from this thread's first on: K-major of t, MN-major of lanes or columns
+  uint4 a[kTurns], b[kTurns];
+
+  // first: the address of (first lane or column, first step of t).
+  __device__ __forceinline__ void set(uint32_t thread, const uint8_t* first, uint64_t ld_, uint32_t extent, uint32_t depth) {
+    const uint32_t c = thread & 7, line = thread >> 3;
+    const uint8_t* p = first + line * ld_ + c * 16;
+    sh = (uint32_t)(uintptr_t)p & 15;
+    at = p - sh;
+    ld = ld_;
+    lines = (int32_t)(MN ? depth : extent) - (int32_t)line;
+    width = (int32_t)(MN ? extent : depth) - (int32_t)(c * 8);
+  }
+  static __device__ __forceinline__ int line_of(int i) { return MN ? (i & 1) * 32 : i * 32; }
+  static __device__ __forceinline__ int chunk_of(int i) { return MN ? i >> 1 : 0; }
+  // Elements of turn i's 16 bytes that exist, 0 to 8.
+  __device__ __forceinline__ int have(int i) const {
+    return line_of(i) < lines ? max(0, min(8, width - chunk_of(i) * 64)) : 0;
+  }
+  __device__ __forceinline__ bool whole() const { return (MN ? lines > 32 : width >= 8) && (!MN || width >= (kTurns > 2 ? 72 : 8)); }
+
+  // No aligned word is read without one of the elements in it.
+  __device__ __forceinline__ void load() {
+    const bool all = whole();
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const uint4* w = reinterpret_cast<const uint4*>(at + line_of(i) * ld + chunk_of(i) * 128);
+      const int n = all ? (MN || line_of(i) < lines ? 8 : 0) : have(i);
+      a[i] = n > 0 ? __ldg(w) : make_uint4(0, 0, 0, 0);
+      b[i] = n > 0 && sh + 2 * n > 16 ? __ldg(w + 1) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t thread, uint8_t* tile) const {
+    const uint32_t c = thread & 7, line = thread >> 3;
+    uint8_t* to = tile + line * 128 + ((c ^ (line & 7)) << 4);
+    const bool all = whole();
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      uint4 v = straddle(a[i], b[i], sh);
+      if (!all) {
+        const int n = have(i);
+        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = n >= 2 * k + 2 ? q[k] : n == 2 * k + 1 ? q[k] & 0xffffu : 0u;
+        v = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+      *reinterpret_cast<uint4*>(to + i * (32 * 128)) = v;
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (MN) {
+      at += kStepK * ld;
+      lines -= kStepK;
+    } else {
+      at += 128;
+      width -= kStepK;
+    }
+  }
+};
+
+// The address of lane or column `first` of an operand at step t.
+template <bool MN>
+__device__ __forceinline__ const uint8_t* operand_at(const CopyOperand& o, uint64_t group, uint64_t first, uint64_t t) {
+  return o.base + group * o.ldg + (MN ? t * o.ld + 2 * first : first * o.ld + 2 * t);
+}
+
+// One CTA a tile of 128 lanes by NT columns, both operands copied.
+
 constexpr int kAnyOut = 4;  // warps that write
 
 template <int NT, int STAGES>
@@ -28,91 +113,9 @@ struct AnySmem {
   int abort;
 };
 
-struct AnyOperand {
-  const uint8_t* base;
-  uint64_t ld, ldg;  // bytes
-};
-
-// A thread's share of one operand's block: 16 bytes of every kCopyThreads/8-th line.
-template <bool MN, int LINES>
-struct Lines {
-  static constexpr int kTurns = (LINES * 8 + kCopyThreads - 1) / kCopyThreads;
-  const uint8_t* at;  // this thread's 16 bytes of its first line, at the block's t
-  uint64_t step;      // to its next line
-  uint64_t ld;
-  int32_t rows;   // K-major: lines that exist; MN-major: steps of t that are left
-  int32_t width;  // elements from this thread's first on: K-major of t, MN-major of lanes or columns
-  uint4 a[kTurns], b[kTurns];
-
-  // first: the address of (first lane or column, first step of t).
-  __device__ __forceinline__ void set(const uint8_t* first, uint64_t ld_, uint32_t extent, uint32_t depth) {
-    const uint32_t c = threadIdx.x & 7, line = threadIdx.x >> 3;
-    ld = ld_;
-    at = first + line * ld_ + c * 16;
-    step = kCopyThreads / 8 * ld_;
-    if (MN) {
-      rows = (int32_t)min(depth, 0x7fffffffu);
-      width = (int32_t)extent - (int32_t)(c * 8);
-      // lines 64.. are the next 64 lanes or columns at the same steps
-    } else {
-      rows = (int32_t)extent;
-      width = (int32_t)min(depth, 0x7fffffffu) - (int32_t)(c * 8);
-    }
-  }
-  static_assert(kCopyThreads / 8 == kStepK, "a turn is one 64 lines: an MN-major chunk");
-
-  // Elements of the 16 bytes of turn i that exist, 0 to 8.
-  __device__ __forceinline__ int have(int i) const {
-    const int line = (int)(threadIdx.x >> 3);
-    const bool there = (MN ? line : line + i * (kCopyThreads / 8)) < rows && (LINES >= kCopyThreads / 8 || line < LINES);
-    const int w = MN ? width - i * 64 : width;
-    return there ? max(0, min(8, w)) : 0;
-  }
-  __device__ __forceinline__ const uint8_t* place(int i) const { return MN ? at + i * 128 : at + i * step; }
-
-  // The aligned words that hold the elements: none is read without one of them.
-  __device__ __forceinline__ void load() {
-#pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      const int n = have(i);
-      const uint8_t* p = place(i);
-      const uint32_t sh = (uint32_t)(uintptr_t)p & 15;
-      const uint4* w = reinterpret_cast<const uint4*>(p - sh);
-      a[i] = n > 0 ? __ldg(w) : make_uint4(0, 0, 0, 0);
-      b[i] = n > 0 && sh + 2 * n > 16 ? __ldg(w + 1) : make_uint4(0, 0, 0, 0);
-    }
-  }
-  __device__ __forceinline__ void store(uint8_t* tile) const {
-    const uint32_t c = threadIdx.x & 7, line = threadIdx.x >> 3;
-    if (LINES < kCopyThreads / 8 && line >= LINES) return;
-    uint8_t* to = tile + line * 128 + ((c ^ (line & 7)) << 4);
-#pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      const int n = have(i);
-      uint4 v = straddle(a[i], b[i], (uint32_t)(uintptr_t)place(i) & 15);
-      if (n < 8) {
-        uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = n >= 2 * k + 2 ? q[k] : n == 2 * k + 1 ? q[k] & 0xffffu : 0u;
-        v = make_uint4(q[0], q[1], q[2], q[3]);
-      }
-      *reinterpret_cast<uint4*>(to + i * (kStepK * 128)) = v;
-    }
-  }
-  __device__ __forceinline__ void next() {
-    if (MN) {
-      at += kStepK * ld;
-      rows -= kStepK;
-    } else {
-      at += 128;
-      width -= kStepK;
-    }
-  }
-};
-
 template <int MODE, typename T, int NT, int STAGES>
 __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
-    product_any_kernel(const AnyOperand A, const AnyOperand B, const __grid_constant__ ProductArgs P,
+    product_any_kernel(const CopyOperand A, const CopyOperand B, const __grid_constant__ ProductArgs P,
                        const StoreTile<MODE, T> out) {
   using Smem = AnySmem<NT, STAGES>;
   constexpr uint32_t kCols = 2 * NT;
@@ -156,12 +159,9 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
     Lines<MODE != kForward, 128> la;
     Lines<MODE == kGradW, NT> lb;
     for (; more; more = walk.next(j)) {
-      // (lane, t) and (col, t) of the operands: K-major ones run along t
-      const uint8_t* a = A.base + (MODE == kGradW ? 0 : j.group * A.ldg);
-      a += MODE == kForward ? j.lane0 * A.ld + 2ull * j.t0 : j.t0 * A.ld + 2ull * j.lane0;
-      const uint8_t* b = B.base + (MODE == kGradW ? j.t0 * B.ld + 2ull * j.col0 : j.col0 * B.ld + 2ull * j.t0);
-      la.set(a, A.ld, P.lanes - j.lane0, j.depth);
-      lb.set(b, B.ld, j.cols, j.depth);
+      la.set(threadIdx.x, operand_at<MODE != kForward>(A, MODE == kGradW ? 0 : j.group, j.lane0, j.t0), A.ld,
+             P.lanes - j.lane0, j.depth);
+      lb.set(threadIdx.x, operand_at<MODE == kGradW>(B, 0, j.col0, j.t0), B.ld, j.cols, j.depth);
       const uint32_t blocks = (j.depth + kStepK - 1) / kStepK;
       bool gone = false;
       if (blocks) {
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
         const uint32_t s = it % STAGES;
         gone = any_of(!mbar_wait(&sm.empty[s], ((it / STAGES) & 1) ^ 1, abort));
         if (gone) break;
-        la.store(sm.stage[s]);
-        lb.store(sm.stage[s] + 128 * 128);
+        la.store(threadIdx.x, sm.stage[s]);
+        lb.store(threadIdx.x, sm.stage[s] + 128 * 128);
         if (kb + 1 < blocks) {  // the next block's loads run beside this one's products
           la.next();
           lb.next();
@@ -516,8 +516,8 @@ int launch_any(const DeviceSlot& D, const Operands& o, const ProductArgs& P, con
   static std::atomic<uint64_t> done{0};
   auto kernel = product_any_kernel<MODE, T, NT, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "product shared memory"));
-  const AnyOperand A{static_cast<const uint8_t*>(o.a), 2 * o.lda, 2 * o.ldga};
-  const AnyOperand B{static_cast<const uint8_t*>(o.b), 2 * o.ldb, 0};
+  const CopyOperand A{static_cast<const uint8_t*>(o.a), 2 * o.lda, 2 * o.ldga};
+  const CopyOperand B{static_cast<const uint8_t*>(o.b), 2 * o.ldb, 0};
   const uint64_t tiles = product_tiles(MODE, P, NT, 128), cap = D.prof.sm_count;
   return launch_rows(kernel, (unsigned)(tiles < cap ? tiles : cap), kCopyThreads + 32 * (1 + kAnyOut), smem, D.stream, 1, A,
                      B, P, out);
@@ -583,7 +583,14 @@ int launch_tile(const DeviceSlot& D, const Operands& o, const ProductArgs& P, Ti
 
 template <int MODE, typename T>
 int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const StoreTile<MODE, T>& out, int otype) {
-  if (!tma_reads(MODE, P, o)) return launch_any<MODE, T, 128, 4>(D, o, P, out);
+  const bool ta = tma_reads_a(MODE, P, o), tb = tma_reads_b(P, o);
+  if (!ta || !tb) {
+    const bool ra = raw_reads(o.rows, o.a_cols, o.lda, MODE == kGradW ? 1 : P.groups, o.ldga);
+    if (getenv("ANY") || !ra || !raw_reads(P.m, o.b_cols, o.ldb, 1, 0)) return launch_any<MODE, T, 128, 4>(D, o, P, out);
+    if (ta) return launch_product_pair<MODE, false, true>(D, o, P, out);
+    if (tb) return launch_product_pair<MODE, true, false>(D, o, P, out);
+    return launch_product_pair<MODE, true, true>(D, o, P, out);
+  }
   if constexpr (MODE != kGradW) {
     static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
                                     {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
@@ -618,7 +625,7 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
         if constexpr (MODE == kForward) return launch_tile<MODE, 16, 32, 4, 7>(D, o, P, O);
     }
   }
-  return launch_product_pair<MODE>(D, o, P, out);
+  return launch_product_pair<MODE, false, false>(D, o, P, out);
 }
 
 int check_site(const MapalProductSite* s) {

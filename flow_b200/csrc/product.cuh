@@ -378,30 +378,112 @@ struct StoreTile {
 // the group's last up to the next 16 (the MMA's step) in both operands, since zero
 // times NaN is not zero, and lets the products go on (fixed).
 
-constexpr int kPairStages = 3, kPairKB = 2, kPairTokens = 256, kPairOut = 8;
+// An operand off 16 bytes (CA, CB) comes by TMA all the same, raw: every eighth of its
+// rows lies 16-byte aligned from the one before, so eight maps, one for each row
+// number's remainder, each with its base rounded down, bring lines with up to 14
+// foreign bytes before them. Copying warps shift them into the swizzled layout:
+// a line's remainder, and so its shift, is the same for all of a thread's lines.
+// Everything else is as with operands in place. A copy loop through registers
+// instead (two aligned words a thread, a block ahead) took 3300 ns a block of
+// both operands, waiting for L1's few lines; this takes MEASURED.
 
+constexpr int kPairTokens = 256, kPairOut = 8;
+constexpr int kCopyGroups = 2, kCopyWarps = 4;  // groups of so many warps take turns at the blocks
+constexpr uint64_t kRawLandNs = 1000000;  // after a wait gave up: for raw loads in flight
+constexpr int kLineK = 144, kLineMN = 272;  // raw bytes of a line: 64 steps, or 128 lanes or columns, and 16 more
+constexpr int kRawOperand = 128 * kLineK;
+static_assert(64 * kLineMN <= kRawOperand, "raw lines");
+
+// STAGES of KB blocks; RAW: raw operands side by side in flight.
+template <int STAGES, int KB, int RAW>
 struct PairSmem {
   static constexpr int kHalf = 128 * 128;  // bytes of a block of lanes, and of columns
-  uint8_t stage[kPairStages][kPairKB * 2 * kHalf];
-  uint64_t full[kPairStages];    // the first CTA's: both CTAs' loads have landed
-  uint64_t empty[kPairStages];   // each CTA's own
-  uint64_t landed[kPairStages];  // each CTA's own: a last block to clear
-  uint64_t fixed[kPairStages];   // the first CTA's: cleared in both
-  uint64_t acc_full[2];          // each CTA's own
-  uint64_t acc_empty[2];         // the first CTA's: both CTAs have read the accumulator
+  uint8_t stage[STAGES][KB * 2 * kHalf];
+  alignas(128) uint8_t raw[RAW == 0 ? 1 : RAW][RAW == 0 ? 16 : kRawOperand];
+  uint64_t full[STAGES];    // the first CTA's: both CTAs' loads have landed
+  uint64_t empty[STAGES];   // each CTA's own
+  uint64_t landed[STAGES];  // each CTA's own: a last block to clear
+  uint64_t fixed[STAGES];   // the first CTA's: cleared in both
+  uint64_t raw_full[RAW == 0 ? 1 : RAW], raw_empty[RAW == 0 ? 1 : RAW];  // each CTA's own
+  uint64_t acc_full[2];     // each CTA's own
+  uint64_t acc_empty[2];    // the first CTA's: both CTAs have read the accumulator
   uint64_t drained;
   alignas(16) uint8_t scratch[kPairOut][kOutScratch];
   uint32_t tmem_base;
   int abort;
 };
-constexpr size_t kPairSmem = sizeof(PairSmem) + 1024;
-static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
-constexpr int pair_threads(int mode) { return 64 + 32 * kPairOut + (mode == kGradW ? 32 : 0); }
+// Copied operands: stages of one block, and raw blocks of 2 (both copied) or 3 (one).
+template <bool CA, bool CB>
+struct PairCut {
+  static constexpr bool kCopy = CA || CB;
+  static constexpr int kStages = kCopy ? 4 : 3, kKB = kCopy ? 1 : 2;
+  static constexpr int kRaw = CA && CB ? 2 : kCopy ? 3 : 0;  // raw blocks
+  using Smem = PairSmem<kStages, kKB, kRaw * (CA + CB)>;
+  static constexpr size_t kSmem = sizeof(Smem) + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+};
+// loads, products, output, grad w: clearing, and copies
+__host__ __device__ constexpr int pair_fixers(int mode, bool ca, bool cb) { return mode == kGradW && !(ca && cb) ? 1 : 0; }
+__host__ __device__ constexpr int pair_threads(int mode, bool ca, bool cb) {
+  return 64 + 32 * kPairOut + 32 * pair_fixers(mode, ca, cb) + (ca || cb ? 32 * kCopyGroups * kCopyWarps : 0);
+}
+
+struct RawMaps {
+  CUtensorMap m[8];
+};
+// A copied operand beside its maps: where row 0 begins in an aligned word and what a row adds.
+struct RawPlace {
+  uint32_t base, ld;  // bytes, modulo 16
+  uint32_t rows;      // from one matrix to the next
+};
+
+// Raw lines of the 128 (K-major: rows from row0 on, steps from x on) or 64 (MN-major:
+// steps from row0 on, 128 lanes or columns from x on) rows of a block.
+template <bool MN>
+__device__ __forceinline__ void raw_load(uint8_t* raw, const RawMaps& maps, uint32_t row0, int x, uint64_t* bar) {
+  constexpr int kRows = MN ? 8 : 16, kLine = MN ? kLineMN : kLineK;
+  mbar_expect_tx(bar, 8 * kRows * kLine);
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i)  // the first rows of each remainder: row0 + i
+    tma_load_2d(raw + ((row0 + i) & 7) * (kRows * kLine), &maps.m[(row0 + i) & 7], x, (int)((row0 + i) >> 3), bar);
+}
+
+// A thread's share of shifting a raw block into the swizzled layout: 16 bytes of every
+// 16th line. left: rows of the block that exist (MN-major; the others become zeros).
+template <bool MN>
+__device__ __forceinline__ void raw_shift(uint32_t thread, const uint8_t* raw, const RawPlace& o, uint32_t row0, uint32_t lines,
+                                          uint32_t left, uint8_t* tile) {
+  constexpr int kRows = MN ? 8 : 16, kLine = MN ? kLineMN : kLineK;
+  constexpr int kApart = kCopyWarps * 4;  // lines from one turn to the next
+  static_assert(kApart == 16, "whole eights of lines, four turns a chunk of 64");
+  const uint32_t c = thread & 7, line = thread >> 3;
+  const uint32_t sh = (o.base + (row0 + line) * o.ld) & 15;
+  const uint32_t s = (row0 + line) & 7, q = (line - ((s - row0) & 7)) >> 3;
+  const uint8_t* from = raw + (s * kRows + q) * kLine + c * 16;
+  uint8_t* to = tile + line * 128 + ((c ^ (line & 7)) << 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = MN ? (i & 3) * 2 * kLine + (i >> 2) * 128 : i * 2 * kLine;
+    if (!MN && line + i * kApart >= lines) break;
+    uint4 v = straddle(*reinterpret_cast<const uint4*>(from + at), *reinterpret_cast<const uint4*>(from + at + 16), sh);
+    if (MN && line + (i & 3) * kApart >= left) v = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(to + i * (kApart * 128)) = v;
+  }
+}
 
 // An arrival at another CTA's barrier that orders nothing but the tensor memory read
 // before it (tcgen05.fence): a release would first wait for the tile's stores.
 __device__ __forceinline__ void arrive_remote_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// An arrival at the first CTA's barrier for what this warp has written to its own
+// CTA's shared memory, where only the tensor cores read it: fence.proxy.async, by
+// every writing lane before, has waited until they see it, so the arrival itself needs
+// no order beyond the CTA. As a release among the CTAs it would take 500 to 1500
+// cycles, the time of two blocks.
+__device__ __forceinline__ void arrive_written(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -419,36 +501,48 @@ __device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, 
       : "memory");
 }
 
-// A CTA's 128 lanes and its half of the columns of one block of t. W's map has the
-// groups as its third dimension.
-template <int MODE>
-__device__ __forceinline__ void pair_load_block(uint8_t* a, const CUtensorMap* map_a, const CUtensorMap* map_b, const Job& j,
+// A CTA's 128 lanes and its half of the columns of one block of t, of the operands
+// that TMA reads. W's map has the groups as its third dimension.
+template <int MODE, bool TA, bool TB>
+__device__ __forceinline__ void pair_load_block(uint8_t* a, uint8_t* b, const CUtensorMap* map_a, const CUtensorMap* map_b, const Job& j,
                                                 int t, int lane0, int col0, uint32_t bar) {
-  uint8_t* b = a + PairSmem::kHalf;
   constexpr int kChunk = kStepK * 128;  // 64 lanes or columns of an MN-major block
-  if constexpr (MODE == kForward) {
-    pair_load_3d(a, map_a, t, lane0, (int)j.group, bar);
-    pair_load_2d(b, map_b, t, col0, bar);
-  } else if constexpr (MODE == kGradX) {
-    pair_load_3d(a, map_a, lane0, t, (int)j.group, bar);
-    pair_load_3d(a + kChunk, map_a, lane0 + 64, t, (int)j.group, bar);
-    pair_load_2d(b, map_b, t, col0, bar);
-  } else {
-    pair_load_2d(a, map_a, lane0, t, bar);
-    pair_load_2d(a + kChunk, map_a, lane0 + 64, t, bar);
-    pair_load_2d(b, map_b, col0, t, bar);
-    pair_load_2d(b + kChunk, map_b, col0 + 64, t, bar);
+  if constexpr (TA) {
+    if constexpr (MODE == kForward) {
+      pair_load_3d(a, map_a, t, lane0, (int)j.group, bar);
+    } else if constexpr (MODE == kGradX) {
+      pair_load_3d(a, map_a, lane0, t, (int)j.group, bar);
+      pair_load_3d(a + kChunk, map_a, lane0 + 64, t, (int)j.group, bar);
+    } else {
+      pair_load_2d(a, map_a, lane0, t, bar);
+      pair_load_2d(a + kChunk, map_a, lane0 + 64, t, bar);
+    }
+  }
+  if constexpr (TB) {
+    if constexpr (MODE == kGradW) {
+      pair_load_2d(b, map_b, col0, t, bar);
+      pair_load_2d(b + kChunk, map_b, col0 + 64, t, bar);
+    } else {
+      pair_load_2d(b, map_b, t, col0, bar);
+    }
   }
 }
 
-template <int MODE, typename Out>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 1)
-    product_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                        const __grid_constant__ ProductArgs P, const __grid_constant__ Out out) {
+// CA, CB: the operand is copied.
+template <int MODE, bool CA, bool CB, typename Out>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, CA, CB), 1)
+    product_pair_kernel(const __grid_constant__ std::conditional_t<CA, RawMaps, CUtensorMap> maps_a,
+                        const __grid_constant__ std::conditional_t<CB, RawMaps, CUtensorMap> maps_b, const RawPlace place_a,
+                        const RawPlace place_b, const __grid_constant__ ProductArgs P, const __grid_constant__ Out out) {
   namespace cg = cooperative_groups;
-  constexpr int NT = kPairTokens;
+  using Cut = PairCut<CA, CB>;
+  using Smem = typename Cut::Smem;
+  constexpr int NT = kPairTokens, kStages = Cut::kStages, kKB = Cut::kKB, kRaw = Cut::kRaw;
+  constexpr bool TA = !CA, TB = !CB;
+  constexpr int kFixer = 2 + kPairOut, kCopier = kFixer + pair_fixers(MODE, CA, CB);  // warps
+  constexpr bool MA = MODE != kForward, MB = MODE == kGradW;  // MN-major
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = blockIdx.x & 1;
   const uint64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
@@ -459,13 +553,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
   };
 
   if (warp == 0 && elect_one()) {
-    prefetch_map(&map_a);
-    prefetch_map(&map_b);
-    for (int s = 0; s < kPairStages; ++s) {
-      mbar_init(&sm.full[s], 1);
+    for (size_t i = 0; i < sizeof(maps_a) / sizeof(CUtensorMap); ++i) prefetch_map(reinterpret_cast<const CUtensorMap*>(&maps_a) + i);
+    for (size_t i = 0; i < sizeof(maps_b) / sizeof(CUtensorMap); ++i) prefetch_map(reinterpret_cast<const CUtensorMap*>(&maps_b) + i);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sm.full[s], (TA || TB) + (Cut::kCopy ? 2 * kCopyWarps : 0));
       mbar_init(&sm.empty[s], 1);
       mbar_init(&sm.landed[s], 1);
       mbar_init(&sm.fixed[s], 2);
+    }
+    for (int i = 0; i < kRaw * (CA + CB); ++i) {
+      mbar_init(&sm.raw_full[i], 1);
+      mbar_init(&sm.raw_empty[i], kCopyWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
@@ -494,34 +592,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
   uint32_t fixes = 0;   // a bit a stage: the parity of its next clearing
 
   auto blocks_of = [](const Job& q) { return (q.depth + kStepK - 1) / kStepK; };
-  // whether the last block holds rows that are not the group's
-  auto to_fix = [&](const Job& q) { return MODE == kGradW && (q.depth & 15) && q.t0 + q.depth < P.m; };
+  // whether the last block holds rows that are not the group's (copied operands have none)
+  auto to_fix = [&](const Job& q) { return MODE == kGradW && (TA || TB) && (q.depth & 15) && q.t0 + q.depth < P.m; };
 
   if (warp == 0) {
     // ---- loads, each CTA its halves, both counted by the first CTA's barrier ----
+    uint32_t raws = 0;  // raw blocks taken
     for (; more; more = walk.next(j)) {
       const uint32_t blocks = blocks_of(j), half = (j.cols + 31) / 32 * 16;  // columns of each CTA
       const bool fix = to_fix(j);
       const int lane0 = (int)(j.lane0 + rank * 128), col0 = (int)(j.col0 + rank * half);
+      const uint32_t row_a = (MODE == kGradW ? 0 : j.group * place_a.rows) + (MA ? j.t0 : (uint32_t)lane0);
       if (elect_one())
-        for (uint32_t kb = 0; kb < blocks; kb += kPairKB, ++it) {
-          const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
-          if (!mbar_wait(&sm.empty[s], ((it / kPairStages) & 1) ^ 1, abort)) {
-            give_up();
-            break;
+        for (uint32_t kb = 0; kb < blocks; kb += kKB, ++it) {
+          const uint32_t s = it % kStages, here = min((uint32_t)kKB, blocks - kb);
+          if (Cut::kCopy) {
+            const uint32_t q = raws % kRaw, parity = (raws / kRaw & 1) ^ 1, t = j.t0 + kb * kStepK;
+            bool ok = true;
+            if (CA) {
+              ok = mbar_wait(&sm.raw_empty[q], parity, abort);
+              if (ok) raw_load<MA>(sm.raw[q], *reinterpret_cast<const RawMaps*>(&maps_a), row_a + (MA ? kb * kStepK : 0), MA ? lane0 : (int)t, &sm.raw_full[q]);
+            }
+            if (CB && ok) {
+              const uint32_t p = q + CA * kRaw;
+              ok = mbar_wait(&sm.raw_empty[p], parity, abort);
+              if (ok) raw_load<MB>(sm.raw[p], *reinterpret_cast<const RawMaps*>(&maps_b), MB ? t : (uint32_t)col0, MB ? col0 : (int)t, &sm.raw_full[p]);
+            }
+            if (!ok) {
+              give_up();
+              break;
+            }
+            ++raws;
           }
-          const bool last = fix && kb + here == blocks;
-          if (rank == 0) mbar_expect_tx(&sm.full[s], (here - last) * 4 * PairSmem::kHalf);
-          if (last) {
-            mbar_expect_tx(&sm.landed[s], 2 * PairSmem::kHalf);
-            fixes ^= 1u << s;
-          }
-          const uint32_t bar = remote(sa(&sm.full[s]), 0);
+          if (TA || TB) {
+            if (!mbar_wait(&sm.empty[s], ((it / kStages) & 1) ^ 1, abort)) {
+              give_up();
+              break;
+            }
+            const bool last = fix && kb + here == blocks;
+            if (rank == 0) mbar_expect_tx(&sm.full[s], (here - last) * 2 * (TA + TB) * Smem::kHalf);
+            if (last) {
+              mbar_expect_tx(&sm.landed[s], (TA + TB) * Smem::kHalf);
+              fixes ^= 1u << s;
+            }
+            const uint32_t bar = remote(sa(&sm.full[s]), 0);
 #pragma unroll
-          for (uint32_t u = 0; u < kPairKB; ++u)
-            if (u < here)
-              pair_load_block<MODE>(sm.stage[s] + 2 * u * PairSmem::kHalf, &map_a, &map_b, j, (int)(j.t0 + (kb + u) * kStepK),
-                                    lane0, col0, last && u + 1 == here ? remote(sa(&sm.landed[s]), rank) : bar);
+            for (uint32_t u = 0; u < kKB; ++u)
+              if (u < here) {
+                uint8_t* to = sm.stage[s] + 2 * u * Smem::kHalf;
+                pair_load_block<MODE, TA, TB>(to, to + Smem::kHalf, reinterpret_cast<const CUtensorMap*>(&maps_a),
+                                              reinterpret_cast<const CUtensorMap*>(&maps_b), j, (int)(j.t0 + (kb + u) * kStepK),
+                                              lane0, col0, last && u + 1 == here ? remote(sa(&sm.landed[s]), rank) : bar);
+              }
+          }
         }
       if (any_of(*abort)) break;
     }
@@ -535,9 +658,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 256, (int)((j.cols + 31) / 32 * 32));
         if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) give_up();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (uint32_t kb = 0; kb < blocks && !*abort; kb += kPairKB, ++it) {
-          const uint32_t s = it % kPairStages, here = min((uint32_t)kPairKB, blocks - kb);
-          bool ok = mbar_wait(&sm.full[s], (it / kPairStages) & 1, abort);
+        for (uint32_t kb = 0; kb < blocks && !*abort; kb += kKB, ++it) {
+          const uint32_t s = it % kStages, here = min((uint32_t)kKB, blocks - kb);
+          bool ok = CA || CB ? mbar_wait_cluster(&sm.full[s], (it / kStages) & 1, abort)
+                             : mbar_wait(&sm.full[s], (it / kStages) & 1, abort);
           if (fix && kb + here == blocks) {
             ok = ok && mbar_wait_cluster(&sm.fixed[s], (fixes >> s) & 1, abort);
             fixes ^= 1u << s;
@@ -547,18 +671,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t da = operand_desc<MODE != kForward>(sm.stage[s]),
-                         db = operand_desc<MODE == kGradW>(sm.stage[s] + PairSmem::kHalf);
+          const uint64_t da = operand_desc<MA>(sm.stage[s]), db = operand_desc<MB>(sm.stage[s] + Smem::kHalf);
 #pragma unroll
-          for (uint32_t u = 0; u < kPairKB; ++u)
+          for (uint32_t u = 0; u < kKB; ++u)
             if (u < here) {
               // grad w: no step behind the group's rows
               const uint32_t left = j.depth - (kb + u) * kStepK;
 #pragma unroll
               for (uint32_t kk = 0; kk < kStepK / 16; ++kk)
                 if (MODE != kGradW || kk * 16 < left)
-                  mma_f16<2>(tmem + b * NT, da + u * (2 * PairSmem::kHalf >> 4) + kk * operand_step<MODE != kForward>(),
-                             db + u * (2 * PairSmem::kHalf >> 4) + kk * operand_step<MODE == kGradW>(), idesc,
+                  mma_f16<2>(tmem + b * NT, da + u * (2 * Smem::kHalf >> 4) + kk * operand_step<MA>(),
+                             db + u * (2 * Smem::kHalf >> 4) + kk * operand_step<MB>(), idesc,
                              kb > 0 || u > 0 || kk > 0);
             }
           pair_commit(&sm.empty[s]);
@@ -567,26 +690,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
       }
       if (any_of(*abort)) break;
     }
-  } else if (MODE == kGradW && warp == 2 + kPairOut) {
+  } else if (warp >= kFixer && warp < kCopier) {
     // ---- last blocks: rows behind the group's become zeros ----
     for (; more; more = walk.next(j)) {
-      const uint32_t blocks = blocks_of(j), fills = (blocks + kPairKB - 1) / kPairKB;
+      const uint32_t blocks = blocks_of(j), fills = (blocks + kKB - 1) / kKB;
       it += fills;
       if (!to_fix(j)) continue;
-      const uint32_t s = (it - 1) % kPairStages;
+      const uint32_t s = (it - 1) % kStages;
       if (any_of(!mbar_wait(&sm.landed[s], (fixes >> s) & 1, abort))) {
         give_up();
         break;
       }
       fixes ^= 1u << s;
       const uint32_t rows = j.depth - (blocks - 1) * kStepK, to = (rows + 15) / 16 * 16;
-      uint8_t* block = sm.stage[s] + (blocks - 1) % kPairKB * (2 * PairSmem::kHalf);
-      for (uint32_t chunk = 0; chunk < 4; ++chunk)
+      uint8_t* block = sm.stage[s] + (blocks - 1) % kKB * (2 * Smem::kHalf);
+      for (uint32_t chunk = TA ? 0 : 2; chunk < (TB ? 4 : 2); ++chunk)
         for (uint32_t i = rows * 8 + lane; i < to * 8; i += 32)
           *reinterpret_cast<uint4*>(block + chunk * (kStepK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_remote(remote(sa(&sm.fixed[s]), 0));
+      if (lane == 0) arrive_written(remote(sa(&sm.fixed[s]), 0));
+    }
+  } else if ((CA || CB) && warp >= kCopier) {
+    // ---- copies ----
+    const uint32_t mine = (warp - kCopier) / kCopyWarps, thread = (threadIdx.x - kCopier * 32) % (32 * kCopyWarps);
+    uint32_t raws = 0;
+    for (; more; more = walk.next(j)) {
+      const uint32_t blocks = blocks_of(j), half = (j.cols + 31) / 32 * 16;
+      const uint32_t lane0 = j.lane0 + rank * 128, col0 = j.col0 + rank * half;
+      const uint32_t row_a = (MODE == kGradW ? 0 : j.group * place_a.rows) + (MA ? j.t0 : lane0);
+      bool gone = false;
+#pragma unroll 1
+      for (uint32_t kb = 0; kb < blocks; ++kb, ++it, ++raws) {
+        const uint32_t s = it % kStages, q = raws % kRaw, parity = raws / kRaw & 1;
+        const uint32_t left = j.depth - kb * kStepK;
+        if (raws % kCopyGroups != mine) continue;
+        gone = !mbar_wait(&sm.empty[s], ((it / kStages) & 1) ^ 1, abort);
+        if (CA && !gone) {
+          gone = !mbar_wait(&sm.raw_full[q], parity, abort);
+          if (!gone)
+            raw_shift<MA>(thread, sm.raw[q], place_a, row_a + (MA ? kb * kStepK : 0), 128, left, sm.stage[s]);
+        }
+        if (CB && !gone) {
+          const uint32_t p = q + CA * kRaw;
+          gone = !mbar_wait(&sm.raw_full[p], parity, abort);
+          if (!gone)
+            raw_shift<MB>(thread, sm.raw[p], place_b, MB ? j.t0 + kb * kStepK : col0, half, left, sm.stage[s] + Smem::kHalf);
+        }
+        gone = any_of(gone);
+        if (gone) break;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if (CA) mbar_arrive(&sm.raw_empty[q]);
+          if (CB) mbar_arrive(&sm.raw_empty[q + CA * kRaw]);
+          arrive_written(remote(sa(&sm.full[s]), 0));
+        }
+      }
+      if (gone) give_up();
+      if (any_of(*abort)) break;
     }
   } else {
     // ---- output ----
@@ -616,11 +778,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
     if (warp == 0 && elect_one()) {
       atomicOr(P.trap, kDeviceTimeout);
       // every stage's last use, in the first CTA for both, and each CTA's own blocks to clear
-      for (uint32_t i = it > kPairStages ? it - kPairStages : 0; i < it; ++i) {
-        if (rank == 0) mbar_wait(&sm.full[i % kPairStages], (i / kPairStages) & 1, nullptr);
+      if (TA || TB)
+        for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) {
+        if (rank == 0) mbar_wait(&sm.full[i % kStages], (i / kStages) & 1, nullptr);
       }
       if (MODE == kGradW)
-        for (int s = 0; s < kPairStages; ++s) mbar_wait(&sm.landed[s], ((fixes >> s) & 1) ^ 1, nullptr);
+        for (int s = 0; s < kStages; ++s) mbar_wait(&sm.landed[s], ((fixes >> s) & 1) ^ 1, nullptr);
+      if (Cut::kCopy) {
+        const uint64_t t0 = now_ns();  // raw lines land within microseconds, whoever waits for them
+        while (now_ns() - t0 < kRawLandNs) {
+        }
+      }
     }
     if (warp == 1 && rank == 0 && elect_one()) {
       pair_commit(&sm.drained);
@@ -681,27 +849,65 @@ struct Operands {
   uint64_t rows, a_cols, b_cols;  // rows and columns of one of A's matrices, columns of B
 };
 
-inline bool tma_reads(int mode, const ProductArgs& P, const Operands& o) {
-  return tma_reads16(o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga) &&
-         tma_reads16(o.b, P.m, o.b_cols, o.ldb, 1, 0);
+inline bool tma_reads_a(int mode, const ProductArgs& P, const Operands& o) {
+  return tma_reads16(o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga);
 }
+inline bool tma_reads_b(const ProductArgs& P, const Operands& o) { return tma_reads16(o.b, P.m, o.b_cols, o.ldb, 1, 0); }
 
 // The maps of tiles of `lanes` and `cols`; an MN-major operand comes in boxes of 64 x 64.
-inline int product_maps(int mode, const ProductArgs& P, const Operands& o, uint32_t lanes, uint32_t cols, CUtensorMap* ma,
-                        CUtensorMap* mb) {
-  MAPAL_TRY(product_map(ma, o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga, mode == kGradW ? 2 : 3,
-                        mode == kForward ? lanes : kStepK));
-  return product_map(mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, mode == kGradW ? kStepK : cols);
+inline int product_map_a(int mode, const ProductArgs& P, const Operands& o, uint32_t lanes, CUtensorMap* map) {
+  return product_map(map, o.a, o.rows, o.a_cols, o.lda, mode == kGradW ? 1 : P.groups, o.ldga, mode == kGradW ? 2 : 3,
+                     mode == kForward ? lanes : kStepK);
+}
+inline int product_map_b(int mode, const ProductArgs& P, const Operands& o, uint32_t cols, CUtensorMap* map) {
+  return product_map(map, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, mode == kGradW ? kStepK : cols);
 }
 
-template <int MODE, typename Out>
+// The eight maps of rows x cols elements at stride ld that lie anywhere: row r by map r
+// modulo 8, from its base rounded down on.
+inline int raw_maps(RawMaps* maps, RawPlace* place, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, bool mn,
+                    uint64_t matrix_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  for (uint64_t s = 0; s < 8; ++s) {
+    const uint64_t row = s < rows ? s : 0;  // a remainder without rows is loaded all the same, and not used
+    const uint64_t p = (uint64_t)(uintptr_t)base + 2 * row * ld, sh = p & 15;
+    cuuint64_t dim[2] = {cols + sh / 2, s < rows ? (rows - s + 7) / 8 : 1};
+    cuuint64_t stride[1] = {dim[1] > 1 ? 16 * ld : (2 * dim[0] + 15) / 16 * 16};
+    cuuint32_t box[2] = {(cuuint32_t)(mn ? kLineMN : kLineK) / 2, mn ? 8u : 16u}, one[2] = {1, 1};
+    const CUresult r = fn(&maps->m[s], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, (void*)(uintptr_t)(p - sh), dim, stride, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(MAPAL_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  }
+  *place = {(uint32_t)((uintptr_t)base & 15), (uint32_t)(2 * ld & 15), (uint32_t)matrix_rows};
+  return 0;
+}
+
+// Whether an operand that lies anywhere can be loaded raw: its matrices are one run of rows.
+inline bool raw_reads(uint64_t rows, uint64_t cols, uint64_t ld, uint64_t mats, uint64_t ldm) {
+  return rows && cols && ld < (1ull << 35) && (mats == 1 || ldm == rows * ld) && mats * rows < (1ull << 31);
+}
+
+template <int MODE, bool CA, bool CB, typename Out>
 int launch_product_pair(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Out& out) {
-  CUtensorMap ma, mb;
-  MAPAL_TRY(product_maps(MODE, P, o, 128, 128, &ma, &mb));
+  std::conditional_t<CA, RawMaps, CUtensorMap> ma;
+  std::conditional_t<CB, RawMaps, CUtensorMap> mb;
+  RawPlace pa{}, pb{};
+  const uint64_t mats = MODE == kGradW ? 1 : P.groups;
+  if constexpr (CA)
+    MAPAL_TRY(raw_maps(&ma, &pa, o.a, mats * o.rows, o.a_cols, o.lda, MODE != kForward, o.rows));
+  else
+    MAPAL_TRY(product_map_a(MODE, P, o, 128, &ma));
+  if constexpr (CB)
+    MAPAL_TRY(raw_maps(&mb, &pb, o.b, P.m, o.b_cols, o.ldb, MODE == kGradW, P.m));
+  else
+    MAPAL_TRY(product_map_b(MODE, P, o, 128, &mb));
   static std::atomic<uint64_t> done{0};
-  auto kernel = product_pair_kernel<MODE, Out>;
-  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, kPairSmem, "product shared memory"));
+  auto kernel = product_pair_kernel<MODE, CA, CB, Out>;
+  constexpr size_t smem = PairCut<CA, CB>::kSmem;
+  MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, smem, "product shared memory"));
   const uint64_t tiles = product_tiles(MODE, P, kPairTokens, 256), cap = D.prof.sm_count / 2;
-  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * 2), pair_threads(MODE), kPairSmem, D.stream, 1, ma, mb,
-                     P, out);
+  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * 2), pair_threads(MODE, CA, CB), smem, D.stream, 1, ma,
+                     mb, pa, pb, P, out);
 }
