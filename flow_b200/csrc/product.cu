@@ -251,10 +251,10 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
 
 // ---- a CTA a tile ------------------------------------------------------------------------
 //
-// Forward and grad x of a few rows: up to 128 columns (NT) and CH lanes. The MMA
-// always has M = 128; with CH below 128 the other rows of its operand are whatever
-// shared memory holds and their results are not read: few rows are bound by reading
-// the weights, and narrower tiles spread them over more SMs.
+// Products of few tiles: up to 128 columns (NT) and CH lanes. The MMA always has
+// M = 128; with CH below 128 the other rows of its operand are whatever shared memory
+// holds and their results are not read: few rows are bound by reading the weights, and
+// narrower tiles spread them over more SMs.
 //
 // Where even that leaves SMs idle, t is split over a cluster of `split` CTAs: each
 // leaves its f32 partial sums in the shared memory of the CTA that writes those
@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(kCopyThreads + 32 * (1 + kAnyOut), 1)
 // A stage holds KB blocks of t. Forward weights come with one load a stage where k
 // and n allow it (multiples of 64 and 8): the map splits k into blocks and channels
 // into eights, so that a stage lies as [eight][block][8 rows][128 bytes] and each row
-// is read KB*128 bytes at a time. Grad x takes 64 lanes by KB*64 steps with a load.
+// is read KB*128 bytes at a time. An MN-major operand comes as 64 lanes or columns by
+// KB*64 steps with a load. grad w: rows behind a group's last are cleared as in pairs.
 
 template <int NT, int CH, int KB, int STAGES>
 struct TileSmem {
@@ -273,7 +274,7 @@ struct TileSmem {
   // lanes of A, in the last stage past its end.
   uint8_t stage[STAGES][kStage];
   uint8_t past[128 - CH > NT ? KB * (128 - CH - NT) * 128 : 16];
-  uint64_t full[STAGES], empty[STAGES];
+  uint64_t full[STAGES], empty[STAGES], fixed[STAGES];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t parts, drained;
   alignas(16) uint8_t scratch[out_warps(NT)][kOutScratch];
@@ -283,7 +284,7 @@ struct TileSmem {
 
 struct TileArgs {
   void* out;
-  uint64_t ld;
+  uint64_t ld, ldg;
   int32_t otype;
   uint32_t split;
   uint32_t wide;    // see StoreTile
@@ -301,23 +302,22 @@ __device__ __forceinline__ void with_type(const TileArgs& O, F&& f) {
     f(static_cast<float*>(O.out));
 }
 
+__host__ __device__ constexpr int tile_threads(int mode, int nt) { return 64 + 32 * out_warps(nt) + (mode == kGradW ? 32 : 0); }
+
 template <int MODE, int NT, int CH, int KB, int STAGES>
-__global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
+__global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
     product_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ ProductArgs P, const __grid_constant__ TileArgs O) {
   using Smem = TileSmem<NT, CH, KB, STAGES>;
   constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
   constexpr int kOut = out_warps(NT);
-  constexpr bool MN = MODE != kForward;
+  constexpr bool MN = MODE != kForward, MB = MODE == kGradW;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* partial = reinterpret_cast<float*>(&sm + 1);  // split > 1: NT x CH partial sums
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t split = O.split, rank = split > 1 ? blockIdx.x % split : 0;
   const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
-  const uint32_t k_blocks = (P.depth + kStepK - 1) / kStepK;
-  const uint32_t kb_lo = (uint32_t)((uint64_t)k_blocks * rank / split);
-  const uint32_t kbs = (uint32_t)((uint64_t)k_blocks * (rank + 1) / split) - kb_lo;
   volatile int* abort = &sm.abort;
 
   if (warp == 0 && elect_one()) {
@@ -326,12 +326,13 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
+      mbar_init(&sm.fixed[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
       mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
     }
-    mbar_init(&sm.parts, split * CH);
+    mbar_init(&sm.parts, split * CH * (kOut / 4));
     mbar_init(&sm.drained, 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -344,27 +345,49 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
   bool more = walk.now(j);
   uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
 
-  const uint32_t fills = (kbs + KB - 1) / KB;  // stages a tile takes
+  uint32_t fixes = 0;  // a bit a stage: the parity of its next clearing
+  uint32_t kb_lo, kbs, fills;  // this CTA's blocks of the tile, and the stages they take
+  auto cut = [&]() {
+    const uint32_t k_blocks = (j.depth + kStepK - 1) / kStepK;
+    kb_lo = split > 1 ? (uint32_t)((uint64_t)k_blocks * rank / split) : 0;
+    kbs = (split > 1 ? (uint32_t)((uint64_t)k_blocks * (rank + 1) / split) : k_blocks) - kb_lo;
+    fills = (kbs + KB - 1) / KB;
+  };
+  if (more) cut();
+  // whether the CTA's last block holds rows that are not the group's
+  auto to_fix = [&]() {
+    return MODE == kGradW && kbs && (j.depth & 15) && (kb_lo + kbs) * kStepK > j.depth && j.t0 + j.depth < P.m;
+  };
   auto blocks_of = [&](uint32_t fill) { return min((uint32_t)KB, kbs - fill * KB); };
   const bool folded = !MN && KB > 1 && O.folded;
   auto load = [&](uint32_t fill) {
     const uint32_t s = it % STAGES, blocks = blocks_of(fill);
     uint8_t* st = sm.stage[s];
-    const int t0 = (int)(kb_lo + fill * KB) * kStepK;
-    mbar_expect_tx(&sm.full[s], (MN || folded ? KB : blocks) * Smem::kATile + blocks * Smem::kBTile);
+    const int t0 = (int)(j.t0 + (kb_lo + fill * KB) * kStepK);
+    mbar_expect_tx(&sm.full[s], (MN || folded ? KB : blocks) * Smem::kATile + (MB ? KB : blocks) * Smem::kBTile);
     if (MN) {
 #pragma unroll
-      for (int c = 0; c < CH / 64; ++c)
-        tma_load_3d(st + c * (KB * kStepK * 128), &map_a, (int)j.lane0 + c * 64, t0, (int)j.group, &sm.full[s]);
+      for (int c = 0; c < CH / 64; ++c) {
+        uint8_t* to = st + c * (KB * kStepK * 128);
+        if (MODE == kGradW)
+          tma_load_2d(to, &map_a, (int)j.lane0 + c * 64, t0, &sm.full[s]);
+        else
+          tma_load_3d(to, &map_a, (int)j.lane0 + c * 64, t0, (int)j.group, &sm.full[s]);
+      }
     } else if (folded) {
       tma_load_5d(st, &map_a, 0, 0, (int)(kb_lo + fill * KB), (int)(j.lane0 / 8), (int)j.group, &sm.full[s]);
+    }
+    if (MB) {
+#pragma unroll
+      for (int c = 0; c < NT / 64; ++c)
+        tma_load_2d(st + KB * Smem::kATile + c * (KB * kStepK * 128), &map_b, (int)j.col0 + c * 64, t0, &sm.full[s]);
     }
 #pragma unroll
     for (uint32_t u = 0; u < KB; ++u)
       if (u < blocks) {
         const int t = t0 + (int)u * kStepK;
         if (!MN && !folded) tma_load_3d(st + u * Smem::kATile, &map_a, t, (int)j.lane0, (int)j.group, &sm.full[s]);
-        tma_load_2d(st + KB * Smem::kATile + u * Smem::kBTile, &map_b, t, (int)j.col0, &sm.full[s]);
+        if (!MB) tma_load_2d(st + KB * Smem::kATile + u * Smem::kBTile, &map_b, t, (int)j.col0, &sm.full[s]);
       }
     ++it;
   };
@@ -388,6 +411,7 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     // ---- loads ----
     uint32_t fill = it;  // of the first tile, some are issued
     for (; more; more = walk.next(j), fill = 0) {
+      cut();
       if (elect_one())
         for (; fill < fills; ++fill) {
           if (!mbar_wait(&sm.empty[it % STAGES], ((it / STAGES) & 1) ^ 1, abort)) {
@@ -403,27 +427,39 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
     uint32_t n = 0;
     for (; more; more = walk.next(j), ++n) {
       const uint32_t b = n & 1;
+      cut();
+      const bool fix = to_fix();
       if (elect_one()) {
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 128, (int)((j.cols + 15) / 16 * 16));
         if (!mbar_wait(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) *abort = 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         for (uint32_t fill = 0; fill < fills && !*abort; ++fill, ++it) {
           const uint32_t s = it % STAGES, blocks = blocks_of(fill);
-          if (!mbar_wait(&sm.full[s], (it / STAGES) & 1, abort)) {
+          bool ok = mbar_wait(&sm.full[s], (it / STAGES) & 1, abort);
+          if (fix && fill + 1 == fills) {
+            ok = ok && mbar_wait(&sm.fixed[s], (fixes >> s) & 1, abort);
+            fixes ^= 1u << s;
+          }
+          if (!ok) {
             *abort = 1;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint64_t da = MN ? desc_mn(sm.stage[s], KB * kStepK * 128) : desc128(sm.stage[s], folded ? KB * 1024 : 1024),
-                         db = desc128(sm.stage[s] + KB * Smem::kATile);
+                         db = MB ? desc_mn(sm.stage[s] + KB * Smem::kATile, KB * kStepK * 128)
+                                 : desc128(sm.stage[s] + KB * Smem::kATile);
           const uint32_t next = (MN ? kStepK * 128 : folded ? 1024 : Smem::kATile) >> 4;
+          const uint32_t next_b = (MB ? kStepK * 128 : Smem::kBTile) >> 4;
 #pragma unroll
           for (uint32_t u = 0; u < KB; ++u)
             if (u < blocks) {
+              // grad w: no step behind the group's rows
+              const uint32_t left = j.depth - (kb_lo + fill * KB + u) * kStepK;
 #pragma unroll
               for (uint32_t kk = 0; kk < kStepK / 16; ++kk)
-                mma_f16<1>(tmem + b * NT, da + u * next + kk * operand_step<MN>(), db + u * (Smem::kBTile >> 4) + kk * 2,
-                           idesc, fill > 0 || u > 0 || kk > 0);
+                if (MODE != kGradW || kk * 16 < left)
+                  mma_f16<1>(tmem + b * NT, da + u * next + kk * operand_step<MN>(), db + u * next_b + kk * operand_step<MB>(),
+                             idesc, fill > 0 || u > 0 || kk > 0);
             }
           mma_commit(&sm.empty[s]);
         }
@@ -431,11 +467,31 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       }
       if (any_of(*abort)) break;
     }
+  } else if (MODE == kGradW && warp == 2 + kOut) {
+    // ---- last blocks: rows behind the group's become zeros ----
+    for (; more; more = walk.next(j)) {
+      cut();
+      it += fills;
+      if (!to_fix()) continue;
+      const uint32_t s = (it - 1) % STAGES;
+      if (any_of(!mbar_wait(&sm.full[s], ((it - 1) / STAGES) & 1, abort))) {
+        *abort = 1;
+        break;
+      }
+      const uint32_t rows = j.depth - (kb_lo + (fills - 1) * KB) * kStepK, to = (rows + 15) / 16 * 16;
+      for (uint32_t chunk = 0; chunk < (CH + NT) / 64; ++chunk)
+        for (uint32_t i = rows * 8 + lane; i < to * 8; i += 32)
+          *reinterpret_cast<uint4*>(sm.stage[s] + chunk * (KB * kStepK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.fixed[s]);
+    }
   } else if ((warp & 3) < CH / 32) {
     // ---- output ----
     const int quarter = warp & 3;  // TMEM lanes 32*quarter to +31
     uint32_t n = 0;
     for (; more; more = walk.next(j), ++n) {
+      cut();
       const uint32_t b = n & 1, at = j.lane0 + quarter * 32 + lane;
       const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
       if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {  // *abort: its commit was an aborted tile's
@@ -446,14 +502,19 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
       const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
       if (split == 1) {
         with_type(O, [&](auto* out) {
-          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, 0, O.wide != 0}.put(
+          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, O.ldg, O.wide != 0}.put(
               P, j, col, j.lane0 + quarter * 32, from, from + NT / (kOut / 4), sm.scratch[warp - 2]);
         });
       } else {
         const uint32_t share = NT / split;
-        for (uint32_t k0 = 0; k0 < j.cols; k0 += 16) {
+        // every writing warp leaves its columns, and writes its share of the CTA's
+        for (uint32_t k0 = from; k0 < min(j.cols, from + NT / (kOut / 4)); k0 += 16) {
           float r[16];
           tmem_ld16f(col + k0, r);
+          if (kbs == 0) {  // none of this CTA's
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = 0.0f;
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint32_t to = ((rank * share + (k0 + i) % share) * CH + quarter * 32 + lane) * 4;
@@ -466,13 +527,13 @@ __global__ void __launch_bounds__(64 + 32 * out_warps(NT), 1)
           *abort = 1;
           break;
         }
-        const uint32_t j0 = rank * share;
+        const uint32_t own = share / (kOut / 4), i0 = (warp - 2) / 4 * own, j0 = rank * share + i0;
         with_type(O, [&](auto* out) {
           using T = std::remove_pointer_t<decltype(out)>;
-          T* c = out + (uint64_t)(j.col0 + j0) * O.ld + at;
-          for (uint32_t i = 0; i < share && j0 + i < j.cols; ++i, c += O.ld) {
+          T* c = out + (MODE == kGradW ? (uint64_t)j.group * O.ldg : 0) + (uint64_t)(j.col0 + j0) * O.ld + at;
+          for (uint32_t i = 0; i < own && j0 + i < j.cols; ++i, c += O.ld) {
             float acc = 0.0f;
-            for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + i) * CH + quarter * 32 + lane];
+            for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + i0 + i) * CH + quarter * 32 + lane];
             if (at < P.lanes) *c = from_f32<T>(acc);
           }
         });
@@ -534,14 +595,15 @@ struct Cut {
 // an SM and 6200 for all. Tiles run in waves, each with a start and an end that
 // nothing overlaps when it is the only one. It ranks cuts; see the 8-bit products
 // for how far it is from a time.
-double cycles_of(int mode, const ProductArgs& P, const Cut& c, int sms) {
+double cycles_of(int mode, const ProductArgs& P, const Cut& c, uint32_t depth, int sms) {
   const bool pair = c.lanes == 256;
   const double tiles = (double)product_tiles(mode, P, c.cols, c.lanes) * c.split, at_once = pair ? sms / 2 : sms;
   const double active = tiles < at_once ? tiles : at_once, ctas = pair ? 2 * active : active;
-  const double blocks = (double)((P.depth + kStepK - 1) / kStepK) / c.split;
+  const double blocks = (double)((depth + kStepK - 1) / kStepK) / c.split;
   const double rate = 6200.0 / ctas < 64.0 ? 6200.0 / ctas : 64.0;
   const double load = (pair ? 256 : c.lanes + c.cols) * 128.0 / rate;
-  const double cols = P.m < c.cols ? (double)((P.m + 15) / 16 * 16) : c.cols;
+  const uint32_t have = mode == kGradW ? P.cols : P.m;
+  const double cols = have < c.cols ? (double)((have + 15) / 16 * 16) : c.cols;
   const double mma = 4 * (cols / 4 + 32 > cols / 2 ? cols / 4 + 32 : cols / 2);
   const double waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
   return waves * (blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
@@ -566,19 +628,22 @@ int launch_tile(const DeviceSlot& D, const Operands& o, const ProductArgs& P, Ti
   using Smem = TileSmem<NT, CH, KB, STAGES>;
   CUtensorMap ma, mb;
   O.folded = MODE == kForward && KB > 1 && o.a_cols % kStepK == 0 && o.rows % 8 == 0 && o.lda < (1ull << 35);
+  const uint64_t mats = MODE == kGradW ? 1 : P.groups;
   if (O.folded)
     MAPAL_TRY(folded_map(&ma, P, o, CH, KB));
   else
-    MAPAL_TRY(product_map(&ma, o.a, o.rows, o.a_cols, o.lda, P.groups, o.ldga, 3, MODE == kForward ? CH : KB * kStepK));
-  MAPAL_TRY(product_map(&mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, NT));
-  constexpr size_t most = sizeof(Smem) + 1024 + (NT <= 64 ? NT * CH * 4 : 0);
-  static_assert(most <= 227 * 1024, "shared memory of a CTA");
+    MAPAL_TRY(product_map(&ma, o.a, o.rows, o.a_cols, o.lda, mats, o.ldga, MODE == kGradW ? 2 : 3,
+                          MODE == kForward ? CH : KB * kStepK));
+  MAPAL_TRY(product_map(&mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, MODE == kGradW ? KB * kStepK : NT));
+  constexpr size_t parts = NT * CH * 4, room = 227 * 1024;
+  constexpr size_t most = sizeof(Smem) + 1024 + (sizeof(Smem) + 1024 + parts <= room ? parts : 0);
+  static_assert(most <= room, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
   auto kernel = product_tile_kernel<MODE, NT, CH, KB, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "product shared memory"));
   const uint64_t tiles = product_tiles(MODE, P, NT, CH), cap = O.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
-  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * O.split), 64 + 32 * out_warps(NT),
-                     sizeof(Smem) + 1024 + (O.split > 1 ? NT * CH * 4 : 0), D.stream, O.split, ma, mb, P, O);
+  return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * O.split), tile_threads(MODE, NT),
+                     sizeof(Smem) + 1024 + (O.split > 1 ? parts : 0), D.stream, O.split, ma, mb, P, O);
 }
 
 template <int MODE, typename T>
@@ -591,29 +656,35 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
     if (tb) return launch_product_pair<MODE, true, false>(D, o, P, out);
     return launch_product_pair<MODE, true, true>(D, o, P, out);
   }
-  if constexpr (MODE != kGradW) {
-    static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
-                                    {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
-    const uint32_t blocks = (P.depth + kStepK - 1) / kStepK;
-    Cut best{};
-    double least = 0;
-    for (Cut c : kCuts) {
-      if (MODE == kGradX && c.lanes == 32) continue;  // an MN-major line is 64 lanes
-      for (c.split = 1; c.split <= 8; c.split *= 2) {
-        if (c.split > 1 && (c.cols > 64 || c.split * 4 > blocks ||
-                            product_tiles(MODE, P, c.cols, c.lanes) * c.split > (uint64_t)D.prof.sm_count))
-          break;
-        const double cy = cycles_of(MODE, P, c, D.prof.sm_count);
-        if (best.lanes == 0 || cy < least) {
-          best = c;
-          least = cy;
-        }
+  static constexpr Cut kCuts[] = {{256, 256, 1}, {128, 128, 1}, {64, 128, 1}, {128, 64, 1}, {64, 64, 1},
+                                  {128, 32, 1},  {64, 32, 1},   {128, 16, 1}, {64, 16, 1},  {32, 16, 1}};
+  // grad w: the groups' rows are on the device; the mean stands for each
+  const uint32_t depth = MODE == kGradW ? (P.m + P.groups - 1) / P.groups : P.depth, blocks = (depth + kStepK - 1) / kStepK;
+  Cut best{};
+  double least = 0;
+  for (Cut c : kCuts) {
+    if (MODE == kGradX && c.lanes == 32) continue;                        // an MN-major line is 64 lanes,
+    if (MODE == kGradW && (c.cols < 128 || c.lanes < 128)) continue;      // or columns
+    for (c.split = 1; c.split <= 8; c.split *= 2) {
+      if (c.split > 1 && (c.lanes == 256 || (c.cols == 128 && c.lanes == 64) || c.split * 4 > blocks ||
+                          product_tiles(MODE, P, c.cols, c.lanes) * c.split > (uint64_t)D.prof.sm_count))
+        break;
+      const double cy = cycles_of(MODE, P, c, depth, D.prof.sm_count);
+      if (best.lanes == 0 || cy < least) {
+        best = c;
+        least = cy;
       }
     }
-    const TileArgs O{out.out, out.ld, otype, best.split, out.wide, 0};
+  }
+  const TileArgs O{out.out, out.ld, out.ldg, otype, best.split, out.wide, 0};
+  switch (best.lanes * 1000 + best.cols) {
+    case 256256: return launch_product_pair<MODE, false, false>(D, o, P, out);
+    case 128128:
+      if (best.split > 1) return launch_tile<MODE, 128, 128, 2, 2>(D, o, P, O);
+      return launch_tile<MODE, 128, 128, 2, 3>(D, o, P, O);
+  }
+  if constexpr (MODE != kGradW) {
     switch (best.lanes * 1000 + best.cols) {
-      case 256256: break;
-      case 128128: return launch_tile<MODE, 128, 128, 2, 3>(D, o, P, O);
       case 64128: return launch_tile<MODE, 128, 64, 2, 4>(D, o, P, O);
       case 128064: return launch_tile<MODE, 64, 128, 2, 3>(D, o, P, O);
       case 64064: return launch_tile<MODE, 64, 64, 2, 6>(D, o, P, O);
@@ -621,11 +692,10 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
       case 64032: return launch_tile<MODE, 32, 64, 4, 4>(D, o, P, O);
       case 128016: return launch_tile<MODE, 16, 128, 2, 5>(D, o, P, O);
       case 64016: return launch_tile<MODE, 16, 64, 4, 4>(D, o, P, O);
-      default:
-        if constexpr (MODE == kForward) return launch_tile<MODE, 16, 32, 4, 7>(D, o, P, O);
     }
+    if constexpr (MODE == kForward) return launch_tile<MODE, 16, 32, 4, 7>(D, o, P, O);
   }
-  return launch_product_pair<MODE, false, false>(D, o, P, out);
+  return set_error(MAPAL_ERR_UNSUPPORTED, "no tile for this product");
 }
 
 int check_site(const MapalProductSite* s) {

@@ -412,12 +412,11 @@ struct PairSmem {
   uint32_t tmem_base;
   int abort;
 };
-// Copied operands: stages of one block, and raw blocks of 2 (both copied) or 3 (one).
 template <bool CA, bool CB>
 struct PairCut {
   static constexpr bool kCopy = CA || CB;
-  static constexpr int kStages = kCopy ? 4 : 3, kKB = kCopy ? 1 : 2;
-  static constexpr int kRaw = CA && CB ? 2 : kCopy ? 3 : 0;  // raw blocks
+  static constexpr int kStages = kCopy && !(CA && CB) ? 4 : 3, kKB = kCopy ? 1 : 2;
+  static constexpr int kRaw = CA && CB ? 3 : kCopy ? 4 : 0;  // raw blocks
   using Smem = PairSmem<kStages, kKB, kRaw * (CA + CB)>;
   static constexpr size_t kSmem = sizeof(Smem) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
