@@ -314,7 +314,6 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
   constexpr bool MN = MODE != kForward, MB = MODE == kGradW;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float* partial = reinterpret_cast<float*>(&sm + 1);  // split > 1: NT x CH partial sums
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t split = O.split, rank = split > 1 ? blockIdx.x % split : 0;
   const uint64_t first = blockIdx.x / split, step = gridDim.x / split;
@@ -332,12 +331,13 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
       mbar_init(&sm.acc_full[b], 1);
       mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
     }
-    mbar_init(&sm.parts, split * CH * (kOut / 4));
+    mbar_init(&sm.parts, 1);
     mbar_init(&sm.drained, 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  if (split > 1 && warp == 0 && elect_one()) mbar_expect_tx(&sm.parts, NT * CH * 4);  // all CTAs' shares
   grid_wait();
   grid_go();
   JobWalk<MODE, NT, CH> walk(P, first, step);
@@ -400,10 +400,7 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  if (split > 1)
-    cg::this_cluster().sync();  // the others' barriers are there before any arrival
-  else
-    __syncthreads();
+  __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
 
@@ -492,55 +489,72 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
     uint32_t n = 0;
     for (; more; more = walk.next(j), ++n) {
       cut();
-      const uint32_t b = n & 1, at = j.lane0 + quarter * 32 + lane;
+      const uint32_t b = n & 1;
       const uint32_t from = (warp - 2) / 4 * (NT / (kOut / 4));
       if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {  // *abort: its commit was an aborted tile's
         *abort = 1;
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t col = tmem + ((uint32_t)(quarter * 32) << 16) + b * NT;
-      if (split == 1) {
-        with_type(O, [&](auto* out) {
-          StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, O.ldg, O.wide != 0}.put(
-              P, j, col, j.lane0 + quarter * 32, from, from + NT / (kOut / 4), sm.scratch[warp - 2]);
-        });
-      } else {
-        const uint32_t share = NT / split;
-        // every writing warp leaves its columns, and writes its share of the CTA's
-        for (uint32_t k0 = from; k0 < min(j.cols, from + NT / (kOut / 4)); k0 += 16) {
-          float r[16];
-          tmem_ld16f(col + k0, r);
-          if (kbs == 0) {  // none of this CTA's
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t to = ((rank * share + (k0 + i) % share) * CH + quarter * 32 + lane) * 4;
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(sa(partial) + to, (k0 + i) / share)), "f"(r[i])
-                         : "memory");
-          }
-        }
-        for (uint32_t q = 0; q < split; ++q) arrive_remote(remote(sa(&sm.parts), q));
-        if (any_of(!mbar_wait_cluster(&sm.parts, 0, abort))) {
-          *abort = 1;
-          break;
-        }
-        const uint32_t own = share / (kOut / 4), i0 = (warp - 2) / 4 * own, j0 = rank * share + i0;
-        with_type(O, [&](auto* out) {
-          using T = std::remove_pointer_t<decltype(out)>;
-          T* c = out + (MODE == kGradW ? (uint64_t)j.group * O.ldg : 0) + (uint64_t)(j.col0 + j0) * O.ld + at;
-          for (uint32_t i = 0; i < own && j0 + i < j.cols; ++i, c += O.ld) {
-            float acc = 0.0f;
-            for (uint32_t q = 0; q < split; ++q) acc += partial[(q * share + i0 + i) * CH + quarter * 32 + lane];
-            if (at < P.lanes) *c = from_f32<T>(acc);
-          }
-        });
-      }
+      if (split > 1) break;  // a cluster's one tile is joined below
+      with_type(O, [&](auto* out) {
+        StoreTile<MODE, std::remove_pointer_t<decltype(out)>>{out, O.ld, O.ldg, O.wide != 0}.put(
+            P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + quarter * 32, from, from + NT / (kOut / 4),
+            sm.scratch[warp - 2]);
+      });
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+
+  if (split > 1) {
+    // ---- the cluster's tile: its parts of t joined ----
+    // Every CTA's products are done, so its stages are free: the partial sums go there, [column][lane], and on to the
+    // CTAs that write them as one bulk copy each. (Stores to other CTAs lane by lane took 8 us for 128 x 128.)
+    __syncwarp();
+    cg::this_cluster().sync();
+    if (more && warp >= 2 && warp < 2 + kOut && (warp & 3) < CH / 32 && !any_of(*abort)) {
+      constexpr int kPart = NT * CH * 4;
+      static_assert(2 * kPart <= (int)sizeof(sm.stage), "own and received sums");
+      const uint32_t quarter = warp & 3, share = NT / split, half = (warp - 2) / 4;
+      float* mine = reinterpret_cast<float*>(sm.stage[0]) + quarter * 32 + lane;
+      const float* received = mine + NT * CH;
+      for (uint32_t k0 = half * (NT / (kOut / 4)); k0 < (half + 1) * (NT / (kOut / 4)); k0 += 16) {
+        float f[16];
+        tmem_ld16f(tmem + ((quarter * 32) << 16) + k0, f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mine[(k0 + i) * CH] = kbs ? f[i] : 0.0f;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(kOut / 4 * CH) : "memory");  // the writing warps
+      if (warp == (CH == 128 ? 2 : 4) && elect_one())                  // the first of them
+        for (uint32_t q = 0; q < split; ++q)
+          asm volatile(
+              "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                  remote(sa(sm.stage[0]) + kPart + rank * share * CH * 4, q)),
+              "r"(sa(sm.stage[0]) + q * share * CH * 4), "r"(share * CH * 4), "r"(remote(sa(&sm.parts), q))
+              : "memory");
+      if (any_of(!mbar_wait_cluster(&sm.parts, 0, abort))) {
+        *abort = 1;
+      } else {
+        const uint32_t own = share / (kOut / 4), i0 = half * own, j0 = rank * share + i0, at = j.lane0 + quarter * 32 + lane;
+        with_type(O, [&](auto* out) {
+          using T = std::remove_pointer_t<decltype(out)>;
+          T* c = out + (MODE == kGradW ? (uint64_t)j.group * O.ldg : 0) + (uint64_t)(j.col0 + j0) * O.ld + at;
+          constexpr uint32_t kTurn = NT / 8 / (kOut / 4) < 8 ? NT / 8 / (kOut / 4) : 8;  // columns at once; split is at most 8
+          for (uint32_t i = 0; i < own && j0 + i < j.cols; i += kTurn, c += kTurn * O.ld) {
+            float acc[kTurn] = {};
+#pragma unroll 2
+            for (uint32_t q = 0; q < split; ++q)
+#pragma unroll
+              for (uint32_t u = 0; u < kTurn; ++u) acc[u] += received[(q * share + i0 + i + u) * CH];
+#pragma unroll
+            for (uint32_t u = 0; u < kTurn; ++u)
+              if (at < P.lanes && j0 + i + u < j.cols) c[u * O.ld] = from_f32<T>(acc[u]);
+          }
+        });
+      }
     }
   }
 
@@ -635,15 +649,14 @@ int launch_tile(const DeviceSlot& D, const Operands& o, const ProductArgs& P, Ti
     MAPAL_TRY(product_map(&ma, o.a, o.rows, o.a_cols, o.lda, mats, o.ldga, MODE == kGradW ? 2 : 3,
                           MODE == kForward ? CH : KB * kStepK));
   MAPAL_TRY(product_map(&mb, o.b, P.m, o.b_cols, o.ldb, 1, 0, 2, MODE == kGradW ? KB * kStepK : NT));
-  constexpr size_t parts = NT * CH * 4, room = 227 * 1024;
-  constexpr size_t most = sizeof(Smem) + 1024 + (sizeof(Smem) + 1024 + parts <= room ? parts : 0);
-  static_assert(most <= room, "shared memory of a CTA");
+  constexpr size_t most = sizeof(Smem) + 1024;
+  static_assert(most <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> done{0};
   auto kernel = product_tile_kernel<MODE, NT, CH, KB, STAGES>;
   MAPAL_TRY(ensure_smem_attr(done, (const void*)kernel, D.device, most, "product shared memory"));
   const uint64_t tiles = product_tiles(MODE, P, NT, CH), cap = O.split > 1 ? tiles : (uint64_t)D.prof.sm_count;
   return launch_rows(kernel, (unsigned)((tiles < cap ? tiles : cap) * O.split), tile_threads(MODE, NT),
-                     sizeof(Smem) + 1024 + (O.split > 1 ? parts : 0), D.stream, O.split, ma, mb, P, O);
+                     most, D.stream, O.split, ma, mb, P, O);
 }
 
 template <int MODE, typename T>
@@ -680,7 +693,6 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
   switch (best.lanes * 1000 + best.cols) {
     case 256256: return launch_product_pair<MODE, false, false>(D, o, P, out);
     case 128128:
-      if (best.split > 1) return launch_tile<MODE, 128, 128, 2, 2>(D, o, P, O);
       return launch_tile<MODE, 128, 128, 2, 3>(D, o, P, O);
   }
   if constexpr (MODE != kGradW) {
