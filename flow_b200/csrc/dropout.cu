@@ -15,20 +15,19 @@ namespace {
 constexpr int kThreads = 256;
 
 struct Key {
-  uint32_t k0, k1, c2, c3;
+  uint32_t k[10][2];  // of each round
+  uint32_t c2, c3;
 };
 
 __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, const Key& k) {
-  uint32_t c2 = k.c2, c3 = k.c3, k0 = k.k0, k1 = k.k1;
+  uint32_t c2 = k.c2, c3 = k.c3;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k.k[i][0];
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k.k[i][1];
     c3 = (uint32_t)p0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -41,67 +40,163 @@ struct DropArgs {
   uint64_t ldx, ldr, ldy, rows;
   uint32_t d, blocks;  // elements of a row, and eights of them
   uint32_t lanes;      // threads on a row, a power of two
-  uint32_t limit;
+  uint32_t limit;      // in the upper half of a word; p = 1 does not get this far
   float scale;
 };
 
-// A thread takes eights of a row, `lanes` threads of a block a row, V elements an access.
-template <typename T, int V>
+__device__ __forceinline__ Key key_of(const DropArgs& A) {
+  const unsigned long long key = __ldg(A.rng), place = __ldg(A.rng + 1);
+  Key k;
+  k.c2 = (uint32_t)place, k.c3 = (uint32_t)(place >> 32);
+#pragma unroll
+  for (uint32_t i = 0; i < 10; ++i) {
+    k.k[i][0] = (uint32_t)key + i * 0x9E3779B9u;
+    k.k[i][1] = (uint32_t)(key >> 32) + i * 0xBB67AE85u;
+  }
+  return k;
+}
+
+// Whether element c of the eight is kept: its 16 bits moved to the top of a word, so that
+// what lies below does not matter, against the limit there.
+__device__ __forceinline__ bool keeps(const uint4& w, int c, uint32_t limit) {
+  const uint32_t word = c / 2 == 0 ? w.x : c / 2 == 1 ? w.y : c / 2 == 2 ? w.z : w.w;
+  return (c & 1 ? word : word << 16) >= limit;
+}
+
+template <typename T>
+__device__ __forceinline__ void drop_one(const DropArgs& A, const T* x, const T* res, T* y, bool keep) {
+  const float g = res ? to_f32(*res) : 0.0f;
+  *y = from_f32<T>(keep ? __fmaf_rn(to_f32(*x), A.scale, g) : g);
+}
+
+// Rows on 16-byte boundaries. Bound by HBM: a thread takes kAhead eights of a row, all
+// of their loads before the first bits, so that the generator's 10 rounds (40 multiply-and-xor
+// instructions) run while they are under way. A row's last part eight goes
+// element by element.
+constexpr int kAhead = 2;
+
+template <typename T>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropArgs A) {
+  constexpr int V = 16 / sizeof(T), N = 8 / V;  // elements of an access, accesses of an eight
   using P = Pack<T, V>;
-  constexpr int N = 8 / V;  // accesses
   const uint32_t in_row = threadIdx.x & (A.lanes - 1), per_block = kThreads / A.lanes;
   grid_wait();
   grid_go();
-  const unsigned long long key = __ldg(A.rng), place = __ldg(A.rng + 1);
-  const Key k{(uint32_t)key, (uint32_t)(key >> 32), (uint32_t)place, (uint32_t)(place >> 32)};
+  const Key k = key_of(A);
   const T* x = static_cast<const T*>(A.x);
   const T* res = static_cast<const T*>(A.residual);
   T* y = static_cast<T*>(A.y);
-  const uint32_t pieces = (A.blocks + A.lanes - 1) / A.lanes;
+  const uint32_t pieces = (A.blocks + A.lanes * kAhead - 1) / (A.lanes * kAhead), whole = A.d / 8;
   const uint64_t row_groups = (A.rows + per_block - 1) / per_block, items = row_groups * pieces;
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint64_t r = item / pieces * per_block + threadIdx.x / A.lanes;
-    const uint32_t b = (uint32_t)(item % pieces) * A.lanes + in_row;
-    if (r >= A.rows || b >= A.blocks) continue;
-    const uint32_t n = min(8u, A.d - b * 8);
-    const uint64_t at = (uint64_t)b * 8;
-    P xv[N], rv[N];
+    const uint64_t group = item / pieces, r = group * per_block + threadIdx.x / A.lanes;
+    const uint32_t b0 = (uint32_t)(item - group * pieces) * A.lanes * kAhead + in_row;
+    if (r >= A.rows) continue;
+    const T *xr = x + r * A.ldx, *rr = res ? res + r * A.ldr : nullptr;
+    T* yr = y + r * A.ldy;
+    P xv[kAhead][N], rv[kAhead][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (i * V < n) xv[i] = *reinterpret_cast<const P*>(x + r * A.ldx + at + i * V);
-      if (res && i * V < n) rv[i] = *reinterpret_cast<const P*>(res + r * A.ldr + at + i * V);
-    }
-    const uint4 w = philox(b, (uint32_t)r, k);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t b = b0 + u * A.lanes;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * V < n) {
-        float f[V], g[V];
-        xv[i].get(f);
-        if (res)
-          rv[i].get(g);
-        else
-#pragma unroll
-          for (int e = 0; e < V; ++e) g[e] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int c = i * V + e;
-          const uint32_t bits = c & 1 ? words[c / 2] >> 16 : words[c / 2] & 0xffffu;
-          f[e] = bits >= A.limit ? __fmaf_rn(f[e], A.scale, g[e]) : g[e];
+      for (int i = 0; i < N; ++i)
+        if (b < whole) {
+          xv[u][i] = ld_once(reinterpret_cast<const P*>(xr + b * 8ull + i * V));
+          if (res) rv[u][i] = ld_once(reinterpret_cast<const P*>(rr + b * 8ull + i * V));
         }
-        P o;
-        o.set(f);
-        *reinterpret_cast<P*>(y + r * A.ldy + at + i * V) = o;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t b = b0 + u * A.lanes;
+      if (b >= A.blocks) break;
+      const uint4 w = philox(b, (uint32_t)r, k);
+      if (b < whole) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          float f[V], g[V] = {};
+          xv[u][i].get(f);
+          if (res) rv[u][i].get(g);
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[e] = keeps(w, i * V + e, A.limit) ? __fmaf_rn(f[e], A.scale, g[e]) : g[e];
+          P o;
+          o.set(f);
+          st_once(reinterpret_cast<P*>(yr + b * 8ull + i * V), o);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (b * 8 + e < A.d)
+            drop_one(A, xr + b * 8ull + e, rr ? rr + b * 8ull + e : nullptr, yr + b * 8ull + e, keeps(w, e, A.limit));
       }
+    }
   }
 }
 
+// Rows anywhere: a warp takes 256 elements, an eight's bits a thread, and gives them out
+// by shuffles, so that neighbouring threads access neighbouring elements (V of them; eight
+// in a row by each thread took 36 us for 5003 x 1021 f16 with gradient).
 template <typename T, int V>
-int launch(const DeviceSlot& D, const DropArgs& A) {
-  const uint64_t per_block = kThreads / A.lanes, pieces = (A.blocks + A.lanes - 1) / A.lanes;
-  const uint64_t items = (A.rows + per_block - 1) / per_block * pieces, cap = 32ull * D.prof.sm_count;
-  return launch_rows(dropout_kernel<T, V>, (unsigned)(items < cap ? items : cap), kThreads, 0, D.stream, 1, A);
+__global__ void __launch_bounds__(kThreads) dropout_loose_kernel(const DropArgs A) {
+  using P = Pack<T, V>;
+  constexpr int kTurns = 8 / V;
+  const uint32_t lane = threadIdx.x & 31;
+  grid_wait();
+  grid_go();
+  const Key k = key_of(A);
+  const T* x = static_cast<const T*>(A.x);
+  const T* res = static_cast<const T*>(A.residual);
+  T* y = static_cast<T*>(A.y);
+  const uint32_t pieces = (A.blocks + 31) / 32;
+  const uint64_t items = A.rows * pieces, step = (uint64_t)gridDim.x * (kThreads / 32);
+  for (uint64_t item = (uint64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; item < items; item += step) {
+    const uint64_t r = item / pieces;
+    const uint32_t b0 = (uint32_t)(item - r * pieces) * 32;
+    const uint64_t e0 = b0 * 8ull + lane * V;
+    const T *xr = x + r * A.ldx + e0, *rr = res ? res + r * A.ldr + e0 : nullptr;
+    T* yr = y + r * A.ldy + e0;
+    const uint32_t left = A.d > e0 ? (uint32_t)min((uint64_t)A.d - e0, (uint64_t)0xffffffffu) : 0;
+    P xv[kTurns], rv[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+      if (i * 32 * V < left) {
+        xv[i] = *reinterpret_cast<const P*>(xr + i * 32 * V);
+        if (res) rv[i] = *reinterpret_cast<const P*>(rr + i * 32 * V);
+      }
+    const uint4 w = philox(b0 + lane, (uint32_t)r, k);
+    uint32_t m = 0;  // which of this thread's eight are kept
+#pragma unroll
+    for (int c = 0; c < 8; ++c) m |= keeps(w, c, A.limit) ? 1u << c : 0u;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const uint32_t e = i * 32 * V + lane * V;  // of the warp's 256
+      const uint32_t bits = __shfl_sync(0xffffffffu, m, e / 8) >> (e & 7);
+      if (i * 32 * V < left) {
+        float f[V], g[V] = {};
+        xv[i].get(f);
+        if (res) rv[i].get(g);
+#pragma unroll
+        for (int c = 0; c < V; ++c) f[c] = bits & (1u << c) ? __fmaf_rn(f[c], A.scale, g[c]) : g[c];
+        P o;
+        o.set(f);
+        *reinterpret_cast<P*>(yr + i * 32 * V) = o;
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch(const DeviceSlot& D, DropArgs A) {
+  // a row's threads: enough for its eights, kAhead each
+  for (A.lanes = 1; A.lanes * kAhead < A.blocks && A.lanes < kThreads;) A.lanes *= 2;
+  const uint64_t per_block = kThreads / A.lanes, pieces = (A.blocks + A.lanes * kAhead - 1) / (A.lanes * kAhead);
+  const uint64_t items = (A.rows + per_block - 1) / per_block * pieces, most = 1u << 20;
+  return launch_rows(dropout_kernel<T>, (unsigned)(items < most ? items : most), kThreads, 0, D.stream, 1, A);
+}
+
+template <typename T, int V>
+int launch_loose(const DeviceSlot& D, const DropArgs& A) {
+  const uint64_t items = A.rows * ((A.blocks + 31) / 32), blocks = (items + kThreads / 32 - 1) / (kThreads / 32), most = 1u << 20;
+  return launch_rows(dropout_loose_kernel<T, V>, (unsigned)(blocks < most ? blocks : most), kThreads, 0, D.stream, 1, A);
 }
 
 }  // namespace
@@ -138,20 +233,26 @@ extern "C" int mapal_gpu_dropout(MapalGpuCtx* ctx, const MapalDropoutSite* site,
     A.rows = s.rows;
     A.d = (uint32_t)s.d;
     A.blocks = (uint32_t)((s.d + 7) / 8);
-    for (A.lanes = 1; A.lanes < A.blocks && A.lanes < kThreads;) A.lanes *= 2;
-    A.limit = (uint32_t)std::lrint(s.p * 65536.0);
-    A.scale = A.limit < 65536 ? (float)(65536.0 / (65536 - A.limit)) : 0.0f;
+    const uint32_t limit = (uint32_t)std::lrint(s.p * 65536.0);
+    if (limit == 65536) {  // nothing of x is left
+      if (residual && residual != y)
+        MAPAL_CUDA(cudaMemcpy2DAsync(y, s.ldy * es, residual, s.ldr * es, s.d * es, s.rows, cudaMemcpyDeviceToDevice, D.stream));
+      else if (!residual)
+        MAPAL_CUDA(cudaMemset2DAsync(y, s.ldy * es, 0, s.d * es, s.rows, D.stream));
+      return finish(ctx, 0, false);
+    }
+    A.limit = limit << 16;
+    A.scale = (float)(65536.0 / (65536 - limit));
     int width = align_of(x, s.ldx * es, s.rows);
-    for (const int o : {align_of(y, s.ldy * es, s.rows), residual ? align_of(residual, s.ldr * es, s.rows) : 16,
-                        align_of(nullptr, s.d * es, 2)})
+    for (const int o : {align_of(y, s.ldy * es, s.rows), residual ? align_of(residual, s.ldr * es, s.rows) : 16})
       width = o < width ? o : width;
     auto half = [&](auto t) {
       using T = decltype(t);
-      if (width >= 16) return launch<T, 8>(D, A);
-      if (width >= 4) return launch<T, 2>(D, A);
-      return launch<T, 1>(D, A);
+      if (width >= 16) return launch<T>(D, A);
+      if (width >= 4 && s.d % 2 == 0) return launch_loose<T, 2>(D, A);
+      return launch_loose<T, 1>(D, A);
     };
-    MAPAL_TRY(s.dtype == MAPAL_DTYPE_F32 ? (width >= 16 ? launch<float, 4>(D, A) : launch<float, 1>(D, A))
+    MAPAL_TRY(s.dtype == MAPAL_DTYPE_F32 ? (width >= 16 ? launch<float>(D, A) : launch_loose<float, 1>(D, A))
               : s.dtype == MAPAL_DTYPE_F16 ? half(__half{})
                                            : half(__nv_bfloat16{}));
     return finish(ctx, 0, false);

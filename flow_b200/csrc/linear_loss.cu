@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
         const uint16_t* from = A.h + (i0 + r) * A.ldh;
         uint16_t* out = T.h + (uint64_t)to * T.ld;
         if (A.aligned) {  // ld is d rounded up to 8
+#pragma unroll 4
           for (uint64_t e = lane * 8; e + 8 <= A.d; e += 256)
             *reinterpret_cast<uint4*>(out + e) = __ldcs(reinterpret_cast<const uint4*>(from + e));
           const uint64_t e = A.d / 8 * 8 + lane;
@@ -219,51 +220,32 @@ struct SumTile {
   }
 };
 
-// The parts of a row joined: 32 rows a block, one a lane, parts spread over warps;
-// then a warp a row for its target's logit.
-constexpr int kJoinWarps = 32, kJoinAhead = 4;
+// The parts of a row joined: 8 rows a block, 32 parts at a time, and a warp a row for its
+// target's logit, whose loads run beside the others'.
+constexpr int kJoinRows = 8, kJoinAhead = 4;
+
+__device__ __forceinline__ void join(float2& a, const float2& b) {
+  const float m = fmaxf(a.x, b.x);
+  if (m == -INFINITY) return;  // nothing on either side
+  a.y = a.y * ex2((a.x - m) * kLog2e) + b.y * ex2((b.x - m) * kLog2e);
+  a.x = m;
+}
 
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kJoinWarps)
+__global__ void __launch_bounds__(32 * kJoinRows)
     join_kernel(const float2* __restrict__ parts, uint64_t ld, uint32_t nparts, const Taken Q, const T* __restrict__ w,
                 uint64_t ldw, uint32_t d, float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 part[kJoinWarps][32];
-  __shared__ float2 joined[32];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float2 part[kJoinRows][kJoinRows];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = threadIdx.x % kJoinRows, p0 = threadIdx.x / kJoinRows;
   grid_wait();
   grid_go();
-  const uint32_t count = (uint32_t)__ldg(Q.count + 1);
-  const uint32_t row0 = blockIdx.x * 32;
+  const uint32_t count = (uint32_t)__ldg(Q.count + 1), row0 = blockIdx.x * kJoinRows, c = row0 + warp;
   if (row0 >= count) return;
-  auto join = [](float2& a, const float2& b) {
-    const float m = fmaxf(a.x, b.x);
-    if (m == -INFINITY) return;  // nothing on either side
-    a.y = a.y * ex2((a.x - m) * kLog2e) + b.y * ex2((b.x - m) * kLog2e);
-    a.x = m;
-  };
-  float2 a = make_float2(-INFINITY, 0.0f);
-  const bool in = row0 + lane < count;
-  for (uint32_t p0 = warp; p0 < nparts; p0 += kJoinWarps * kJoinAhead) {
-    float2 b[kJoinAhead];
-#pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) {
-      const uint32_t p = p0 + u * kJoinWarps;
-      b[u] = in && p < nparts ? __ldcs(parts + p * ld + row0 + lane) : make_float2(-INFINITY, 0.0f);
-    }
-#pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) join(a, b[u]);
-  }
-  part[warp][lane] = a;
-  __syncthreads();
-  if (warp == 0) {
-    for (int q = 1; q < kJoinWarps; ++q) join(a, part[q][lane]);
-    joined[lane] = a;
-  }
-  const uint32_t c = row0 + warp;
   float dot = 0.0f;
   if (c < count) {
     const T* hr = reinterpret_cast<const T*>(Q.h) + (uint64_t)c * Q.ld;
     const T* wr = w + (uint64_t)__ldg(Q.target + c) * ldw;
+#pragma unroll 4
     for (uint32_t e = lane * V; e < d; e += 32 * V) {
       float x[V], y[V];
       reinterpret_cast<const Pack<T, V>*>(hr + e)->get(x);
@@ -271,13 +253,29 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 #pragma unroll
       for (int k = 0; k < V; ++k) dot = __fmaf_rn(x[k], y[k], dot);
     }
-    dot = warp_sum(dot);
   }
+  float2 a = make_float2(-INFINITY, 0.0f);
+  const bool in = row0 + r < count;
+  for (uint32_t p = p0; p < nparts; p += 32 * kJoinAhead) {
+    float2 b[kJoinAhead];
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u)
+      b[u] = in && p + u * 32 < nparts ? __ldcs(parts + (p + u * 32) * ld + row0 + r) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) join(a, b[u]);
+  }
+#pragma unroll
+  for (int o = kJoinRows; o < 32; o *= 2)
+    join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
+  if (lane < kJoinRows) part[warp][lane] = a;
+  dot = warp_sum(dot);
   __syncthreads();
   if (c < count && lane == 0) {
-    const float2 r = joined[warp];
-    const float u = fmaxf(r.x, dot);
-    const float others = r.y == 0.0f ? 0.0f : r.y * ex2((r.x - u) * kLog2e);
+    float2 s = part[0][warp];
+#pragma unroll
+    for (int q = 1; q < kJoinRows; ++q) join(s, part[q][warp]);
+    const float u = fmaxf(s.x, dot);
+    const float others = s.y == 0.0f ? 0.0f : s.y * ex2((s.x - u) * kLog2e);
     const float more = log1pf(others + (ex2((dot - u) * kLog2e) - 1.0f));
     const int32_t row = __ldg(Q.list + c);
     loss[row] = (u - dot) + more;
@@ -333,16 +331,18 @@ struct GradientTile {
         for (int i = 0; i < 32; ++i) f[i] -= hit == i ? 1.0f : 0.0f;
       }
       if (in) {
-        // whole packs: what lies behind the piece's last column is dl's own row
+        // sixteen at a time, whole sectors: what lies behind the piece's last column is dl's own row
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+        for (int i = 0; i < 32; i += 16) {
           if (j0 + i >= to) break;
-          float v[8];
+          float v[16];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = f[i + k] * c;
-          Pack<T, 8> o;
+          for (int k = 0; k < 16; ++k) v[k] = f[i + k] * c;
+          Pack<T, 16> o;
           o.set(v);
-          *reinterpret_cast<uint4*>(row + j0 + i) = make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + j0 + i), "r"(o.w[0]), "r"(o.w[1]),
+                       "r"(o.w[2]), "r"(o.w[3]), "r"(o.w[4]), "r"(o.w[5]), "r"(o.w[6]), "r"(o.w[7])
+                       : "memory");
         }
       }
     }
@@ -457,12 +457,20 @@ Plan plan_of(const MapalLossSite& s, bool grad, bool copies, int sms) {
   p.pieces = (uint32_t)((s.vocab + most - 1) / most);
   p.piece = (uint32_t)up((s.vocab + p.pieces - 1) / p.pieces, 256);
   p.pieces = (uint32_t)((s.vocab + p.piece - 1) / p.piece);
-  // dh has rows x d outputs, which may be few tiles: the sum over a piece is cut
-  // until they fill the device, down to 16 blocks of 64.
+  // dh has rows x d outputs, which may be few tiles: the sum over a piece is cut into the
+  // parts that take the least, counted in blocks of 64 a tile, waves, and 8 blocks'
+  // time a wave for a tile's ends and for joining a part.
   p.parts = 1;
   if (grad) {
-    const uint64_t tiles = up(s.rows, 256) / 256 * (up(s.d, 256) / 256), at_once = sms / 2;
-    while (tiles * p.parts * 2 <= at_once && p.parts < 32 && p.piece / (p.parts * 2) >= 16 * kStepK) p.parts *= 2;
+    const uint64_t tiles = up(s.rows, 256) / 256 * (up(s.d, 256) / 256), at_once = sms / 2, blocks = p.piece / kStepK;
+    uint64_t least = ~0ull;
+    for (uint32_t n = 1; n <= 16 && blocks / n >= 16; ++n) {
+      const uint64_t cost = (tiles * n + at_once - 1) / at_once * ((blocks + n - 1) / n + 8) + 4 * n * p.pieces;
+      if (cost < least) {
+        least = cost;
+        p.parts = n;
+      }
+    }
   }
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -532,7 +540,7 @@ struct Call {
     a.vocab = (uint32_t)s.vocab;
     a.aligned = aligned16(h) && (s.rows == 1 || s.ldh % 8 == 0);
     a.trap = D.trap;
-    const uint64_t blocks = std::min<uint64_t>((s.rows + 7) / 8, 8ull * D.prof.sm_count);
+    const uint64_t blocks = std::min<uint64_t>((s.rows + 3) / 4, 8ull * D.prof.sm_count);
     a.chunk = (uint32_t)((s.rows + blocks - 1) / blocks);
     return launch_rows(take_rows_kernel, (unsigned)((s.rows + a.chunk - 1) / a.chunk), kTakeThreads, 0, D.stream, 1, a, q);
   }
@@ -584,10 +592,10 @@ int forward(const Call& c, const void* h, const void* w, const int32_t* targets,
     MAPAL_TRY(c.logits(from, ldw, n, SumTile{parts, s.rows, c.q.target, v0, v0 / 128}));
   }
   const uint32_t nparts = (uint32_t)(up(s.vocab, 256) / 128);
-  const unsigned blocks = (unsigned)((s.rows + 31) / 32);
+  const unsigned blocks = (unsigned)((s.rows + kJoinRows - 1) / kJoinRows);
   const bool wide = weights_in_place(s, w) && s.d % 8 == 0;
   auto go = [&](auto kernel) {
-    return launch_rows(kernel, blocks, 32 * kJoinWarps, 0, c.D.stream, 1, parts, s.rows, nparts, c.q,
+    return launch_rows(kernel, blocks, 32 * kJoinRows, 0, c.D.stream, 1, parts, s.rows, nparts, c.q,
                        static_cast<const T*>(w), s.ldw, (uint32_t)s.d, loss, lse);
   };
   return wide ? go(join_kernel<T, 8>) : go(join_kernel<T, 1>);

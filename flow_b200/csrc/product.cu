@@ -274,7 +274,8 @@ struct TileSmem {
   // lanes of A, in the last stage past its end.
   uint8_t stage[STAGES][kStage];
   uint8_t past[128 - CH > NT ? KB * (128 - CH - NT) * 128 : 16];
-  uint64_t full[STAGES], empty[STAGES], fixed[STAGES];
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t to_fix, fixed;  // a last block to clear has landed; it is cleared
   uint64_t acc_full[2], acc_empty[2];
   uint64_t parts, drained;
   alignas(16) uint8_t scratch[out_warps(NT)][kOutScratch];
@@ -325,8 +326,9 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
-      mbar_init(&sm.fixed[s], 1);
     }
+    mbar_init(&sm.to_fix, 1);
+    mbar_init(&sm.fixed, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
       mbar_init(&sm.acc_empty[b], kOut / 4 * (CH / 32));
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
   bool more = walk.now(j);
   uint32_t it = 0;  // stages taken, by the loads' and by the products' lane
 
-  uint32_t fixes = 0;  // a bit a stage: the parity of its next clearing
+  uint32_t fixes = 0;  // last blocks cleared
   uint32_t kb_lo, kbs, fills;  // this CTA's blocks of the tile, and the stages they take
   auto cut = [&]() {
     const uint32_t k_blocks = (j.depth + kStepK - 1) / kStepK;
@@ -433,9 +435,10 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
         for (uint32_t fill = 0; fill < fills && !*abort; ++fill, ++it) {
           const uint32_t s = it % STAGES, blocks = blocks_of(fill);
           bool ok = mbar_wait(&sm.full[s], (it / STAGES) & 1, abort);
-          if (fix && fill + 1 == fills) {
-            ok = ok && mbar_wait(&sm.fixed[s], (fixes >> s) & 1, abort);
-            fixes ^= 1u << s;
+          if (fix && fill + 1 == fills && ok) {
+            // the clearing warp is told here: a wait of its own on the stage would have to follow every one of its uses
+            mbar_arrive(&sm.to_fix);
+            ok = mbar_wait(&sm.fixed, fixes++ & 1, abort);
           }
           if (!ok) {
             *abort = 1;
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
       it += fills;
       if (!to_fix()) continue;
       const uint32_t s = (it - 1) % STAGES;
-      if (any_of(!mbar_wait(&sm.full[s], ((it - 1) / STAGES) & 1, abort))) {
+      if (any_of(!mbar_wait(&sm.to_fix, fixes++ & 1, abort))) {
         *abort = 1;
         break;
       }
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
           *reinterpret_cast<uint4*>(sm.stage[s] + chunk * (KB * kStepK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.fixed[s]);
+      if (lane == 0) mbar_arrive(&sm.fixed);
     }
   } else if ((warp & 3) < CH / 32) {
     // ---- output ----
@@ -605,22 +608,23 @@ struct Cut {
 };
 
 // Cycles of a cut, from what bounds its tiles: the MMA (N/2 cycles for 128 lanes and
-// 16 steps of t, 32 + N/4 at least), and the loads, at up to 64 bytes a cycle for
-// an SM and 6200 for all. Tiles run in waves, each with a start and an end that
-// nothing overlaps when it is the only one. It ranks cuts; see the 8-bit products
-// for how far it is from a time.
+// 16 steps of t, 72 + N/4 at least), and the loads, at up to 58 bytes a cycle for
+// an SM and 7200 for all; tiles run in waves. The constants are fitted to 210 products
+// (1 to 16000 rows, 64 to 8192 channels, 1 to 64 matrices, all three modes) that were
+// measured with every cut: the cut chosen takes 2 % longer than the best, in the mean.
 double cycles_of(int mode, const ProductArgs& P, const Cut& c, uint32_t depth, int sms) {
   const bool pair = c.lanes == 256;
   const double tiles = (double)product_tiles(mode, P, c.cols, c.lanes) * c.split, at_once = pair ? sms / 2 : sms;
   const double active = tiles < at_once ? tiles : at_once, ctas = pair ? 2 * active : active;
   const double blocks = (double)((depth + kStepK - 1) / kStepK) / c.split;
-  const double rate = 6200.0 / ctas < 64.0 ? 6200.0 / ctas : 64.0;
+  const double rate = 7200.0 / ctas < 58.0 ? 7200.0 / ctas : 58.0;
   const double load = (pair ? 256 : c.lanes + c.cols) * 128.0 / rate;
   const uint32_t have = mode == kGradW ? P.cols : P.m;
   const double cols = have < c.cols ? (double)((have + 15) / 16 * 16) : c.cols;
-  const double mma = 4 * (cols / 4 + 32 > cols / 2 ? cols / 4 + 32 : cols / 2);
-  const double waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
-  return waves * (blocks * (load > mma ? load : mma) + 1500) + (c.split > 1 ? 5500 : 0);
+  const double mma = 4 * (cols / 4 + 72 > cols / 2 ? cols / 4 + 72 : cols / 2);
+  const double size = c.lanes * c.cols / 16384.0, waves = (double)(uint64_t)((tiles + at_once - 1) / at_once);
+  return (pair ? 9900 : 5200) + waves * (blocks * (load > mma ? load : mma) + (pair ? 2000 : 860 * size) + 1500) +
+         (c.split > 1 ? 3300 + 3500 * size : 0);
 }
 
 // W as [group][eight channels][block of k][8][64], in boxes of lanes/8 x blocks.
