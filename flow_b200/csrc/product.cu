@@ -1,6 +1,5 @@
 // product.cu — products in 16-bit floats with one matrix or one per group of rows,
 // and their gradients (mapal_gpu_product*). No counterpart in the reference.
-#include <cstdlib>
 #include "product.cuh"
 
 namespace cg = cooperative_groups;
@@ -668,7 +667,7 @@ int run(const DeviceSlot& D, const Operands& o, const ProductArgs& P, const Stor
   const bool ta = tma_reads_a(MODE, P, o), tb = tma_reads_b(P, o);
   if (!ta || !tb) {
     const bool ra = raw_reads(o.rows, o.a_cols, o.lda, MODE == kGradW ? 1 : P.groups, o.ldga);
-    if (getenv("ANY") || !ra || !raw_reads(P.m, o.b_cols, o.ldb, 1, 0)) return launch_any<MODE, T, 128, 4>(D, o, P, out);
+    if (!ra || !raw_reads(P.m, o.b_cols, o.ldb, 1, 0)) return launch_any<MODE, T, 128, 4>(D, o, P, out);
     if (ta) return launch_product_pair<MODE, false, true>(D, o, P, out);
     if (tb) return launch_product_pair<MODE, true, false>(D, o, P, out);
     return launch_product_pair<MODE, true, true>(D, o, P, out);
