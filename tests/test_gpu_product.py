@@ -224,3 +224,45 @@ def test_two_streams():
         assert torch.equal(a, b)
     for c in ctxs:
         c.close()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,n,k,groups,gap", [(300, 64, 72, 3, 1), (300, 65, 131, 3, 1), (90, 33, 47, 5, 2), (700, 257, 129, 2, 3)])
+def test_matrices_apart(ctx, m, n, k, groups, gap, dtype):
+    """Rows between one matrix and the next, which are left as they were in dw."""
+    x, dy, off = whole((m, k), dtype, 1), whole((m, n), dtype, 2), ragged(m, groups, 3)
+    buf = torch.full((groups, n + gap, k), float("nan"), dtype=dtype, device="cuda")
+    w = buf[:, :n].copy_(whole((groups, n, k), dtype, 4))
+    out = torch.full((groups, n + gap, k), 77.0, dtype=dtype, device="cuda")
+    y, dx = torch.empty(m, n, dtype=dtype, device="cuda"), torch.empty(m, k, dtype=dtype, device="cuda")
+    site = fb.product_site(m, n, k, dtype, groups=groups, ldg=(n + gap) * k, lddg=(n + gap) * k)
+    ctx.product(site, x, w, y, offsets=off)
+    ctx.product_grad(site, x, w, dy, dx, out[:, :n], offsets=off)
+    wy, wdx, wdw = wants(x, w, dy, off)
+    assert torch.equal(y, wy.to(dtype)) and torch.equal(dx, wdx.to(dtype)) and torch.equal(out[:, :n], wdw.to(dtype))
+    assert (out[:, n:] == 77).all()
+
+
+@pytest.mark.parametrize("m,n,k,groups", [(4096, 128, 128, 1), (3000, 136, 264, 2), (5000, 64, 200, 1), (2049, 512, 128, 3), (1100, 250, 131, 1)])
+def test_long_sums_of_few_outputs(ctx, m, n, k, groups):
+    """The weights' gradient of many rows and few weights, whose rows are cut over several CTAs; ragged groups, so that
+    some cuts are empty and last blocks hold the next group's rows."""
+    check(ctx, m, n, k, groups, torch.bfloat16, behind=7 if groups > 1 else 0)
+    check(ctx, m, n, k, groups, torch.float16, ytype=torch.float32, dwtype=torch.float32, seed=9)
+
+
+def test_past_two_to_the_31(ctx):
+    """Operands and outputs of more than 2^31 elements: the last rows and the last matrix."""
+    t, m, k, n = torch.bfloat16, 70000, 32768, 8
+    x = torch.zeros(m, k, dtype=t, device="cuda")
+    w, dy = whole((1, n, k), t, 1), whole((m, n), t, 2)
+    x[-3:] = whole((3, k), t, 3)
+    site = fb.product_site(m, n, k, t)
+    y, dw = torch.empty(m, n, dtype=t, device="cuda"), torch.empty(1, n, k, dtype=t, device="cuda")
+    ctx.product(site, x, w, y)
+    ctx.product_grad(site, x, w, dy, None, dw)
+    want, _, wdw = wants(x[-3:], w, dy[-3:], None)
+    assert torch.equal(y[-3:], want.to(t)) and not y[:-3].any() and torch.equal(dw, wdw.to(t))
+    ctx.product_grad(site, x, w, dy, x, None)  # dx into the rows
+    _, wdx, _ = wants(torch.zeros(3, k, device="cuda"), w, dy[-3:], None)
+    assert torch.equal(x[-3:], wdx.to(t))
