@@ -177,6 +177,13 @@ __global__ void __launch_bounds__(256) copy_weights_kernel(const uint16_t* __res
 
 // ---- forward -------------------------------------------------------------------------
 
+// The tensor cores cut a sum towards zero at each step of 16 products. A logit loses
+// 2^-26 of itself a step by that, in the mean (measured over logits above 2: 4.2e-7,
+// 1.9e-6 and 3.9e-6 of them at d = 512, 2048 and 4096; f32 sums that round leave a
+// spread of that size and no mean), and lse, which is an average of them, the same. The
+// factor gives the mean back; it goes into the exponent's own.
+__device__ __forceinline__ float uncut(const ProductArgs& P) { return 1.0f + (float)((P.depth + 15) / 16) * 0x1p-26f; }
+
 // A tile of logits, rows on the lanes and 128 of the vocabulary's columns a warp:
 // each thread keeps the running maximum of its row and the sum of exponentials
 // against it, the target's column left out, and writes one pair.
@@ -192,6 +199,7 @@ struct SumTile {
     const bool in = lane < P.lanes;
     const uint32_t end = min(to, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;  // the target's column of this tile
+    const float whole = uncut(P), log2e = kLog2e * whole;
     float m = -INFINITY, s = 0.0f;
     for (uint32_t j0 = from; j0 < end; j0 += 32) {
       float f[32];
@@ -209,14 +217,14 @@ struct SumTile {
 #pragma unroll
       for (int i = 1; i < 32; ++i) top = fmaxf(top, f[i]);
       const float next = fmaxf(m, top);
-      const float base = next == -INFINITY ? 0.0f : -next * kLog2e;
+      const float base = next == -INFINITY ? 0.0f : -next * log2e;
       float sum[4] = {};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(__fmaf_rn(f[i], kLog2e, base));
-      s = __fmaf_rn(s, ex2(__fmaf_rn(m, kLog2e, base)), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(__fmaf_rn(f[i], log2e, base));
+      s = __fmaf_rn(s, ex2(__fmaf_rn(m, log2e, base)), (sum[0] + sum[1]) + (sum[2] + sum[3]));
       m = next;
     }
-    if (in) parts[(uint64_t)(part0 + j.col0 / 128 + from / 128) * ld + lane] = make_float2(m, s);
+    if (in) parts[(uint64_t)(part0 + j.col0 / 128 + from / 128) * ld + lane] = make_float2(m * whole, s);
   }
 };
 
@@ -319,12 +327,13 @@ struct GradientTile {
     to = min(to, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;
     const float base = in ? -__ldg(lse + lane) * kLog2e : 0.0f, c = in ? __ldg(g + lane) * scale_up(most) : 0.0f;
+    const float log2e = kLog2e * uncut(P);
     T* row = dl + (uint64_t)(in ? lane : 0) * ld + j.col0;
     for (uint32_t j0 = from; j0 < to; j0 += 32) {
       float f[32];
       tmem_ld32f(taddr + j0, f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = ex2(__fmaf_rn(f[i], kLog2e, base));
+      for (int i = 0; i < 32; ++i) f[i] = ex2(__fmaf_rn(f[i], log2e, base));
       const uint32_t hit = (uint32_t)(mine - (int32_t)j0);
       if (any_of(hit < 32)) {
 #pragma unroll
