@@ -390,13 +390,13 @@ struct StoreTile {
 // a line's remainder, and so its shift, is the same for all of a thread's lines.
 // Everything else is as with operands in place. A copy loop through registers
 // instead (two aligned words a thread, a block ahead) took 3300 ns a block of
-// both operands, waiting for L1's few lines; this takes 810, and 530 where one is
-// copied (4096 x 4096 x 4097: 212 us forward, 138 for either gradient; the products
-// alone take 270 a block). Shared memory bounds it: two reads and a write of every
+// both operands, waiting for L1's few lines; this takes 770, and 550 where one
+// is copied (4096 x 4096 x 4097: 200 us forward, 142 and 153 for the gradients; the
+// products alone take 270 a block; with two groups of warps 212 us). Shared memory bounds it: two reads and a write of every
 // 16 bytes, 384 cycles an operand's block.
 
 constexpr int kPairTokens = 256, kPairOut = 8;
-constexpr int kCopyGroups = 2, kCopyWarps = 4;  // groups of so many warps take turns at the blocks
+constexpr int kCopyGroups = 3, kCopyWarps = 4;  // groups of so many warps take turns at the blocks
 constexpr uint64_t kRawLandNs = 1000000;  // after a wait gave up: for raw loads in flight
 constexpr int kLineK = 144, kLineMN = 272;  // raw bytes of a line: 64 steps, or 128 lanes or columns, and 16 more
 constexpr int kRawOperand = 128 * kLineK;
