@@ -285,3 +285,21 @@ def test_two_streams():
     assert_within(outs[0][0], *want[0])
     for c in ctxs:
         c.close()
+
+
+def test_the_mean_cut_of_the_sums_is_given_back(ctx):
+    """The tensor cores cut a sum at each step of 16 products: d/16 * 2^-26 of a logit in the mean. lse, an average of
+    logits, would be that much of their average too small for every row; at most a quarter of it is left in the mean."""
+    rows, vocab, d = 256, 20000, 2048
+    g = torch.Generator(device="cuda").manual_seed(13)
+    w = (torch.randn(vocab, d, generator=g, device="cuda") * (1.5 / d ** 0.5)).to(torch.bfloat16)
+    h = torch.randn(rows, d, generator=g, device="cuda").to(torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    site = fb.loss_site(rows, vocab, d, torch.bfloat16)
+    work = torch.empty(ctx.linear_loss_workspace(site, grad=False), dtype=torch.uint8, device="cuda")
+    loss, lse = (torch.empty(rows, device="cuda") for _ in range(2))
+    ctx.linear_loss(site, h, w, t, loss, lse, work)
+    l = h.double() @ w.double().t()
+    want = torch.logsumexp(l, 1)
+    average = (torch.softmax(l, 1) * l).sum(1).mean()
+    assert (lse.double() - want).mean().abs() <= 0.25 * d / 16 * 2.0 ** -26 * average
