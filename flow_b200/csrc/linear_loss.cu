@@ -16,6 +16,9 @@
 // Bound by the tensor cores: 2 rows*vocab*d operations forward, three times that
 // backward. The rows with a target come first of all, side by side (list, hc), so
 // that the others cost nothing and whatever they hold is not read.
+// Measured on a B200: 8192 rows, 128000 x 4096 bf16, forward and backward 26.7 ms (1.28
+// PFLOP/s over four products, at the power limit); 2401 rows, 50257 x 1000 216 and
+// 653 us; 16 rows, 50257 x 2048 57 and 155 us (the weights, once and three times: 32 and 96).
 #include <algorithm>
 
 #include "product.cuh"
