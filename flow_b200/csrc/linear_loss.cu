@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict
   const uint64_t n = (uint64_t)count * d;
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
     float s = 0.0f;
+#pragma unroll 8
     for (uint32_t p = 0; p < parts; ++p) s += __ldcs(sums + p * ldp + i);
     dh[(uint64_t)__ldg(Q.list + i / d) * lddh + i % d] = from_f32<T>(s * down);
   }
@@ -470,14 +471,16 @@ Plan plan_of(const MapalLossSite& s, bool grad, bool copies, int sms) {
   p.piece = (uint32_t)up((s.vocab + p.pieces - 1) / p.pieces, 256);
   p.pieces = (uint32_t)((s.vocab + p.piece - 1) / p.piece);
   // dh has rows x d outputs, which may be few tiles: the sum over a piece is cut into the
-  // parts that take the least, counted in blocks of 64 a tile, waves, and 8 blocks'
-  // time a wave for a tile's ends and for joining a part.
+  // parts that take the least, counted in the time of a block of 64 (270 ns, 2 MB from
+  // HBM): a tile's blocks and 8 for its ends, in waves; a part's sums, written and read;
+  // and half a block for each that the join adds in turn.
   p.parts = 1;
   if (grad) {
     const uint64_t tiles = up(s.rows, 256) / 256 * (up(s.d, 256) / 256), at_once = sms / 2, blocks = p.piece / kStepK;
     uint64_t least = ~0ull;
-    for (uint32_t n = 1; n <= 16 && blocks / n >= 16; ++n) {
-      const uint64_t cost = (tiles * n + at_once - 1) / at_once * ((blocks + n - 1) / n + 8) + 4 * n * p.pieces;
+    for (uint32_t n = 1; n <= 64 && blocks / n >= 8; ++n) {
+      const uint64_t sums = n > 1 ? n * (s.rows * s.d * 8 >> 21) + n / 2 : 0;
+      const uint64_t cost = (tiles * n + at_once - 1) / at_once * ((blocks + n - 1) / n + 8) + sums;
       if (cost < least) {
         least = cost;
         p.parts = n;
