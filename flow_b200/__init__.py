@@ -589,8 +589,9 @@ class Context:
 
     def linear_loss(self, site: LossSite, h, w, targets, loss, lse, work) -> None:
         """loss[i] = lse[i] - <h[i], w[targets[i]]> with lse[i] the log of the summed exponentials of <h[i], w[v]> over
-        the vocabulary, both f32 (lse may be None); 0 where the target is -1. `work`: a contiguous CUDA buffer of at
-        least linear_loss_workspace(site) bytes, its own for calls that may overlap."""
+        the vocabulary, both f32; a row whose target is -1 has a loss of 0. lse may be None, and rows without a target
+        are then not read. `work`: a contiguous CUDA buffer of at least linear_loss_workspace(site) bytes, its own for
+        calls that may overlap."""
         rc = _direct.linear_loss(self._h, self.devices[0], site, h, w, targets, loss, lse, work)
         if rc is not None and rc != _SHORT:
             if rc:

@@ -14,8 +14,9 @@
 // dl from which both sums are products. The logits are never in memory.
 //
 // Bound by the tensor cores: 2 rows*vocab*d operations forward, three times that
-// backward. The rows with a target come first of all, side by side (list, hc), so
-// that the others cost nothing and whatever they hold is not read.
+// backward. The rows that a call takes come first of all, side by side (list, h):
+// those with a target, and all of them where lse is asked for, which every row has.
+// The others cost nothing and whatever they hold is not read.
 // Measured on a B200: 8192 rows, 128000 x 4096 bf16, forward and backward 26.7 ms (1.28
 // PFLOP/s over four products, at the power limit); 2401 rows, 50257 x 1000 216 and
 // 653 us; 16 rows, 50257 x 2048 57 and 155 us (the weights, once and three times: 32 and 96).
@@ -49,13 +50,13 @@ __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&f)[32]) {
   for (int i = 0; i < 32; ++i) f[i] = __int_as_float(r[i]);
 }
 
-// ---- rows with a target --------------------------------------------------------------
+// ---- rows taken ------------------------------------------------------------------------
 //
-// The rows that have a target, in order: list[c] = row, and their h, target,
-// log-sum and gradient side by side. count = {0, how many}, the offsets of one
-// group. Each block counts the targets before its rows itself (they are few bytes),
-// so no scan goes before. Rows without a target get what they are due: a loss and
-// a log-sum of 0, or a gradient of zeros.
+// The rows that have a target (all: every row), in order: list[c] = row, and their
+// h, target (-1: none), log-sum and gradient side by side. count = {0, how many}, the
+// offsets of one group. Each block counts the targets before its rows itself (they
+// are few bytes), so no scan goes before. Rows that are not taken get what they are
+// due: a loss of 0, or a gradient of zeros.
 
 struct Taken {
   int32_t* list;
@@ -73,11 +74,10 @@ struct TakeArgs {
   const float* lse;
   const float* dloss;
   float* loss_out;  // forward
-  float* lse_out;
-  uint16_t* dh;  // backward, may be null
+  uint16_t* dh;     // backward, may be null
   uint64_t ldh, lddh, rows, d;
   uint32_t vocab, chunk;  // rows a block takes
-  uint32_t grad, aligned;
+  uint32_t grad, all, aligned;
   unsigned* trap;
 };
 
@@ -93,7 +93,10 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
   grid_go();
   const uint64_t lo = (uint64_t)blockIdx.x * A.chunk, hi = min(lo + A.chunk, A.rows);
   uint32_t n = 0;
-  for (uint64_t i = threadIdx.x; i < lo; i += kTakeThreads) n += is_target(__ldg(A.targets + i), A.vocab);
+  if (A.all)
+    n = threadIdx.x == 0 ? (uint32_t)lo : 0;
+  else
+    for (uint64_t i = threadIdx.x; i < lo; i += kTakeThreads) n += is_target(__ldg(A.targets + i), A.vocab);
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0) sums[warp] = n;
   __syncthreads();
@@ -106,13 +109,13 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
     const int32_t t = i < hi ? __ldg(A.targets + i) : -1;
     const bool ok = is_target(t, A.vocab);
     if (warp == 0 && !ok && t != -1) atomicMax(A.trap, kTrapOob);
-    const uint32_t which = __ballot_sync(0xffffffffu, ok);
+    const uint32_t which = __ballot_sync(0xffffffffu, ok || (A.all && i < hi));
     const uint32_t c = before + __popc(which & ((1u << lane) - 1));
     before += __popc(which);
     if (warp == 0 && i < hi) {
-      if (ok) {
+      if (ok || A.all) {
         T.list[c] = (int32_t)i;
-        T.target[c] = t;
+        T.target[c] = ok ? t : -1;
         if (A.grad) {
           const float g = A.dloss ? __ldg(A.dloss + i) : 1.0f;
           T.lse[c] = __ldg(A.lse + i);
@@ -121,7 +124,6 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
         }
       } else if (!A.grad) {
         A.loss_out[i] = 0.0f;
-        if (A.lse_out) A.lse_out[i] = 0.0f;
       }
     }
     for (uint32_t r = warp; r < 32 && i0 + r < hi; r += kTakeThreads / 32) {
@@ -253,9 +255,10 @@ __global__ void __launch_bounds__(32 * kJoinRows)
   const uint32_t count = (uint32_t)__ldg(Q.count + 1), row0 = blockIdx.x * kJoinRows, c = row0 + warp;
   if (row0 >= count) return;
   float dot = 0.0f;
-  if (c < count) {
+  const int32_t target = c < count ? __ldg(Q.target + c) : -1;
+  if (target >= 0) {
     const T* hr = reinterpret_cast<const T*>(Q.h) + (uint64_t)c * Q.ld;
-    const T* wr = w + (uint64_t)__ldg(Q.target + c) * ldw;
+    const T* wr = w + (uint64_t)target * ldw;
 #pragma unroll 4
     for (uint32_t e = lane * V; e < d; e += 32 * V) {
       float x[V], y[V];
@@ -285,10 +288,15 @@ __global__ void __launch_bounds__(32 * kJoinRows)
     float2 s = part[0][warp];
 #pragma unroll
     for (int q = 1; q < kJoinRows; ++q) join(s, part[q][warp]);
+    const int32_t row = __ldg(Q.list + c);
+    if (target < 0) {  // s is of all the vocabulary
+      loss[row] = 0.0f;
+      if (lse) lse[row] = s.x + logf(s.y);
+      return;
+    }
     const float u = fmaxf(s.x, dot);
     const float others = s.y == 0.0f ? 0.0f : s.y * ex2((s.x - u) * kLog2e);
     const float more = log1pf(others + (ex2((dot - u) * kLog2e) - 1.0f));
-    const int32_t row = __ldg(Q.list + c);
     loss[row] = (u - dot) + more;
     if (lse) lse[row] = u + more;
   }
@@ -596,7 +604,7 @@ int forward(const Call& c, const void* h, const void* w, const int32_t* targets,
   const MapalLossSite& s = c.s;
   TakeArgs a{};
   a.loss_out = loss;
-  a.lse_out = lse;
+  a.all = lse != nullptr;
   MAPAL_TRY(c.take(a, h, targets));
   float2* parts = c.template at<float2>(c.p.sums);
   for (uint32_t i = 0; i < c.p.pieces; ++i) {

@@ -688,9 +688,10 @@ int mapal_gpu_linear_loss_workspace(MapalGpuCtx* ctx, const MapalLossSite* site,
  * loss[i] = lse[i] - l[i, t]. Logits are f32 (products exact, sums on the
  * tensor cores, the target's by itself), and the loss of a target that is
  * nearly certain is the others' share, not what is left of two large numbers.
- * targets: one of [0, vocab) a row; -1: the row has none, its loss and lse are
- * 0 and its H is not read. Any other target traps index_oob; its row is
- * treated as one without. lse may be NULL (the gradient needs it). `work` is
+ * targets: one of [0, vocab) a row; -1: the row has none and its loss is 0. Any
+ * other target traps index_oob; its row is treated as one without. lse is every
+ * row's, with a target or without; it may be NULL (the gradient needs it), and
+ * rows without a target then cost nothing and their H is not read. `work` is
  * scratch of at least the stated bytes, 16-byte aligned, used until the
  * call's work has finished: calls that may overlap need one each. */
 int mapal_gpu_linear_loss(MapalGpuCtx* ctx, const MapalLossSite* site, const void* h, const void* w,

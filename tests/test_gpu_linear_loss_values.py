@@ -1,0 +1,137 @@
+"""The loss of a large vocabulary on a B200 where its values could go wrong: the log-sum of rows without a target."""
+import pytest
+import torch
+
+import flow_b200 as fb
+from _rows import U32, Guarded, assert_within, replayed
+from test_gpu_linear_loss import HALF, formula, inputs
+from test_gpu_training_step import Step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = fb.Context((0,))
+    yield c
+    c.close()
+
+
+def sums(h, w, t):
+    """lse of every row, the loss (0 without a target) in f64, and bounds on both: a logit's, of the exponentials and
+    of their sum as in test_gpu_linear_loss.py."""
+    h, w, there = h.double(), w.double(), t >= 0
+    l, size = h @ w.t(), h.abs() @ w.abs().t()
+    err_l = ((h.shape[1] + 16) * 17 / 16 * 2 * U32 * size).amax(1)
+    big = l.abs().amax(1)
+    lse = torch.logsumexp(l, 1)
+    loss = torch.where(there, lse - l.gather(1, t.long().clamp(min=0)[:, None])[:, 0], 0.0)
+    err = err_l + 8 * U32 * big * (1 + 1.4427) + 2.0 ** -22 + 2.0 ** -19
+    return (lse, err), (loss, torch.where(there, err + err_l + 8 * U32 * loss, 0.0))
+
+
+def forward(ctx, h, w, t, ask=True, call=lambda f: f()):
+    rows, d = h.t.shape
+    site = fb.loss_site(rows, w.t.shape[0], d, h.t.dtype, ldh=h.ld, ldw=w.ld)
+    work = torch.full((ctx.linear_loss_workspace(site, w=w.t, grad=False),), 0xFF, dtype=torch.uint8, device="cuda")  # NaN
+    loss, lse = (torch.full((rows,), 9.0, device="cuda") for _ in range(2))
+    call(lambda: ctx.linear_loss(site, h.t, w.t, t, loss, lse if ask else None, work))
+    return loss, lse
+
+
+def check(ctx, h, w, t, dloss, opads=(0, 0), call=lambda f: f()):
+    """The loss, every row's lse and both gradients, with nothing written around them or behind work."""
+    (rows, d), (vocab, dtype) = h.t.shape, (w.t.shape[0], h.t.dtype)
+    (_, _, *want), lse32 = formula(h.t, w.t, t, dloss, dtype)
+    lse_loss = sums(h.t, w.t, t)
+    dh, dw = Guarded(rows, d, dtype, opads[0], opads[0]), Guarded(vocab, d, dtype, opads[1], opads[1])
+    site = fb.loss_site(rows, vocab, d, dtype, ldh=h.ld, ldw=w.ld, lddh=dh.ld, lddw=dw.ld)
+    n = ctx.linear_loss_workspace(site, w=w.t)
+    buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    lse, loss = (torch.full((rows + 1,), 9.0, device="cuda") for _ in range(2))
+
+    def go():
+        ctx.linear_loss(site, h.t, w.t, t, loss, lse, buf[:n])
+        ctx.linear_loss_grad(site, h.t, w.t, t, lse32, dloss, dh.t, dw.t, buf[:n])
+
+    call(go)
+    for got, (value, bound), what in zip((lse[:rows], loss[:rows], dh.t, dw.t), (*lse_loss, *want), ("lse", "loss", "dh", "dw")):
+        assert_within(got, value, bound, what)
+    assert (loss[rows] == 9.0) and (lse[rows] == 9.0) and dh.intact() and dw.intact() and (buf[n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("ignored", [0.0, 0.1, 0.5, 0.97, 1.0])
+@pytest.mark.parametrize("rows,vocab,d", [(40, 300, 64), (700, 1000, 136), (2000, 515, 33)])
+def test_gradients_beside_rows_without_a_target(ctx, rows, vocab, d, ignored, dtype):
+    check(ctx, *inputs(rows, vocab, d, dtype, rows, ignored))
+
+
+@pytest.mark.parametrize("pads,offsets,opads", [((8, 8), (0, 0), (8, 16)), ((1, 0), (0, 0), (1, 3)), ((0, 5), (0, 0), (0, 0)),
+                                                ((8, 8), (1, 0), (0, 0)), ((8, 8), (0, 3), (2, 0)), ((16, 24), (8, 16), (3, 5))])
+@pytest.mark.parametrize("rows,vocab,d", [(70, 600, 72), (300, 1300, 131)])
+def test_strides_and_places(ctx, rows, vocab, d, pads, offsets, opads):
+    check(ctx, *inputs(rows, vocab, d, torch.float16, 5, 0.2, pads=pads, offsets=offsets), opads=opads)
+
+
+def test_several_pieces_and_captured(ctx):
+    check(ctx, *inputs(9000, 33000, 72, torch.bfloat16, 3, 0.05), call=lambda f: replayed(ctx, f))
+
+
+def test_the_loss_of_a_training_step(ctx):
+    """On what a step of a layer of experts gave it, forty rows of padding among its rows."""
+    s = Step()
+    s.run(ctx)
+    (lse, elses), (loss, eloss) = sums(s.out, s.wv, s.targets)
+    assert_within(s.lse, lse, elses, "lse")
+    assert_within(s.loss, loss, eloss, "loss")
+    (_, _, (dh, edh), (dw, edw)), _ = formula(s.out, s.wv, s.targets, s.g, s.t)
+    # the step's own lse goes into its gradient: its error is a relative one of p
+    assert_within(s.dout, dh, edh + 2 * elses.max() * (s.g.max() * s.wv.double().abs().sum(0)), "dh")
+    assert_within(s.dwv, dw, edw + 2 * elses.max() * (s.g.double() @ s.out.double().abs()), "dw")
+    assert not s.dout[s.T - 40:].any() and torch.isfinite(s.dx.float()).all()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("ignored", [0.0, 0.1, 0.97, 1.0])
+@pytest.mark.parametrize("rows,vocab,d,pads,offsets", [(1, 1, 1, (0, 0), (0, 0)), (1, 300, 64, (0, 0), (0, 0)),
+                                                       (40, 129, 7, (1, 0), (0, 3)), (700, 1000, 136, (8, 16), (0, 0)),
+                                                       (2500, 515, 33, (0, 0), (1, 0)), (300, 70001, 2051, (0, 0), (0, 0))])
+def test_every_row_has_a_log_sum(ctx, rows, vocab, d, pads, offsets, ignored, dtype):
+    """With a target or without; a row without one has a loss of 0. The losses are the same where lse is not asked for."""
+    h, w, t, _ = inputs(rows, vocab, d, dtype, rows + vocab, ignored, pads=pads, offsets=offsets)
+    (want_lse, err_lse), (want_loss, err_loss) = sums(h.t, w.t, t)
+    loss, lse = forward(ctx, h, w, t)
+    assert_within(lse, want_lse, err_lse, "lse")
+    assert_within(loss, want_loss, err_loss, "loss")
+    assert torch.equal(forward(ctx, h, w, t, ask=False)[0], loss)
+
+
+def test_a_log_sum_for_bad_targets_and_in_a_graph(ctx):
+    h, w, t, _ = inputs(200, 700, 72, torch.bfloat16, 3, 0.3)
+    loss, lse = forward(ctx, h, w, t)
+    again = forward(ctx, h, w, t, call=lambda f: replayed(ctx, f))
+    assert torch.equal(again[0], loss) and torch.equal(again[1], lse)
+    at = int(torch.nonzero(t < 0)[0])
+    t[at] = 700
+    with pytest.raises(fb.MapalTrap, match="index_oob"):
+        forward(ctx, h, w, t)
+
+
+def test_what_rows_without_a_target_hold(ctx):
+    """Their own log-sum alone depends on it; without lse they are not read, and the gradients never read them."""
+    h, w, t, dloss = inputs(300, 500, 64, torch.bfloat16, 7, 0.4)
+    site, none = fb.loss_site(300, 500, 64, torch.bfloat16), t == -1
+    out = []
+    for bad in (0.0, float("nan"), float("inf")):
+        h.t[none] = bad
+        (loss, lse), alone = forward(ctx, h, w, t), forward(ctx, h, w, t, ask=False)[0]
+        assert torch.equal(loss, alone) and not loss[none].any()
+        work = torch.full((ctx.linear_loss_workspace(site),), 0xFF, dtype=torch.uint8, device="cuda")
+        dh, dw = torch.empty(300, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(500, 64, dtype=torch.bfloat16, device="cuda")
+        ctx.linear_loss_grad(site, h.t, w.t, t, lse, torch.where(none, bad, dloss), dh, dw, work)
+        assert torch.isfinite(lse[none]).any() == (bad == 0.0) and not dh[none].any()
+        out.append((loss, lse[~none], dh, dw))
+    for o in out[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out[0], o))
+    assert all(torch.isfinite(x).all() for x in out[0])
