@@ -309,7 +309,9 @@ __global__ void __launch_bounds__(tile_threads(MODE, NT), 1)
     product_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ ProductArgs P, const __grid_constant__ TileArgs O) {
   using Smem = TileSmem<NT, CH, KB, STAGES>;
-  constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+  // two accumulators of NT columns; 16 of them are read with the 16 columns behind
+  constexpr uint32_t kCols = NT < kTurnCols ? 2 * kTurnCols : 2 * NT;
+  static_assert(NT + (NT < kTurnCols ? kTurnCols : NT) <= kCols, "the second accumulator's reads stay in what is allocated");
   constexpr int kOut = out_warps(NT);
   constexpr bool MN = MODE != kForward, MB = MODE == kGradW;
   extern __shared__ __align__(1024) uint8_t smem_raw[];

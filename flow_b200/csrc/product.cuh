@@ -241,6 +241,7 @@ __device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, float (&f)[16]) {
 }
 
 constexpr int kOutScratch = 32 * 64;  // bytes of shared memory that a writing warp needs
+constexpr int kTurnCols = 32;  // columns of tensor memory that it reads at a time, whatever is left of the tile
 
 // Columns [from, to) of a warp's 32 lanes, of which `left` exist, as 16-bit values: 32
 // columns at a time are turned in shared memory (stmatrix, transposed) so that a
@@ -269,7 +270,7 @@ __device__ __forceinline__ void put_turned(uint32_t taddr, uint32_t from, uint32
     return;
   }
   if (from < to) load(from);
-  for (uint32_t j0 = from; j0 < to; j0 += 32) {
+  for (uint32_t j0 = from; j0 < to; j0 += kTurnCols) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(f[0][i]), "+f"(f[1][i]));
@@ -285,7 +286,7 @@ __device__ __forceinline__ void put_turned(uint32_t taddr, uint32_t from, uint32
         o.set(v);
         w[q][2 * h] = o.w[0], w[q][2 * h + 1] = o.w[1];
       }
-    if (j0 + 32 < to) load(j0 + 32);  // beside the stores
+    if (j0 + kTurnCols < to) load(j0 + kTurnCols);  // beside the stores
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + q * 512),
