@@ -351,7 +351,8 @@ struct GradientTile {
         for (int i = 0; i < 32; ++i) f[i] -= hit == i ? 1.0f : 0.0f;
       }
       if (in) {
-        // sixteen at a time, whole sectors: what lies behind the piece's last column is dl's own row
+        // sixteen at a time, whole sectors (dl, its rows and j0 lie on 32 bytes): what lies behind the piece's last
+        // column is dl's own row
 #pragma unroll
         for (int i = 0; i < 32; i += 16) {
           if (j0 + i >= to) break;
@@ -451,10 +452,11 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict
 // ---- host ------------------------------------------------------------------------------
 
 constexpr uint64_t kPieceBytes = 256ull << 20;  // of dl, and of copied weights, about
+constexpr uint64_t kWorkAligned = 16, kStoreAligned = 32;  // what `work` is, and what dl's widest stores need
 
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
-// How a call is cut, and where its scratch lies.
+// How a call is cut, and where its scratch lies: offsets from the first 32-byte boundary in `work`.
 struct Plan {
   uint64_t ld;              // of h's rows side by side, and of copied weights
   uint32_t piece, pieces;   // of the vocabulary, a multiple of 256
@@ -515,7 +517,7 @@ Plan plan_of(const MapalLossSite& s, bool grad, bool copies, int sms) {
   } else {
     p.sums = take(8 * s.rows * (up(s.vocab, 256) / 128));
   }
-  p.bytes = at;
+  p.bytes = at + (kStoreAligned - kWorkAligned);
   return p;
 }
 
@@ -548,7 +550,7 @@ struct Call {
     return reinterpret_cast<T*>(work + offset);
   }
   Call(DeviceSlot& d, const MapalLossSite& site, const Plan& plan, void* w, bool grad)
-      : D(d), s(site), p(plan), work(static_cast<uint8_t*>(w)) {
+      : D(d), s(site), p(plan), work(reinterpret_cast<uint8_t*>(up((uintptr_t)w, kStoreAligned))) {
     q = {at<int32_t>(p.list), at<int32_t>(p.count), at<int32_t>(p.target), at<float>(p.lse), at<float>(p.g),
          grad && s.dtype == MAPAL_DTYPE_F16 ? at<unsigned>(p.most) : nullptr, at<uint16_t>(p.h), p.ld};
   }
@@ -681,7 +683,7 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
 int check_work(const Plan& p, const void* work, uint64_t bytes) {
   if (bytes < p.bytes || !work)
     return set_error(MAPAL_ERR_INVALID, "work is shorter than mapal_gpu_linear_loss_workspace says for these arrays");
-  if ((uintptr_t)work & 15) return set_error(MAPAL_ERR_INVALID, "work is not on a 16-byte boundary");
+  if ((uintptr_t)work & (kWorkAligned - 1)) return set_error(MAPAL_ERR_INVALID, "work is not on a 16-byte boundary");
   return 0;
 }
 

@@ -39,25 +39,27 @@ def forward(ctx, h, w, t, ask=True, call=lambda f: f()):
     return loss, lse
 
 
-def check(ctx, h, w, t, dloss, opads=(0, 0), call=lambda f: f()):
-    """The loss, every row's lse and both gradients, with nothing written around them or behind work."""
+def check(ctx, h, w, t, dloss, opads=(0, 0), call=lambda f: f(), at=0):
+    """The loss, every row's lse and both gradients, with nothing written around them or around work, which begins `at`
+    bytes behind a boundary of 256."""
     (rows, d), (vocab, dtype) = h.t.shape, (w.t.shape[0], h.t.dtype)
     (_, _, *want), lse32 = formula(h.t, w.t, t, dloss, dtype)
     lse_loss = sums(h.t, w.t, t)
     dh, dw = Guarded(rows, d, dtype, opads[0], opads[0]), Guarded(vocab, d, dtype, opads[1], opads[1])
     site = fb.loss_site(rows, vocab, d, dtype, ldh=h.ld, ldw=w.ld, lddh=dh.ld, lddw=dw.ld)
     n = ctx.linear_loss_workspace(site, w=w.t)
-    buf = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    buf = torch.full((at + n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    work = buf[at:at + n]
     lse, loss = (torch.full((rows + 1,), 9.0, device="cuda") for _ in range(2))
 
     def go():
-        ctx.linear_loss(site, h.t, w.t, t, loss, lse, buf[:n])
-        ctx.linear_loss_grad(site, h.t, w.t, t, lse32, dloss, dh.t, dw.t, buf[:n])
+        ctx.linear_loss(site, h.t, w.t, t, loss, lse, work)
+        ctx.linear_loss_grad(site, h.t, w.t, t, lse32, dloss, dh.t, dw.t, work)
 
     call(go)
     for got, (value, bound), what in zip((lse[:rows], loss[:rows], dh.t, dw.t), (*lse_loss, *want), ("lse", "loss", "dh", "dw")):
         assert_within(got, value, bound, what)
-    assert (loss[rows] == 9.0) and (lse[rows] == 9.0) and dh.intact() and dw.intact() and (buf[n:] == 0xA5).all()
+    assert (loss[rows] == 9.0) and (lse[rows] == 9.0) and dh.intact() and dw.intact() and (buf[:at] == 0xA5).all() and (buf[at + n:] == 0xA5).all()
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -72,6 +74,14 @@ def test_gradients_beside_rows_without_a_target(ctx, rows, vocab, d, ignored, dt
 @pytest.mark.parametrize("rows,vocab,d", [(70, 600, 72), (300, 1300, 131)])
 def test_strides_and_places(ctx, rows, vocab, d, pads, offsets, opads):
     check(ctx, *inputs(rows, vocab, d, torch.float16, 5, 0.2, pads=pads, offsets=offsets), opads=opads)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("at", [16, 32, 48, 128, 240])
+@pytest.mark.parametrize("rows,vocab,d,offset", [(40, 300, 64, 0), (700, 1000, 136, 0), (300, 600, 33, 1)])
+def test_scratch_on_any_16_bytes(ctx, rows, vocab, d, offset, at, dtype):
+    """As a slice of an arena lies: on 16 bytes, whatever lies on 32 of its own."""
+    check(ctx, *inputs(rows, vocab, d, dtype, rows, 0.2, offsets=(0, offset)), at=at)
 
 
 def test_several_pieces_and_captured(ctx):
@@ -135,3 +145,14 @@ def test_what_rows_without_a_target_hold(ctx):
     for o in out[1:]:
         assert all(torch.equal(a, b) for a, b in zip(out[0], o))
     assert all(torch.isfinite(x).all() for x in out[0])
+
+
+def test_scratch_off_16_bytes_is_refused(ctx):
+    h, w, t, dloss = inputs(40, 300, 64, torch.bfloat16, 1)
+    site = fb.loss_site(40, 300, 64, torch.bfloat16)
+    buf, loss = torch.empty(ctx.linear_loss_workspace(site) + 64, dtype=torch.uint8, device="cuda"), torch.empty(40, device="cuda")
+    for at in (1, 4, 8, 24):
+        with pytest.raises(fb.MapalInfraError, match="16-byte boundary"):
+            ctx.linear_loss(site, h.t, w.t, t, loss, loss, buf[at:])
+        with pytest.raises(fb.MapalInfraError, match="16-byte boundary"):
+            ctx.linear_loss_grad(site, h.t, w.t, t, loss, None, h.t, None, buf[at:])
