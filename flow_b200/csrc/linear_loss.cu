@@ -239,7 +239,10 @@ constexpr int kJoinRows = 8, kJoinAhead = 4;
 
 __device__ __forceinline__ void join(float2& a, const float2& b) {
   const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) return;  // nothing on either side
+  if (m == -INFINITY) {  // no number on either side: sums of nothing, or of NaN, which a maximum passes over
+    a.y += b.y;
+    return;
+  }
   a.y = a.y * ex2((a.x - m) * kLog2e) + b.y * ex2((b.x - m) * kLog2e);
   a.x = m;
 }

@@ -156,3 +156,23 @@ def test_scratch_off_16_bytes_is_refused(ctx):
             ctx.linear_loss(site, h.t, w.t, t, loss, loss, buf[at:])
         with pytest.raises(fb.MapalInfraError, match="16-byte boundary"):
             ctx.linear_loss_grad(site, h.t, w.t, t, loss, None, h.t, None, buf[at:])
+
+
+@pytest.mark.parametrize("ask", [True, False])
+@pytest.mark.parametrize("rows,vocab,spoilt", [(5, 129, slice(128, 129)), (40, 4000, slice(128, 256)), (3, 2, slice(1, 2)), (3, 2, slice(0, 1)),
+                                               (40, 4000, slice(3999, 4000)), (40, 4000, slice(0, 4000)), (300, 9000, slice(0, 128)),
+                                               (300, 9000, slice(7000, 7001)), (40, 300, slice(17, 18)), (40, 600, slice(256, 512))])
+def test_a_logit_that_is_no_number_is_not_lost(ctx, rows, vocab, spoilt, ask):
+    """Weights of NaN, the target's or others, in part of a tile of the vocabulary or in whole ones: every row's loss
+    and lse are NaN, as the formula's. A row of h with a NaN spoils itself alone."""
+    h, w, t, _ = inputs(rows, vocab, 72, torch.bfloat16, 2, 0.2 if rows > 5 else 0.0)
+    clean = [x.clone() for x in forward(ctx, h, w, t, ask)]
+    h.t[rows // 2, 5] = float("nan")
+    loss, lse = forward(ctx, h, w, t, ask)
+    there, other = t >= 0, torch.arange(rows, device="cuda") != rows // 2
+    for got, was in zip((loss, lse), clean):
+        assert torch.equal(got[other], was[other])
+    assert torch.isnan(loss[rows // 2]) == there[rows // 2] and (not ask or torch.isnan(lse[rows // 2]))
+    w.t[spoilt] = float("nan")
+    loss, lse = forward(ctx, h, w, t, ask)
+    assert torch.isnan(loss[there]).all() and not loss[~there].any() and (not ask or torch.isnan(lse).all())
