@@ -191,7 +191,8 @@ __device__ __forceinline__ float uncut(const ProductArgs& P) { return 1.0f + (fl
 
 // A tile of logits, rows on the lanes and 128 of the vocabulary's columns a warp:
 // each thread keeps the running maximum of its row and the sum of exponentials
-// against it, the target's column left out, and writes one pair.
+// against it, the target's column left out, and writes one pair. Against a maximum
+// that is infinite the sum is of exp(l) itself: inf, or NaN with one among them.
 struct SumTile {
   float2* parts;  // [part][row]
   uint64_t ld;
@@ -222,7 +223,7 @@ struct SumTile {
 #pragma unroll
       for (int i = 1; i < 32; ++i) top = fmaxf(top, f[i]);
       const float next = fmaxf(m, top);
-      const float base = next == -INFINITY ? 0.0f : -next * log2e;
+      const float base = isinf(next) ? 0.0f : -next * log2e;
       float sum[4] = {};
 #pragma unroll
       for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(__fmaf_rn(f[i], log2e, base));
@@ -239,11 +240,8 @@ constexpr int kJoinRows = 8, kJoinAhead = 4;
 
 __device__ __forceinline__ void join(float2& a, const float2& b) {
   const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) {  // no number on either side: sums of nothing, or of NaN, which a maximum passes over
-    a.y += b.y;
-    return;
-  }
-  a.y = a.y * ex2((a.x - m) * kLog2e) + b.y * ex2((b.x - m) * kLog2e);
+  // -inf: no number on either side, sums of nothing, or of NaN, which a maximum passes over
+  a.y = isinf(m) ? a.y + b.y : a.y * ex2((a.x - m) * kLog2e) + b.y * ex2((b.x - m) * kLog2e);
   a.x = m;
 }
 
@@ -298,6 +296,12 @@ __global__ void __launch_bounds__(32 * kJoinRows)
       return;
     }
     const float u = fmaxf(s.x, dot);
+    if (isinf(u)) {  // as the limits are: lse is infinite, and so is the loss unless the target's logit is too
+      const float sum = isnan(s.y) || isnan(dot) ? NAN : u;
+      loss[row] = sum - dot;
+      if (lse) lse[row] = sum;
+      return;
+    }
     const float others = s.y == 0.0f ? 0.0f : s.y * ex2((s.x - u) * kLog2e);
     const float more = log1pf(others + (ex2((dot - u) * kLog2e) - 1.0f));
     loss[row] = (u - dot) + more;

@@ -176,3 +176,39 @@ def test_a_logit_that_is_no_number_is_not_lost(ctx, rows, vocab, spoilt, ask):
     w.t[spoilt] = float("nan")
     loss, lse = forward(ctx, h, w, t, ask)
     assert torch.isnan(loss[there]).all() and not loss[~there].any() and (not ask or torch.isnan(lse).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("vocab", [2, 100, 129, 700, 5000])
+def test_infinite_logits(ctx, vocab, dtype):
+    """Weights of infinities and none of h at zero: lse is the limit, inf where a logit is, -inf where all are; the loss
+    is inf where others outweigh the target, NaN where lse and the target's logit are the same infinity."""
+    rows, d, inf = 12, 8, float("inf")
+    h, w, t, _ = inputs(rows, vocab, d, dtype, 5)
+    h.t.fill_(0)
+    h.t[:, 0], h.t[::2, 1] = 1, 0.5
+    h.t[:, 1] += 0.25
+    t[:] = torch.arange(rows, device="cuda") % vocab
+    t[rows - 1] = -1
+
+    def holds(lse_want):
+        loss, lse = forward(ctx, h, w, t)
+        l = h.t.double() @ w.t.double().t()
+        want = torch.logsumexp(l, 1)
+        there = t >= 0
+        want_loss = torch.where(there, want - l.gather(1, t.long().clamp(min=0)[:, None])[:, 0], 0.0)
+        assert torch.isinf(want).all() == lse_want and not torch.isnan(want).any()
+        assert_within(lse, want, torch.where(torch.isinf(want), 0.0, 1e-4), "lse")
+        assert_within(loss, want_loss, torch.where(torch.isinf(want_loss), 0.0, 1e-4), "loss")
+
+    w.t[:, 1] = 1
+    w.t[vocab - 1, 0] = -inf  # a logit that adds nothing; a loss of inf for its own rows
+    holds(False)
+    w.t[1:, 0] = -inf
+    holds(False)
+    w.t[:, 0] = -inf
+    holds(True)
+    w.t[vocab - 1, 0] = inf
+    holds(True)
+    w.t[:, 0] = inf
+    holds(True)
