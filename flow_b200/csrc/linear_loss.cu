@@ -34,22 +34,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&f)[32]) {
-  int r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __int_as_float(r[i]);
-}
-
 // ---- rows taken ------------------------------------------------------------------------
 //
 // The rows that have a target (all: every row), in order: list[c] = row, and their
@@ -182,34 +166,37 @@ __global__ void __launch_bounds__(256) copy_weights_kernel(const uint16_t* __res
 
 // ---- forward -------------------------------------------------------------------------
 
-// The tensor cores cut a sum towards zero at each step of 16 products. A logit loses
-// 2^-26 of itself a step by that, in the mean (measured over logits above 2: 4.2e-7,
-// 1.9e-6 and 3.9e-6 of them at d = 512, 2048 and 4096; f32 sums that round leave a
-// spread of that size and no mean), and lse, which is an average of them, the same. The
-// factor gives the mean back; it goes into the exponent's own.
-__device__ __forceinline__ float uncut(const ProductArgs& P) { return 1.0f + (float)((P.depth + 15) / 16) * 0x1p-26f; }
+// The tensor cores cut a sum towards zero at each step of 16 products: in one sum over
+// d = 4096 a logit loses 4e-6 of itself in the mean, and lse, which is an average of
+// logits, the same. In runs of 256 elements (Out::kRun) whose sums are added in f32 the
+// cut is of small sums.
+constexpr int kLogitRun = 4;
 
 // A tile of logits, rows on the lanes and 128 of the vocabulary's columns a warp:
 // each thread keeps the running maximum of its row and the sum of exponentials
 // against it, the target's column left out, and writes one pair. Against a maximum
 // that is infinite the sum is of exp(l) itself: inf, or NaN with one among them.
 struct SumTile {
+  static constexpr int kRun = kLogitRun;
   float2* parts;  // [part][row]
   uint64_t ld;
   const int32_t* target;
   uint32_t v0, part0;
 
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
-                                      uint32_t to, uint8_t* scratch) const {
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, float (&l)[kHalfTokens], uint32_t lane0,
+                                      uint32_t from) const {
     const uint32_t lane = lane0 + (threadIdx.x & 31);
     const bool in = lane < P.lanes;
-    const uint32_t end = min(to, j.cols);
+    const uint32_t end = min(from + kHalfTokens, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;  // the target's column of this tile
-    const float whole = uncut(P), log2e = kLog2e * whole;
     float m = -INFINITY, s = 0.0f;
-    for (uint32_t j0 = from; j0 < end; j0 += 32) {
+#pragma unroll
+    for (int q = 0; q < kHalfTokens / 32; ++q) {
+      const uint32_t j0 = from + q * 32;
+      if (j0 >= end) break;
       float f[32];
-      tmem_ld32f(taddr + j0, f);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = l[q * 32 + i];
       if (j0 + 32 > end) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = j0 + i < end ? f[i] : -INFINITY;
@@ -223,14 +210,14 @@ struct SumTile {
 #pragma unroll
       for (int i = 1; i < 32; ++i) top = fmaxf(top, f[i]);
       const float next = fmaxf(m, top);
-      const float base = isinf(next) ? 0.0f : -next * log2e;
+      const float base = isinf(next) ? 0.0f : -next * kLog2e;
       float sum[4] = {};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(__fmaf_rn(f[i], log2e, base));
-      s = __fmaf_rn(s, ex2(__fmaf_rn(m, log2e, base)), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(__fmaf_rn(f[i], kLog2e, base));
+      s = __fmaf_rn(s, ex2(__fmaf_rn(m, kLog2e, base)), (sum[0] + sum[1]) + (sum[2] + sum[3]));
       m = next;
     }
-    if (in) parts[(uint64_t)(part0 + j.col0 / 128 + from / 128) * ld + lane] = make_float2(m * whole, s);
+    if (in) parts[(uint64_t)(part0 + j.col0 / 128 + from / 128) * ld + lane] = make_float2(m, s);
   }
 };
 
@@ -330,6 +317,7 @@ __device__ __forceinline__ float scale_down(const unsigned* most) {
 // which the tensor cores take no wider.
 template <typename T>
 struct GradientTile {
+  static constexpr int kRun = kLogitRun;
   T* dl;
   uint64_t ld;
   const int32_t* target;
@@ -338,20 +326,21 @@ struct GradientTile {
   const unsigned* most;
   uint32_t v0;
 
-  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, uint32_t taddr, uint32_t lane0, uint32_t from,
-                                      uint32_t to, uint8_t* scratch) const {
+  __device__ __forceinline__ void put(const ProductArgs& P, const Job& j, float (&l)[kHalfTokens], uint32_t lane0,
+                                      uint32_t from) const {
     const uint32_t lane = lane0 + (threadIdx.x & 31);
     const bool in = lane < (uint32_t)__ldg(P.lane_count);
-    to = min(to, j.cols);
+    const uint32_t to = min(from + kHalfTokens, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;
     const float base = in ? -__ldg(lse + lane) * kLog2e : 0.0f, c = in ? __ldg(g + lane) * scale_up(most) : 0.0f;
-    const float log2e = kLog2e * uncut(P);
     T* row = dl + (uint64_t)(in ? lane : 0) * ld + j.col0;
-    for (uint32_t j0 = from; j0 < to; j0 += 32) {
-      float f[32];
-      tmem_ld32f(taddr + j0, f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = ex2(__fmaf_rn(f[i], log2e, base));
+    for (int q = 0; q < kHalfTokens / 32; ++q) {
+      const uint32_t j0 = from + q * 32;
+      if (j0 >= to) break;
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = ex2(__fmaf_rn(l[q * 32 + i], kLog2e, base));
       const uint32_t hit = (uint32_t)(mine - (int32_t)j0);
       if (any_of(hit < 32)) {
 #pragma unroll
@@ -381,6 +370,7 @@ struct GradientTile {
 // `sums`, are added first. place: where column j's row goes (null: j itself).
 template <typename T, bool ADD>
 struct SumsTile {
+  static constexpr int kRun = 0;
   T* out;
   const float* sums;
   const int32_t* place;

@@ -318,6 +318,7 @@ __device__ __forceinline__ void put_turned(uint32_t taddr, uint32_t from, uint32
 // group's matrix), lanes along the row. wide: 16-bit rows on 16-byte boundaries.
 template <int MODE, typename T>
 struct StoreTile {
+  static constexpr int kRun = 0;  // see the pair of CTAs
   T* out;
   uint64_t ld, ldg;  // rows, groups' matrices
   bool wide;
@@ -379,6 +380,10 @@ struct StoreTile {
 // block is counted by a barrier of its own (landed); a warp clears the rows behind
 // the group's last up to the next 16 (the MMA's step) in both operands, since zero
 // times NaN is not zero, and lets the products go on (fixed).
+//
+// Where the sum's own error counts (Out::kRun, blocks), t is taken in runs: each run's
+// sums start from zero in tensor memory, where every step cuts what it adds up, and
+// the output warps add the runs up in registers, rounded.
 //
 // Bound by the tensor cores: 4096^3 bf16 in 95 us (1.45 PFLOP/s, cuBLAS 93), 16384 rows
 // of 16 matrices of 4096 x 4096 in 411, 475 and 415 us (1.16 to 1.34 PFLOP/s, at the
@@ -600,6 +605,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
   uint32_t fixes = 0;   // a bit a stage: the parity of its next clearing
 
   auto blocks_of = [](const Job& q) { return (q.depth + kStepK - 1) / kStepK; };
+  constexpr uint32_t kRun = Out::kRun;
+  static_assert(kRun % kKB == 0, "runs of whole stages");
   // whether the last block holds rows that are not the group's (copied operands have none)
   auto to_fix = [&](const Job& q) { return MODE == kGradW && (TA || TB) && (q.depth & 15) && q.t0 + q.depth < P.m; };
 
@@ -661,16 +668,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
     }
   } else if (warp == 1) {
     // ---- products, by the first CTA ----
-    uint32_t n = 0;
-    for (; rank == 0 && more; more = walk.next(j), ++n) {
-      const uint32_t b = n & 1, blocks = blocks_of(j);
+    uint32_t n = 0, b = 0;  // accumulators taken, this one
+    for (; rank == 0 && more; more = walk.next(j)) {
+      const uint32_t blocks = blocks_of(j);
       const bool fix = to_fix(j);
       if (elect_one()) {
         const uint32_t idesc = idesc_f16<MODE>(P.bf16, 256, (int)((j.cols + 31) / 32 * 32));
-        if (!mbar_wait_cluster(&sm.acc_empty[b], ((n >> 1) & 1) ^ 1, abort)) give_up();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        auto accumulator = [&]() {  // the next one, once it has been read
+          b = n++ & 1;
+          if (!mbar_wait_cluster(&sm.acc_empty[b], (((n - 1) >> 1) & 1) ^ 1, abort)) give_up();
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        };
+        accumulator();
         for (uint32_t kb = 0; kb < blocks && !*abort; kb += kKB, ++it) {
           const uint32_t s = it % kStages, here = min((uint32_t)kKB, blocks - kb);
+          const bool starts = kRun ? kb % kRun == 0 : kb == 0;
+          if (kRun && starts && kb) {
+            pair_commit(&sm.acc_full[b]);
+            accumulator();
+            if (*abort) break;
+          }
           bool ok = CA || CB ? mbar_wait_cluster(&sm.full[s], (it / kStages) & 1, abort)
                              : mbar_wait(&sm.full[s], (it / kStages) & 1, abort);
           if (fix && kb + here == blocks) {
@@ -693,7 +710,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
                 if (MODE != kGradW || kk * 16 < left)
                   mma_f16<2>(tmem + b * NT, da + u * (2 * Smem::kHalf >> 4) + kk * operand_step<MA>(),
                              db + u * (2 * Smem::kHalf >> 4) + kk * operand_step<MB>(), idesc,
-                             kb > 0 || u > 0 || kk > 0);
+                             !starts || u > 0 || kk > 0);
             }
           pair_commit(&sm.empty[s]);
         }
@@ -765,19 +782,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
     // ---- output ----
     const int quarter = warp & 3;
     const uint32_t from = (warp - 2) / 4 * kHalfTokens;
-    uint32_t n = 0;
-    for (; more; more = walk.next(j), ++n) {
-      const uint32_t b = n & 1;
-      if (any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort)) {
-        give_up();
-        break;
-      }
+    uint32_t n = 0, b = 0;
+    auto filled = [&]() {  // the next accumulator, in which a tile or a run has ended
+      b = n & 1;
+      const bool ok = !any_of(!mbar_wait(&sm.acc_full[b], (n >> 1) & 1, abort) || *abort);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      out.put(P, j, tmem + ((uint32_t)(quarter * 32) << 16) + b * NT, j.lane0 + rank * 128 + quarter * 32, from,
-              from + kHalfTokens, sm.scratch[warp - 2]);
+      ++n;
+      return ok;
+    };
+    auto read = [&]() {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive_remote_relaxed(remote(sa(&sm.acc_empty[b]), 0));
+    };
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+    for (; more; more = walk.next(j)) {
+      const uint32_t lane0 = j.lane0 + rank * 128 + quarter * 32;
+      bool ok = filled();
+      if constexpr (kRun == 0) {
+        if (ok) {
+          out.put(P, j, mine + b * NT, lane0, from, from + kHalfTokens, sm.scratch[warp - 2]);
+          read();
+        }
+      } else {
+        float sums[kHalfTokens];
+#pragma unroll
+        for (int i = 0; i < kHalfTokens; ++i) sums[i] = 0.0f;
+        const uint32_t runs = (blocks_of(j) + kRun - 1) / kRun;  // at least one: t is never empty here
+#pragma unroll 1
+        for (uint32_t r = 0; r < runs && ok; ++r) {
+          if (r) ok = filled();
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < kHalfTokens / 16; ++q)
+            if (from + q * 16 < j.cols) {
+              float f[16];
+              tmem_ld16f(mine + b * NT + from + q * 16, f);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sums[q * 16 + i] += f[i];
+            }
+          read();
+        }
+        if (ok) out.put(P, j, sums, lane0, from);
+      }
+      if (!ok) {
+        give_up();
+        break;
+      }
     }
   }
 

@@ -212,3 +212,61 @@ def test_infinite_logits(ctx, vocab, dtype):
     holds(True)
     w.t[:, 0] = inf
     holds(True)
+
+
+def exact_sums(h, w, t):
+    """As sums(), for logits that are exact in f32: the exponent is off by two roundings of l*log2(e), the sum of
+    exponentials by 2^-22 + 2^-19, lse and the loss by their own rounding."""
+    (lse, _), (loss, _) = sums(h, w, t)
+    big = (h.double() @ w.double().t()).abs().amax(1)
+    err = 2 * 1.4427 * U32 * big + 2.0 ** -22 + 2.0 ** -19
+    return (lse, err + U32 * lse.abs()), (loss, torch.where(t >= 0, err + 2 * U32 * (lse.abs() + loss.abs()), 0.0))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d", [1024, 2048, 2056, 4096])
+@pytest.mark.parametrize("form", ["identical", "one channel", "powers of two"])
+def test_logits_that_are_exact(ctx, form, d, dtype):
+    """No sum of these rounds, however long: the vocabulary's rows are all the same (lse is l + log(vocab)), h has one
+    channel each, or every product is the same power of two."""
+    rows, vocab = 70, 700
+    h, w, t, _ = inputs(rows, vocab, d, dtype, 4)
+    r, v = torch.arange(rows, device="cuda"), torch.arange(vocab, device="cuda")
+    if form == "identical":
+        w.t[:] = 1 / 64
+        h.t[:] = ((r % 5 - 2) / 2)[:, None]  # up to 64 at d = 4096
+    elif form == "one channel":
+        h.t.zero_()
+        h.t[r, r * 37 % d] = 1
+        w.t[:] = (torch.randint(-2048, 2048, (vocab, d), device="cuda") / 64).to(dtype)
+    else:
+        w.t[:] = (2.0 ** -(v % 3 + 6))[:, None]
+        h.t[:] = (2.0 ** (r % 3 - 1))[:, None]
+    (want_lse, err_lse), (want_loss, err_loss) = exact_sums(h.t, w.t, t)
+    loss, lse = forward(ctx, h, w, t)
+    assert_within(lse, want_lse, err_lse, "lse")
+    assert_within(loss, want_loss, err_loss, "loss")
+
+
+@pytest.mark.parametrize("where", ["first", "last", "spread"])
+def test_a_sum_is_not_cut_whatever_its_order(ctx, where):
+    """Logits of some 25 that a few channels make, first, last or among the others. In one sum on the tensor cores each
+    of the d/16 steps cuts 2^-26 of what is there, in the mean: d/16 * 2^-26 of the logit where the large channels
+    come first. At most a quarter of that is left in the mean of lse, as for sums of like channels."""
+    rows, vocab, d, large = 256, 6000, 4096, 32
+    g = torch.Generator(device="cuda").manual_seed(17)
+    at = {"first": slice(0, large), "last": slice(d - large, d), "spread": slice(5, d, d // large)}[where]
+    w = torch.randn(vocab, d, generator=g, device="cuda") / d ** 0.5
+    h = torch.randn(rows, d, generator=g, device="cuda")
+    w[:, at] = 0.75 + 0.1 * torch.rand(vocab, large, generator=g, device="cuda")
+    h[:, at] = 1 + 0.1 * torch.rand(rows, large, generator=g, device="cuda")
+    w, h = w.to(torch.bfloat16), h.to(torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    site = fb.loss_site(rows, vocab, d, torch.bfloat16)
+    work = torch.empty(ctx.linear_loss_workspace(site, grad=False), dtype=torch.uint8, device="cuda")
+    loss, lse = (torch.empty(rows, device="cuda") for _ in range(2))
+    ctx.linear_loss(site, h, w, t, loss, lse, work)
+    l = h.double() @ w.double().t()
+    want = torch.logsumexp(l, 1)
+    average = (torch.softmax(l, 1) * l).sum(1).mean()
+    assert average > 20 and (lse.double() - want).mean().abs() <= 0.25 * d / 16 * 2.0 ** -26 * average
