@@ -12,6 +12,9 @@
 //   dl_iv = g_i (exp(l_iv - lse_i) - [v = t_i]),  dh_i = sum_v dl_iv w_v,  dw_v = sum_i dl_iv h_i
 // takes the logits again, a piece of the vocabulary at a time, as one 16-bit matrix
 // dl from which both sums are products. The logits are never in memory.
+// The target's own p - 1 is expm1(l_it - lse_i) with the logit that lse was made of, the
+// same dot product: where the target is nearly certain, another sum of the same
+// products is off by more than p - 1 is.
 //
 // Bound by the tensor cores: 2 rows*vocab*d operations forward, three times that
 // backward. The rows that a call takes come first of all, side by side (list, h):
@@ -48,20 +51,23 @@ struct Taken {
   int32_t* target;
   float* lse;
   float* g;
+  float* missing;  // the target's probability less 1
   unsigned* most;  // the bits of the largest |g| (f16 alone; 0 before)
   uint16_t* h;     // stride ld, zeros from d up to it
   uint64_t ld;
 };
 struct TakeArgs {
   const uint16_t* h;
+  const void* w;  // backward
   const int32_t* targets;
   const float* lse;
   const float* dloss;
   float* loss_out;  // forward
   uint16_t* dh;     // backward, may be null
-  uint64_t ldh, lddh, rows, d;
+  uint64_t ldh, ldw, lddh, rows, d;
   uint32_t vocab, chunk;  // rows a block takes
   uint32_t grad, all, aligned;
+  uint32_t wide;  // h's rows side by side and the weights can be read eight at a time
   unsigned* trap;
 };
 
@@ -69,6 +75,23 @@ constexpr int kTakeThreads = 256;
 
 __device__ __forceinline__ bool is_target(int32_t t, uint32_t vocab) { return (uint32_t)t < vocab; }
 
+// A lane's share of a row's target logit, V elements an access. The loss and its gradient
+// take the same V, so that both have the same bits.
+template <typename T, int V>
+__device__ __forceinline__ float target_dot(const T* h, const T* w, uint32_t d) {
+  float dot = 0.0f;
+#pragma unroll 4
+  for (uint32_t e = (threadIdx.x & 31) * V; e < d; e += 32 * V) {
+    float x[V], y[V];
+    reinterpret_cast<const Pack<T, V>*>(h + e)->get(x);
+    reinterpret_cast<const Pack<T, V>*>(w + e)->get(y);
+#pragma unroll
+    for (int k = 0; k < V; ++k) dot = __fmaf_rn(x[k], y[k], dot);
+  }
+  return dot;
+}
+
+template <typename E>
 __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs A, const Taken T) {
   __shared__ uint32_t sums[kTakeThreads / 32];
   __shared__ uint32_t total;
@@ -113,6 +136,7 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
     for (uint32_t r = warp; r < 32 && i0 + r < hi; r += kTakeThreads / 32) {
       const bool take = (which >> r) & 1;
       const uint32_t to = __shfl_sync(0xffffffffu, c, r);
+      const int32_t target = __shfl_sync(0xffffffffu, t, r);
       if (take) {
         const uint16_t* from = A.h + (i0 + r) * A.ldh;
         uint16_t* out = T.h + (uint64_t)to * T.ld;
@@ -124,6 +148,13 @@ __global__ void __launch_bounds__(kTakeThreads) take_rows_kernel(const TakeArgs 
           if (e < T.ld) out[e] = e < A.d ? from[e] : (uint16_t)0;
         } else {
           for (uint64_t e = lane; e < T.ld; e += 32) out[e] = e < A.d ? __ldg(from + e) : (uint16_t)0;
+        }
+        if (A.grad) {
+          __syncwarp();  // the row as it lies now, whatever its own place
+          const E* h = reinterpret_cast<const E*>(out);
+          const E* w = static_cast<const E*>(A.w) + (uint64_t)target * A.ldw;
+          const float dot = warp_sum(A.wide ? target_dot<E, 8>(h, w, (uint32_t)A.d) : target_dot<E, 1>(h, w, (uint32_t)A.d));
+          if (lane == 0) T.missing[to] = expm1f(dot - __ldg(A.lse + i0 + r));
         }
       } else if (A.dh) {
         uint16_t* out = A.dh + (i0 + r) * A.lddh;
@@ -244,18 +275,7 @@ __global__ void __launch_bounds__(32 * kJoinRows)
   if (row0 >= count) return;
   float dot = 0.0f;
   const int32_t target = c < count ? __ldg(Q.target + c) : -1;
-  if (target >= 0) {
-    const T* hr = reinterpret_cast<const T*>(Q.h) + (uint64_t)c * Q.ld;
-    const T* wr = w + (uint64_t)target * ldw;
-#pragma unroll 4
-    for (uint32_t e = lane * V; e < d; e += 32 * V) {
-      float x[V], y[V];
-      reinterpret_cast<const Pack<T, V>*>(hr + e)->get(x);
-      reinterpret_cast<const Pack<T, V>*>(wr + e)->get(y);
-#pragma unroll
-      for (int k = 0; k < V; ++k) dot = __fmaf_rn(x[k], y[k], dot);
-    }
-  }
+  if (target >= 0) dot = target_dot<T, V>(reinterpret_cast<const T*>(Q.h) + (uint64_t)c * Q.ld, w + (uint64_t)target * ldw, d);
   float2 a = make_float2(-INFINITY, 0.0f);
   const bool in = row0 + r < count;
   for (uint32_t p = p0; p < nparts; p += 32 * kJoinAhead) {
@@ -323,6 +343,7 @@ struct GradientTile {
   const int32_t* target;
   const float* lse;
   const float* g;
+  const float* missing;
   const unsigned* most;
   uint32_t v0;
 
@@ -332,7 +353,8 @@ struct GradientTile {
     const bool in = lane < (uint32_t)__ldg(P.lane_count);
     const uint32_t to = min(from + kHalfTokens, j.cols);
     const int32_t mine = in ? __ldg(target + lane) - (int32_t)(v0 + j.col0) : -1;
-    const float base = in ? -__ldg(lse + lane) * kLog2e : 0.0f, c = in ? __ldg(g + lane) * scale_up(most) : 0.0f;
+    const float base = in ? -__ldg(lse + lane) * kLog2e : 0.0f, c = in ? __ldg(g + lane) * scale_up(most) : 0.0f,
+                less = in ? __ldg(missing + lane) : 0.0f;
     T* row = dl + (uint64_t)(in ? lane : 0) * ld + j.col0;
 #pragma unroll
     for (int q = 0; q < kHalfTokens / 32; ++q) {
@@ -344,7 +366,7 @@ struct GradientTile {
       const uint32_t hit = (uint32_t)(mine - (int32_t)j0);
       if (any_of(hit < 32)) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] -= hit == i ? 1.0f : 0.0f;
+        for (int i = 0; i < 32; ++i) f[i] = hit == i ? less : f[i];
       }
       if (in) {
         // sixteen at a time, whole sectors (dl, its rows and j0 lie on 32 bytes): what lies behind the piece's last
@@ -459,12 +481,15 @@ struct Plan {
   uint32_t piece, pieces;   // of the vocabulary, a multiple of 256
   uint32_t parts;           // of a piece, in dh
   bool copies;              // weights that TMA cannot read
-  uint64_t list, count, target, lse, g, most, h, w, sums, dl, bytes;  // offsets
+  uint64_t list, count, target, lse, g, missing, most, h, w, sums, dl, bytes;  // offsets
 };
 
 bool weights_in_place(const MapalLossSite& s, const void* w) {
   return aligned16(w) && (s.vocab == 1 || s.ldw % 8 == 0);
 }
+
+// Whether the targets' logits are taken eight elements at a time.
+bool dots_wide(const MapalLossSite& s, const void* w) { return weights_in_place(s, w) && s.d % 8 == 0; }
 
 Plan plan_of(const MapalLossSite& s, bool grad, bool copies, int sms) {
   Plan p{};
@@ -508,6 +533,7 @@ Plan plan_of(const MapalLossSite& s, bool grad, bool copies, int sms) {
   if (grad) {
     p.lse = take(4 * s.rows);
     p.g = take(4 * s.rows);
+    p.missing = take(4 * s.rows);
     p.most = take(4);
     p.dl = take(2 * s.rows * p.piece);
     if (p.pieces > 1 || p.parts > 1) p.sums = take(4 * s.rows * s.d * p.parts);
@@ -548,14 +574,18 @@ struct Call {
   }
   Call(DeviceSlot& d, const MapalLossSite& site, const Plan& plan, void* w, bool grad)
       : D(d), s(site), p(plan), work(reinterpret_cast<uint8_t*>(up((uintptr_t)w, kStoreAligned))) {
-    q = {at<int32_t>(p.list), at<int32_t>(p.count), at<int32_t>(p.target), at<float>(p.lse), at<float>(p.g),
+    q = {at<int32_t>(p.list), at<int32_t>(p.count), at<int32_t>(p.target), at<float>(p.lse), at<float>(p.g), at<float>(p.missing),
          grad && s.dtype == MAPAL_DTYPE_F16 ? at<unsigned>(p.most) : nullptr, at<uint16_t>(p.h), p.ld};
   }
 
-  int take(TakeArgs a, const void* h, const int32_t* targets) const {
+  template <typename T>
+  int take(TakeArgs a, const void* h, const void* w, const int32_t* targets) const {
     a.h = static_cast<const uint16_t*>(h);
+    a.w = w;
     a.targets = targets;
     a.ldh = s.ldh;
+    a.ldw = s.ldw;
+    a.wide = dots_wide(s, w);
     a.lddh = s.lddh;
     a.rows = s.rows;
     a.d = s.d;
@@ -564,7 +594,7 @@ struct Call {
     a.trap = D.trap;
     const uint64_t blocks = std::min<uint64_t>((s.rows + 3) / 4, 8ull * D.prof.sm_count);
     a.chunk = (uint32_t)((s.rows + blocks - 1) / blocks);
-    return launch_rows(take_rows_kernel, (unsigned)((s.rows + a.chunk - 1) / a.chunk), kTakeThreads, 0, D.stream, 1, a, q);
+    return launch_rows(take_rows_kernel<T>, (unsigned)((s.rows + a.chunk - 1) / a.chunk), kTakeThreads, 0, D.stream, 1, a, q);
   }
   // The weights of a piece where TMA can read them.
   int weights(const void* w, uint32_t v0, uint32_t n, const void** out, uint64_t* ld) const {
@@ -604,7 +634,7 @@ int forward(const Call& c, const void* h, const void* w, const int32_t* targets,
   TakeArgs a{};
   a.loss_out = loss;
   a.all = lse != nullptr;
-  MAPAL_TRY(c.take(a, h, targets));
+  MAPAL_TRY(c.take<T>(a, h, w, targets));
   float2* parts = c.template at<float2>(c.p.sums);
   for (uint32_t i = 0; i < c.p.pieces; ++i) {
     const uint32_t v0 = i * c.p.piece, n = (uint32_t)std::min<uint64_t>(c.p.piece, s.vocab - v0);
@@ -615,12 +645,11 @@ int forward(const Call& c, const void* h, const void* w, const int32_t* targets,
   }
   const uint32_t nparts = (uint32_t)(up(s.vocab, 256) / 128);
   const unsigned blocks = (unsigned)((s.rows + kJoinRows - 1) / kJoinRows);
-  const bool wide = weights_in_place(s, w) && s.d % 8 == 0;
   auto go = [&](auto kernel) {
     return launch_rows(kernel, blocks, 32 * kJoinRows, 0, c.D.stream, 1, parts, s.rows, nparts, c.q,
                        static_cast<const T*>(w), s.ldw, (uint32_t)s.d, loss, lse);
   };
-  return wide ? go(join_kernel<T, 8>) : go(join_kernel<T, 1>);
+  return dots_wide(s, w) ? go(join_kernel<T, 8>) : go(join_kernel<T, 1>);
 }
 
 template <typename T>
@@ -634,7 +663,7 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
   a.dloss = dloss;
   a.dh = static_cast<uint16_t*>(dh);
   a.grad = 1;
-  MAPAL_TRY(c.take(a, h, targets));
+  MAPAL_TRY(c.take<T>(a, h, w, targets));
   T* dl = c.template at<T>(p.dl);
   float* sums = c.template at<float>(p.sums);
   const uint64_t ldp = s.rows * s.d;
@@ -643,7 +672,7 @@ int backward(const Call& c, const void* h, const void* w, const int32_t* targets
     const void* from;
     uint64_t ldw;
     MAPAL_TRY(c.weights(w, v0, n, &from, &ldw));
-    MAPAL_TRY(c.logits(from, ldw, n, GradientTile<T>{dl, p.piece, c.q.target, c.q.lse, c.q.g, c.q.most, v0}));
+    MAPAL_TRY(c.logits(from, ldw, n, GradientTile<T>{dl, p.piece, c.q.target, c.q.lse, c.q.g, c.q.missing, c.q.most, v0}));
     ProductArgs P = c.args();
     P.offsets = c.q.count;
     P.m = (uint32_t)s.rows;

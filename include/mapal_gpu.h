@@ -701,7 +701,8 @@ int mapal_gpu_linear_loss(MapalGpuCtx* ctx, const MapalLossSite* site, const voi
  * dl[i, v] = dloss[i]*(exp(l[i, v] - lse[i]) - (v == t)) (dloss NULL: 1),
  *   dH[i] = sum over v of dl[i, v]*W[v],  dW[v] = sum over i of dl[i, v]*H[i],
  * written (not added to); either may be NULL. dl is taken for a piece of the
- * vocabulary at a time and rounded to the rows' type, f16 after a power of two
+ * vocabulary at a time (its target's exp - 1 without their difference, from
+ * the logit that lse has) and rounded to the rows' type, f16 after a power of two
  * that keeps a mean's small gradients in its range; sums are f32. A row without
  * a target has a dH of zeros and adds nothing to dW, whatever it holds. */
 int mapal_gpu_linear_loss_grad(MapalGpuCtx* ctx, const MapalLossSite* site, const void* h, const void* w,

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import flow_b200 as fb
-from _rows import U32, Guarded, assert_within, replayed
+from _rows import U32, Guarded, assert_within, half_step, out_error, replayed
 from test_gpu_linear_loss import HALF, formula, inputs
 from test_gpu_training_step import Step
 
@@ -270,3 +270,46 @@ def test_a_sum_is_not_cut_whatever_its_order(ctx, where):
     want = torch.logsumexp(l, 1)
     average = (torch.softmax(l, 1) * l).sum(1).mean()
     assert average > 20 and (lse.double() - want).mean().abs() <= 0.25 * d / 16 * 2.0 ** -26 * average
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d,offset", [(136, 0), (2048, 0), (4096, 0), (4099, 1)])
+@pytest.mark.parametrize("order", [1, -1])
+def test_the_gradient_of_nearly_certain_targets(ctx, order, d, offset, dtype):
+    """1 - p of a target with a logit of some 20 that its first (or last) channels make, from the loss's own lse. Row i
+    alone has channel i, of which the weights are 0, so that dw[:, i] is dl of row i, rounded twice (f16: at a scale
+    that brings 1 to 2^14). lse is rounded by U32 of itself and the difference to it is exact; the others' sum has
+    their logits' errors."""
+    rows, vocab, large = 24, 5000, 48
+    g = torch.Generator(device="cuda").manual_seed(23)
+    h, w, t, _ = inputs(rows, vocab, d, dtype, 9, offsets=(0, offset))
+    t[:] = torch.randperm(vocab, generator=g, device="cuda")[:rows]
+    h.t.mul_(0.5)
+    w.t.mul_(0.5)
+    lead = torch.arange(rows, rows + large, device="cuda") if order > 0 else torch.arange(d - large, d, device="cuda")
+    signs = torch.randint(0, 2, (rows, large), generator=g, device="cuda") * 2.0 - 1
+    h.t[:, lead] = (signs * (0.6 + 0.1 * torch.rand(rows, large, generator=g, device="cuda"))).to(dtype)
+    w.t[:, lead] = (0.1 * torch.randn(vocab, large, generator=g, device="cuda")).to(dtype)
+    w.t[t.long()[:, None], lead] = (signs * 0.65).to(dtype)
+    h.t[:, :rows] = torch.eye(rows, device="cuda").to(dtype)
+    w.t[:, :rows] = 0
+    site = fb.loss_site(rows, vocab, d, dtype, ldh=h.ld, ldw=w.ld)
+    work = torch.empty(ctx.linear_loss_workspace(site, w=w.t), dtype=torch.uint8, device="cuda")
+    loss, lse = (torch.empty(rows, device="cuda") for _ in range(2))
+    dh, dw = torch.empty(rows, d, dtype=dtype, device="cuda"), torch.empty(vocab, d, dtype=dtype, device="cuda")
+    ctx.linear_loss(site, h.t, w.t, t, loss, lse, work)
+    ctx.linear_loss_grad(site, h.t, w.t, t, lse, None, dh, dw, work)
+    h64, w64, at = h.t.double(), w.t.double(), t.long()[:, None]
+    l = h64 @ w64.t()
+    p = torch.softmax(l, 1)
+    missing = p.scatter(1, at, 0.0).sum(1)  # 1 - p of the target, without the difference
+    assert missing.max() < 2e-3 and missing.min() < 2e-5
+    size = (h64.abs() @ w64.abs().t()).amax(1)
+    rel = (d + 16) * 17 / 16 * 2 * U32 * size + 8 * U32 * l.abs().amax(1) + 2.0 ** -18
+    tiny = 2.0 ** -38 if dtype == torch.float16 else 0.0
+    err = 2 * U32 * lse.double() + missing * (rel + 2 * half_step(dtype)) + tiny + out_error(missing, dtype)
+    got = -dw[t.long(), torch.arange(rows, device="cuda")].double()
+    assert_within(got, missing, err, "1 - p")
+    others = p.scatter(1, at, 0.0).t()
+    err = others * (2 * rel[None] + 2 * half_step(dtype)) + tiny + out_error(others, dtype)
+    assert_within(dw[:, :rows].double().scatter(0, at.t(), 0.0), others, err, "p")
