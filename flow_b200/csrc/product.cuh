@@ -403,7 +403,8 @@ struct StoreTile {
 
 constexpr int kPairTokens = 256, kPairOut = 8;
 constexpr int kCopyGroups = 3, kCopyWarps = 4;  // groups of so many warps take turns at the blocks
-constexpr uint64_t kRawLandNs = 1000000;  // after a wait gave up: for raw loads in flight
+constexpr uint32_t kToldBytes = 16;
+constexpr uint64_t kRawLandNs = 1000000;  // after a wait gave up: for copies in flight that nothing waits for
 constexpr int kLineK = 144, kLineMN = 272;  // raw bytes of a line: 64 steps, or 128 lanes or columns, and 16 more
 constexpr int kRawOperand = 128 * kLineK;
 static_assert(64 * kLineMN <= kRawOperand, "raw lines");
@@ -414,7 +415,7 @@ struct PairSmem {
   static constexpr int kHalf = 128 * 128;  // bytes of a block of lanes, and of columns
   uint8_t stage[STAGES][KB * 2 * kHalf];
   alignas(128) uint8_t raw[RAW == 0 ? 1 : RAW][RAW == 0 ? 16 : kRawOperand];
-  uint64_t full[STAGES];    // the first CTA's: both CTAs' loads have landed
+  uint64_t full[STAGES];    // the first CTA's: both CTAs' loads have landed, their copies are written
   uint64_t empty[STAGES];   // each CTA's own
   uint64_t landed[STAGES];  // each CTA's own: a last block to clear
   uint64_t fixed[STAGES];   // the first CTA's: cleared in both
@@ -423,6 +424,7 @@ struct PairSmem {
   uint64_t acc_empty[2];    // the first CTA's: both CTAs have read the accumulator
   uint64_t drained;
   alignas(16) uint8_t scratch[kPairOut][kOutScratch];
+  alignas(16) uint8_t told[kCopyGroups * kCopyWarps + 1][kToldBytes];  // where tell_written's copies go, a warp's each
   uint32_t tmem_base;
   int abort;
 };
@@ -490,13 +492,21 @@ __device__ __forceinline__ void arrive_remote_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// An arrival at the first CTA's barrier for what this warp has written to its own
-// CTA's shared memory, where only the tensor cores read it: fence.proxy.async, by
-// every writing lane before, has waited until they see it, so the arrival itself needs
-// no order beyond the CTA. As a release among the CTAs it would take 500 to 1500
-// cycles, the time of two blocks.
-__device__ __forceinline__ void arrive_written(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Tells the first CTA's barrier that this warp has written to its own CTA's shared memory,
+// `written` among it, which the pair's MMA reads from both CTAs; every writing lane has made
+// its part visible to the asynchronous proxy before. The second CTA tells it by a copy of
+// 16 bytes between the CTAs: the copy follows what was written, and its completion is a
+// release among the CTAs, which a thread's own arrival can be too, but for 500 to 1800
+// cycles in which the thread waits for its SM's stores (4096 x 4096 x 4097: 275 us). The
+// first CTA's arrival expects the bytes.
+__device__ __forceinline__ void tell_written(uint64_t* bar, const void* written, const void* to, uint32_t rank) {
+  if (rank == 0)
+    mbar_expect_tx(bar, kToldBytes);
+  else
+    asm volatile(
+        "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(remote(sa(to), 0)),
+        "r"(sa(written)), "r"(kToldBytes), "r"(remote(sa(bar), 0))
+        : "memory");
 }
 
 __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -569,10 +579,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
     for (size_t i = 0; i < sizeof(maps_a) / sizeof(CUtensorMap); ++i) prefetch_map(reinterpret_cast<const CUtensorMap*>(&maps_a) + i);
     for (size_t i = 0; i < sizeof(maps_b) / sizeof(CUtensorMap); ++i) prefetch_map(reinterpret_cast<const CUtensorMap*>(&maps_b) + i);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full[s], (TA || TB) + (Cut::kCopy ? 2 * kCopyWarps : 0));
+      mbar_init(&sm.full[s], (TA || TB) + (Cut::kCopy ? kCopyWarps : 0));
       mbar_init(&sm.empty[s], 1);
       mbar_init(&sm.landed[s], 1);
-      mbar_init(&sm.fixed[s], 2);
+      mbar_init(&sm.fixed[s], 1);
     }
     for (int i = 0; i < kRaw * (CA + CB); ++i) {
       mbar_init(&sm.raw_full[i], 1);
@@ -737,7 +747,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
           *reinterpret_cast<uint4*>(block + chunk * (kStepK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_written(remote(sa(&sm.fixed[s]), 0));
+      if (lane == 0) tell_written(&sm.fixed[s], block + (TA ? 0 : Smem::kHalf) + rows * 128, sm.told[kCopyGroups * kCopyWarps], rank);
     }
   } else if ((CA || CB) && warp >= kCopier) {
     // ---- copies ----
@@ -772,7 +782,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
         if (lane == 0) {
           if (CA) mbar_arrive(&sm.raw_empty[q]);
           if (CB) mbar_arrive(&sm.raw_empty[q + CA * kRaw]);
-          arrive_written(remote(sa(&sm.full[s]), 0));
+          tell_written(&sm.full[s], sm.stage[s] + (CA ? 0 : Smem::kHalf) + (thread >> 3) * 128, sm.told[warp - kCopier], rank);
         }
       }
       if (gone) give_up();
@@ -846,8 +856,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE, C
       }
       if (MODE == kGradW)
         for (int s = 0; s < kStages; ++s) mbar_wait(&sm.landed[s], ((fixes >> s) & 1) ^ 1, nullptr);
-      if (Cut::kCopy) {
-        const uint64_t t0 = now_ns();  // raw lines land within microseconds, whoever waits for them
+      if (Cut::kCopy || MODE == kGradW) {
+        const uint64_t t0 = now_ns();  // raw lines and words that tell land within microseconds, whoever waits for them
         while (now_ns() - t0 < kRawLandNs) {
         }
       }

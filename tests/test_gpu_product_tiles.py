@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import flow_b200 as fb
-from test_gpu_product import HALF, check
+from test_gpu_product import HALF, check, operands, ragged, wants
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,25 @@ def test_few_rows_and_many_channels(ctx, m, n, k, groups, dtype):
     gradient (k large), with rows on 16-byte boundaries and, the outputs alone, off them."""
     check(ctx, m, n, k, groups, dtype)
     check(ctx, m, n, k, groups, dtype, opads=(3, 5, 0), seed=5)
+
+
+@pytest.mark.parametrize("m,n,k,groups,pads", [(1500, 516, 771, 11, (0, 0, 0)), (1500, 520, 776, 11, (8, 0, 8)), (1500, 520, 771, 11, (0, 0, 0)),
+                                               (1501, 517, 776, 11, (0, 0, 0)), (900, 1029, 2051, 1, (0, 0, 0)), (2000, 768, 768, 60, (0, 0, 0))])
+def test_copied_operands_and_last_blocks_many_times(ctx, m, n, k, groups, pads):
+    """What one CTA of a pair writes to its shared memory is read by the other's products: copied blocks, and last blocks
+    whose rows of the next group are cleared. Forty passes, each from other contents of shared memory, bit for bit."""
+    dtype = torch.bfloat16
+    sets = [operands(m, n, k, groups, dtype, pads=pads, seed=s) for s in (1, 11)]
+    off = ragged(m, groups, 3) if groups > 1 else None
+    site = fb.product_site(m, n, k, dtype, groups=groups, ldx=sets[0][0].ld, ldw=sets[0][1].ld, lddy=sets[0][2].ld)
+    want = []
+    for x, w, dy in sets:
+        y, dx, dw = wants(x.t, w.t.reshape(groups, n, k), dy.t, off)
+        want.append((y.to(dtype), dx.to(dtype), dw.to(dtype)))
+    y, dx, dw = (torch.empty(s, dtype=dtype, device="cuda") for s in ((m, n), (m, k), (groups, n, k)))
+    for i in range(40):
+        x, w, dy = sets[i % 2]
+        ctx.product(site, x.t, w.t, y, offsets=off)
+        ctx.product_grad(site, x.t, w.t, dy.t, dx, dw, offsets=off)
+        for got, right, what in zip((y, dx, dw), want[i % 2], ("y", "dx", "dw")):
+            assert torch.equal(got, right), (i, what)
