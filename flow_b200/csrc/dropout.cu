@@ -242,10 +242,7 @@ extern "C" int mapal_gpu_dropout(MapalGpuCtx* ctx, const MapalDropoutSite* site,
     A.blocks = (uint32_t)((s.d + 7) / 8);
     const uint32_t limit = (uint32_t)std::lrint(s.p * 65536.0);
     if (limit == 65536) {  // nothing of x is left
-      if (residual && residual != y)
-        MAPAL_CUDA(cudaMemcpy2DAsync(y, s.ldy * es, residual, s.ldr * es, s.d * es, s.rows, cudaMemcpyDeviceToDevice, D.stream));
-      else if (!residual)
-        MAPAL_CUDA(cudaMemset2DAsync(y, s.ldy * es, 0, s.d * es, s.rows, D.stream));
+      if (residual != y) MAPAL_TRY(copy_rows(y, s.ldy * es, residual, s.ldr * es, s.d * es, s.rows, D.stream));
       return finish(ctx, 0, false);
     }
     A.limit = limit * 0x10001u;

@@ -768,7 +768,7 @@ extern "C" int mapal_gpu_linear_loss_grad(MapalGpuCtx* ctx, const MapalLossSite*
     MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
     if (s.rows == 0) {
-      if (dw) MAPAL_CUDA(cudaMemset2DAsync(dw, 2 * s.lddw, 0, 2 * s.d, s.vocab, D.stream));
+      if (dw) MAPAL_TRY(copy_rows(dw, 2 * s.lddw, nullptr, 0, 2 * s.d, s.vocab, D.stream));
       return finish(ctx, 0, false);
     }
     const Plan p = plan_of(s, true, !weights_in_place(s, w), D.prof.sm_count);

@@ -277,6 +277,33 @@ inline bool rows_ok(uint64_t rows, uint64_t cols, uint64_t ld, uint64_t elem) {
   return ld <= lim / elem && (rows - 1) <= (lim / elem - cols) / ld;
 }
 
+// `bytes` of each of some rows copied, or set to zeros (from null), at strides in bytes.
+// One row's stride may be anything, and the runtime's own two-dimensional calls take
+// strides up to 2^31 - 1: longer ones are some hundred rows at most in a device's memory.
+inline int copy_rows(void* to, uint64_t ldt, const void* from, uint64_t ldf, uint64_t bytes, uint64_t rows, cudaStream_t stream) {
+  if (rows <= 1 || (ldt == bytes && (!from || ldf == bytes))) {
+    bytes *= rows;
+    rows = 1;
+    ldt = ldf = bytes;
+  }
+  const uint64_t most = 0x7fffffff;
+  if (rows > 1 && ldt <= most && (!from || ldf <= most)) {
+    if (from)
+      MAPAL_CUDA(cudaMemcpy2DAsync(to, ldt, from, ldf, bytes, rows, cudaMemcpyDeviceToDevice, stream));
+    else
+      MAPAL_CUDA(cudaMemset2DAsync(to, ldt, 0, bytes, rows, stream));
+    return 0;
+  }
+  for (uint64_t r = 0; r < rows; ++r) {
+    uint8_t* p = static_cast<uint8_t*>(to) + r * ldt;
+    if (from)
+      MAPAL_CUDA(cudaMemcpyAsync(p, static_cast<const uint8_t*>(from) + r * ldf, bytes, cudaMemcpyDeviceToDevice, stream));
+    else
+      MAPAL_CUDA(cudaMemsetAsync(p, 0, bytes, stream));
+  }
+  return 0;
+}
+
 // The widest access of 16, 8, 4, 2 or 1 bytes that a pointer and a row stride
 // (in bytes; ignored for a single row) are multiples of.
 inline int align_of(const void* p, uint64_t stride_bytes, uint64_t rows) {
