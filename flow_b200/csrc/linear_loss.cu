@@ -761,6 +761,9 @@ extern "C" int mapal_gpu_linear_loss_grad(MapalGpuCtx* ctx, const MapalLossSite*
     const MapalLossSite& s = *site;
     if (!dh && !dw) return 0;
     if (s.rows && (!h || !w || !targets || !lse)) return set_error(MAPAL_ERR_INVALID, "null h, w, targets or lse");
+    // a piece's dw is written before its w has gone into dh; h is gathered before anything is written
+    if (s.rows && ((dw && (dw == h || dw == dh || (dh && dw == w))) || (dh && (dh == w || (dh == h && s.rows > 1 && s.lddh != s.ldh)))))
+      return set_error(MAPAL_ERR_INVALID, "dh or dw is an array that the call reads");
     if (((uintptr_t)h | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)dw) & 1 ||
         ((uintptr_t)targets | (uintptr_t)lse | (uintptr_t)dloss) & 3)
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");

@@ -784,6 +784,7 @@ extern "C" int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site,
     if (!y || (s.k && (!x || !w))) return set_error(MAPAL_ERR_INVALID, "null x, w or y");
     if (!on_type(x, s.dtype) || !on_type(w, s.dtype) || !on_type(y, s.ytype) || ((uintptr_t)offsets & 3))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
+    if (s.k && (y == x || y == w)) return set_error(MAPAL_ERR_INVALID, "y is x or w");
     const OnDevice on(ctx);
     MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];
@@ -816,6 +817,10 @@ extern "C" int mapal_gpu_product_grad(MapalGpuCtx* ctx, const MapalProductSite* 
     if (!on_type(x, s.dtype) || !on_type(w, s.dtype) || !on_type(dy, s.dtype) || !on_type(dx, s.dtype) ||
         !on_type(dw, s.dwtype) || ((uintptr_t)offsets & 3))
       return set_error(MAPAL_ERR_INVALID, "a pointer is not aligned to its type");
+    // an output may be an operand that the call does not read: x without dw, w without dx
+    const bool reads = s.m && s.n;
+    if (reads && ((do_x && (dx == dy || dx == w || (do_w && dx == x))) || (do_w && (dw == dy || dw == x || (do_x && dw == w)))))
+      return set_error(MAPAL_ERR_INVALID, "dx or dw is an array that the call reads");
     const OnDevice on(ctx);
     MAPAL_TRY(on.rc);
     DeviceSlot& D = ctx->dev[0];

@@ -648,7 +648,8 @@ typedef struct MapalProductSite {
  * offsets[g + 1] (groups + 1 values on the device, as mapal_gpu_expert_sort
  * writes them) belong to g; rows of Y in no group are left as they were.
  * Offsets that descend or leave [0, m] trap index_oob and are taken as the
- * largest up to them, clamped to [0, m]. k = 0 gives zeros. */
+ * largest up to them, clamped to [0, m]. k = 0 gives zeros. Y overlaps neither X
+ * nor W. */
 int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site, const void* x, const void* w,
                       const int32_t* offsets, void* y);
 
@@ -658,7 +659,8 @@ int mapal_gpu_product(MapalGpuCtx* ctx, const MapalProductSite* site, const void
  * written (not added to). dx (m x k) or dw (groups of n x k) may be NULL, then
  * w or x is not read. Rows of dX in no group are left as they were; a group
  * without rows has a dW of zeros. Bad offsets trap index_oob; dW[g] is then
- * the sum over its range's rows that exist. */
+ * the sum over its range's rows that exist. The outputs overlap nothing that the
+ * call reads: dX may be X, or dW W, where it is the only one asked for. */
 int mapal_gpu_product_grad(MapalGpuCtx* ctx, const MapalProductSite* site, const void* x, const void* w,
                            const int32_t* offsets, const void* dy, void* dx, void* dw);
 
@@ -704,7 +706,9 @@ int mapal_gpu_linear_loss(MapalGpuCtx* ctx, const MapalLossSite* site, const voi
  * vocabulary at a time (its target's exp - 1 without their difference, from
  * the logit that lse has) and rounded to the rows' type, f16 after a power of two
  * that keeps a mean's small gradients in its range; sums are f32. A row without
- * a target has a dH of zeros and adds nothing to dW, whatever it holds. */
+ * a target has a dH of zeros and adds nothing to dW, whatever it holds. The
+ * outputs overlap no operand, but dH may be H (same pointer and stride), and dW
+ * may be W where dH is NULL. */
 int mapal_gpu_linear_loss_grad(MapalGpuCtx* ctx, const MapalLossSite* site, const void* h, const void* w,
                                const int32_t* targets, const float* lse, const float* dloss, void* dh, void* dw,
                                void* work, uint64_t work_bytes);
