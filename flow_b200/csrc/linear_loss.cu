@@ -20,9 +20,11 @@
 // backward. The rows that a call takes come first of all, side by side (list, h):
 // those with a target, and all of them where lse is asked for, which every row has.
 // The others cost nothing and whatever they hold is not read.
-// Measured on a B200: 8192 rows, 128000 x 4096 bf16, forward and backward 26.7 ms (1.28
-// PFLOP/s over four products, at the power limit); 2401 rows, 50257 x 1000 216 and
-// 653 us; 16 rows, 50257 x 2048 57 and 155 us (the weights, once and three times: 32 and 96).
+// Measured on a B200, graph replays, forward and backward: 8192 rows, 128000 x 4096 bf16
+// 6.6 and 20.6 ms (1.27 PFLOP/s over four products, at the power limit); 2401 rows,
+// 50257 x 1000 222 and 643 us in bf16, 287 and 700 in f16; 3001 rows of which 600 have no
+// target, f16, 331 (270 without lse) and 779 us; 16 rows, 50257 x 2048 bf16 58 and 161 us
+// (the weights, once and three times: 32 and 96).
 #include <algorithm>
 
 #include "product.cuh"

@@ -612,7 +612,8 @@ struct Cut {
 // 16 steps of t, 72 + N/4 at least), and the loads, at up to 58 bytes a cycle for
 // an SM and 7200 for all; tiles run in waves. The constants are fitted to 210 products
 // (1 to 16000 rows, 64 to 8192 channels, 1 to 64 matrices, all three modes) that were
-// measured with every cut: the cut chosen takes 2 % longer than the best, in the mean.
+// measured with every cut. grad w: a group's rows are on the device, and the mean
+// stands for each, which groups of very different sizes are cut the worse for.
 double cycles_of(int mode, const ProductArgs& P, const Cut& c, uint32_t depth, int sms) {
   const bool pair = c.lanes == 256;
   const double tiles = (double)product_tiles(mode, P, c.cols, c.lanes) * c.split, at_once = pair ? sms / 2 : sms;

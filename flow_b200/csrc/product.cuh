@@ -397,7 +397,7 @@ struct StoreTile {
 // Everything else is as with operands in place. A copy loop through registers
 // instead (two aligned words a thread, a block ahead) took 3300 ns a block of
 // both operands, waiting for L1's few lines; this takes 770, and 550 where one
-// is copied (4096 x 4096 x 4097: 200 us forward, 142 and 153 for the gradients; the
+// is copied (4096 x 4096 x 4097: 204 us forward, 137 and 152 for the gradients; the
 // products alone take 270 a block; with two groups of warps 212 us). Shared memory bounds it: two reads and a write of every
 // 16 bytes, 384 cycles an operand's block.
 

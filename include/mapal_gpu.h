@@ -643,7 +643,9 @@ typedef struct MapalProductSite {
 } MapalProductSite;
 
 /* Y[i, j] = sum over t of X[i, t]*W[g][j, t], the products exact, the sum in f32
- * on the tensor cores, in an order fixed by the record and the device. offsets
+ * on the tensor cores, in an order fixed by the record and the device. They cut
+ * a sum towards zero at each step of 16 products, which f32 outputs show: some
+ * 4e-6 of a sum of 4096 like terms. offsets
  * NULL: groups is 1 and every row belongs to it. Otherwise rows offsets[g] to
  * offsets[g + 1] (groups + 1 values on the device, as mapal_gpu_expert_sort
  * writes them) belong to g; rows of Y in no group are left as they were.
@@ -687,8 +689,8 @@ int mapal_gpu_linear_loss_workspace(MapalGpuCtx* ctx, const MapalLossSite* site,
 
 /* Softmax cross entropy of the logits l[i, v] = <H[i], W[v]>, which are never
  * in memory: with lse[i] = log(sum over v of exp(l[i, v])) and target t,
- * loss[i] = lse[i] - l[i, t]. Logits are f32 (products exact, sums on the
- * tensor cores, the target's by itself), and the loss of a target that is
+ * loss[i] = lse[i] - l[i, t]. Logits are f32 (products exact, sums of 256 on the
+ * tensor cores, which cut them, added in f32; the target's by itself), and the loss of a target that is
  * nearly certain is the others' share, not what is left of two large numbers.
  * targets: one of [0, vocab) a row; -1: the row has none and its loss is 0. Any
  * other target traps index_oob; its row is treated as one without. lse is every
